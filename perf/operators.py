@@ -387,7 +387,8 @@ def _branch_plain(s):
     begin = need.cumsum(0) - need
     free = torch.sort((refs > 0).int(), stable=True).indices
     fresh = torch.where(copied, free[begin], last)
-    kv[:, :, fresh] = kv[:, :, last]
+    filled = torch.arange(P, device=DEV) < (length % P)[:, None]         # the rows that the last page holds
+    kv[:, :, fresh] = torch.where(filled[:, None, :, None], kv[:, :, last], kv[:, :, fresh])
     refs.index_add_(0, last, -copied.int())
     j = torch.arange(-(-c["new"] // P) + 1, device=DEV)
     page = free[(begin + copied.long())[:, None] + j]
@@ -529,7 +530,7 @@ def _branch_exact(s, plan):
         at, length = table[p + i], lens[p + i]
         if length % P and then[at[length // P]] > 1:
             old, page = at[length // P], free.pop(0)
-            kv[:, :, page] = kv[:, :, old]
+            kv[:, :, page, :, :length % P] = kv[:, :, old, :, :length % P]
             refs[old] -= 1
             refs[page] = 1
             at[length // P] = page
