@@ -227,9 +227,10 @@ def prepare(case, seed):
         rows = dict(enumerate(zip(plan["rows"], plan["lens"])))
         s["table"], s["lens"], s["refs"] = _tables(plan, rows)
         s.update(table_sent=s["table"].clone(), lens_sent=s["lens"].clone(), refs_sent=s["refs"].clone())
-    if own:            # the handle that a program opens once for its cache
+    if own:            # the handle that a program opens once for its cache, and the library's stream for torch
         from mod_amd import ops
         s["cache"] = ops.KvCache(kv, s["table"], s["lens"], s["refs"])
+        s["stream"] = torch.cuda.ExternalStream(ops.lib.get_current_stream())
     return s
 
 
@@ -248,15 +249,10 @@ def run(state):
             _branch_own(s)
         else:
             _branch_plain(s)
+    elif own:
+        _compact_own(s)
     else:
-        # the tables as the scheduler sends them
-        s["table"].copy_(s["table_sent"])
-        s["lens"].copy_(s["lens_sent"])
-        s["refs"].copy_(s["refs_sent"])
-        if own:
-            _compact_own(s)
-        else:
-            _compact_plain(s)
+        _compact_plain(s)
     return dict(table=s["table"], lens=s["lens"], refs=s["refs"], kv=s["kv"])
 
 
@@ -288,7 +284,16 @@ def _branch_own(s):
 
 def _compact_own(s):
     from mod_amd import ops
+    with torch.cuda.stream(s["stream"]):
+        _send_tables(s)
     ops.kv_compact(s["cache"])
+
+
+def _send_tables(s):
+    """The tables as the scheduler sends them."""
+    s["table"].copy_(s["table_sent"])
+    s["lens"].copy_(s["lens_sent"])
+    s["refs"].copy_(s["refs_sent"])
 
 
 def _attention_plain(s):
@@ -411,6 +416,7 @@ def _branch_plain(s):
 
 
 def _compact_plain(s):
+    _send_tables(s)
     kv, table, refs = s["kv"], s["table"], s["refs"]
     live = refs > 0
     index = torch.arange(refs.shape[0], device=DEV)
