@@ -305,6 +305,122 @@ int pio_moe_w8a8(const void* x, int x_dtype, const float* logits, const int8_t* 
                  void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Paged key / value cache of many sequences (no counterpart in the reference,
+ * whose one cache is a dense tensor per layer, architecture.py:195-201, and
+ * whose paged attention kernel is never launched, tensor_ops_cuda.cu:582-618).
+ *
+ * The caller owns the memory; all of it is on the device, so that a step's
+ * calls can be captured into a HIP graph and need no host round trip:
+ *   kv     fp32|fp16 [n_layers][2 (k, v)][n_pages][n_kv_heads][page_size][head_dim]
+ *   table  int32 [max_seqs][max_pages]  page ids of each sequence, -1 behind its last
+ *   lens   int32 [max_seqs]             tokens of each sequence
+ *   refs   int32 [n_pages]              table entries that hold each page, 0 = free
+ *   work   int32, pio_kv_work_bytes()   plans of the calls below and their status
+ * Sequences may share pages (pio_kv_fork). page_size is a power of two from 1 to
+ * 1024, head_dim a multiple of 8 up to 256; kv is 16-byte aligned, table rows
+ * and the other arrays 4-byte. The lists of sequence ids and counts are int32
+ * on the device as well. Calls on one cache are ordered by the caller (one
+ * stream, or events): each reads what the one before it left.
+ *
+ * Arguments that the host can see are checked there. What only the device can
+ * see (a sequence id outside the cache, one id twice, too few free pages) is
+ * checked by the kernels: such a request changes nothing, and
+ * pio_kv_status reports it. At most 2^20 pages, sequences and pages a sequence.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    void* kv;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    int32_t* work;
+    int kv_dtype, n_layers, n_kv_heads, head_dim, page_size, n_pages, max_seqs, max_pages;
+} pio_kv_cache;
+
+/* Requests that one pio_kv_reserve / fork / drop / write call takes. */
+#define PIO_KV_MAX_REQUESTS 4096
+
+/* Bytes of `work` (0 for a struct that no call would take). */
+size_t pio_kv_work_bytes(const pio_kv_cache* cache);
+/* Empties the cache: no sequence holds a page. The pages' contents stay. */
+int pio_kv_init(const pio_kv_cache* cache, void* stream);
+/* Waits for `stream` and reports what the kernels of the calls before found
+ * wrong since the last pio_kv_status: PIO_OK, PIO_ERR_OOM (a pio_kv_reserve
+ * found too few free pages or too short table rows) or PIO_ERR_INVALID (bad
+ * sequence id, count or page, one sequence twice, a fork onto a sequence that
+ * is not empty). */
+int pio_kv_status(const pio_kv_cache* cache, void* stream);
+/* Room for count[i] more tokens of sequence seq[i], i < n: the pages it needs
+ * join its table row, the lowest free ones in the order of the requests, and
+ * its length grows by count[i]. Where the new tokens begin inside a page that
+ * another table entry holds as well, the sequence gets a copy of it first: the
+ * rows in use, in every layer (two requests that share such a page each get
+ * one). All or nothing: if any request is refused, or the free pages do not
+ * suffice, no request is served. */
+int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t* count, int n, void* stream);
+/* Keys and values of each sequence's last tokens: rows row_start[i] ..
+ * row_start[i + 1] - 1 of k and v become the last positions of seq[i], in
+ * `layers` layers from `layer`. k and v [layers][rows][n_kv_heads * head_dim]
+ * with rows `row_stride` and layers `layer_stride` elements apart (each a
+ * multiple of 8, or 0 for dense rows / layers), fp32|fp16, rounded to the
+ * cache's type, 16-byte aligned. row_start int32 [n + 1], ascending; rows at
+ * and behind row_start[n] are not read. */
+int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
+                 int n, const void* k, const void* v, int dtype, int rows, int64_t row_stride,
+                 int64_t layer_stride, void* stream);
+/* dst[i] becomes a copy of src[i] that shares all its pages. dst[i] must be
+ * empty and may not be a source of the same call; a source may come often. */
+int pio_kv_fork(const pio_kv_cache* cache, const int32_t* src, const int32_t* dst, int n, void* stream);
+/* The last count[i] tokens of seq[i] go (all of them where it has fewer, or
+ * where count is null); pages that no table entry holds any longer are free. */
+int pio_kv_drop(const pio_kv_cache* cache, const int32_t* seq, const int32_t* count, int n, void* stream);
+/* Moves the pages in use to the lowest slots (the k-th page in use behind them
+ * to the k-th free one among them) and rewrites the tables. */
+int pio_kv_compact(const pio_kv_cache* cache, void* stream);
+
+/* Causal attention of a batch over one layer of the cache:
+ *   out[r, h] = sum_t softmax_t(q[r, h] . k[t, h / G] * scale) v[t, h / G]
+ * with G = n_heads / n_kv_heads. Rows row_start[i] .. row_start[i + 1] - 1 are
+ * the queries of seq[i]'s last tokens (already in the cache): the last row sees
+ * all of its keys, the one before it all but the last, and so on. A row that
+ * sees no key gets 0; rows at and behind row_start[n] are left as they are.
+ * The first `shared` tokens are the same for every sequence of the batch (a
+ * common system prompt, say; 0: none): they are read through the table row of
+ * seq[0], once for all queries. q and out fp32|fp16 [rows, n_heads, head_dim],
+ * rows q_stride / out_stride elements apart (multiples of 8), 16-byte aligned;
+ * out may be q. max_rows: the most queries that one sequence has (larger ones
+ * are served too, but slower). A sequence id or a page outside the cache gives
+ * NaN rows. Products and sums in fp32: of fp16 queries over an fp16 cache on
+ * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32
+ * queries over an fp16 cache with queries and weights as two fp16 parts each;
+ * over an fp32 cache on the fp32 matrix cores. */
+int pio_kv_attention(const pio_kv_cache* cache, int layer, const int32_t* seq, const int32_t* row_start, int n,
+                     int shared, const void* q, void* out, int dtype, int rows, int n_heads, int64_t q_stride,
+                     int64_t out_stride, int max_rows, float scale, void* stream);
+
+/* Speculative sampling's verification of drafted tokens. Rows row_start[i] ..
+ * row_start[i + 1] - 1 belong to request i: row r holds the target's
+ * probabilities of the token at its place (target[r]), and, in all but a
+ * request's last row, the drafted token ids[r] and the draft's probabilities
+ * draft[r]. A drafted token is accepted while u[r] * draft[r, ids[r]] <
+ * target[r, ids[r]]. At the first that is not, the token that follows is drawn
+ * from max(target[r] - draft[r], 0), after all were accepted from target of the
+ * last row: the smallest v whose weights up to v sum to more than u_next[i] *
+ * (sum of all weights), or the last v with a weight if rounding leaves none.
+ * If the difference has no weight, target[r] itself is drawn from; if that has
+ * none either, the token is -1. Weights that are not finite count as 0, a
+ * drafted id outside the vocabulary is not accepted. Comparisons and sums are
+ * in 64 bits. draft null: the drafted tokens were certain (probability 1).
+ *   target, draft  fp32|fp16 (one type) [rows, vocab], rows *_stride elements apart
+ *   ids int32, u fp32 [rows], read in rows with a drafted token; u_next fp32 [n]
+ *   accepted  int32 [n]: drafted tokens accepted
+ *   tokens    int32 [rows]: the accepted ones, the drawn one, then -1
+ *   rejected  int32 [n] or null: drafted tokens not accepted (for pio_kv_drop)
+ * A request without rows gets accepted 0. `rows` bounds row_start. */
+int pio_verify_draft(const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int dtype,
+                     const int32_t* ids, const float* u, const float* u_next, const int32_t* row_start, int n,
+                     int rows, int vocab, int32_t* accepted, int32_t* tokens, int32_t* rejected, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Int8 Qwen3-style decoder (greedy decode at batch 1). Replaces the decode
  * loop of Qwen3ForCausalLM.generate / Qwen3DecoderLayer.forward
  * (ip/models/qwen3_0_6b/architecture.py:124-221) with one device-driven step:

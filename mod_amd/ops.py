@@ -46,6 +46,16 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 
+class CKvCache(ctypes.Structure):
+    """pio_kv_cache of include/tensor_rocm.h."""
+    _fields_ = [(n, _vp) for n in ("kv", "table", "lens", "refs", "work")] + \
+               [(n, _i) for n in ("kv_dtype", "n_layers", "n_kv_heads", "head_dim", "page_size", "n_pages",
+                                  "max_seqs", "max_pages")]
+
+
+_cp = ctypes.POINTER(CKvCache)
+_i64 = ctypes.c_int64
+
 # Every symbol declared in include/tensor_rocm.h: name -> (restype, argtypes).
 SIGNATURES: dict[str, tuple] = {
     "create_tensor": (TP, [ctypes.POINTER(ctypes.c_int), _i, _i]),
@@ -146,6 +156,16 @@ SIGNATURES: dict[str, tuple] = {
     "pio_moe_workspace": (_sz, [_i, _i, _i, _i, _i]),
     "pio_moe_w8a8": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
                           _vp, _vp]),
+    "pio_kv_work_bytes": (_sz, [_cp]),
+    "pio_kv_init": (_i, [_cp, _vp]),
+    "pio_kv_status": (_i, [_cp, _vp]),
+    "pio_kv_reserve": (_i, [_cp, _vp, _vp, _i, _vp]),
+    "pio_kv_write": (_i, [_cp, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i64, _i64, _vp]),
+    "pio_kv_fork": (_i, [_cp, _vp, _vp, _i, _vp]),
+    "pio_kv_drop": (_i, [_cp, _vp, _vp, _i, _vp]),
+    "pio_kv_compact": (_i, [_cp, _vp]),
+    "pio_kv_attention": (_i, [_cp, _i, _vp, _vp, _i, _i, _vp, _vp, _i, _i, _i, _i64, _i64, _i, ctypes.c_float, _vp]),
+    "pio_verify_draft": (_i, [_vp, _i64, _vp, _i64, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp]),
     "pio_qwen3_create": (_vp, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "pio_qwen3_destroy": (None, [_vp]),
     "pio_qwen3_reset": (_i, [_vp, _vp, _i]),
@@ -303,6 +323,108 @@ def moe_w8a8(x, logits, w_gu, s_gu, w_down, s_down, out, T: int, H: int, I: int,
     check(lib.pio_moe_w8a8(_ptr(x), _dt(x), _ptr(logits), _ptr(w_gu), _ptr(s_gu), _ptr(w_down),
                            _ptr(s_down), _ptr(out), _dt(out), T, H, I, E, k, int(renorm),
                            _ptr(workspace), _stream(stream)), "pio_moe_w8a8")
+
+
+class KvCache:
+    """A paged key / value cache over memory that the caller owns: kv
+    [layers, 2, pages, kv heads, page size, head dim] fp32 | fp16, table [sequences,
+    pages of a sequence], lens [sequences] and refs [pages] int32, all dense on
+    one device (torch or backend tensors; kept alive by this object). The plans'
+    workspace is allocated here, and the tables are taken as they are: kv_init
+    empties a new cache."""
+
+    def __init__(self, kv, table, lens, refs):
+        if len(kv.shape) != 6 or kv.shape[1] != 2:
+            raise ValueError(f"KvCache: kv of shape {tuple(kv.shape)}, not [layers, 2, pages, heads, page, dim]")
+        L, _, pages, heads, page, dim = (int(v) for v in kv.shape)
+        if len(table.shape) != 2:
+            raise ValueError(f"KvCache: table of shape {tuple(table.shape)}, not [sequences, pages]")
+        seqs, width = (int(v) for v in table.shape)
+        for name, t, shape in (("table", table, (seqs, width)), ("lens", lens, (seqs,)), ("refs", refs, (pages,))):
+            if tuple(int(v) for v in t.shape) != shape or _dt(t) != I32:
+                raise ValueError(f"KvCache: {name} must be int32 {list(shape)}")
+        for name, t in (("kv", kv), ("table", table), ("lens", lens), ("refs", refs)):
+            if hasattr(t, "is_contiguous") and not t.is_contiguous():
+                raise ValueError(f"KvCache: {name} is not dense")
+            if str(t.device) != str(kv.device):
+                raise ValueError(f"KvCache: {name} is on {t.device}, kv on {kv.device}")
+        device = str(kv.device)
+        if device.split(":")[0] not in ("cuda", "rocm"):
+            raise ValueError(f"KvCache: the cache is on {device}, not on a GPU")
+        self.tensors = (kv, table, lens, refs)
+        self.c = CKvCache(_ptr(kv), _ptr(table), _ptr(lens), _ptr(refs), None, _dt(kv), L, heads, dim, page, pages,
+                          seqs, width)
+        words = lib.pio_kv_work_bytes(ctypes.byref(self.c)) // 4
+        self._work = lib.create_tensor_typed((ctypes.c_int * 1)(words), 1,
+                                             int(device.split(":")[1]) if ":" in device else 0, I32)
+        if not self._work:
+            raise RocmError(f"KvCache: {last_error()}")
+        zero = (ctypes.c_int * words)()
+        check(lib.tensor_load_bytes_status(self._work, zero, 4 * words), "KvCache")
+        self.c.work = ctypes.cast(self._work.contents.data, ctypes.c_void_p).value
+        self.ref = ctypes.byref(self.c)
+
+    def __del__(self):
+        h = getattr(self, "_work", None)
+        if h:
+            try:
+                lib.free_tensor(h)
+            except Exception:
+                pass
+            self._work = None
+
+
+def kv_init(cache: KvCache, stream=None) -> None:
+    check(lib.pio_kv_init(cache.ref, _stream(stream)), "pio_kv_init")
+
+
+def kv_status(cache: KvCache, stream=None) -> None:
+    """Waits for the stream and raises RocmError for what the cache's calls found wrong on the device."""
+    check(lib.pio_kv_status(cache.ref, _stream(stream)), "pio_kv_status")
+
+
+def kv_reserve(cache: KvCache, seq, count, n: int, stream=None) -> None:
+    check(lib.pio_kv_reserve(cache.ref, _ptr(seq), _ptr(count), n, _stream(stream)), "pio_kv_reserve")
+
+
+def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, row_stride: int = 0,
+             layer_stride: int = 0, stream=None) -> None:
+    check(lib.pio_kv_write(cache.ref, layer, layers, _ptr(seq), _ptr(row_start), n, _ptr(k), _ptr(v), _dt(k), rows,
+                           row_stride, layer_stride, _stream(stream)), "pio_kv_write")
+
+
+def kv_fork(cache: KvCache, src, dst, n: int, stream=None) -> None:
+    check(lib.pio_kv_fork(cache.ref, _ptr(src), _ptr(dst), n, _stream(stream)), "pio_kv_fork")
+
+
+def kv_drop(cache: KvCache, seq, count, n: int, stream=None) -> None:
+    """count None: all tokens of each sequence."""
+    check(lib.pio_kv_drop(cache.ref, _ptr(seq), _ptr(count), n, _stream(stream)), "pio_kv_drop")
+
+
+def kv_compact(cache: KvCache, stream=None) -> None:
+    check(lib.pio_kv_compact(cache.ref, _stream(stream)), "pio_kv_compact")
+
+
+def kv_attention(cache: KvCache, layer: int, seq, row_start, n: int, q, out, rows: int, n_heads: int, scale: float,
+                 shared: int = 0, max_rows: int = 1, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
+    """out[r, h] = softmax(scale q[r, h] k^T) v, causal, over each sequence's pages; the first `shared`
+    tokens are common to the batch and read once."""
+    if _dt(q) != _dt(out):
+        raise TypeError("kv_attention: q and out differ in dtype")
+    check(lib.pio_kv_attention(cache.ref, layer, _ptr(seq), _ptr(row_start), n, shared, _ptr(q), _ptr(out), _dt(q),
+                               rows, n_heads, q_stride, out_stride, max_rows, scale, _stream(stream)),
+          "pio_kv_attention")
+
+
+def verify_draft(target, draft, ids, u, u_next, row_start, n: int, rows: int, vocab: int, accepted, tokens,
+                 rejected=None, target_stride: int = 0, draft_stride: int = 0, stream=None) -> None:
+    """draft None: the drafted tokens were certain."""
+    if draft is not None and _dt(draft) != _dt(target):
+        raise TypeError("verify_draft: target and draft differ in dtype")
+    check(lib.pio_verify_draft(_ptr(target), target_stride, _ptr(draft), draft_stride, _dt(target), _ptr(ids), _ptr(u),
+                               _ptr(u_next), _ptr(row_start), n, rows, vocab, _ptr(accepted), _ptr(tokens),
+                               _ptr(rejected), _stream(stream)), "pio_verify_draft")
 
 
 def pool_stats() -> dict:
