@@ -10,6 +10,7 @@ namespace pio {
 
 constexpr int VD_THREADS = 256;
 constexpr int VD_WAVES = VD_THREADS / 64;
+constexpr int VD_UNIT = 8 * VD_THREADS;      // tokens whose weights are summed together
 
 struct VdArgs {
     const void *target, *draft;
@@ -19,6 +20,8 @@ struct VdArgs {
     const int32_t* row_start;
     int32_t *accepted, *tokens, *rejected;
     int n, rows, vocab;
+    int units, per_block;
+    double* sums;          // [n][units]
 };
 
 // The weight that the next token is drawn with: p - q where that is positive.
@@ -67,80 +70,180 @@ __device__ __forceinline__ VdRow vd_accept(const VdArgs& a, int i, int* sh) {
     return r;
 }
 
-// The weight of token v in a request's row: from the difference, or from the
-// target alone.
+// 8 consecutive tokens' probabilities from v of a row (0 behind its end). Rows may
+// begin at any element, so the wide loads are unaligned ones.
 template <typename PT>
-__device__ __forceinline__ double vd_at(const VdArgs& a, const VdRow& r, int id, bool difference, int v) {
-    const double p = (double)((const PT*)a.target)[r.row * a.target_stride + v];
-    double q = 0.0;
-    if (difference) q = a.draft ? (double)((const PT*)a.draft)[r.row * a.draft_stride + v] : v == id ? 1.0 : 0.0;
-    return vd_weight(p, q);
+__device__ __forceinline__ void vd_load8(const PT* row, int v, int vocab, double (&x)[8]) {
+    typedef PT V __attribute__((ext_vector_type(16 / sizeof(PT)), aligned(sizeof(PT))));
+    if (v + 8 <= vocab) {
+        V r[8 * sizeof(PT) / 16];
+#pragma unroll
+        for (int i = 0; i < (int)(8 * sizeof(PT) / 16); i++) r[i] = *(const V*)(row + v + i * (16 / (int)sizeof(PT)));
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = (double)r[e * sizeof(PT) / 16][e % (16 / sizeof(PT))];
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = v + e < vocab ? (double)row[v + e] : 0.0;
+    }
 }
 
-__device__ __forceinline__ double vd_shfl_up(double x, int o) { return __shfl_up(x, o, 64); }
-
-// One workgroup per request: it sums the weights, then walks them again for the
-// place. Every thread has a run of consecutive tokens of each piece of the row.
+// The weights of 8 consecutive tokens of a request's row: from the difference, or
+// from the target alone.
 template <typename PT>
-__global__ __launch_bounds__(VD_THREADS) void vd_simple_kernel(VdArgs a) {
-    __shared__ int sh, place, last;
+__device__ __forceinline__ void vd_weights(const VdArgs& a, const VdRow& r, int id, bool difference, int v, double (&w)[8]) {
+    double p[8];
+    vd_load8<PT>((const PT*)a.target + r.row * a.target_stride, v, a.vocab, p);
+    if (difference && a.draft) {
+        double q[8];
+        vd_load8<PT>((const PT*)a.draft + r.row * a.draft_stride, v, a.vocab, q);
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = vd_weight(p[e], q[e]);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = vd_weight(p[e], difference && v + e == id ? 1.0 : 0.0);
+    }
+}
+__device__ __forceinline__ double vd_sum8(const double (&w)[8]) {
+    return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+}
+// Sum over the workgroup.
+__device__ __forceinline__ double vd_block_sum(double x, double* red) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) x += __shfl_xor(x, o, 64);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+// Sums of the threads before this one; `total` gets the sum of all.
+__device__ __forceinline__ double vd_block_scan(double x, double* red, double& total) {
+    const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    double up = x;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(up, o, 64);
+        if (lane >= o) up += y;
+    }
+    const double before = __shfl_up(up, 1, 64);
+    __syncthreads();
+    if (lane == 63) red[wv] = up;
+    __syncthreads();
+    double base = 0.0;
+    for (int k = 0; k < wv; k++) base += red[k];
+    total = (red[0] + red[1]) + (red[2] + red[3]);
+    return lane ? base + before : base;
+}
+
+// First launch, (units of a row / per_block, requests): every workgroup finds its
+// request's row and sums the weights of a few units of 2048 tokens; the first also
+// writes what is accepted.
+template <typename PT>
+__global__ __launch_bounds__(VD_THREADS) void vd_sum_kernel(VdArgs a) {
+    __shared__ int sh;
     __shared__ double red[VD_WAVES];
-    const int i = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int i = blockIdx.y, tid = threadIdx.x;
     const VdRow r = vd_accept<PT>(a, i, &sh);
-    if (r.count == 0) {
+    if (blockIdx.x == 0) {
         if (tid == 0) {
-            a.accepted[i] = 0;
-            if (a.rejected) a.rejected[i] = 0;
+            a.accepted[i] = r.accepted;
+            if (a.rejected) a.rejected[i] = max(r.count - 1, 0) - r.accepted;
         }
-        return;
+        for (int j = tid; j < r.count; j += VD_THREADS)
+            if (j != r.accepted) a.tokens[r.first + j] = j < r.accepted ? a.ids[r.first + j] : -1;
     }
+    if (r.count == 0) return;
     const int id = r.rejects ? a.ids[r.row] : -1;
+    const int u1 = min(a.units, (int)(blockIdx.x + 1) * a.per_block);
+    for (int u = blockIdx.x * a.per_block; u < u1; u++) {
+        double w[8];
+        vd_weights<PT>(a, r, id, r.rejects, u * VD_UNIT + 8 * tid, w);
+        const double s = vd_block_sum(vd_sum8(w), red);
+        if (tid == 0) a.sums[(int64_t)i * a.units + u] = s;
+    }
+}
+
+// Second launch, one workgroup per request: the unit whose weights reach u_next *
+// total, and the token in it.
+template <typename PT>
+__global__ __launch_bounds__(VD_THREADS) void vd_pick_kernel(VdArgs a) {
+    __shared__ int unit, place, last;
+    __shared__ double red[VD_WAVES], before_unit;
+    const int i = blockIdx.x, tid = threadIdx.x;
+    VdRow r;
+    const int r0 = min(max(a.row_start[i], 0), a.rows), r1 = min(max(a.row_start[i + 1], r0), a.rows);
+    if (r1 <= r0) return;
+    r.first = r0;
+    r.count = r1 - r0;
+    r.accepted = a.accepted[i];
+    r.row = r0 + r.accepted;
+    r.rejects = r.accepted < r.count - 1;
+    const int id = r.rejects ? a.ids[r.row] : -1;
+    double* sums = a.sums + (int64_t)i * a.units;
     bool difference = r.rejects;
-    double total = 0.0;
+    double total;
     for (;;) {
-        double sum = 0.0;
-        for (int v = tid; v < a.vocab; v += VD_THREADS) sum += vd_at<PT>(a, r, id, difference, v);
-        for (int o = 32; o >= 1; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        __syncthreads();
-        if (lane == 0) red[wv] = sum;
-        __syncthreads();
-        total = (red[0] + red[1]) + (red[2] + red[3]);
+        double x = 0.0;
+        for (int u = tid; u < a.units; u += VD_THREADS) x += sums[u];
+        total = vd_block_sum(x, red);
         if (total > 0.0 || !difference) break;
+        // nothing is left of the target above the draft: the target's own weights
         difference = false;
-    }
-    const double bar = (double)a.u_next[i] * total;
-    if (tid == 0) {
-        place = INT_MAX;
-        last = -1;
-    }
-    double before = 0.0;
-    for (int v0 = 0; v0 < a.vocab; v0 += VD_THREADS) {
-        const int v = v0 + tid;
-        const double w = v < a.vocab ? vd_at<PT>(a, r, id, difference, v) : 0.0;
-        double x = w;
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = vd_shfl_up(x, o);
-            if (lane >= o) x += y;
+        for (int u = 0; u < a.units; u++) {
+            double w[8];
+            vd_weights<PT>(a, r, id, false, u * VD_UNIT + 8 * tid, w);
+            const double s = vd_block_sum(vd_sum8(w), red);
+            if (tid == 0) sums[u] = s;
         }
         __syncthreads();
-        if (lane == 63) red[wv] = x;
-        __syncthreads();
-        double base = before;
-        for (int k = 0; k < wv; k++) base += red[k];
-        if (w > 0.0) atomicMax(&last, v);
-        if (w > 0.0 && base + x > bar) atomicMin(&place, v);
-        before += (red[0] + red[1]) + (red[2] + red[3]);
-        __syncthreads();
-        if (place != INT_MAX) break;
+    }
+    if (tid == 0) {
+        unit = INT_MAX;
+        last = -1;
+        place = INT_MAX;
     }
     __syncthreads();
-    const int drafted = r.count - 1, next = place != INT_MAX ? place : last;
-    for (int j = tid; j < r.count; j += VD_THREADS)
-        a.tokens[r.first + j] = j < r.accepted ? a.ids[r.first + j] : j == r.accepted ? next : -1;
-    if (tid == 0) {
-        a.accepted[i] = r.accepted;
-        if (a.rejected) a.rejected[i] = drafted - r.accepted;
+    const double bar = (double)a.u_next[i] * total;
+    double before = 0.0;
+    for (int u0 = 0; u0 < a.units; u0 += VD_THREADS) {
+        const int u = u0 + tid;
+        const double s = u < a.units ? sums[u] : 0.0;
+        double all;
+        const double base = before + vd_block_scan(s, red, all);
+        if (s > 0.0) {
+            atomicMax(&last, u);
+            if (base + s > bar) atomicMin(&unit, u);
+        }
+        __syncthreads();
+        if (unit == u) before_unit = base;
+        if (unit != INT_MAX) break;
+        before += all;
     }
+    __syncthreads();
+    // rounding (or u_next = 1) left none: the last one with a weight
+    const bool over = unit != INT_MAX;
+    const int u = over ? unit : last;
+    if (u >= 0) {
+        double w[8], all;
+        const int v = u * VD_UNIT + 8 * tid;
+        vd_weights<PT>(a, r, id, difference, v, w);
+        double sum = (over ? before_unit : 0.0) + vd_block_scan(vd_sum8(w), red, all);
+        __syncthreads();
+        if (tid == 0) last = -1;
+        __syncthreads();
+        int some = -1, first = INT_MAX;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            sum += w[e];
+            if (w[e] > 0.0) {
+                some = v + e;
+                if (over && sum > bar) first = min(first, v + e);
+            }
+        }
+        if (some >= 0) atomicMax(&last, some);
+        if (first != INT_MAX) atomicMin(&place, first);
+        __syncthreads();
+    }
+    if (tid == 0) a.tokens[r.row] = place != INT_MAX ? place : last;
 }
 
 }  // namespace pio
@@ -182,8 +285,29 @@ PIO_EXPORT int pio_verify_draft(const void* target, int64_t target_stride, const
     a.rows = rows;
     a.vocab = vocab;
     hipStream_t st = pick_stream(stream);
-    if (dtype == PIO_F32) vd_simple_kernel<float><<<n, VD_THREADS, 0, st>>>(a);
-    else vd_simple_kernel<_Float16><<<n, VD_THREADS, 0, st>>>(a);
-    PIO_LAUNCHED();
+    a.units = ceil_div(vocab, VD_UNIT);
+    Scratch ws;
+    PIO_TRY(ws.get((size_t)n * a.units * sizeof(double), st));
+    a.sums = (double*)ws.ptr;
+    // a few thousand workgroups are enough for the device, and each has its row to find first
+    a.per_block = (int)std::max<int64_t>(1, (int64_t)n * a.units / 2048);
+    for (int i0 = 0; i0 < n; i0 += 65535) {        // the grid's second dimension
+        VdArgs b = a;
+        b.n = std::min(n - i0, 65535);
+        b.u_next += i0;
+        b.row_start += i0;
+        b.accepted += i0;
+        if (b.rejected) b.rejected += i0;
+        b.sums += (int64_t)i0 * a.units;
+        const dim3 grid(ceil_div(a.units, a.per_block), b.n);
+        if (dtype == PIO_F32) {
+            vd_sum_kernel<float><<<grid, VD_THREADS, 0, st>>>(b);
+            vd_pick_kernel<float><<<b.n, VD_THREADS, 0, st>>>(b);
+        } else {
+            vd_sum_kernel<_Float16><<<grid, VD_THREADS, 0, st>>>(b);
+            vd_pick_kernel<_Float16><<<b.n, VD_THREADS, 0, st>>>(b);
+        }
+        PIO_LAUNCHED();
+    }
     return PIO_OK;
 }
