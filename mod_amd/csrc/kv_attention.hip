@@ -146,58 +146,89 @@ typedef __fp16 ka_p4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void ka_lds_t;
 typedef __attribute__((address_space(3))) ka_p4 ka_lds_p4;
 
-constexpr int KA_COLS = 32;      // columns of a tile
-constexpr int KA_KEYS = 32;      // keys of a tile
 constexpr float KA_LOG2E = 1.44269504088896340736f;
 // fp16 weights are held times 2^10, so that those down to 2^-24 of the largest are normal
 // numbers; the sum is scaled alike.
 constexpr float KA_LIFT = 10.f;
 constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column's largest is 2^12 .. 2^13
 
-// Geometry of a cache row and of its image in LDS: rows of RB bytes in 16-byte
-// slots, slot s of row r holding chunk s ^ swz(r), so that 16 consecutive rows'
-// reads of one chunk fall into different banks.
-template <typename KT, int D>
+// A tile of keys x COLS columns (16 or 32) on v_mfma_*_COLSxCOLS: lane l holds
+// column l % COLS and is one of PL = 64 / COLS parts q = l / COLS of it.
+//   S^T: accumulator e of part q is key COLS * (e / E) + sub(e % E, q)
+//   O^T: NT tiles of COLS dimensions
+// A row of the cache is RB bytes in 16-byte chunks; in LDS, slot s of row r holds
+// chunk s ^ swz(r), so that 16 consecutive rows' reads of one chunk fall into
+// different banks.
+template <typename KT, int D, int COLS_>
 struct Ka {
     static constexpr bool F16 = sizeof(KT) == 2;
-    static constexpr int NT = D / 32;                  // O^T tiles
+    static constexpr int COLS = COLS_, PL = 64 / COLS;
+    static constexpr int KEYS = F16 ? 32 : 16;         // keys of a tile: the depth of fp16's product with V
+    static constexpr int E = COLS * COLS / 64;         // accumulators of one COLS x COLS tile
+    static constexpr int ST = KEYS / COLS;             // S^T tiles
+    static constexpr int NS = ST * E;                  // a lane's scores
+    static constexpr int NT = D / COLS;
     static constexpr int RB = D * (int)sizeof(KT), SL = RB / 16;
     static constexpr int RPI = 64 / SL;                // rows of one copy instruction
-    static constexpr int NI = KA_KEYS / RPI;           // copies of a tile of K (or V)
-    static constexpr int TILE = KA_KEYS * RB;          // bytes
-    static constexpr int QC = F16 ? D / 16 : D / 8;    // operand groups of a score
+    static constexpr int NI = KEYS / RPI;              // copies of a tile of K (or V)
+    static constexpr int TILE = KEYS * RB;             // bytes
+    static constexpr int QC = SL / PL;                 // operand chunks of a lane in a score
     static constexpr int OP = D + 4;                   // LDS pitch of a column's output (floats)
+    typedef typename std::conditional<COLS == 32, ka_v16, ka_f4>::type Acc;
     __device__ static int swz(int r) { return RB == 128 ? (r >> 1) & 7 : r & 15; }
     __device__ static int slot(int r, int chunk) { return r * RB + ((chunk ^ swz(r)) << 4); }
-    // dimension that register e of O^T tile n holds in half h
-    __device__ static int dim(int n, int e, int h) {
-        const int i = 8 * (e >> 2) + 4 * h + (e & 3);
-        return F16 ? 32 * n + i : NT * i + n;
+    // row of a COLS x COLS accumulator tile that element e of part q is
+    __device__ static int sub(int e, int q) { return COLS == 32 ? 8 * (e >> 2) + 4 * q + (e & 3) : 4 * q + e; }
+    // key of score i of part q
+    __device__ static int key(int i, int q) { return COLS * (i / E) + sub(i % E, q); }
+    // dimension that element e of O^T tile n is in part q. fp32: a lane reads 16 bytes of
+    // V at a time, dimensions 4 i .. 4 i + 3 of each 64, so a tile's row i is dimension 4 i + n % 4.
+    __device__ static int dim(int n, int e, int q) {
+        return F16 ? COLS * n + sub(e, q) : 4 * sub(e, q) + (n & 3) + 64 * (n >> 2);
+    }
+    __device__ static Acc mfma(ka_h8 a, ka_h8 b, Acc c) {
+        if constexpr (COLS == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+        else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    __device__ static Acc zero() {
+        Acc c;
+#pragma unroll
+        for (int e = 0; e < E; e++) c[e] = 0.f;
+        return c;
     }
 };
 
-// A column's query as operands, and the factor of its scores (base 2).
-template <typename KT, int D, int XP>
+// A column's query as operands (chunk PL c + q of its row), and the factor of its
+// scores (base 2).
+template <typename KT, int D, int COLS, int XP>
 struct KaQ {
-    ka_h8 h[XP][Ka<KT, D>::QC];
+    ka_h8 h[XP][Ka<KT, D, COLS>::QC];
     float cs;
 };
-template <int D>
-struct KaQ<float, D, 1> {
-    ka_f4 f[D / 8];
+template <int D, int COLS>
+struct KaQ<float, D, COLS, 1> {
+    ka_f4 f[Ka<float, D, COLS>::QC];
     float cs;
 };
 
-// q of (row, head), this lane's half of every group; zeros for a column without a row.
-template <typename KT, int D, int XP>
-__device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bool live, int h, KaQ<KT, D, XP>& q) {
-    constexpr int QC = Ka<KT, D>::QC;
-    const int64_t at = (live ? row * a.q_stride + (int64_t)head * D : 0);
+// Maximum over the parts of a column.
+template <int COLS>
+__device__ __forceinline__ float ka_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 32, 64));
+    if constexpr (COLS == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return v;
+}
+
+// q of (row, head); zeros for a column without a row.
+template <typename KT, int D, int COLS, int XP>
+__device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bool live, int part, KaQ<KT, D, COLS, XP>& q) {
+    using T = Ka<KT, D, COLS>;
+    const int64_t at = live ? row * a.q_stride + (int64_t)head * D : 0;
     q.cs = a.scale * KA_LOG2E;
-    if constexpr (!Ka<KT, D>::F16) {
+    if constexpr (!T::F16) {
 #pragma unroll
-        for (int c = 0; c < QC; c++) {
-            const int64_t e0 = at + 8 * c + 4 * h;
+        for (int c = 0; c < T::QC; c++) {
+            const int64_t e0 = at + 4 * (T::PL * c + part);
             if (a.q16) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) q.f[c][e] = (float)((const _Float16*)a.q)[e0 + e];
@@ -208,30 +239,29 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
         }
     } else if constexpr (XP == 1) {
 #pragma unroll
-        for (int c = 0; c < QC; c++) {
-            q.h[0][c] = *(const ka_h8*)((const _Float16*)a.q + at + 16 * c + 8 * h);
+        for (int c = 0; c < T::QC; c++) {
+            q.h[0][c] = *(const ka_h8*)((const _Float16*)a.q + at + 8 * (T::PL * c + part));
             if (!live) q.h[0][c] = ka_h8{0, 0, 0, 0, 0, 0, 0, 0};
         }
     } else {
-        float x[QC][8], most = 0.f;
-        bool odd = false;
+        float x[T::QC][8], most = 0.f, odd = 0.f;
 #pragma unroll
-        for (int c = 0; c < QC; c++) {
-            load8<float>((const float*)a.q + at + 16 * c + 8 * h, x[c]);
+        for (int c = 0; c < T::QC; c++) load8<float>((const float*)a.q + at + 8 * (T::PL * c + part), x[c]);
+#pragma unroll
+        for (int c = 0; c < T::QC; c++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 if (!live) x[c][e] = 0.f;
                 most = fmaxf(most, fabsf(x[c][e]));
-                odd |= !(fabsf(x[c][e]) <= FLT_MAX);
+                odd += x[c][e] * 0.f;                  // NaN if any is inf or NaN
             }
-        }
-        most = fmaxf(most, __shfl_xor(most, 32, 64));
-        odd = odd || __shfl_xor((int)odd, 32, 64);
+        most = ka_max<COLS>(most);
+        odd = ka_max<COLS>(odd == 0.f ? 0.f : 1.f);
         int ex = 0;
-        if (most > 0.f && !odd) frexpf(most, &ex);     // most = 2^ex * [0.5, 1)
+        if (most > 0.f && most <= FLT_MAX) frexpf(most, &ex);     // most = 2^ex * [0.5, 1)
         ex = KA_Q_EXP + 1 - ex;
 #pragma unroll
-        for (int c = 0; c < QC; c++)
+        for (int c = 0; c < T::QC; c++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = ldexpf(x[c][e], ex);
@@ -239,55 +269,57 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
                 q.h[0][c][e] = hi;
                 q.h[XP - 1][c][e] = (_Float16)(v - (float)hi);
             }
-        q.cs = odd ? NAN : ldexpf(q.cs, -ex);
+        q.cs = odd > 0.f ? NAN : ldexpf(q.cs, -ex);
     }
 }
 
-// S^T of one tile of 32 keys; kt: K's rows in LDS.
-template <typename KT, int D, int XP>
-__device__ __forceinline__ ka_v16 ka_scores(const char* kt, const KaQ<KT, D, XP>& q, int lane) {
-    using T = Ka<KT, D>;
-    const int key = lane & 31, h = lane >> 5;
-    ka_v16 s;
+// S^T of one tile; kt: K's rows in LDS.
+template <typename KT, int D, int COLS, int XP>
+__device__ __forceinline__ void ka_scores(const char* kt, const KaQ<KT, D, COLS, XP>& q, int lane,
+                                          float (&s)[Ka<KT, D, COLS>::NS]) {
+    using T = Ka<KT, D, COLS>;
+    const int part = lane / COLS;
 #pragma unroll
-    for (int e = 0; e < 16; e++) s[e] = 0.f;
-    if constexpr (T::F16) {
+    for (int st = 0; st < T::ST; st++) {
+        const int key = COLS * st + lane % COLS;
+        if constexpr (T::F16) {
+            typename T::Acc c = T::zero();
 #pragma unroll
-        for (int c = 0; c < T::QC; c++) {
-            const ka_h8 k = *(const ka_h8*)(kt + T::slot(key, 2 * c + h));
-            s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.h[0][c], s, 0, 0, 0);
-            if constexpr (XP == 2) s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.h[XP - 1][c], s, 0, 0, 0);
+            for (int i = 0; i < T::QC; i++) {
+                const ka_h8 k = *(const ka_h8*)(kt + T::slot(key, T::PL * i + part));
+                c = T::mfma(k, q.h[0][i], c);
+                if constexpr (XP == 2) c = T::mfma(k, q.h[XP - 1][i], c);
+            }
+#pragma unroll
+            for (int e = 0; e < T::E; e++) s[st * T::E + e] = c[e];
+        } else {
+            ka_f4 c[4];                // 4 chains: half the rounding of one, and the MFMAs need not wait for each other
+#pragma unroll
+            for (int ch = 0; ch < 4; ch++) c[ch] = T::zero();
+#pragma unroll
+            for (int i = 0; i < T::QC; i++) {
+                const ka_f4 k = *(const ka_f4*)(kt + T::slot(key, T::PL * i + part));
+#pragma unroll
+                for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q.f[i][e], c[e], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = (c[0][e] + c[1][e]) + (c[2][e] + c[3][e]);
         }
-    } else {
-        // 4 chains: half the rounding of one
-        ka_v16 sum[4];
-#pragma unroll
-        for (int ch = 0; ch < 4; ch++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) sum[ch][e] = 0.f;
-#pragma unroll
-        for (int c = 0; c < T::QC; c++) {
-            const ka_f4 k = *(const ka_f4*)(kt + T::slot(key, 2 * c + h));
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                sum[c % 4] = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q.f[c][e], sum[c % 4], 0, 0, 0);
-        }
-#pragma unroll
-        for (int e = 0; e < 16; e++) s[e] = (sum[0][e] + sum[1][e]) + (sum[2][e] + sum[3][e]);
     }
-    return s;
 }
 
-// A lane's 8 values of V^T (O^T tile n, key group kc of 16): one dimension, the
-// keys of S^T's registers 8 kc .. 8 kc + 7.
-template <int D>
+// A lane's 8 values of V^T (O^T tile n, key group kc): one dimension, the keys of
+// scores 8 kc .. 8 kc + 7.
+template <int D, int COLS>
 __device__ __forceinline__ ka_h8 ka_vt(const char* vt, int n, int kc, int lane) {
-    using T = Ka<_Float16, D>;
-    const int i = lane & 15, g = lane >> 4, h = g >> 1;
+    using T = Ka<_Float16, D, COLS>;
+    const int i = lane & 15, part = lane / COLS;
     ka_h8 v;
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-        const int row = 16 * kc + 8 * b + 4 * h + (i >> 2), chunk = 4 * n + 2 * (g & 1) + ((i >> 1) & 1);
+        // 16 lanes read 16 dimensions of 4 keys, 8 bytes each, and get one dimension of the 4
+        const int row = T::key(8 * kc + 4 * b, part) + (i >> 2);
+        const int chunk = COLS / 8 * n + (COLS == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((i >> 1) & 1);
         const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)(vt + T::slot(row, chunk) + 8 * (i & 1)));
 #pragma unroll
         for (int e = 0; e < 4; e++) v[4 * b + e] = (_Float16)r[e];
@@ -295,12 +327,12 @@ __device__ __forceinline__ ka_h8 ka_vt(const char* vt, int n, int kc, int lane) 
     return v;
 }
 
-// Whether any of a tile's 32 rows of V holds inf or NaN.
-template <typename KT, int D>
+// Whether any row of a tile of V holds inf or NaN.
+template <typename KT, int D, int COLS>
 __device__ __forceinline__ bool ka_odd(const char* vt, int lane) {
     bool odd = false;
-#pragma unroll 4
-    for (int u = lane; u < Ka<KT, D>::TILE / 16; u += 64) {
+#pragma unroll 1
+    for (int u = lane; u < Ka<KT, D, COLS>::TILE / 16; u += 64) {
         const uint4 x = *(const uint4*)(vt + 16 * u);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -313,60 +345,53 @@ __device__ __forceinline__ bool ka_odd(const char* vt, int lane) {
 }
 
 // A column's running softmax: (max, sum) in base 2, O^T.
-template <typename KT, int D>
+template <typename KT, int D, int COLS>
 struct KaAcc {
     float m, l;
-    ka_v16 o[Ka<KT, D>::NT];
+    typename Ka<KT, D, COLS>::Acc o[Ka<KT, D, COLS>::NT];
     __device__ void clear() {
         m = -FLT_MAX;
         l = 0.f;
 #pragma unroll
-        for (int n = 0; n < Ka<KT, D>::NT; n++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) o[n][e] = 0.f;
+        for (int n = 0; n < Ka<KT, D, COLS>::NT; n++) o[n] = Ka<KT, D, COLS>::zero();
     }
 };
 
 // Scores -> weights (in s), and the running maximum and sum. The tile's keys
 // from t0; edge (wave-uniform): some column does not see all of them.
-template <typename KT, int D>
-__device__ __forceinline__ void ka_softmax(KaAcc<KT, D>& x, ka_v16& s, float cs, int t0, int limit, bool edge, int h) {
-    constexpr float lift = Ka<KT, D>::F16 ? KA_LIFT : 0.f;
-    float top = -INFINITY;
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ void ka_softmax(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs, int t0,
+                                           int limit, bool edge, int part) {
+    using T = Ka<KT, D, COLS>;
+    constexpr float lift = T::F16 ? KA_LIFT : 0.f;
+#pragma unroll
+    for (int e = 0; e < T::NS; e++) s[e] *= cs;
     if (edge) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const bool seen = t0 + 8 * (e >> 2) + 4 * h + (e & 3) < limit;
-            s[e] = seen ? s[e] * cs : -INFINITY;
-            top = fmaxf(top, s[e]);
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            s[e] *= cs;
-            top = fmaxf(top, s[e]);
-        }
+        for (int e = 0; e < T::NS; e++) s[e] = t0 + T::key(e, part) < limit ? s[e] : -INFINITY;
     }
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float m = fmaxf(x.m, top);
+    float top = x.m;
+#pragma unroll
+    for (int e = 0; e < T::NS; e++) top = fmaxf(top, s[e]);
+    const float m = ka_max<COLS>(top);
     if (__any(m != x.m)) {
         const float corr = __builtin_amdgcn_exp2f(x.m - m);
         x.l *= corr;
 #pragma unroll
-        for (int n = 0; n < Ka<KT, D>::NT; n++)
+        for (int n = 0; n < T::NT; n++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) x.o[n][e] *= corr;
+            for (int e = 0; e < T::E; e++) x.o[n][e] *= corr;
         x.m = m;
     }
     const float base = m - lift;
-    float sum[16];
+    float sum[T::NS];
 #pragma unroll
-    for (int e = 0; e < 16; e++) {
+    for (int e = 0; e < T::NS; e++) {
         s[e] = __builtin_amdgcn_exp2f(s[e] - base);     // -inf: 0 (the maximum is finite, or the scores are no numbers)
         sum[e] = s[e];
     }
 #pragma unroll
-    for (int n = 8; n >= 1; n >>= 1)
+    for (int n = T::NS / 2; n >= 1; n >>= 1)
 #pragma unroll
         for (int e = 0; e < n; e++) sum[e] += sum[e + n];
     x.l += sum[0];
@@ -375,21 +400,18 @@ __device__ __forceinline__ void ka_softmax(KaAcc<KT, D>& x, ka_v16& s, float cs,
 // O^T += V^T P^T over one tile. `odd`: V holds inf or NaN and some column does not
 // see all keys: 0 * inf would make those columns NaN, so inf and NaN are taken out of
 // the product and added where a column sees them (their weights are positive).
-template <typename KT, int D, int XP>
-__device__ __forceinline__ void ka_values(KaAcc<KT, D>& x, const ka_v16& p, const char* vt, int lane, bool odd, int t0,
-                                          int limit) {
-    using T = Ka<KT, D>;
-    const int h = lane >> 5;
-    typedef typename std::conditional<T::NT == 4, ka_f4, ka_f2>::type V;
-    auto row = [&](int e) {                // fp32: dimensions NT i .. of the key of register e
-        const int r = 8 * (e >> 2) + 4 * h + (e & 3), i = lane & 31;
-        if constexpr (T::NT == 4) return *(const V*)(vt + T::slot(r, i));
-        else return *(const V*)(vt + T::slot(r, i >> 1) + 8 * (i & 1));
+template <typename KT, int D, int COLS, int XP>
+__device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], const char* vt,
+                                          int lane, bool odd, int t0, int limit) {
+    using T = Ka<KT, D, COLS>;
+    const int part = lane / COLS;
+    auto row = [&](int e, int half) {      // fp32: 4 dimensions of the key of score e
+        return *(const ka_f4*)(vt + T::slot(T::key(e, part), 16 * half + lane % COLS));
     };
     auto product = [&](auto finite) {
         if constexpr (T::F16) {
 #pragma unroll
-            for (int kc = 0; kc < 2; kc++) {
+            for (int kc = 0; kc < T::NS / 8; kc++) {
                 ka_h8 w[XP];
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
@@ -399,25 +421,28 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D>& x, const ka_v16& p, cons
                 }
 #pragma unroll
                 for (int n = 0; n < T::NT; n++) {
-                    ka_h8 v = ka_vt<D>(vt, n, kc, lane);
+                    ka_h8 v = ka_vt<D, COLS>(vt, n, kc, lane);
                     if constexpr (!decltype(finite)::value) {
 #pragma unroll
                         for (int e = 0; e < 8; e++) v[e] = fabsf((float)v[e]) <= 65504.f ? v[e] : (_Float16)0;
                     }
-                    x.o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[0], x.o[n], 0, 0, 0);
-                    if constexpr (XP == 2) x.o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w[XP - 1], x.o[n], 0, 0, 0);
+                    x.o[n] = T::mfma(v, w[0], x.o[n]);
+                    if constexpr (XP == 2) x.o[n] = T::mfma(v, w[XP - 1], x.o[n]);
                 }
             }
         } else {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                V v = row(e);
+            for (int e = 0; e < T::NS; e++)
 #pragma unroll
-                for (int n = 0; n < T::NT; n++) {
-                    if constexpr (!decltype(finite)::value) v[n] = fabsf(v[n]) <= FLT_MAX ? v[n] : 0.f;
-                    x.o[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(v[n], p[e], x.o[n], 0, 0, 0);
+                for (int half = 0; half < T::NT / 4; half++) {
+                    ka_f4 v = row(e, half);
+#pragma unroll
+                    for (int n = 0; n < 4; n++) {
+                        if constexpr (!decltype(finite)::value) v[n] = fabsf(v[n]) <= FLT_MAX ? v[n] : 0.f;
+                        ka_f4& o = x.o[4 * half + n];
+                        o = __builtin_amdgcn_mfma_f32_16x16x4f32(v[n], p[e], o, 0, 0, 0);
+                    }
                 }
-            }
         }
     };
     if (!odd) {
@@ -431,141 +456,62 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D>& x, const ka_v16& p, cons
 #pragma unroll 1
         for (int kind = 0; kind < 3; kind++) {
             const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-            ka_v16 c;
-#pragma unroll
-            for (int e = 0; e < 16; e++) c[e] = 0.f;
+            typename T::Acc c = T::zero();
             auto is = [&](float f) { return kind == 2 ? f != f : f == what; };
-            auto sees = [&](int e) { return t0 + 8 * (e >> 2) + 4 * h + (e & 3) < limit; };
+            auto sees = [&](int e) { return t0 + T::key(e, part) < limit; };
             if constexpr (T::F16) {
 #pragma unroll 1
-                for (int kc = 0; kc < 2; kc++) {
-                    const ka_h8 v = ka_vt<D>(vt, n, kc, lane);
+                for (int kc = 0; kc < T::NS / 8; kc++) {
+                    const ka_h8 v = ka_vt<D, COLS>(vt, n, kc, lane);
                     ka_h8 k, w;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
                         k[e] = is((float)v[e]) ? (_Float16)1 : (_Float16)0;
                         w[e] = sees(8 * kc + e) ? (_Float16)1 : (_Float16)0;
                     }
-                    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, w, c, 0, 0, 0);
+                    c = T::mfma(k, w, c);
                 }
             } else {
-#pragma unroll 1
-                for (int e = 0; e < 16; e++)
-                    c = __builtin_amdgcn_mfma_f32_32x32x2f32(is(row(e)[n]) ? 1.f : 0.f, sees(e) ? 1.f : 0.f, c, 0, 0, 0);
+#pragma unroll
+                for (int e = 0; e < T::NS; e++)
+                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(is(row(e, n >> 2)[n & 3]) ? 1.f : 0.f, sees(e) ? 1.f : 0.f, c,
+                                                             0, 0, 0);
             }
 #pragma unroll
-            for (int e = 0; e < 16; e++)
+            for (int e = 0; e < T::E; e++)
                 if (c[e] > 0.5f) x.o[n][e] += what;
         }
     }
 }
 
-// ---- one item by 4 waves: 32 columns, every 4th tile of the keys each, from a
-// piece of LDS of the wave's own (one tile of K, one of V). The next K tile is
-// copied during this one's softmax and product with V, the next V tile during the
-// next scores. No barriers: a wave waits for its own copies.
-template <int N>
-__device__ __forceinline__ void ka_wait_copies() {
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
-    asm volatile("" ::: "memory");
-}
-__device__ __forceinline__ void ka_wait_reads() {     // the wave's LDS reads are done: copies may overwrite them
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_waitcnt(0xC07F);               // lgkmcnt(0)
-    asm volatile("" ::: "memory");
+// A lane's part of an accumulated column, times f, into LDS (column's row at `to`),
+// or added to what is there.
+template <typename KT, int D, int COLS, bool ADD>
+__device__ __forceinline__ void ka_spill(const KaAcc<KT, D, COLS>& x, float f, float* to, int part) {
+    using T = Ka<KT, D, COLS>;
+#pragma unroll
+    for (int n = 0; n < T::NT; n += T::F16 ? 1 : 4)
+#pragma unroll
+        for (int e = 0; e < T::E; e += T::F16 ? 4 : 1) {
+            ka_f4 v;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = (T::F16 ? x.o[n][e + j] : x.o[n + j][e]) * f;
+            ka_f4* at = (ka_f4*)(to + T::dim(n, e, part));
+            *at = ADD ? *at + v : v;
+        }
 }
 
-struct KaKeys {
-    const int32_t* row;      // the table row that the keys are read through
+// ---- what an item is: columns of a batch or a request, a run of keys of one kv head
+struct KaItem {
+    const int32_t* table;    // the table row that the keys are read through
     int g, k0, k1;           // kv head, keys
+    int row0, ncols;         // columns: (row0 + c / G, head g * G + c % G), c < ncols
+    int first_limit;         // tails: keys that row0 sees, each row behind it one more
+    int slot;                // of the workspace
+    bool bad;                // no such sequence: the rows become NaN
 };
 
-template <typename KT, int D, int XP>
-__device__ __forceinline__ void ka_walk(const KaArgs& a, const KaKeys& keys, char* mine, int w, int lane, int limit,
-                                        int least, const KaQ<KT, D, XP>& q, KaAcc<KT, D>& x, bool& bad) {
-    using T = Ka<KT, D>;
-    const pio_kv_cache& c = a.c;
-    const int h = lane >> 5, lg = kv_log2(c.page_size), mask = c.page_size - 1, per_page = c.n_kv_heads * c.page_size;
-    const char* kb = (const char*)c.kv + ((int64_t)(2 * a.layer) * c.n_pages * per_page + (int64_t)keys.g * c.page_size) * T::RB;
-    const char* vb = kb + (int64_t)c.n_pages * per_page * T::RB;
-    char *kt = mine, *vt = mine + T::TILE;
-    const int tiles = (keys.k1 - keys.k0 + KA_KEYS - 1) / KA_KEYS;
-    // cache row of this lane's key of tile j (keys behind the last one re-read it)
-    auto key_row = [&](int j) -> uint32_t {
-        const int t = min(keys.k0 + min(j, tiles - 1) * KA_KEYS + (lane & 31), keys.k1 - 1);
-        int page = keys.row[t >> lg];
-        if (page < 0 || page >= c.n_pages) {
-            bad = true;
-            page = 0;
-        }
-        return (uint32_t)page * (uint32_t)per_page + (uint32_t)(t & mask);
-    };
-    int64_t off[T::NI];
-    auto offsets = [&](uint32_t row) {
-#pragma unroll
-        for (int i = 0; i < T::NI; i++) {
-            const int r = T::RPI * i + lane / T::SL;
-            off[i] = (int64_t)(uint32_t)__shfl((int)row, r, 64) * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
-        }
-    };
-    auto copy = [&](const char* from, char* to) {
-#pragma unroll
-        for (int i = 0; i < T::NI; i++)
-            __builtin_amdgcn_global_load_lds((const void*)(from + off[i]), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
-    };
-    if (w >= tiles) return;
-    uint32_t next = key_row(w);
-    offsets(next);
-    next = key_row(w + 4);
-    copy(kb, kt);
-    copy(vb, vt);
-    for (int j = w; j < tiles; j += 4) {
-        const int t0 = keys.k0 + j * KA_KEYS;
-        const bool more = j + 4 < tiles, edge = t0 + KA_KEYS > least;
-        ka_wait_copies<T::NI>();
-        ka_v16 s = ka_scores<KT, D, XP>(kt, q, lane);
-        ka_wait_reads();
-        if (more) {
-            offsets(next);
-            copy(kb, kt);
-            next = key_row(j + 8);
-        }
-        ka_softmax<KT, D>(x, s, q.cs, t0, limit, edge, h);
-        if (more) ka_wait_copies<T::NI + 1>();
-        else ka_wait_copies<0>();
-        const bool odd = edge && ka_odd<KT, D>(vt, lane);
-        ka_values<KT, D, XP>(x, s, vt, lane, odd, t0, limit);
-        ka_wait_reads();
-        if (more) copy(vb, vt);
-    }
-}
-
-// A lane's part of an accumulated column, times f, into LDS (column's row at `to`).
-template <typename KT, int D>
-__device__ __forceinline__ void ka_spill(const KaAcc<KT, D>& x, float f, float* to, int h) {
-    using T = Ka<KT, D>;
-    if constexpr (T::F16) {
-#pragma unroll
-        for (int n = 0; n < T::NT; n++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *(ka_f4*)(to + T::dim(n, e, h)) = ka_f4{x.o[n][e] * f, x.o[n][e + 1] * f, x.o[n][e + 2] * f, x.o[n][e + 3] * f};
-    } else {
-#pragma unroll
-        for (int e = 0; e < 16; e++)
-#pragma unroll
-            for (int n = 0; n < T::NT; n++) to[T::dim(n, e, h)] = x.o[n][e] * f;
-    }
-}
-
-// 4 consecutive dimensions from d of column (row, head): an item's part of it, or
-// the result.
-__device__ __forceinline__ void ka_put(const KaArgs& a, int D, int slot, int row, int head, int d, ka_f4 v, float m, float l) {
-    const int64_t at = (int64_t)slot * a.rows * a.H + (int64_t)row * a.H + head;
-    *(ka_f4*)(a.part_o + at * D + d) = v;
-    if (d == 0) *(ka_f2*)(a.part_ml + 2 * at) = ka_f2{m, l};
-}
+// 4 dimensions from d of column (row, head): an item's part of it, or the result.
 __device__ __forceinline__ void ka_out(const KaArgs& a, int D, int row, int head, int d, ka_f4 v) {
     const int64_t at = row * a.out_stride + (int64_t)head * D + d;
     if (a.q16) {
@@ -578,32 +524,33 @@ __device__ __forceinline__ void ka_out(const KaArgs& a, int D, int row, int head
         *(ka_f4*)((float*)a.out + at) = v;
     }
 }
-
-// Keys of tail split z of a request: from `from` to `len`, in runs of whole rounds
-// of 4 tiles; how many runs there are.
-__host__ __device__ __forceinline__ int ka_tail_runs(int from, int len, int splits, int& keys) {
-    constexpr int ROUND = 4 * KA_KEYS;
-    if (len <= from) {
-        keys = 0;
-        return 0;
+__device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it, int col, int d, ka_f4 v, float m, float l) {
+    const int r = col / a.G, row = it.row0 + r, head = it.g * a.G + col - r * a.G;
+    if (a.direct) {
+        v = v / l;
+        if (it.first_limit + r <= 0 && l == 0.f) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
+        ka_out(a, D, row, head, d, v);
+        return;
     }
-    const int rounds = (len - from + ROUND - 1) / ROUND;
-    const int per = (rounds + splits - 1) / splits;
-    keys = per * ROUND;
+    const int64_t at = ((int64_t)it.slot * a.rows + row) * a.H + head;
+    *(ka_f4*)(a.part_o + at * D + d) = v;
+    if (d == 0) *(ka_f2*)(a.part_ml + 2 * at) = ka_f2{m, l};
+}
+
+constexpr int KA_ROUND = 128;          // keys that runs are multiples of
+// The runs of a tail's keys (from `from` to `len`): how many, and the keys of each.
+__device__ __forceinline__ int ka_tail_runs(int from, int len, int splits, int& keys) {
+    keys = 0;
+    if (len <= from) return 0;
+    const int rounds = (len - from + KA_ROUND - 1) / KA_ROUND, per = (rounds + splits - 1) / splits;
+    keys = per * KA_ROUND;
     return (rounds + per - 1) / per;
 }
 
-// Rows in LDS that a tile of columns has: limit (keys that the row sees) and
-// whether a request has the row.
-template <int N>
-struct KaRows {
-    int limit[N];
-};
-
-// The limits of rows first .. first + N - 1 of the batch, by the whole workgroup.
-template <int N>
-__device__ __forceinline__ void ka_limits(const KaArgs& a, int first, KaRows<N>& r) {
-    for (int i = threadIdx.x; i < N; i += blockDim.x) r.limit[i] = -1;
+// Keys that each of N rows of the batch from `first` sees, -1 for a row that no
+// request has; by the whole workgroup.
+__device__ __forceinline__ void ka_limits(const KaArgs& a, int first, int* limit, int N) {
+    for (int i = threadIdx.x; i < N; i += blockDim.x) limit[i] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
         int r0, r1;
@@ -612,7 +559,7 @@ __device__ __forceinline__ void ka_limits(const KaArgs& a, int first, KaRows<N>&
         if (lo >= hi) continue;
         const int L = kv_seq_len(a.c, a.seq[i]);
         if (L < 0) continue;
-        for (int row = lo; row < hi; row++) r.limit[row - first] = max(L - (r1 - row) + 1, 0);
+        for (int row = lo; row < hi; row++) limit[row - first] = max(L - (r1 - row) + 1, 0);
     }
     __syncthreads();
 }
@@ -623,133 +570,228 @@ __device__ __forceinline__ int ka_wave_min(int v) {
     return v;
 }
 
-// Workgroup items. GROUPS groups of 4 waves; WIDE: the prefix is taken by 8 waves
-// together (128 columns, below), else by groups of 4 as the tails are.
-template <typename KT, int D, int GROUPS>
+// Where a layer's K of kv head g begins (V: a plane behind it).
+template <int RB>
+__device__ __forceinline__ const char* ka_base(const KaArgs& a, int g) {
+    const pio_kv_cache& c = a.c;
+    return (const char*)c.kv + (((int64_t)2 * a.layer * c.n_pages * c.n_kv_heads + g) * c.page_size) * RB;
+}
+template <int RB>
+__device__ __forceinline__ int64_t ka_plane(const KaArgs& a) {
+    return (int64_t)a.c.n_pages * a.c.n_kv_heads * a.c.page_size * RB;
+}
+
+// ---- narrow items: 4 waves, 16 columns, every 4th tile of the keys each, from a
+// piece of LDS of the wave's own (one tile of K, one of V). The next K tile is
+// copied during this one's softmax and product with V, the next V tile during the
+// next scores. No barriers: a wave waits for its own copies.
+constexpr int KA_COLS = 16;
+
+template <int N>
+__device__ __forceinline__ void ka_wait_copies() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((N & 0xF) | (0x7 << 4) | (0xF << 8) | ((N >> 4) << 14));
+    asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void ka_wait_reads() {     // the wave's LDS reads are done: copies may overwrite them
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xC07F);               // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+template <typename KT, int D, int XP>
+__device__ __forceinline__ void ka_walk(const KaArgs& a, const KaItem& it, char* mine, int w, int lane, int limit,
+                                        int row, int head, bool has, KaAcc<KT, D, KA_COLS>& x, bool& bad) {
+    using T = Ka<KT, D, KA_COLS>;
+    const pio_kv_cache& c = a.c;
+    const int part = lane / KA_COLS, lg = kv_log2(c.page_size), mask = c.page_size - 1;
+    const int per_page = c.n_kv_heads * c.page_size;
+    const char* kb = ka_base<T::RB>(a, it.g);
+    const char* vb = kb + ka_plane<T::RB>(a);
+    char *kt = mine, *vt = mine + T::TILE;
+    const int tiles = (it.k1 - it.k0 + T::KEYS - 1) / T::KEYS;
+    if (w >= tiles) return;
+    // cache row of this lane's key of tile j (keys behind the last one re-read it)
+    auto key_row = [&](int j) -> uint32_t {
+        const int t = min(it.k0 + min(j, tiles - 1) * T::KEYS + lane % T::KEYS, it.k1 - 1);
+        int page = it.table[t >> lg];
+        if (page < 0 || page >= c.n_pages) {
+            bad = true;
+            page = 0;
+        }
+        return (uint32_t)page * (uint32_t)per_page + (uint32_t)(t & mask);
+    };
+    int64_t off[T::NI];
+    auto offsets = [&](uint32_t r0) {
+#pragma unroll
+        for (int i = 0; i < T::NI; i++) {
+            const int r = T::RPI * i + lane / T::SL;
+            off[i] = (int64_t)(uint32_t)__shfl((int)r0, r, 64) * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
+        }
+    };
+    auto copy = [&](const char* from, char* to) {
+#pragma unroll
+        for (int i = 0; i < T::NI; i++)
+            __builtin_amdgcn_global_load_lds((const void*)(from + off[i]), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
+    };
+    uint32_t next = key_row(w);
+    offsets(next);
+    next = key_row(w + 4);
+    copy(kb, kt);
+    copy(vb, vt);
+    KaQ<KT, D, KA_COLS, XP> q;
+    ka_load_q<KT, D, KA_COLS, XP>(a, row, head, has, part, q);
+    const int least = ka_wave_min(limit);
+    ka_wait_copies<0>();                   // the query too: below only copies and one page id are counted
+    for (int j = w; j < tiles; j += 4) {
+        const int t0 = it.k0 + j * T::KEYS;
+        const bool more = j + 4 < tiles, edge = t0 + T::KEYS > least;
+        ka_wait_copies<T::NI>();
+        float s[T::NS];
+        ka_scores<KT, D, KA_COLS, XP>(kt, q, lane, s);
+        ka_wait_reads();
+        if (more) {
+            offsets(next);
+            copy(kb, kt);
+            next = key_row(j + 8);
+        }
+        ka_softmax<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
+        if (more) ka_wait_copies<T::NI + 1>();
+        else ka_wait_copies<0>();
+        const bool odd = edge && ka_odd<KT, D, KA_COLS>(vt, lane);
+        ka_values<KT, D, KA_COLS, XP>(x, s, vt, lane, odd, t0, limit);
+        ka_wait_reads();
+        if (more) copy(vb, vt);
+    }
+}
+
+template <typename KT, int D>
 constexpr size_t ka_group_bytes() {
-    using T = Ka<KT, D>;
+    using T = Ka<KT, D, KA_COLS>;
     return std::max<size_t>(4 * 2 * T::TILE, (size_t)4 * KA_COLS * T::OP * 4);
 }
 
+// A group's 16 columns from c0 joined over its 4 waves and written.
+template <typename KT, int D>
+__device__ __forceinline__ void ka_join(const KaArgs& a, const KaItem& it, KaAcc<KT, D, KA_COLS>& x, char* lds,
+                                        float (*ml)[KA_COLS][2], int w, int lane, bool bad, int c0, bool on) {
+    using T = Ka<KT, D, KA_COLS>;
+    const int col = lane % KA_COLS, part = lane / KA_COLS;
+    x.l += __shfl_xor(x.l, 32, 64);
+    x.l += __shfl_xor(x.l, 16, 64);
+    if (__any(bad)) x.l = NAN;
+    if (part == 0) {
+        ml[w][col][0] = x.m;
+        ml[w][col][1] = x.l;
+    }
+    __syncthreads();                       // and every wave is done with its tiles
+    float mx = ml[0][col][0];
+#pragma unroll
+    for (int i = 1; i < 4; i++) mx = fmaxf(mx, ml[i][col][0]);
+    ka_spill<KT, D, KA_COLS, false>(x, __builtin_amdgcn_exp2f(x.m - mx), (float*)lds + (w * KA_COLS + col) * T::OP, part);
+    __syncthreads();
+    if (!on) return;
+    for (int i = w * 64 + lane; i < min(KA_COLS, it.ncols - c0) * (D / 4); i += 256) {
+        const int c = i / (D / 4), d = (i % (D / 4)) * 4;
+        float m = ml[0][c][0], l = 0.f;
+#pragma unroll
+        for (int k = 1; k < 4; k++) m = fmaxf(m, ml[k][c][0]);
+        ka_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            v += *(const ka_f4*)((const float*)lds + (k * KA_COLS + c) * T::OP + d);
+            l += ml[k][c][1] * __builtin_amdgcn_exp2f(ml[k][c][0] - m);
+        }
+        ka_emit(a, D, it, c0 + c, d, v, m, l);
+    }
+}
+
+// ---- wide items: 8 waves, 128 columns, 4 tiles of 32 by waves w % 4, the two halves
+// of every 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in
+// LDS that all waves copy together: K and V cross from L2 once for 128 columns.
 constexpr int KA_WIDE_MIN = 64;      // columns from which on
 constexpr int KA_WIDE_COLS = 128, KA_WIDE_KEYS = 64, KA_STAGES = 4, KA_WIDE_PAGES = 4096;
 template <int D>
 constexpr size_t ka_wide_bytes() {
     return std::max<size_t>({(size_t)KA_STAGES * 2 * KA_WIDE_KEYS * D * 2, (size_t)KA_WIDE_COLS * (D + 4) * 4,
-                             2 * ka_group_bytes<_Float16, D, 2>()});
+                             2 * ka_group_bytes<_Float16, D>()});
 }
 
-// A group's columns joined over its 4 waves and written. first_limit: keys that row
-// row0 sees (fewer than one: none; each row behind it sees one more).
-template <typename KT, int D>
-__device__ __forceinline__ void ka_join(const KaArgs& a, KaAcc<KT, D>& x, char* lds, float (*ml)[KA_COLS][2], int w, int lane,
-                                        bool bad, int slot, int row0, int g, int c0, int ncols, bool live,
-                                        int first_limit = 1) {
-    using T = Ka<KT, D>;
-    const int col = lane & 31, h = lane >> 5;
-    x.l += __shfl_xor(x.l, 32, 64);
-    if (__any(bad)) x.l = NAN;
-    if (h == 0) {
-        ml[w][col][0] = x.m;
-        ml[w][col][1] = x.l;
-    }
-    __syncthreads();
-    float mx = ml[0][col][0];
-#pragma unroll
-    for (int i = 1; i < 4; i++) mx = fmaxf(mx, ml[i][col][0]);
-    ka_spill<KT, D>(x, __builtin_amdgcn_exp2f(x.m - mx), (float*)lds + (w * KA_COLS + col) * T::OP, h);
-    __syncthreads();
-    if (live)
-        for (int i = w * 64 + lane; i < KA_COLS * (D / 4); i += 256) {
-            const int c = i / (D / 4), d = (i % (D / 4)) * 4;
-            if (c0 + c >= ncols) break;
-            float m = ml[0][c][0], l = 0.f;
-#pragma unroll
-            for (int k = 1; k < 4; k++) m = fmaxf(m, ml[k][c][0]);
-            ka_f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                v += *(const ka_f4*)((const float*)lds + (k * KA_COLS + c) * T::OP + d);
-                l += ml[k][c][1] * __builtin_amdgcn_exp2f(ml[k][c][0] - m);
-            }
-            const int row = row0 + (c0 + c) / a.G, head = g * a.G + (c0 + c) % a.G;
-            if (a.direct) {
-                v = v / l;
-                if (first_limit + row - row0 <= 0 && l == 0.f) v = ka_f4{0.f, 0.f, 0.f, 0.f};
-                ka_out(a, D, row, head, d, v);
-            }
-            else ka_put(a, D, slot, row, head, d, v, m, l);
-        }
-}
-
-// The prefix item of 8 waves: 128 columns, 4 tiles of 32 by waves w % 4, the two
-// halves of every 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES
-// stages in LDS that all waves copy together.
 template <int D, int XP>
-__device__ __forceinline__ void ka_wide(const KaArgs& a, char* lds, int* pages, float (*ml)[KA_COLS][2], KaRows<128>& rows,
-                                        int g, int split, int ct) {
+__device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char* lds, int* pages,
+                                        float (*ml)[32][2], const int* limits, int base) {
     typedef _Float16 KT;
-    using T = Ka<KT, D>;
+    using T = Ka<KT, D, 32>;
     const pio_kv_cache& c = a.c;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), cg = w & 3, kg = w >> 2;
     const int col = lane & 31, h = lane >> 5;
     const int lg = kv_log2(c.page_size), mask = c.page_size - 1, per_page = c.n_kv_heads * c.page_size;
-    const int k0 = split * a.pre_keys, k1 = min(k0 + a.pre_keys, a.shared);
-    const int ncols = a.rows * a.G, c0 = ct * KA_WIDE_COLS + cg * KA_COLS, first = ct * KA_WIDE_COLS / a.G;
-    bool bad = a.seq[0] < 0 || a.seq[0] >= c.max_seqs;
-    const int32_t* trow = c.table + (int64_t)(bad ? 0 : a.seq[0]) * c.max_pages;
-    const int p0 = k0 >> lg, np = ((k1 - 1) >> lg) - p0 + 1;
-    for (int i = tid; i < np; i += 512) {
-        int page = trow[p0 + i];
-        if (page < 0 || page >= c.n_pages) {
-            bad = true;
-            page = 0;
-        }
-        pages[i] = page;
+    const int c0 = base + cg * 32;
+    const bool has = c0 + col < it.ncols;
+    const int r = has ? (c0 + col) / a.G : 0, row = it.row0 + r, head = it.g * a.G + (has ? (c0 + col) - r * a.G : 0);
+    // limits: of the rows from base / G (prefix); else by first_limit
+    int limit = it.k1;
+    if (has) {
+        const int n = limits ? limits[r - base / a.G] : it.first_limit + r;
+        if (!limits || n >= 0) limit = min(n, it.k1);
     }
-    ka_limits(a, first, rows);
-    const bool has = c0 + col < ncols;
-    const int row = has ? (c0 + col) / a.G : 0, head = g * a.G + (has ? (c0 + col) % a.G : 0);
-    int limit = has ? rows.limit[row - first] : -1;
-    limit = limit < 0 ? k1 : min(limit, k1);
     const int least = ka_wave_min(limit);
-    KaQ<KT, D, XP> q;
-    ka_load_q<KT, D, XP>(a, row, head, has, h, q);
-    KaAcc<KT, D> x;
+    KaQ<KT, D, 32, XP> q;
+    ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
+    KaAcc<KT, D, 32> x;
     x.clear();
+    bool bad = it.bad;
 
-    const char* kb = (const char*)c.kv + ((int64_t)(2 * a.layer) * c.n_pages * per_page + (int64_t)g * c.page_size) * T::RB;
-    const char* vb = kb + (int64_t)c.n_pages * per_page * T::RB;
+    const char* kb = ka_base<T::RB>(a, it.g);
+    const char* vb = kb + ka_plane<T::RB>(a);
     constexpr int STAGE = 2 * KA_WIDE_KEYS * T::RB, PW = 8 / T::RPI;    // copies of a wave: PW of K, PW of V
-    // stage s: its rows 8 w .. 8 w + 7 (keys behind the last one re-read it)
-    auto copy = [&](int s) {
-        char* to = lds + (s % KA_STAGES) * STAGE + 8 * w * T::RB;
-#pragma unroll
-        for (int i = 0; i < PW; i++) {
-            const int r = 8 * w + T::RPI * i + lane / T::SL, t = min(k0 + s * KA_WIDE_KEYS + r, k1 - 1);
-            const uint32_t at = (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
-            const int64_t off = (int64_t)at * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
-            __builtin_amdgcn_global_load_lds((const void*)(kb + off), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const void*)(vb + off), (ka_lds_t*)(to + KA_WIDE_KEYS * T::RB + i * 1024), 16, 0, 0);
+    const int chunk = (KA_WIDE_PAGES - 1) * min(c.page_size, 1 << 16) / KA_WIDE_KEYS * KA_WIDE_KEYS;
+    for (int k0 = it.k0; k0 < it.k1; k0 += chunk) {    // as many keys as page ids fit
+        const int k1 = min(it.k1 - k0, chunk) + k0, p0 = k0 >> lg, np = ((k1 - 1) >> lg) - p0 + 1;
+        if (k0 != it.k0) __syncthreads();
+        for (int i = tid; i < np; i += 512) {
+            int page = it.table[p0 + i];
+            if (page < 0 || page >= c.n_pages) {
+                bad = true;
+                page = 0;
+            }
+            pages[i] = page;
         }
-    };
-    const int stages = (k1 - k0 + KA_WIDE_KEYS - 1) / KA_WIDE_KEYS;
-    ka_wait_copies<0>();               // q is here: the waits below count copies alone
+        __syncthreads();
+        // stage s: its rows 8 w .. 8 w + 7 (keys behind the last one re-read it)
+        auto copy = [&](int s) {
+            char* to = lds + (s % KA_STAGES) * STAGE + 8 * w * T::RB;
 #pragma unroll
-    for (int s = 0; s < KA_STAGES - 1; s++) copy(s);
-    for (int s = 0; s < stages; s++) {
-        stage_barrier<(KA_STAGES - 2) * 2 * PW>();
-        // into the stage that every wave has read before this barrier; past the end the last key again
-        copy(s + KA_STAGES - 1);
-        const char* kt = lds + (s % KA_STAGES) * STAGE + kg * T::TILE;
-        const char* vt = kt + KA_WIDE_KEYS * T::RB;
-        const int t0 = k0 + s * KA_WIDE_KEYS + kg * KA_KEYS;
-        const bool edge = t0 + KA_KEYS > least;
-        ka_v16 sc = ka_scores<KT, D, XP>(kt, q, lane);
-        ka_softmax<KT, D>(x, sc, q.cs, t0, limit, edge, h);
-        const bool odd = edge && ka_odd<KT, D>(vt, lane);
-        ka_values<KT, D, XP>(x, sc, vt, lane, odd, t0, limit);
+            for (int i = 0; i < PW; i++) {
+                const int rr = 8 * w + T::RPI * i + lane / T::SL, t = min(k0 + s * KA_WIDE_KEYS + rr, k1 - 1);
+                const uint32_t at = (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
+                const int64_t off = (int64_t)at * T::RB + (((lane % T::SL) ^ T::swz(rr)) << 4);
+                __builtin_amdgcn_global_load_lds((const void*)(kb + off), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void*)(vb + off), (ka_lds_t*)(to + KA_WIDE_KEYS * T::RB + i * 1024), 16, 0, 0);
+            }
+        };
+        const int stages = (k1 - k0 + KA_WIDE_KEYS - 1) / KA_WIDE_KEYS;
+        ka_wait_copies<0>();               // q is here: the waits below count copies alone
+#pragma unroll
+        for (int s = 0; s < KA_STAGES - 1; s++) copy(s);
+        for (int s = 0; s < stages; s++) {
+            stage_barrier<(KA_STAGES - 2) * 2 * PW>();
+            // into the stage that every wave has read before this barrier; past the end the last key again
+            copy(s + KA_STAGES - 1);
+            const char* kt = lds + (s % KA_STAGES) * STAGE + kg * T::TILE;
+            const char* vt = kt + KA_WIDE_KEYS * T::RB;
+            const int t0 = k0 + s * KA_WIDE_KEYS + kg * T::KEYS;
+            // (a chunk's end is not the item's: keys behind it come with the next chunk)
+            const int end = min(limit, k1);
+            const bool edge = t0 + T::KEYS > min(least, k1);
+            float sc[T::NS];
+            ka_scores<KT, D, 32, XP>(kt, q, lane, sc);
+            ka_softmax<KT, D, 32>(x, sc, q.cs, t0, end, edge, h);
+            const bool odd = edge && ka_odd<KT, D, 32>(vt, lane);
+            ka_values<KT, D, 32, XP>(x, sc, vt, lane, odd, t0, end);
+        }
     }
+    ka_wait_copies<0>();                   // those past the end too: the stages are overwritten
     // the halves of the keys meet in LDS
     x.l += __shfl_xor(x.l, 32, 64);
     if (h == 0) {
@@ -759,116 +801,133 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, char* lds, int* pages, 
     const bool any_bad = __syncthreads_or(bad);        // and every copy has landed, every stage is read
     if (any_bad && tid == 0) atomicOr(c.work, KV_BAD);
     const float mx = fmaxf(ml[cg][col][0], ml[cg + 4][col][0]), f = __builtin_amdgcn_exp2f(x.m - mx);
-    float* ob = (float*)lds + (cg * KA_COLS + col) * T::OP;
-    if (kg) ka_spill<KT, D>(x, f, ob, h);
+    float* ob = (float*)lds + (cg * 32 + col) * T::OP;
+    if (kg) ka_spill<KT, D, 32, false>(x, f, ob, h);
     __syncthreads();
-    if (!kg) {
-#pragma unroll
-        for (int n = 0; n < T::NT; n++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                ka_f4* at = (ka_f4*)(ob + T::dim(n, e, h));
-                *at += ka_f4{x.o[n][e] * f, x.o[n][e + 1] * f, x.o[n][e + 2] * f, x.o[n][e + 3] * f};
-            }
-    }
+    if (!kg) ka_spill<KT, D, 32, true>(x, f, ob, h);
     __syncthreads();
-    for (int i = tid; i < KA_WIDE_COLS * (D / 4); i += 512) {
-        const int cc = i / (D / 4), d = (i % (D / 4)) * 4, at = ct * KA_WIDE_COLS + cc;
-        if (at >= ncols) break;
+    for (int i = tid; i < min(KA_WIDE_COLS, it.ncols - base) * (D / 4); i += 512) {
+        const int cc = i / (D / 4), d = (i % (D / 4)) * 4;
         const float m0 = ml[cc >> 5][cc & 31][0], m1 = ml[4 + (cc >> 5)][cc & 31][0], m = fmaxf(m0, m1);
         float l = ml[cc >> 5][cc & 31][1] * __builtin_amdgcn_exp2f(m0 - m) +
                   ml[4 + (cc >> 5)][cc & 31][1] * __builtin_amdgcn_exp2f(m1 - m);
         if (any_bad) l = NAN;
-        ka_put(a, D, split, at / a.G, g * a.G + at % a.G, d, *(const ka_f4*)((const float*)lds + cc * T::OP + d), m, l);
+        ka_emit(a, D, it, base + cc, d, *(const ka_f4*)((const float*)lds + cc * T::OP + d), m, l);
     }
 }
 
-// Workgroups: the prefix's items, then the tails'. WIDE: 8 waves, prefix items of
-// all of them and tail items of 4; else 4 waves, items of 4.
-template <typename KT, int D, int XP, bool WIDE>
-__global__ __launch_bounds__(WIDE ? 512 : 256, sizeof(KT) == 4 ? 1 : 2) void ka_kernel(KaArgs a) {
-    constexpr int GROUPS = WIDE ? 2 : 1;
+// The prefix item of a workgroup: false for one beyond them.
+__device__ __forceinline__ bool ka_prefix(const KaArgs& a, KaItem& it, int& ct) {
+    // the column tiles of a (kv head, run of keys) on one XCD, next to each other: they read the same K and V
+    const int x = blockIdx.x & 7, y = blockIdx.x >> 3, unit = (y / a.pre_tiles) * 8 + x;
+    ct = y % a.pre_tiles;
+    if (unit >= a.c.n_kv_heads * a.pre_splits) return false;
+    it.slot = unit / a.c.n_kv_heads;
+    it.g = unit - it.slot * a.c.n_kv_heads;
+    it.k0 = it.slot * a.pre_keys;
+    it.k1 = min(it.k0 + a.pre_keys, a.shared);
+    it.row0 = 0;
+    it.ncols = a.rows * a.G;
+    it.first_limit = 1;
+    const int s = a.seq[0];
+    it.bad = s < 0 || s >= a.c.max_seqs;
+    it.table = a.c.table + (int64_t)(it.bad ? 0 : s) * a.c.max_pages;
+    return true;
+}
+// Run z of the tail of request i; false: it has none.
+__device__ __forceinline__ bool ka_tail(const KaArgs& a, KaItem& it, int i, int g, int z) {
+    it = KaItem{};
+    if (i >= a.n) return false;
+    int r0, r1, keys;
+    ka_rows(a, i, r0, r1);
+    const int s = a.seq[i], L = kv_seq_len(a.c, s);
+    const int runs = ka_tail_runs(a.shared, L, a.tail_splits, keys);
+    it.g = g;
+    it.k0 = a.shared + z * keys;
+    it.k1 = z < runs ? min(it.k0 + keys, L) : it.k0;
+    it.row0 = r0;
+    it.ncols = max(r1 - r0, 0) * a.G;
+    it.first_limit = L - (r1 - r0) + 1;
+    it.slot = a.pre_splits + z;
+    it.bad = L < 0;
+    it.table = a.c.table + (int64_t)(it.bad ? 0 : s) * a.c.max_pages;
+    return it.ncols > 0 && (a.direct || z < runs);     // (direct: rows without a key, and without a sequence, are written too)
+}
+
+// Workgroups: the prefix's items, then the tails'.
+//   WIDE 0: 4 waves, narrow items
+//   WIDE 1: 8 waves, wide prefix items, narrow tail items (two to a workgroup)
+//   WIDE 2: 8 waves, wide items
+template <typename KT, int D, int XP, int WIDE>
+__global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
+    constexpr int GROUPS = WIDE == 1 ? 2 : 1;
     extern __shared__ __attribute__((aligned(16))) char ka_lds[];
-    __shared__ float ml[4 * GROUPS][KA_COLS][2];
-    __shared__ KaRows<WIDE ? 128 : KA_COLS> rows;
-    const pio_kv_cache& c = a.c;
-    const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3, grp = w8 >> 2;
-    const int col = lane & 31, h = lane >> 5, Hk = c.n_kv_heads;
-    if ((int)blockIdx.x < a.pre_items) {
-        // the column tiles of a (kv head, run of keys) on one XCD, next to each other: they read the same K and V
-        const int x = blockIdx.x & 7, y = blockIdx.x >> 3, ct = y % a.pre_tiles, unit = (y / a.pre_tiles) * 8 + x;
-        if (unit >= Hk * a.pre_splits) return;
-        const int g = unit % Hk, split = unit / Hk;
+    __shared__ float ml[WIDE ? 8 * 32 * 2 : 4 * KA_COLS * 2];
+    __shared__ int limits[WIDE ? KA_WIDE_COLS : KA_COLS];
+    const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3;
+    const bool prefix = (int)blockIdx.x < a.pre_items;
+    KaItem it;
+    int ct = 0, step = 1;                  // first column tile, tiles to the next
+    if (prefix) {
+        if (!ka_prefix(a, it, ct)) return;
+        step = INT_MAX / 256;              // one only
         if constexpr (WIDE) {
-            ka_wide<D, XP>(a, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), ml, rows, g, split, ct);
+            ka_limits(a, ct * KA_WIDE_COLS / a.G, limits, KA_WIDE_COLS);
+            ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, limits, ct * KA_WIDE_COLS);
+            return;
         } else {
-            const int ncols = a.rows * a.G, c0 = ct * KA_COLS, first = c0 / a.G;
-            bool bad = a.seq[0] < 0 || a.seq[0] >= c.max_seqs;
-            KaKeys keys{c.table + (int64_t)(bad ? 0 : a.seq[0]) * c.max_pages, g, split * a.pre_keys, 0};
-            keys.k1 = min(keys.k0 + a.pre_keys, a.shared);
-            ka_limits(a, first, rows);
-            const bool has = c0 + col < ncols;
-            const int row = has ? (c0 + col) / a.G : 0, head = g * a.G + (has ? (c0 + col) % a.G : 0);
-            int limit = has ? rows.limit[row - first] : -1;
-            limit = limit < 0 ? keys.k1 : min(limit, keys.k1);
-            KaQ<KT, D, XP> q;
-            ka_load_q<KT, D, XP>(a, row, head, has, h, q);
-            KaAcc<KT, D> acc;
+            ka_limits(a, ct * KA_COLS / a.G, limits, KA_COLS);
+        }
+    }
+    bool live = true;
+    if (!prefix) {
+        // (request, kv head, column tile, run), neighbours in one workgroup
+        int item = ((int)blockIdx.x - a.pre_items) * GROUPS + (GROUPS == 2 ? w8 >> 2 : 0);
+        const int z = item % a.tail_splits;
+        item /= a.tail_splits;
+        ct = item % a.tail_tiles;
+        item /= a.tail_tiles;
+        step = a.tail_tiles;
+        live = ka_tail(a, it, item / a.c.n_kv_heads, item % a.c.n_kv_heads, z);
+    }
+    if constexpr (WIDE == 2) {
+        // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
+        for (int base = ct * KA_WIDE_COLS; live && base < it.ncols; base += step * KA_WIDE_COLS) {
+            __syncthreads();
+            ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, nullptr, base);
+        }
+    } else {
+        const int grp = GROUPS == 2 ? w8 >> 2 : 0;
+        char* lds = ka_lds + grp * ka_group_bytes<KT, D>();
+        float (*gml)[KA_COLS][2] = (float (*)[KA_COLS][2])ml + 4 * grp;
+        const int ct1 = live ? (it.ncols + KA_COLS - 1) / KA_COLS : 0;
+        int rounds = prefix ? 1 : ct < ct1 ? (ct1 - ct + step - 1) / step : 0;
+        if constexpr (GROUPS == 2) {       // both groups make as many rounds, for the barriers
+            __shared__ int most[2];
+            if ((tid & 255) == 0) most[grp] = rounds;
+            __syncthreads();
+            rounds = max(most[0], most[1]);
+        }
+        for (int r = 0; r < rounds; r++) {
+            const int c0 = (ct + r * step) * KA_COLS, col = c0 + lane % KA_COLS;
+            const bool on = live && c0 < it.ncols;
+            bool bad = it.bad;
+            KaAcc<KT, D, KA_COLS> acc;
             acc.clear();
-            ka_walk<KT, D, XP>(a, keys, ka_lds + w * 2 * Ka<KT, D>::TILE, w, lane, limit, ka_wave_min(limit), q, acc, bad);
-            if (__any(bad) && lane == 0) atomicOr(c.work, KV_BAD);
-            ka_join<KT, D>(a, acc, ka_lds, ml, w, lane, bad, split, 0, g, c0, ncols, true);
+            if (on && it.k0 < it.k1) {
+                const bool has = col < it.ncols;
+                const int q = has ? col / a.G : 0, head = it.g * a.G + (has ? col - q * a.G : 0);
+                int limit = it.k1;
+                if (has) {
+                    const int n = prefix ? limits[q - c0 / a.G] : it.first_limit + q;
+                    if (!prefix || n >= 0) limit = min(n, it.k1);
+                }
+                ka_walk<KT, D, XP>(a, it, lds + w * 2 * Ka<KT, D, KA_COLS>::TILE, w, lane, limit, it.row0 + q, head, has, acc, bad);
+            }
+            if (on && __any(bad) && lane == 0) atomicOr(a.c.work, KV_BAD);
+            if (r) __syncthreads();        // the last round's output is out of LDS
+            ka_join<KT, D>(a, it, acc, lds, gml, w, lane, bad, c0, on);
         }
-        return;
-    }
-    // tails: (request, kv head, column tile, run), two neighbours per workgroup of 8 waves
-    int item = ((int)blockIdx.x - a.pre_items) * GROUPS + grp;
-    const int z = item % a.tail_splits;
-    item /= a.tail_splits;
-    const int ct0 = item % a.tail_tiles;
-    item /= a.tail_tiles;
-    const int g = item % Hk, i = item / Hk;
-    int r0 = 0, r1 = 0, L = -1, s = -1, keys_per = 0, runs = 0;
-    if (i < a.n) {
-        ka_rows(a, i, r0, r1);
-        s = a.seq[i];
-        L = kv_seq_len(c, s);
-        runs = ka_tail_runs(a.shared, L, a.tail_splits, keys_per);
-    }
-    char* lds = ka_lds + grp * ka_group_bytes<KT, D, GROUPS>();
-    float (*gml)[KA_COLS][2] = ml + 4 * grp;
-    const int ncols = max(r1 - r0, 0) * a.G;
-    // columns beyond the tiles of the grid (a request of more rows than announced): more rounds.
-    // Both groups of a workgroup make as many, for the barriers.
-    const bool live = i < a.n && (a.direct || z < runs);
-    int rounds = live ? (ncols + KA_COLS - 1) / KA_COLS - ct0 : 0;
-    rounds = rounds > 0 ? (rounds + a.tail_tiles - 1) / a.tail_tiles : 0;
-    if constexpr (GROUPS == 2) {
-        __shared__ int most[2];
-        if ((tid & 255) == 0) most[grp] = rounds;
-        __syncthreads();
-        rounds = max(most[0], most[1]);
-    }
-    for (int r = 0; r < rounds; r++) {
-        const int c0 = (ct0 + r * a.tail_tiles) * KA_COLS;
-        const bool on = live && c0 < ncols;
-        bool bad = L < 0;
-        KaAcc<KT, D> acc;
-        acc.clear();
-        if (on && z < runs) {
-            const bool has = c0 + col < ncols;
-            const int row = has ? r0 + (c0 + col) / a.G : r0, head = g * a.G + (has ? (c0 + col) % a.G : 0);
-            KaKeys keys{c.table + (int64_t)s * c.max_pages, g, a.shared + z * keys_per, 0};
-            keys.k1 = min(keys.k0 + keys_per, L);
-            const int limit = has ? min(L - (r1 - row) + 1, keys.k1) : keys.k1;
-            KaQ<KT, D, XP> q;
-            ka_load_q<KT, D, XP>(a, row, head, has, h, q);
-            ka_walk<KT, D, XP>(a, keys, lds + w * 2 * Ka<KT, D>::TILE, w, lane, limit, ka_wave_min(limit), q, acc, bad);
-        }
-        if (on && __any(bad) && lane == 0) atomicOr(c.work, KV_BAD);
-        if (r) __syncthreads();        // the last round's output is out of LDS
-        ka_join<KT, D>(a, acc, lds, gml, w, lane, bad, a.pre_splits + z, r0, g, c0, ncols, on,
-                        L - (r1 - r0) + 1);
     }
 }
 
@@ -932,14 +991,14 @@ __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
     if (bad && tid == 0) atomicOr(c.work, KV_BAD);
 }
 
-template <typename KT, int D, int XP, bool WIDE>
+template <typename KT, int D, int XP, int WIDE>
 static int ka_launch(const KaArgs& a, hipStream_t st) {
-    constexpr int GROUPS = WIDE ? 2 : 1;
-    size_t lds = ka_group_bytes<KT, D, GROUPS>();
+    constexpr int GROUPS = WIDE == 1 ? 2 : 1;
+    size_t lds = ka_group_bytes<KT, D>();
     if constexpr (WIDE) lds = ka_wide_bytes<D>() + KA_WIDE_PAGES * sizeof(int);
     const int64_t tails = (int64_t)a.n * a.c.n_kv_heads * a.tail_tiles * a.tail_splits;
     PIO_TRY((allow_lds<ka_kernel<KT, D, XP, WIDE>>(lds)));
-    ka_kernel<KT, D, XP, WIDE><<<(unsigned)(a.pre_items + (tails + GROUPS - 1) / GROUPS), 256 * GROUPS, lds, st>>>(a);
+    ka_kernel<KT, D, XP, WIDE><<<(unsigned)(a.pre_items + (tails + GROUPS - 1) / GROUPS), WIDE ? 512 : 256, lds, st>>>(a);
     PIO_LAUNCHED();
     if (!a.direct) {
         ka_merge_kernel<D><<<a.rows * a.H, 256, 0, st>>>(a);
@@ -948,39 +1007,40 @@ static int ka_launch(const KaArgs& a, hipStream_t st) {
     return PIO_OK;
 }
 
+template <int D, int XP>
+static int ka_route16(const KaArgs& a, int wide, hipStream_t st) {
+    return wide == 2 ? ka_launch<_Float16, D, XP, 2>(a, st)
+           : wide    ? ka_launch<_Float16, D, XP, 1>(a, st)
+                     : ka_launch<_Float16, D, XP, 0>(a, st);
+}
 template <int D>
-static int ka_route(const KaArgs& a, bool wide, hipStream_t st) {
-    if (a.c.kv_dtype == PIO_F32) return ka_launch<float, D, 1, false>(a, st);
-    if (a.q16) return wide ? ka_launch<_Float16, D, 1, true>(a, st) : ka_launch<_Float16, D, 1, false>(a, st);
-    return wide ? ka_launch<_Float16, D, 2, true>(a, st) : ka_launch<_Float16, D, 2, false>(a, st);
+static int ka_route(const KaArgs& a, int wide, hipStream_t st) {
+    if (a.c.kv_dtype == PIO_F32) return ka_launch<float, D, 1, 0>(a, st);
+    return a.q16 ? ka_route16<D, 1>(a, wide, st) : ka_route16<D, 2>(a, wide, st);
 }
 
 // Items for the matrix core kernels.
 static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
     const bool f16 = a.c.kv_dtype == PIO_F16;
-    const int64_t cols = (int64_t)a.rows * a.G;
-    const bool wide = f16 && a.shared > 0 && cols > KA_WIDE_MIN;
+    const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
+    const int wide = !f16 ? 0 : tail_cols > KA_WIDE_MIN ? 2 : a.shared > 0 && cols > KA_WIDE_MIN ? 1 : 0;
     if (a.shared > 0) {
-        // prefix: as many items as the device holds at once, each of at least a few tiles of keys
-        const int width = wide ? KA_WIDE_COLS : KA_COLS, round = wide ? KA_WIDE_KEYS : 4 * KA_KEYS;
-        const int at_once = wide || !f16 ? cus : 2 * cus;
+        // prefix: as many items as the device holds at once, each of at least KA_ROUND keys
+        const int width = wide ? KA_WIDE_COLS : KA_COLS, at_once = wide ? cus : 2 * cus;
         a.pre_tiles = ceil_div(cols, width);
-        int64_t splits = std::max<int64_t>(1, at_once / std::max<int64_t>(1, (int64_t)Hk * a.pre_tiles));
-        splits = std::min<int64_t>(splits, ceil_div(a.shared, 4 * KA_KEYS));
-        int keys = ceil_div(ceil_div(a.shared, splits), round) * round;
-        if (wide) keys = (int)std::min<int64_t>(keys, (int64_t)(KA_WIDE_PAGES - 1) * a.c.page_size / round * round);
-        a.pre_keys = keys;
-        a.pre_splits = ceil_div(a.shared, keys);
+        const int64_t splits = std::max<int64_t>(1, at_once / std::max<int64_t>(1, (int64_t)Hk * a.pre_tiles));
+        a.pre_keys = ceil_div(ceil_div(a.shared, std::min<int64_t>(splits, a.shared)), KA_ROUND) * KA_ROUND;
+        a.pre_splits = ceil_div(a.shared, a.pre_keys);
         const int64_t items = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
         PIO_REQUIRE(items <= INT_MAX / 2, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)items;
     }
-    a.tail_tiles = ceil_div((int64_t)std::min(max_rows, a.rows) * a.G, KA_COLS);
+    a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
     const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
     PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    a.tail_splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / items, 32, ceil_div(longest, 4 * KA_KEYS)}));
+    a.tail_splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / items, 32, ceil_div(longest, KA_ROUND)}));
     a.direct = a.shared == 0 && a.tail_splits == 1;
     Scratch ws;
     if (!a.direct) {
