@@ -325,7 +325,8 @@ int pio_moe_w8a8(const void* x, int x_dtype, const float* logits, const int8_t* 
  * Arguments that the host can see are checked there. What only the device can
  * see (a sequence id outside the cache, one id twice, too few free pages) is
  * checked by the kernels: such a request changes nothing, and
- * pio_kv_status reports it. At most 2^20 pages, sequences and pages a sequence.
+ * pio_kv_status reports it. At most 2^20 pages, sequences and pages a sequence, 2^28
+ * tokens a sequence.
  * ------------------------------------------------------------------------- */
 typedef struct {
     void* kv;

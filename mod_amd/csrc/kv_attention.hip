@@ -42,10 +42,11 @@ struct KaArgs {
     bool q16;
     // items of the matrix core kernels
     int pre_items, pre_tiles, pre_splits, pre_keys;   // workgroups; column tiles; runs of keys, keys of each
-    int tail_tiles, tail_splits;                      // per (request, kv head)
+    int tail_tiles, tail_runs, max_runs;              // column tiles; runs of all requests that are aimed at, and of one
     bool direct;                                      // one item per column: it writes out itself
-    float* part_o;                                    // [pre_splits + tail_splits][rows * H][D]
+    float* part_o;                                    // [pre_splits + max_runs][rows * H][D]
     float* part_ml;                                   // [..][rows * H][2]
+    int* part_n;                                      // [rows]: tail runs, 0 for a row that is written already
 };
 
 // Rows of request i, kept inside q whatever row_start holds.
@@ -150,6 +151,8 @@ constexpr float KA_LOG2E = 1.44269504088896340736f;
 // fp16 weights are held times 2^10, so that those down to 2^-24 of the largest are normal
 // numbers; the sum is scaled alike.
 constexpr float KA_LIFT = 10.f;
+// Least maximum of a column that sees a key; one that sees none keeps -FLT_MAX.
+constexpr float KA_SEEN = -3.4e38f;
 constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column's largest is 2^12 .. 2^13
 
 // A tile of keys x COLS columns (16 or 32) on v_mfma_*_COLSxCOLS: lane l holds
@@ -273,22 +276,47 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
     }
 }
 
+// Operand addresses. A lane's reads of a tile differ in bits that the swizzle
+// XORs, so all are (x ^ constant) + base + constant, one instruction from one
+// register; opaque in the loop, or the compiler would hold each in a register.
+typedef __attribute__((address_space(3))) char ka_lds_c;
+__device__ __forceinline__ uint32_t ka_addr(const char* p) { return (uint32_t)(uintptr_t)(ka_lds_c*)p; }
+template <typename V>
+__device__ __forceinline__ V ka_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)(uintptr_t)at; }
+__device__ __forceinline__ uint32_t ka_opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+// K: row lane % COLS, chunk part
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ uint32_t ka_kx(int lane) { return Ka<KT, D, COLS>::slot(lane % COLS, lane / COLS); }
+// V, fp16: 16 lanes read 16 dimensions of 4 keys, 8 bytes each; fp32: 4 dimensions of the part's first key
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ uint32_t ka_vx(int lane) {
+    using T = Ka<KT, D, COLS>;
+    const int i = lane & 15, part = lane / COLS;
+    if constexpr (T::F16) return T::slot(4 * part + (i >> 2), (COLS == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((i >> 1) & 1)) + 8 * (i & 1);
+    else return T::slot(4 * part, i);
+}
+
 // S^T of one tile; kt: K's rows in LDS.
 template <typename KT, int D, int COLS, int XP>
-__device__ __forceinline__ void ka_scores(const char* kt, const KaQ<KT, D, COLS, XP>& q, int lane,
+__device__ __forceinline__ void ka_scores(uint32_t kt, uint32_t kx, const KaQ<KT, D, COLS, XP>& q,
                                           float (&s)[Ka<KT, D, COLS>::NS]) {
     using T = Ka<KT, D, COLS>;
-    const int part = lane / COLS;
+    typedef typename std::conditional<T::F16, ka_h8, ka_f4>::type K;
+    kx = ka_opaque(kx);
 #pragma unroll
     for (int st = 0; st < T::ST; st++) {
-        const int key = COLS * st + lane % COLS;
+        K k[T::QC];                    // all reads in flight together
+#pragma unroll
+        for (int i = 0; i < T::QC; i++) k[i] = ka_read<K>((kx ^ (T::PL * i << 4)) + kt + st * COLS * T::RB);
         if constexpr (T::F16) {
             typename T::Acc c = T::zero();
 #pragma unroll
             for (int i = 0; i < T::QC; i++) {
-                const ka_h8 k = *(const ka_h8*)(kt + T::slot(key, T::PL * i + part));
-                c = T::mfma(k, q.h[0][i], c);
-                if constexpr (XP == 2) c = T::mfma(k, q.h[XP - 1][i], c);
+                c = T::mfma(k[i], q.h[0][i], c);
+                if constexpr (XP == 2) c = T::mfma(k[i], q.h[XP - 1][i], c);
             }
 #pragma unroll
             for (int e = 0; e < T::E; e++) s[st * T::E + e] = c[e];
@@ -297,11 +325,9 @@ __device__ __forceinline__ void ka_scores(const char* kt, const KaQ<KT, D, COLS,
 #pragma unroll
             for (int ch = 0; ch < 4; ch++) c[ch] = T::zero();
 #pragma unroll
-            for (int i = 0; i < T::QC; i++) {
-                const ka_f4 k = *(const ka_f4*)(kt + T::slot(key, T::PL * i + part));
+            for (int i = 0; i < T::QC; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[e], q.f[i][e], c[e], 0, 0, 0);
-            }
+                for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][e], q.f[i][e], c[e], 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < 4; e++) s[e] = (c[0][e] + c[1][e]) + (c[2][e] + c[3][e]);
         }
@@ -311,16 +337,15 @@ __device__ __forceinline__ void ka_scores(const char* kt, const KaQ<KT, D, COLS,
 // A lane's 8 values of V^T (O^T tile n, key group kc): one dimension, the keys of
 // scores 8 kc .. 8 kc + 7.
 template <int D, int COLS>
-__device__ __forceinline__ ka_h8 ka_vt(const char* vt, int n, int kc, int lane) {
+__device__ __forceinline__ ka_h8 ka_vt(uint32_t vt, uint32_t vx, int n, int kc) {
     using T = Ka<_Float16, D, COLS>;
-    const int i = lane & 15, part = lane / COLS;
     ka_h8 v;
 #pragma unroll
     for (int b = 0; b < 2; b++) {
-        // 16 lanes read 16 dimensions of 4 keys, 8 bytes each, and get one dimension of the 4
-        const int row = T::key(8 * kc + 4 * b, part) + (i >> 2);
-        const int chunk = COLS / 8 * n + (COLS == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((i >> 1) & 1);
-        const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)(vt + T::slot(row, chunk) + 8 * (i & 1)));
+        // 32 columns: the second 4 keys are 8 rows on, another swizzle; 16 columns: 16 rows, the same
+        const uint32_t flip = COLS == 32 ? b * (T::RB == 128 ? 4 : 8) << 4 : 0;
+        const uint32_t at = (vx ^ ((COLS / 8 * n << 4) ^ flip)) + vt + (16 * kc + (COLS == 32 ? 8 : 16) * b) * T::RB;
+        const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)(uintptr_t)at);
 #pragma unroll
         for (int e = 0; e < 4; e++) v[4 * b + e] = (_Float16)r[e];
     }
@@ -370,7 +395,7 @@ __device__ __forceinline__ void ka_softmax(KaAcc<KT, D, COLS>& x, float (&s)[Ka<
 #pragma unroll
         for (int e = 0; e < T::NS; e++) s[e] = t0 + T::key(e, part) < limit ? s[e] : -INFINITY;
     }
-    float top = x.m;
+    float top = fmaxf(x.m, t0 < limit ? KA_SEEN : -FLT_MAX);
 #pragma unroll
     for (int e = 0; e < T::NS; e++) top = fmaxf(top, s[e]);
     const float m = ka_max<COLS>(top);
@@ -401,12 +426,12 @@ __device__ __forceinline__ void ka_softmax(KaAcc<KT, D, COLS>& x, float (&s)[Ka<
 // see all keys: 0 * inf would make those columns NaN, so inf and NaN are taken out of
 // the product and added where a column sees them (their weights are positive).
 template <typename KT, int D, int COLS, int XP>
-__device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], const char* vt,
-                                          int lane, bool odd, int t0, int limit) {
+__device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], uint32_t vt,
+                                          uint32_t vx, int part, bool odd, int t0, int limit) {
     using T = Ka<KT, D, COLS>;
-    const int part = lane / COLS;
+    vx = ka_opaque(vx);
     auto row = [&](int e, int half) {      // fp32: 4 dimensions of the key of score e
-        return *(const ka_f4*)(vt + T::slot(T::key(e, part), 16 * half + lane % COLS));
+        return ka_read<ka_f4>((vx ^ ((e ^ 16 * half) << 4)) + vt + e * T::RB);
     };
     auto product = [&](auto finite) {
         if constexpr (T::F16) {
@@ -419,16 +444,19 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p
                     w[0][e] = hi;
                     if constexpr (XP == 2) w[XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
                 }
+                ka_h8 v[T::NT];
 #pragma unroll
-                for (int n = 0; n < T::NT; n++) {
-                    ka_h8 v = ka_vt<D, COLS>(vt, n, kc, lane);
-                    if constexpr (!decltype(finite)::value) {
+                for (int n = 0; n < T::NT; n++) v[n] = ka_vt<D, COLS>(vt, vx, n, kc);
+                if constexpr (!decltype(finite)::value) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = fabsf((float)v[e]) <= 65504.f ? v[e] : (_Float16)0;
-                    }
-                    x.o[n] = T::mfma(v, w[0], x.o[n]);
-                    if constexpr (XP == 2) x.o[n] = T::mfma(v, w[XP - 1], x.o[n]);
+                    for (int n = 0; n < T::NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) v[n][e] = fabsf((float)v[n][e]) <= 65504.f ? v[n][e] : (_Float16)0;
                 }
+#pragma unroll
+                for (int part2 = 0; part2 < XP; part2++)
+#pragma unroll
+                    for (int n = 0; n < T::NT; n++) x.o[n] = T::mfma(v[n], w[part2], x.o[n]);
             }
         } else {
 #pragma unroll
@@ -462,7 +490,7 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p
             if constexpr (T::F16) {
 #pragma unroll 1
                 for (int kc = 0; kc < T::NS / 8; kc++) {
-                    const ka_h8 v = ka_vt<D, COLS>(vt, n, kc, lane);
+                    const ka_h8 v = ka_vt<D, COLS>(vt, vx, n, kc);
                     ka_h8 k, w;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -509,6 +537,7 @@ struct KaItem {
     int first_limit;         // tails: keys that row0 sees, each row behind it one more
     int slot;                // of the workspace
     bool bad;                // no such sequence: the rows become NaN
+    bool direct;             // the columns' only item: it writes the result
 };
 
 // 4 dimensions from d of column (row, head): an item's part of it, or the result.
@@ -526,9 +555,9 @@ __device__ __forceinline__ void ka_out(const KaArgs& a, int D, int row, int head
 }
 __device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it, int col, int d, ka_f4 v, float m, float l) {
     const int r = col / a.G, row = it.row0 + r, head = it.g * a.G + col - r * a.G;
-    if (a.direct) {
+    if (it.direct) {
         v = v / l;
-        if (it.first_limit + r <= 0 && l == 0.f) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
+        if (m == -FLT_MAX && l == 0.f) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
         ka_out(a, D, row, head, d, v);
         return;
     }
@@ -538,13 +567,72 @@ __device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it
 }
 
 constexpr int KA_ROUND = 128;          // keys that runs are multiples of
-// The runs of a tail's keys (from `from` to `len`): how many, and the keys of each.
-__device__ __forceinline__ int ka_tail_runs(int from, int len, int splits, int& keys) {
-    keys = 0;
-    if (len <= from) return 0;
-    const int rounds = (len - from + KA_ROUND - 1) / KA_ROUND, per = (rounds + splits - 1) / splits;
-    keys = per * KA_ROUND;
-    return (rounds + per - 1) / per;
+
+// Sum over the workgroup's threads before this one, and over all.
+__device__ __forceinline__ int ka_scan(int v, int* red, int& total) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int y = __shfl_up(x, o, 64);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 63) red[w] = x;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int i = 0; i < waves; i++) {
+        if (i < w) before += red[i];
+        total += red[i];
+    }
+    return before + x - v;
+}
+
+// Which tail items there are: the tails are cut into runs of about equal length,
+// however uneven they are (every request with rows has at least one). By the whole
+// workgroup; it gets the request, run and geometry of run number `run` (two of them
+// for two groups), false if there are fewer.
+struct KaRun {
+    int i, z, runs, per;     // request, run of it, runs of it, rounds of KA_ROUND keys of a run
+    int r0, r1, s, L;        // rows, sequence, its length (-1: none such)
+};
+template <int GROUPS>
+__device__ __forceinline__ void ka_runs(const KaArgs& a, const int (&run)[GROUPS], KaRun* found, int* red) {
+    const int tid = threadIdx.x, threads = blockDim.x;
+    KaRun r{};
+    auto rounds = [&](int i) {
+        r.i = i;
+        if (i >= a.n) return 0;
+        ka_rows(a, i, r.r0, r.r1);
+        r.s = a.seq[i];
+        r.L = kv_seq_len(a.c, r.s);
+        if (r.r1 <= r.r0) return 0;
+        return r.L <= a.shared ? 1 : (r.L - a.shared + KA_ROUND - 1) / KA_ROUND;
+    };
+    if (tid < GROUPS) found[tid].i = -1;
+    int n = rounds(tid), total, sum;
+    ka_scan(n, red, total);
+    for (int i0 = threads; i0 < a.n; i0 += threads) {
+        ka_scan(rounds(i0 + tid), red, sum);
+        total += min(sum, INT_MAX - total);
+    }
+    const int most = max(1, (int)(((int64_t)total + a.tail_runs - 1) / a.tail_runs));
+    int before = 0;
+    for (int i0 = 0; i0 < a.n; i0 += threads) {
+        if (a.n > threads) n = rounds(i0 + tid);
+        r.per = max(most, (n + a.max_runs - 1) / a.max_runs);
+        r.runs = (n + r.per - 1) / r.per;
+        const int at = before + ka_scan(r.runs, red, sum);
+        before += sum;
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++)
+            if (run[k] >= at && run[k] < at + r.runs) {
+                r.z = run[k] - at;
+                found[k] = r;
+            }
+    }
+    __syncthreads();
 }
 
 // Keys that each of N rows of the batch from `first` sees, -1 for a row that no
@@ -599,71 +687,88 @@ __device__ __forceinline__ void ka_wait_reads() {     // the wave's LDS reads ar
     asm volatile("" ::: "memory");
 }
 
-template <typename KT, int D, int XP>
-__device__ __forceinline__ void ka_walk(const KaArgs& a, const KaItem& it, char* mine, int w, int lane, int limit,
-                                        int row, int head, bool has, KaAcc<KT, D, KA_COLS>& x, bool& bad) {
+template <typename KT, int D>
+struct KaWalk {
     using T = Ka<KT, D, KA_COLS>;
-    const pio_kv_cache& c = a.c;
-    const int part = lane / KA_COLS, lg = kv_log2(c.page_size), mask = c.page_size - 1;
-    const int per_page = c.n_kv_heads * c.page_size;
-    const char* kb = ka_base<T::RB>(a, it.g);
-    const char* vb = kb + ka_plane<T::RB>(a);
-    char *kt = mine, *vt = mine + T::TILE;
-    const int tiles = (it.k1 - it.k0 + T::KEYS - 1) / T::KEYS;
-    if (w >= tiles) return;
-    // cache row of this lane's key of tile j (keys behind the last one re-read it)
-    auto key_row = [&](int j) -> uint32_t {
+    const char *kb, *vb;
+    char *kt, *vt;
+    int tiles, per_page, lg, mask;
+    uint32_t next;                         // cache row of this lane's key of the next tile
+    int64_t off[T::NI];
+    bool bad = false;
+
+    // (keys behind the last one re-read it)
+    __device__ uint32_t key_row(const KaArgs& a, const KaItem& it, int j, int lane) {
         const int t = min(it.k0 + min(j, tiles - 1) * T::KEYS + lane % T::KEYS, it.k1 - 1);
         int page = it.table[t >> lg];
-        if (page < 0 || page >= c.n_pages) {
+        if (page < 0 || page >= a.c.n_pages) {
             bad = true;
             page = 0;
         }
         return (uint32_t)page * (uint32_t)per_page + (uint32_t)(t & mask);
-    };
-    int64_t off[T::NI];
-    auto offsets = [&](uint32_t r0) {
+    }
+    __device__ void offsets(int lane) {
 #pragma unroll
         for (int i = 0; i < T::NI; i++) {
             const int r = T::RPI * i + lane / T::SL;
-            off[i] = (int64_t)(uint32_t)__shfl((int)r0, r, 64) * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
+            off[i] = (int64_t)(uint32_t)__shfl((int)next, r, 64) * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
         }
-    };
-    auto copy = [&](const char* from, char* to) {
+    }
+    __device__ void copy(const char* from, char* to) {
 #pragma unroll
         for (int i = 0; i < T::NI; i++)
             __builtin_amdgcn_global_load_lds((const void*)(from + off[i]), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
-    };
-    uint32_t next = key_row(w);
-    offsets(next);
-    next = key_row(w + 4);
-    copy(kb, kt);
-    copy(vb, vt);
-    KaQ<KT, D, KA_COLS, XP> q;
-    ka_load_q<KT, D, KA_COLS, XP>(a, row, head, has, part, q);
-    const int least = ka_wave_min(limit);
-    ka_wait_copies<0>();                   // the query too: below only copies and one page id are counted
-    for (int j = w; j < tiles; j += 4) {
-        const int t0 = it.k0 + j * T::KEYS;
-        const bool more = j + 4 < tiles, edge = t0 + T::KEYS > least;
-        ka_wait_copies<T::NI>();
-        float s[T::NS];
-        ka_scores<KT, D, KA_COLS, XP>(kt, q, lane, s);
-        ka_wait_reads();
-        if (more) {
-            offsets(next);
-            copy(kb, kt);
-            next = key_row(j + 8);
-        }
-        ka_softmax<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
-        if (more) ka_wait_copies<T::NI + 1>();
-        else ka_wait_copies<0>();
-        const bool odd = edge && ka_odd<KT, D, KA_COLS>(vt, lane);
-        ka_values<KT, D, KA_COLS, XP>(x, s, vt, lane, odd, t0, limit);
-        ka_wait_reads();
-        if (more) copy(vb, vt);
     }
-}
+    // The first tile's copies, if the wave has one.
+    __device__ void begin(const KaArgs& a, const KaItem& it, char* mine, int w, int lane) {
+        lg = kv_log2(a.c.page_size);
+        mask = a.c.page_size - 1;
+        per_page = a.c.n_kv_heads * a.c.page_size;
+        kb = ka_base<T::RB>(a, it.g);
+        vb = kb + ka_plane<T::RB>(a);
+        kt = mine;
+        vt = mine + T::TILE;
+        tiles = (it.k1 - it.k0 + T::KEYS - 1) / T::KEYS;
+        if (w >= tiles) return;
+        next = key_row(a, it, w, lane);
+        const uint32_t then = key_row(a, it, w + 4, lane);
+        offsets(lane);
+        next = then;
+        copy(kb, kt);
+        copy(vb, vt);
+    }
+    template <int XP>
+    __device__ void run(const KaArgs& a, const KaItem& it, int w, int lane, int limit, int row, int head, bool has,
+                        KaAcc<KT, D, KA_COLS>& x) {
+        if (w >= tiles) return;
+        const int part = lane / KA_COLS;
+        KaQ<KT, D, KA_COLS, XP> q;
+        ka_load_q<KT, D, KA_COLS, XP>(a, row, head, has, part, q);
+        const int least = ka_wave_min(limit);
+        const uint32_t kx = ka_kx<KT, D, KA_COLS>(lane), vx = ka_vx<KT, D, KA_COLS>(lane);
+        ka_wait_copies<0>();               // the query too: below only copies and one page id are counted
+        for (int j = w; j < tiles; j += 4) {
+            const int t0 = it.k0 + j * T::KEYS;
+            const bool more = j + 4 < tiles, edge = t0 + T::KEYS > least;
+            ka_wait_copies<T::NI>();
+            float s[T::NS];
+            ka_scores<KT, D, KA_COLS, XP>(ka_addr(kt), kx, q, s);
+            ka_wait_reads();
+            if (more) {
+                offsets(lane);
+                copy(kb, kt);
+                next = key_row(a, it, j + 8, lane);
+            }
+            ka_softmax<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
+            if (more) ka_wait_copies<T::NI + 1>();
+            else ka_wait_copies<0>();
+            const bool odd = edge && ka_odd<KT, D, KA_COLS>(vt, lane);
+            ka_values<KT, D, KA_COLS, XP>(x, s, ka_addr(vt), vx, part, odd, t0, limit);
+            ka_wait_reads();
+            if (more) copy(vb, vt);
+        }
+    }
+};
 
 template <typename KT, int D>
 constexpr size_t ka_group_bytes() {
@@ -709,7 +814,6 @@ __device__ __forceinline__ void ka_join(const KaArgs& a, const KaItem& it, KaAcc
 // ---- wide items: 8 waves, 128 columns, 4 tiles of 32 by waves w % 4, the two halves
 // of every 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in
 // LDS that all waves copy together: K and V cross from L2 once for 128 columns.
-constexpr int KA_WIDE_MIN = 64;      // columns from which on
 constexpr int KA_WIDE_COLS = 128, KA_WIDE_KEYS = 64, KA_STAGES = 4, KA_WIDE_PAGES = 4096;
 template <int D>
 constexpr size_t ka_wide_bytes() {
@@ -719,7 +823,7 @@ constexpr size_t ka_wide_bytes() {
 
 template <int D, int XP>
 __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char* lds, int* pages,
-                                        float (*ml)[32][2], const int* limits, int base) {
+                                        float (*ml)[32][2], int* limits, int base) {
     typedef _Float16 KT;
     using T = Ka<KT, D, 32>;
     const pio_kv_cache& c = a.c;
@@ -729,18 +833,13 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
     const int c0 = base + cg * 32;
     const bool has = c0 + col < it.ncols;
     const int r = has ? (c0 + col) / a.G : 0, row = it.row0 + r, head = it.g * a.G + (has ? (c0 + col) - r * a.G : 0);
-    // limits: of the rows from base / G (prefix); else by first_limit
-    int limit = it.k1;
-    if (has) {
-        const int n = limits ? limits[r - base / a.G] : it.first_limit + r;
-        if (!limits || n >= 0) limit = min(n, it.k1);
-    }
-    const int least = ka_wave_min(limit);
+    int limit = it.k1, least = 0;
     KaQ<KT, D, 32, XP> q;
-    ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
+    if constexpr (XP == 1) ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
     KaAcc<KT, D, 32> x;
     x.clear();
     bool bad = it.bad;
+    const uint32_t kx = ka_kx<KT, D, 32>(lane), vx = ka_vx<KT, D, 32>(lane);
 
     const char* kb = ka_base<T::RB>(a, it.g);
     const char* vb = kb + ka_plane<T::RB>(a);
@@ -771,9 +870,20 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
             }
         };
         const int stages = (k1 - k0 + KA_WIDE_KEYS - 1) / KA_WIDE_KEYS;
-        ka_wait_copies<0>();               // q is here: the waits below count copies alone
+        ka_wait_copies<0>();
 #pragma unroll
         for (int s = 0; s < KA_STAGES - 1; s++) copy(s);
+        if (k0 == it.k0) {
+            // under the first copies' way; limits: of the rows from base / G (prefix), else by first_limit
+            if (limits) ka_limits(a, base / a.G, limits, KA_WIDE_COLS);
+            if (has) {
+                const int n = limits ? limits[r - base / a.G] : it.first_limit + r;
+                if (!limits || n >= 0) limit = min(n, it.k1);
+            }
+            least = ka_wave_min(limit);
+            if constexpr (XP == 2) ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
+            ka_wait_copies<0>();           // q is here: the waits below count copies alone
+        }
         for (int s = 0; s < stages; s++) {
             stage_barrier<(KA_STAGES - 2) * 2 * PW>();
             // into the stage that every wave has read before this barrier; past the end the last key again
@@ -785,10 +895,10 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
             const int end = min(limit, k1);
             const bool edge = t0 + T::KEYS > min(least, k1);
             float sc[T::NS];
-            ka_scores<KT, D, 32, XP>(kt, q, lane, sc);
+            ka_scores<KT, D, 32, XP>(ka_addr(kt), kx, q, sc);
             ka_softmax<KT, D, 32>(x, sc, q.cs, t0, end, edge, h);
             const bool odd = edge && ka_odd<KT, D, 32>(vt, lane);
-            ka_values<KT, D, 32, XP>(x, sc, vt, lane, odd, t0, end);
+            ka_values<KT, D, 32, XP>(x, sc, ka_addr(vt), vx, h, odd, t0, end);
         }
     }
     ka_wait_copies<0>();                   // those past the end too: the stages are overwritten
@@ -829,29 +939,28 @@ __device__ __forceinline__ bool ka_prefix(const KaArgs& a, KaItem& it, int& ct) 
     it.row0 = 0;
     it.ncols = a.rows * a.G;
     it.first_limit = 1;
+    it.direct = false;
     const int s = a.seq[0];
     it.bad = s < 0 || s >= a.c.max_seqs;
     it.table = a.c.table + (int64_t)(it.bad ? 0 : s) * a.c.max_pages;
     return true;
 }
-// Run z of the tail of request i; false: it has none.
-__device__ __forceinline__ bool ka_tail(const KaArgs& a, KaItem& it, int i, int g, int z) {
+// A run of a request's tail; false: there is none.
+__device__ __forceinline__ bool ka_tail(const KaArgs& a, KaItem& it, const KaRun& r, int g) {
     it = KaItem{};
-    if (i >= a.n) return false;
-    int r0, r1, keys;
-    ka_rows(a, i, r0, r1);
-    const int s = a.seq[i], L = kv_seq_len(a.c, s);
-    const int runs = ka_tail_runs(a.shared, L, a.tail_splits, keys);
+    if (r.i < 0) return false;
+    const int keys = r.per * KA_ROUND;
     it.g = g;
-    it.k0 = a.shared + z * keys;
-    it.k1 = z < runs ? min(it.k0 + keys, L) : it.k0;
-    it.row0 = r0;
-    it.ncols = max(r1 - r0, 0) * a.G;
-    it.first_limit = L - (r1 - r0) + 1;
-    it.slot = a.pre_splits + z;
-    it.bad = L < 0;
-    it.table = a.c.table + (int64_t)(it.bad ? 0 : s) * a.c.max_pages;
-    return it.ncols > 0 && (a.direct || z < runs);     // (direct: rows without a key, and without a sequence, are written too)
+    it.k0 = a.shared + r.z * keys;
+    it.k1 = max(it.k0, min(it.k0 + keys, r.L));
+    it.row0 = r.r0;
+    it.ncols = (r.r1 - r.r0) * a.G;
+    it.first_limit = r.L - (r.r1 - r.r0) + 1;
+    it.slot = a.pre_splits + r.z;
+    it.bad = r.L < 0;
+    it.direct = r.runs == 1 && a.pre_splits == 0;
+    it.table = a.c.table + (int64_t)(it.bad ? 0 : r.s) * a.c.max_pages;
+    return true;
 }
 
 // Workgroups: the prefix's items, then the tails'.
@@ -872,23 +981,28 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
         if (!ka_prefix(a, it, ct)) return;
         step = INT_MAX / 256;              // one only
         if constexpr (WIDE) {
-            ka_limits(a, ct * KA_WIDE_COLS / a.G, limits, KA_WIDE_COLS);
             ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, limits, ct * KA_WIDE_COLS);
             return;
-        } else {
-            ka_limits(a, ct * KA_COLS / a.G, limits, KA_COLS);
         }
     }
     bool live = true;
     if (!prefix) {
-        // (request, kv head, column tile, run), neighbours in one workgroup
-        int item = ((int)blockIdx.x - a.pre_items) * GROUPS + (GROUPS == 2 ? w8 >> 2 : 0);
-        const int z = item % a.tail_splits;
-        item /= a.tail_splits;
-        ct = item % a.tail_tiles;
-        item /= a.tail_tiles;
+        // (run, column tile, kv head)
+        __shared__ KaRun found[GROUPS];
+        __shared__ int red[8];
+        const int grp = GROUPS == 2 ? w8 >> 2 : 0, per_run = a.tail_tiles * a.c.n_kv_heads;
+        const int item0 = ((int)blockIdx.x - a.pre_items) * GROUPS, item = item0 + grp;
+        int run[GROUPS];
+#pragma unroll
+        for (int k = 0; k < GROUPS; k++) run[k] = (item0 + k) / per_run;
+        ka_runs<GROUPS>(a, run, found, red);
+        const int in_run = item - (GROUPS == 2 && grp ? run[GROUPS - 1] : run[0]) * per_run;
+        ct = in_run / a.c.n_kv_heads;
         step = a.tail_tiles;
-        live = ka_tail(a, it, item / a.c.n_kv_heads, item % a.c.n_kv_heads, z);
+        const KaRun r = found[grp];
+        live = ka_tail(a, it, r, in_run - ct * a.c.n_kv_heads);
+        if (live && !a.direct && it.g == 0 && ct == 0 && r.z == 0)
+            for (int i = tid & 255; i < it.ncols / a.G; i += 256) a.part_n[it.row0 + i] = it.direct ? 0 : r.runs;
     }
     if constexpr (WIDE == 2) {
         // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
@@ -909,12 +1023,17 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
             rounds = max(most[0], most[1]);
         }
         for (int r = 0; r < rounds; r++) {
+            if (r) __syncthreads();        // the last round's output is out of LDS
             const int c0 = (ct + r * step) * KA_COLS, col = c0 + lane % KA_COLS;
             const bool on = live && c0 < it.ncols;
             bool bad = it.bad;
             KaAcc<KT, D, KA_COLS> acc;
             acc.clear();
-            if (on && it.k0 < it.k1) {
+            const bool walks = on && it.k0 < it.k1;
+            KaWalk<KT, D> walk;
+            if (walks) walk.begin(a, it, lds + w * 2 * Ka<KT, D, KA_COLS>::TILE, w, lane);
+            if (WIDE == 0 && prefix) ka_limits(a, c0 / a.G, limits, KA_COLS);
+            if (walks) {
                 const bool has = col < it.ncols;
                 const int q = has ? col / a.G : 0, head = it.g * a.G + (has ? col - q * a.G : 0);
                 int limit = it.k1;
@@ -922,45 +1041,32 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
                     const int n = prefix ? limits[q - c0 / a.G] : it.first_limit + q;
                     if (!prefix || n >= 0) limit = min(n, it.k1);
                 }
-                ka_walk<KT, D, XP>(a, it, lds + w * 2 * Ka<KT, D, KA_COLS>::TILE, w, lane, limit, it.row0 + q, head, has, acc, bad);
+                walk.template run<XP>(a, it, w, lane, limit, it.row0 + q, head, has, acc);
+                bad |= walk.bad;
             }
             if (on && __any(bad) && lane == 0) atomicOr(a.c.work, KV_BAD);
-            if (r) __syncthreads();        // the last round's output is out of LDS
             ka_join<KT, D>(a, it, acc, lds, gml, w, lane, bad, c0, on);
         }
     }
 }
 
-// A column's items joined, one workgroup per column; D / 4 lanes have its dimensions,
-// the groups of them take every such item.
-template <int D>
+// A column's items joined: D / 4 lanes have its dimensions, Z groups of them take
+// every Z-th item, all loads of a few in flight together. Z = 8: few columns, where
+// latency counts; Z = 1: 8 (16) columns to a workgroup.
+template <int D, int Z>
 __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
-    constexpr int TPC = D / 4, Z = 256 / TPC;
-    __shared__ __attribute__((aligned(16))) float so[Z][D];
-    __shared__ float sml[Z][2];
-    __shared__ int req, behind;
-    const pio_kv_cache& c = a.c;
-    const int tid = threadIdx.x, zg = tid / TPC, d = (tid % TPC) * 4, row = blockIdx.x / a.H, head = blockIdx.x - row * a.H;
-    if (tid == 0) req = -1;
-    __syncthreads();
-    for (int i = tid; i < a.n; i += 256) {
-        int r0, r1;
-        ka_rows(a, i, r0, r1);
-        if (row >= r0 && row < r1) {
-            req = i;
-            behind = r1 - row;
-        }
-    }
-    __syncthreads();
-    if (req < 0) return;               // behind the last request
-    const int s = a.seq[req], L = kv_seq_len(c, s);
-    const bool bad = L < 0 || (a.shared > 0 && kv_seq_len(c, a.seq[0]) < 0);
-    int keys;
-    const int runs = bad ? 0 : ka_tail_runs(a.shared, L, a.tail_splits, keys), parts = bad ? 0 : a.pre_splits + runs;
-    const int64_t step = (int64_t)a.rows * a.H, at = (int64_t)blockIdx.x;
+    constexpr int TPC = D / 4, GRP = 256 / TPC, COLS = GRP / Z;
+    __shared__ __attribute__((aligned(16))) float so[GRP][D];
+    __shared__ float sml[GRP][2];
+    const int tid = threadIdx.x, grp = tid / TPC, d = (tid % TPC) * 4, zg = grp % Z;
+    const int64_t at = (int64_t)blockIdx.x * COLS + grp / Z, step = (int64_t)a.rows * a.H;
+    const int row = at < step ? (int)(at / a.H) : a.rows, head = (int)(at - (int64_t)row * a.H);
+    const bool has = row >= a.row_start[0] && row < min(a.row_start[a.n], a.rows);
+    // (0: the row's only item wrote it)
+    const int runs = has ? min(max(a.part_n[row], 0), a.max_runs) : 0, parts = runs ? a.pre_splits + runs : 0;
     float m = -FLT_MAX, l = 0.f;
     ka_f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+#pragma unroll 4
     for (int z = zg; z < parts; z += Z) {
         const ka_f2 ml = *(const ka_f2*)(a.part_ml + 2 * (at + z * step));
         const ka_f4 o = *(const ka_f4*)(a.part_o + (at + z * step) * D + d);
@@ -969,26 +1075,29 @@ __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
         v = v * f + o * fz;
         m = nm;
     }
-    *(ka_f4*)&so[zg][d] = v;
-    if (d == 0) {
-        sml[zg][0] = m;
-        sml[zg][1] = l;
+    if constexpr (Z > 1) {
+        *(ka_f4*)&so[grp][d] = v;
+        if (d == 0) {
+            sml[grp][0] = m;
+            sml[grp][1] = l;
+        }
+        __syncthreads();
+        if (zg) return;
+#pragma unroll
+        for (int z = 1; z < Z; z++) m = fmaxf(m, sml[grp + z][0]);
+        l = 0.f;
+        v = ka_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int z = 0; z < Z; z++) {
+            const float f = __builtin_amdgcn_exp2f(sml[grp + z][0] - m);
+            l += sml[grp + z][1] * f;
+            v += *(const ka_f4*)&so[grp + z][d] * f;
+        }
     }
-    __syncthreads();
-    if (zg) return;
-    for (int z = 1; z < Z; z++) m = fmaxf(m, sml[z][0]);
-    l = 0.f;
-    v = ka_f4{0.f, 0.f, 0.f, 0.f};
-    for (int z = 0; z < Z; z++) {
-        const float f = __builtin_amdgcn_exp2f(sml[z][0] - m);
-        l += sml[z][1] * f;
-        v += *(const ka_f4*)&so[z][d] * f;
-    }
+    if (parts == 0) return;
     v = v / l;
-    if (L - behind + 1 <= 0) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
-    if (bad) v = ka_f4{NAN, NAN, NAN, NAN};
+    if (l == 0.f && m == -FLT_MAX) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
     ka_out(a, D, row, head, d, v);
-    if (bad && tid == 0) atomicOr(c.work, KV_BAD);
 }
 
 template <typename KT, int D, int XP, int WIDE>
@@ -996,12 +1105,16 @@ static int ka_launch(const KaArgs& a, hipStream_t st) {
     constexpr int GROUPS = WIDE == 1 ? 2 : 1;
     size_t lds = ka_group_bytes<KT, D>();
     if constexpr (WIDE) lds = ka_wide_bytes<D>() + KA_WIDE_PAGES * sizeof(int);
-    const int64_t tails = (int64_t)a.n * a.c.n_kv_heads * a.tail_tiles * a.tail_splits;
+    // the aimed at runs, and up to one more for each request
+    const int64_t tails = (int64_t)(a.direct ? a.n : a.n + a.tail_runs) * a.c.n_kv_heads * a.tail_tiles;
     PIO_TRY((allow_lds<ka_kernel<KT, D, XP, WIDE>>(lds)));
     ka_kernel<KT, D, XP, WIDE><<<(unsigned)(a.pre_items + (tails + GROUPS - 1) / GROUPS), WIDE ? 512 : 256, lds, st>>>(a);
     PIO_LAUNCHED();
     if (!a.direct) {
-        ka_merge_kernel<D><<<a.rows * a.H, 256, 0, st>>>(a);
+        constexpr int GRP = 1024 / D;
+        const int cols = a.rows * a.H;
+        if (cols <= 2048) ka_merge_kernel<D, 8><<<ceil_div(cols, GRP / 8), 256, 0, st>>>(a);
+        else ka_merge_kernel<D, 1><<<ceil_div(cols, GRP), 256, 0, st>>>(a);
         PIO_LAUNCHED();
     }
     return PIO_OK;
@@ -1024,30 +1137,42 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
     const bool f16 = a.c.kv_dtype == PIO_F16;
     const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
-    const int wide = !f16 ? 0 : tail_cols > KA_WIDE_MIN ? 2 : a.shared > 0 && cols > KA_WIDE_MIN ? 1 : 0;
+    const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : a.shared > 0 && cols > 64 ? 1 : 0;
+    a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
+    const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
+    PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
+    // tails: as many runs as the device holds at once, in all and of one request (up to one
+    // more for each request comes on top)
+    const int groups = wide == 2 ? cus : 2 * cus;
+    const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
+    const int64_t runs = groups / ((int64_t)Hk * a.tail_tiles);
+    a.tail_runs = (int)std::max<int64_t>({1, runs - a.n, runs / 2});
+    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND)});
+    a.direct = a.shared == 0 && a.max_runs == 1;
     if (a.shared > 0) {
         // prefix: as many items as the device holds at once, each of at least KA_ROUND keys
-        const int width = wide ? KA_WIDE_COLS : KA_COLS, at_once = wide ? cus : 2 * cus;
+        const int width = wide ? KA_WIDE_COLS : KA_COLS;
+        int at_once = wide ? cus : 2 * cus;
+        if (wide == 1) {
+            // CUs kept free for the tails, 5 us a workgroup of them beside the prefix's time at 700 TFLOP/s
+            const double pre_us = 4.0 * a.c.head_dim * a.H * a.rows * a.shared * (a.q16 ? 1 : 2) / 700e6;
+            at_once -= (int)std::min<double>(cus / 3, items / 2 * 5.0 / pre_us);
+        }
         a.pre_tiles = ceil_div(cols, width);
         const int64_t splits = std::max<int64_t>(1, at_once / std::max<int64_t>(1, (int64_t)Hk * a.pre_tiles));
         a.pre_keys = ceil_div(ceil_div(a.shared, std::min<int64_t>(splits, a.shared)), KA_ROUND) * KA_ROUND;
         a.pre_splits = ceil_div(a.shared, a.pre_keys);
-        const int64_t items = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
-        PIO_REQUIRE(items <= INT_MAX / 2, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
-        a.pre_items = (int)items;
+        const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
+        PIO_REQUIRE(pre <= INT_MAX / 2, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
+        a.pre_items = (int)pre;
     }
-    a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
-    const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
-    PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
-    const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    a.tail_splits = (int)std::max<int64_t>(1, std::min<int64_t>({4 * cus / items, 32, ceil_div(longest, KA_ROUND)}));
-    a.direct = a.shared == 0 && a.tail_splits == 1;
     Scratch ws;
     if (!a.direct) {
-        const size_t parts = (size_t)(a.pre_splits + a.tail_splits) * a.rows * a.H;
-        PIO_TRY(ws.get(parts * (a.c.head_dim + 2) * sizeof(float), st));
+        const size_t parts = (size_t)(a.pre_splits + a.max_runs) * a.rows * a.H;
+        PIO_TRY(ws.get(parts * (a.c.head_dim + 2) * sizeof(float) + a.rows * sizeof(int), st));
         a.part_o = (float*)ws.ptr;
         a.part_ml = a.part_o + parts * a.c.head_dim;
+        a.part_n = (int*)(a.part_ml + 2 * parts);
     }
     return a.c.head_dim == 128 ? ka_route<128>(a, wide, st) : ka_route<64>(a, wide, st);
 }

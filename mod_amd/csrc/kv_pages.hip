@@ -50,8 +50,8 @@ int kv_check(const pio_kv_cache* c, const char* what) {
                 "%s: head_dim %d (a multiple of 8 up to 256)", what, c->head_dim);
     PIO_REQUIRE(c->page_size >= 1 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0,
                 "%s: page_size %d (a power of two up to 1024)", what, c->page_size);
-    // positions, and the pages that a plan's 1024 requests need, are counted in 32 bits
-    PIO_REQUIRE((int64_t)c->max_pages * c->page_size <= INT_MAX, "%s: table rows of over 2^31 positions", what);
+    // positions, and the pages or rounds of keys that 1024 requests need, are counted in 32 bits
+    PIO_REQUIRE((int64_t)c->max_pages * c->page_size <= 1 << 28, "%s: table rows of over 2^28 positions", what);
     PIO_REQUIRE(c->n_pages <= 1 << 20 && c->max_seqs <= 1 << 20 && c->max_pages <= 1 << 20,
                 "%s: over 2^20 pages, sequences or pages of a sequence", what);
     PIO_REQUIRE((int64_t)c->n_kv_heads * c->head_dim <= 1 << 20, "%s: n_kv_heads x head_dim over 2^20", what);

@@ -24,7 +24,7 @@ BAD_CACHES = [
     (dict(head_dim=264), "head_dim"), (dict(page_size=0), "page_size"), (dict(page_size=24), "page_size"),
     (dict(page_size=2048), "page_size"), (dict(kv=4104), "16-byte"), (dict(table=4098), "4-byte"),
     (dict(refs=4097), "4-byte"), (dict(n_pages=(1 << 20) + 1), "2\\^20"), (dict(max_pages=(1 << 20) + 1), "2\\^20"),
-    (dict(max_pages=1 << 20, page_size=1024 * 2), "page_size"), (dict(max_seqs=1 << 21), "2\\^20"),
+    (dict(max_pages=1 << 20, page_size=1024), "2\\^28"), (dict(max_seqs=1 << 21), "2\\^20"),
     (dict(n_kv_heads=1 << 18), "n_kv_heads"),
 ]
 
