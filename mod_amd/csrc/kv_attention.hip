@@ -148,9 +148,11 @@ typedef __attribute__((address_space(3))) void ka_lds_t;
 typedef __attribute__((address_space(3))) ka_p4 ka_lds_p4;
 
 constexpr float KA_LOG2E = 1.44269504088896340736f;
-// fp16 weights are held times 2^10, so that those down to 2^-24 of the largest are normal
-// numbers; the sum is scaled alike.
-constexpr float KA_LIFT = 10.f;
+// A column's reference (the exponent that its weights are relative to) follows its
+// maximum only when that has grown by KA_SLACK: rescaling O^T for every new maximum of 32
+// columns cost as much as a tile's exponentials. fp16 weights are held times 2^10, so that they
+// stay below 2^15, and are normal numbers down to 2^-24 of the reference.
+constexpr float KA_LIFT = 10.f, KA_SLACK = 5.f;
 // Least maximum of a column that sees a key; one that sees none keeps -FLT_MAX.
 constexpr float KA_SEEN = -3.4e38f;
 constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column's largest is 2^12 .. 2^13
@@ -160,8 +162,10 @@ constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column'
 //   S^T: accumulator e of part q is key COLS * (e / E) + sub(e % E, q)
 //   O^T: NT tiles of COLS dimensions
 // A row of the cache is RB bytes in 16-byte chunks; in LDS, slot s of row r holds
-// chunk s ^ swz(r), so that 16 consecutive rows' reads of one chunk fall into
-// different banks.
+// chunk s ^ swz(r), a permutation of the row's 4 low bits: 16 consecutive rows' reads
+// of one chunk (K) fall into different banks, and so do 4 or 8 rows' reads of 2 or 4
+// neighbouring chunks (V, transposed), whose rows differ in the low bits: those go
+// to the slot's high ones (the plain r & 15 put 4 rows on the same banks).
 template <typename KT, int D, int COLS_>
 struct Ka {
     static constexpr bool F16 = sizeof(KT) == 2;
@@ -178,7 +182,9 @@ struct Ka {
     static constexpr int QC = SL / PL;                 // operand chunks of a lane in a score
     static constexpr int OP = D + 4;                   // LDS pitch of a column's output (floats)
     typedef typename std::conditional<COLS == 32, ka_v16, ka_f4>::type Acc;
-    __device__ static int swz(int r) { return RB == 128 ? (r >> 1) & 7 : r & 15; }
+    __device__ static int swz(int r) {
+        return RB == 128 ? (r << 1 & 4) | (r >> 1 & 2) | (r >> 3 & 1) : (r << 2 & 12) | (r >> 1 & 2) | (r >> 3 & 1);
+    }
     __device__ static int slot(int r, int chunk) { return r * RB + ((chunk ^ swz(r)) << 4); }
     // row of a COLS x COLS accumulator tile that element e of part q is
     __device__ static int sub(int e, int q) { return COLS == 32 ? 8 * (e >> 2) + 4 * q + (e & 3) : 4 * q + e; }
@@ -227,7 +233,9 @@ template <typename KT, int D, int COLS, int XP>
 __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bool live, int part, KaQ<KT, D, COLS, XP>& q) {
     using T = Ka<KT, D, COLS>;
     const int64_t at = live ? row * a.q_stride + (int64_t)head * D : 0;
-    q.cs = a.scale * KA_LOG2E;
+    // (a maximum of scores is one of their products with it; a masked score, -inf, times it is -inf)
+    q.cs = fmaxf(fabsf(a.scale) * KA_LOG2E, FLT_MIN);
+    const bool neg = a.scale < 0.f;
     if constexpr (!T::F16) {
 #pragma unroll
         for (int c = 0; c < T::QC; c++) {
@@ -238,12 +246,14 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
             } else {
                 q.f[c] = *(const ka_f4*)((const float*)a.q + e0);
             }
+            if (neg) q.f[c] = -q.f[c];
             if (!live) q.f[c] = ka_f4{0.f, 0.f, 0.f, 0.f};
         }
     } else if constexpr (XP == 1) {
 #pragma unroll
         for (int c = 0; c < T::QC; c++) {
             q.h[0][c] = *(const ka_h8*)((const _Float16*)a.q + at + 8 * (T::PL * c + part));
+            if (neg) q.h[0][c] = -q.h[0][c];
             if (!live) q.h[0][c] = ka_h8{0, 0, 0, 0, 0, 0, 0, 0};
         }
     } else {
@@ -267,12 +277,12 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
         for (int c = 0; c < T::QC; c++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float v = ldexpf(x[c][e], ex);
+                const float v = ldexpf(neg ? -x[c][e] : x[c][e], ex);
                 const _Float16 hi = (_Float16)v;
                 q.h[0][c][e] = hi;
                 q.h[XP - 1][c][e] = (_Float16)(v - (float)hi);
             }
-        q.cs = odd > 0.f ? NAN : ldexpf(q.cs, -ex);
+        q.cs = odd > 0.f ? NAN : fmaxf(ldexpf(q.cs, -ex), FLT_MIN);
     }
 }
 
@@ -280,9 +290,12 @@ __device__ __forceinline__ void ka_load_q(const KaArgs& a, int row, int head, bo
 // XORs, so all are (x ^ constant) + base + constant, one instruction from one
 // register; opaque in the loop, or the compiler would hold each in a register.
 typedef __attribute__((address_space(3))) char ka_lds_c;
-__device__ __forceinline__ uint32_t ka_addr(const char* p) { return (uint32_t)(uintptr_t)(ka_lds_c*)p; }
+// (offsets from the LDS array's own name: with an address of unknown origin the
+// compiler waits for every copy in flight before each read)
+extern __shared__ __attribute__((aligned(256))) char ka_lds[];
 template <typename V>
-__device__ __forceinline__ V ka_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)(uintptr_t)at; }
+__device__ __forceinline__ V ka_read(uint32_t at) { return *(const __attribute__((address_space(3))) V*)((ka_lds_c*)ka_lds + at); }
+__device__ __forceinline__ uint32_t ka_addr(const char* p) { return (uint32_t)(p - ka_lds); }
 __device__ __forceinline__ uint32_t ka_opaque(uint32_t x) {
     asm volatile("" : "+v"(x));
     return x;
@@ -299,24 +312,32 @@ __device__ __forceinline__ uint32_t ka_vx(int lane) {
     else return T::slot(4 * part, i);
 }
 
-// S^T of one tile; kt: K's rows in LDS.
-template <typename KT, int D, int COLS, int XP>
-__device__ __forceinline__ void ka_scores(uint32_t kt, uint32_t kx, const KaQ<KT, D, COLS, XP>& q,
-                                          float (&s)[Ka<KT, D, COLS>::NS]) {
+// S^T of one tile: K's operands (rows at kt), all reads in flight together, and the products.
+template <typename KT, int D, int COLS>
+struct KaKeysOf {
     using T = Ka<KT, D, COLS>;
     typedef typename std::conditional<T::F16, ka_h8, ka_f4>::type K;
-    kx = ka_opaque(kx);
+    K k[T::ST][T::QC];
+    __device__ __forceinline__ void read(uint32_t kt, uint32_t kx) {
+        kx = ka_opaque(kx);
+#pragma unroll
+        for (int st = 0; st < T::ST; st++)
+#pragma unroll
+            for (int i = 0; i < T::QC; i++) k[st][i] = ka_read<K>((kx ^ (T::PL * i << 4)) + kt + st * COLS * T::RB);
+    }
+};
+template <typename KT, int D, int COLS, int XP>
+__device__ __forceinline__ void ka_scores(const KaKeysOf<KT, D, COLS>& k, const KaQ<KT, D, COLS, XP>& q,
+                                          float (&s)[Ka<KT, D, COLS>::NS]) {
+    using T = Ka<KT, D, COLS>;
 #pragma unroll
     for (int st = 0; st < T::ST; st++) {
-        K k[T::QC];                    // all reads in flight together
-#pragma unroll
-        for (int i = 0; i < T::QC; i++) k[i] = ka_read<K>((kx ^ (T::PL * i << 4)) + kt + st * COLS * T::RB);
         if constexpr (T::F16) {
             typename T::Acc c = T::zero();
 #pragma unroll
             for (int i = 0; i < T::QC; i++) {
-                c = T::mfma(k[i], q.h[0][i], c);
-                if constexpr (XP == 2) c = T::mfma(k[i], q.h[XP - 1][i], c);
+                c = T::mfma(k.k[st][i], q.h[0][i], c);
+                if constexpr (XP == 2) c = T::mfma(k.k[st][i], q.h[XP - 1][i], c);
             }
 #pragma unroll
             for (int e = 0; e < T::E; e++) s[st * T::E + e] = c[e];
@@ -327,7 +348,7 @@ __device__ __forceinline__ void ka_scores(uint32_t kt, uint32_t kx, const KaQ<KT
 #pragma unroll
             for (int i = 0; i < T::QC; i++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[i][e], q.f[i][e], c[e], 0, 0, 0);
+                for (int e = 0; e < 4; e++) c[e] = __builtin_amdgcn_mfma_f32_16x16x4f32(k.k[st][i][e], q.f[i][e], c[e], 0, 0, 0);
 #pragma unroll
             for (int e = 0; e < 4; e++) s[e] = (c[0][e] + c[1][e]) + (c[2][e] + c[3][e]);
         }
@@ -343,9 +364,9 @@ __device__ __forceinline__ ka_h8 ka_vt(uint32_t vt, uint32_t vx, int n, int kc) 
 #pragma unroll
     for (int b = 0; b < 2; b++) {
         // 32 columns: the second 4 keys are 8 rows on, another swizzle; 16 columns: 16 rows, the same
-        const uint32_t flip = COLS == 32 ? b * (T::RB == 128 ? 4 : 8) << 4 : 0;
+        const uint32_t flip = COLS == 32 ? b << 4 : 0;
         const uint32_t at = (vx ^ ((COLS / 8 * n << 4) ^ flip)) + vt + (16 * kc + (COLS == 32 ? 8 : 16) * b) * T::RB;
-        const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)(uintptr_t)at);
+        const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)((ka_lds_c*)ka_lds + at));
 #pragma unroll
         for (int e = 0; e < 4; e++) v[4 * b + e] = (_Float16)r[e];
     }
@@ -369,7 +390,7 @@ __device__ __forceinline__ bool ka_odd(const char* vt, int lane) {
     return __any(odd);
 }
 
-// A column's running softmax: (max, sum) in base 2, O^T.
+// A column's running softmax: (reference, sum) in base 2, O^T.
 template <typename KT, int D, int COLS>
 struct KaAcc {
     float m, l;
@@ -382,25 +403,25 @@ struct KaAcc {
     }
 };
 
-// Scores -> weights (in s), and the running maximum and sum. The tile's keys
-// from t0; edge (wave-uniform): some column does not see all of them.
+// Scores -> weights (in s), and the running reference and sum, in two steps: the
+// reference, then the exponentials. The tile's keys from t0; edge (wave-uniform):
+// some column does not see all of them.
 template <typename KT, int D, int COLS>
-__device__ __forceinline__ void ka_softmax(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs, int t0,
-                                           int limit, bool edge, int part) {
+__device__ __forceinline__ void ka_reference(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs, int t0,
+                                             int limit, bool edge, int part) {
     using T = Ka<KT, D, COLS>;
-    constexpr float lift = T::F16 ? KA_LIFT : 0.f;
-#pragma unroll
-    for (int e = 0; e < T::NS; e++) s[e] *= cs;
     if (edge) {
+        const int left = ka_opaque(limit - t0 - T::key(0, part));      // (in this branch alone, not hoisted out of it)
 #pragma unroll
-        for (int e = 0; e < T::NS; e++) s[e] = t0 + T::key(e, part) < limit ? s[e] : -INFINITY;
+        for (int e = 0; e < T::NS; e++) s[e] = T::key(e, 0) < left ? s[e] : -INFINITY;
     }
-    float top = fmaxf(x.m, t0 < limit ? KA_SEEN : -FLT_MAX);
+    float top = s[0];
 #pragma unroll
-    for (int e = 0; e < T::NS; e++) top = fmaxf(top, s[e]);
-    const float m = ka_max<COLS>(top);
-    if (__any(m != x.m)) {
-        const float corr = __builtin_amdgcn_exp2f(x.m - m);
+    for (int e = 1; e < T::NS; e++) top = fmaxf(top, s[e]);
+    // (a score of -inf, and one times no scale, are no numbers to compare with)
+    top = ka_max<COLS>(fmaxf(top * cs, t0 < limit ? KA_SEEN : -FLT_MAX));
+    if (__any(top > x.m + KA_SLACK)) {
+        const float m = fmaxf(x.m, top), corr = __builtin_amdgcn_exp2f(x.m - m);
         x.l *= corr;
 #pragma unroll
         for (int n = 0; n < T::NT; n++)
@@ -408,11 +429,15 @@ __device__ __forceinline__ void ka_softmax(KaAcc<KT, D, COLS>& x, float (&s)[Ka<
             for (int e = 0; e < T::E; e++) x.o[n][e] *= corr;
         x.m = m;
     }
-    const float base = m - lift;
+}
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ void ka_weights(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs) {
+    using T = Ka<KT, D, COLS>;
+    const float base = (T::F16 ? KA_LIFT : 0.f) - x.m;
     float sum[T::NS];
 #pragma unroll
     for (int e = 0; e < T::NS; e++) {
-        s[e] = __builtin_amdgcn_exp2f(s[e] - base);     // -inf: 0 (the maximum is finite, or the scores are no numbers)
+        s[e] = __builtin_amdgcn_exp2f(fmaf(s[e], cs, base));
         sum[e] = s[e];
     }
 #pragma unroll
@@ -431,7 +456,7 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p
     using T = Ka<KT, D, COLS>;
     vx = ka_opaque(vx);
     auto row = [&](int e, int half) {      // fp32: 4 dimensions of the key of score e
-        return ka_read<ka_f4>((vx ^ ((e ^ 16 * half) << 4)) + vt + e * T::RB);
+        return ka_read<ka_f4>((vx ^ ((4 * e ^ 16 * half) << 4)) + vt + e * T::RB);
     };
     auto product = [&](auto finite) {
         if constexpr (T::F16) {
@@ -752,14 +777,17 @@ struct KaWalk {
             const bool more = j + 4 < tiles, edge = t0 + T::KEYS > least;
             ka_wait_copies<T::NI>();
             float s[T::NS];
-            ka_scores<KT, D, KA_COLS, XP>(ka_addr(kt), kx, q, s);
+            KaKeysOf<KT, D, KA_COLS> k;
+            k.read(ka_addr(kt), kx);
+            ka_scores<KT, D, KA_COLS, XP>(k, q, s);
             ka_wait_reads();
             if (more) {
                 offsets(lane);
                 copy(kb, kt);
                 next = key_row(a, it, j + 8, lane);
             }
-            ka_softmax<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
+            ka_reference<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
+            ka_weights<KT, D, KA_COLS>(x, s, q.cs);
             if (more) ka_wait_copies<T::NI + 1>();
             else ka_wait_copies<0>();
             const bool odd = edge && ka_odd<KT, D, KA_COLS>(vt, lane);
@@ -884,21 +912,45 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
             if constexpr (XP == 2) ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
             ka_wait_copies<0>();           // q is here: the waits below count copies alone
         }
-        for (int s = 0; s < stages; s++) {
+        // The scores run one stage ahead of the softmax: their products fill the matrix cores
+        // while the exponentials fill the VALU. (A workgroup's waves pass the barriers together,
+        // and so do not cover each other.) Two parts of 128 dimensions leave no registers for it.
+        constexpr bool AHEAD = XP == 1 || D < 128;
+        auto tile = [&](int s) { return ka_addr(lds + (s % KA_STAGES) * STAGE + kg * T::TILE); };
+        KaKeysOf<KT, D, 32> k;
+        float sc[T::NS], next[T::NS];
+        if constexpr (AHEAD) {
             stage_barrier<(KA_STAGES - 2) * 2 * PW>();
+            k.read(tile(0), kx);
+            ka_scores<KT, D, 32, XP>(k, q, sc);
+        }
+        for (int s = 0; s < stages; s++) {
+            stage_barrier<(KA_STAGES - (AHEAD ? 3 : 2)) * 2 * PW>();
             // into the stage that every wave has read before this barrier; past the end the last key again
             copy(s + KA_STAGES - 1);
-            const char* kt = lds + (s % KA_STAGES) * STAGE + kg * T::TILE;
-            const char* vt = kt + KA_WIDE_KEYS * T::RB;
+            k.read(tile(AHEAD ? s + 1 : s), kx);
+            if constexpr (!AHEAD) ka_scores<KT, D, 32, XP>(k, q, sc);
             const int t0 = k0 + s * KA_WIDE_KEYS + kg * T::KEYS;
             // (a chunk's end is not the item's: keys behind it come with the next chunk)
             const int end = min(limit, k1);
             const bool edge = t0 + T::KEYS > min(least, k1);
-            float sc[T::NS];
-            ka_scores<KT, D, 32, XP>(ka_addr(kt), kx, q, sc);
-            ka_softmax<KT, D, 32>(x, sc, q.cs, t0, end, edge, h);
-            const bool odd = edge && ka_odd<KT, D, 32>(vt, lane);
-            ka_values<KT, D, 32, XP>(x, sc, ka_addr(vt), vx, h, odd, t0, end);
+            ka_reference<KT, D, 32>(x, sc, q.cs, t0, end, edge, h);
+            ka_weights<KT, D, 32>(x, sc, q.cs);
+            if constexpr (AHEAD) {
+                ka_scores<KT, D, 32, XP>(k, q, next);
+#pragma unroll
+                for (int i = 0; i < T::QC * XP; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                   // a product
+                    __builtin_amdgcn_sched_group_barrier(0x402, 64 / (T::QC * XP), 0);   // its share of the VALU's work
+                }
+            }
+            const uint32_t vt = tile(s) + KA_WIDE_KEYS * T::RB;
+            const bool odd = edge && ka_odd<KT, D, 32>(lds + vt, lane);
+            ka_values<KT, D, 32, XP>(x, sc, vt, vx, h, odd, t0, end);
+            if constexpr (AHEAD) {
+#pragma unroll
+                for (int e = 0; e < T::NS; e++) sc[e] = next[e];
+            }
         }
     }
     ka_wait_copies<0>();                   // those past the end too: the stages are overwritten
@@ -970,7 +1022,6 @@ __device__ __forceinline__ bool ka_tail(const KaArgs& a, KaItem& it, const KaRun
 template <typename KT, int D, int XP, int WIDE>
 __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
     constexpr int GROUPS = WIDE == 1 ? 2 : 1;
-    extern __shared__ __attribute__((aligned(16))) char ka_lds[];
     __shared__ float ml[WIDE ? 8 * 32 * 2 : 4 * KA_COLS * 2];
     __shared__ int limits[WIDE ? KA_WIDE_COLS : KA_COLS];
     const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3;
@@ -1146,7 +1197,8 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int groups = wide == 2 ? cus : 2 * cus;
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
     const int64_t runs = groups / ((int64_t)Hk * a.tail_tiles);
-    a.tail_runs = (int)std::max<int64_t>({1, runs - a.n, runs / 2});
+    // (with 8 waves a workgroup, those beyond one a CU wait for a second round)
+    a.tail_runs = (int)std::max<int64_t>({1, runs - (wide ? a.n : 0), runs / 2});
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND)});
     a.direct = a.shared == 0 && a.max_runs == 1;
     if (a.shared > 0) {

@@ -394,6 +394,21 @@ def test_attention_large_scores(torch, ops):
         assert np.isfinite(got.astype(np.float64)).all()
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1e-30, 3.0])
+def test_attention_scales(torch, ops, scale):
+    """No scale (the mean over what a row sees), a negative one, a tiny and a large one."""
+    for kv, x in [("float32", "float32"), ("float16", "float32"), ("float16", "float16")]:
+        for D, G in [(64, 2), (128, 20)]:
+            rng = np.random.default_rng(12)
+            p = Pair(torch, ops, 1, 2, D, 16, 60, 5, 20, kv, fill=np.nan)
+            _prefix(p, rng, 3, 150, [30, 1, 77])
+            seq, start = [1, 2, 3], [0, 2, 3, 6]
+            q = rng.standard_normal((6, 2 * G, D)).astype(x)
+            ref = p.ref.attention(0, seq, start, q, scale, np.zeros(q.shape))
+            got = _attend(p, torch, ops, 0, seq, start, q, scale, 150, 3)
+            assert np.abs(got.astype(np.float64) - ref).max() <= _tolerance(p, 0, seq, start, q, scale, x == "float16")
+
+
 def test_attention_strides_and_in_place(torch, ops):
     rng = np.random.default_rng(10)
     p = Pair(torch, ops, 1, 2, 64, 16, 30, 5, 10, "float16")
