@@ -161,11 +161,12 @@ constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column'
 // column l % COLS and is one of PL = 64 / COLS parts q = l / COLS of it.
 //   S^T: accumulator e of part q is key COLS * (e / E) + sub(e % E, q)
 //   O^T: NT tiles of COLS dimensions
-// A row of the cache is RB bytes in 16-byte chunks; in LDS, slot s of row r holds
-// chunk s ^ swz(r), a permutation of the row's 4 low bits: 16 consecutive rows' reads
-// of one chunk (K) fall into different banks, and so do 4 or 8 rows' reads of 2 or 4
-// neighbouring chunks (V, transposed), whose rows differ in the low bits: those go
-// to the slot's high ones (the plain r & 15 put 4 rows on the same banks).
+// A row of the cache is RB bytes in 16-byte chunks. In LDS a tile is RB / 128 blocks of
+// KEYS rows of 128 bytes (a copy instruction fills 8 of them: whole lines of 8 rows),
+// where slot s of row r holds chunk s ^ swz(r), a permutation of the bits of r above the
+// lowest: 16 consecutive rows' reads of one chunk (K) fall into different banks, and so do
+// 4 or 8 rows' reads of 4 or 2 neighbouring chunks (V, transposed; the plain bits in order
+// would put such rows on the same banks).
 template <typename KT, int D, int COLS_>
 struct Ka {
     static constexpr bool F16 = sizeof(KT) == 2;
@@ -175,17 +176,18 @@ struct Ka {
     static constexpr int ST = KEYS / COLS;             // S^T tiles
     static constexpr int NS = ST * E;                  // a lane's scores
     static constexpr int NT = D / COLS;
-    static constexpr int RB = D * (int)sizeof(KT), SL = RB / 16;
-    static constexpr int RPI = 64 / SL;                // rows of one copy instruction
-    static constexpr int NI = KEYS / RPI;              // copies of a tile of K (or V)
-    static constexpr int TILE = KEYS * RB;             // bytes
-    static constexpr int QC = SL / PL;                 // operand chunks of a lane in a score
+    static constexpr int RB = D * (int)sizeof(KT), CB = RB / 128;
+    static constexpr int NB = KEYS / 8;                // groups of 8 rows: CB copies each of a tile of K (or V)
+    static constexpr int NI = NB * CB;
+    static constexpr int BLOCK = KEYS * 128, TILE = CB * BLOCK;    // bytes
+    static constexpr int QC = RB / 16 / PL;            // operand chunks of a lane in a score
     static constexpr int OP = D + 4;                   // LDS pitch of a column's output (floats)
     typedef typename std::conditional<COLS == 32, ka_v16, ka_f4>::type Acc;
-    __device__ static int swz(int r) {
-        return RB == 128 ? (r << 1 & 4) | (r >> 1 & 2) | (r >> 3 & 1) : (r << 2 & 12) | (r >> 1 & 2) | (r >> 3 & 1);
-    }
-    __device__ static int slot(int r, int chunk) { return r * RB + ((chunk ^ swz(r)) << 4); }
+    __device__ static int swz(int r) { return (r << 1 & 4) | (r >> 1 & 2) | (r >> 3 & 1); }
+    __device__ static int slot(int r, int chunk) { return (chunk >> 3) * BLOCK + r * 128 + (((chunk & 7) ^ swz(r)) << 4); }
+    // where chunk c of a row lies beside the row's chunk 0 (c a multiple of what lanes add): XOR and offset
+    static constexpr uint32_t flip(int c) { return (c & 7) << 4; }
+    static constexpr uint32_t block(int c) { return (c >> 3) * BLOCK; }
     // row of a COLS x COLS accumulator tile that element e of part q is
     __device__ static int sub(int e, int q) { return COLS == 32 ? 8 * (e >> 2) + 4 * q + (e & 3) : 4 * q + e; }
     // key of score i of part q
@@ -323,7 +325,8 @@ struct KaKeysOf {
 #pragma unroll
         for (int st = 0; st < T::ST; st++)
 #pragma unroll
-            for (int i = 0; i < T::QC; i++) k[st][i] = ka_read<K>((kx ^ (T::PL * i << 4)) + kt + st * COLS * T::RB);
+            for (int i = 0; i < T::QC; i++)
+                k[st][i] = ka_read<K>((kx ^ T::flip(T::PL * i)) + kt + T::block(T::PL * i) + st * COLS * 128);
     }
 };
 template <typename KT, int D, int COLS, int XP>
@@ -355,23 +358,69 @@ __device__ __forceinline__ void ka_scores(const KaKeysOf<KT, D, COLS>& k, const 
     }
 }
 
-// A lane's 8 values of V^T (O^T tile n, key group kc): one dimension, the keys of
-// scores 8 kc .. 8 kc + 7.
-template <int D, int COLS>
-__device__ __forceinline__ ka_h8 ka_vt(uint32_t vt, uint32_t vx, int n, int kc) {
-    using T = Ka<_Float16, D, COLS>;
-    ka_h8 v;
-#pragma unroll
-    for (int b = 0; b < 2; b++) {
-        // 32 columns: the second 4 keys are 8 rows on, another swizzle; 16 columns: 16 rows, the same
-        const uint32_t flip = COLS == 32 ? b << 4 : 0;
-        const uint32_t at = (vx ^ ((COLS / 8 * n << 4) ^ flip)) + vt + (16 * kc + (COLS == 32 ? 8 : 16) * b) * T::RB;
-        const ka_p4 r = __builtin_amdgcn_ds_read_tr16_b64_v4f16((ka_lds_p4*)((ka_lds_c*)ka_lds + at));
-#pragma unroll
-        for (int e = 0; e < 4; e++) v[4 * b + e] = (_Float16)r[e];
-    }
-    return v;
+// Pairs of transposed reads, OFF bytes apart, from each address, and the wait for them in
+// one piece: the compiler cannot tell what a transposed read does not alias, and would wait
+// for every copy in flight before the first (a round trip to memory in every tile).
+template <int OFF>
+__device__ __forceinline__ void ka_read_tr(const uint32_t (&a)[4], ka_p4 (&r)[4][2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %8\n ds_read_b64_tr_b16 %1, %8 offset:%12\n"
+                 "ds_read_b64_tr_b16 %2, %9\n ds_read_b64_tr_b16 %3, %9 offset:%12\n"
+                 "ds_read_b64_tr_b16 %4, %10\n ds_read_b64_tr_b16 %5, %10 offset:%12\n"
+                 "ds_read_b64_tr_b16 %6, %11\n ds_read_b64_tr_b16 %7, %11 offset:%12\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]),
+                   "=&v"(r[3][0]), "=&v"(r[3][1])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "n"(OFF));
 }
+template <int OFF>
+__device__ __forceinline__ void ka_read_tr(const uint32_t (&a)[8], ka_p4 (&r)[8][2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %16\n ds_read_b64_tr_b16 %1, %16 offset:%24\n"
+                 "ds_read_b64_tr_b16 %2, %17\n ds_read_b64_tr_b16 %3, %17 offset:%24\n"
+                 "ds_read_b64_tr_b16 %4, %18\n ds_read_b64_tr_b16 %5, %18 offset:%24\n"
+                 "ds_read_b64_tr_b16 %6, %19\n ds_read_b64_tr_b16 %7, %19 offset:%24\n"
+                 "ds_read_b64_tr_b16 %8, %20\n ds_read_b64_tr_b16 %9, %20 offset:%24\n"
+                 "ds_read_b64_tr_b16 %10, %21\n ds_read_b64_tr_b16 %11, %21 offset:%24\n"
+                 "ds_read_b64_tr_b16 %12, %22\n ds_read_b64_tr_b16 %13, %22 offset:%24\n"
+                 "ds_read_b64_tr_b16 %14, %23\n ds_read_b64_tr_b16 %15, %23 offset:%24\n"
+                 "s_waitcnt lgkmcnt(0)"
+                 : "=&v"(r[0][0]), "=&v"(r[0][1]), "=&v"(r[1][0]), "=&v"(r[1][1]), "=&v"(r[2][0]), "=&v"(r[2][1]),
+                   "=&v"(r[3][0]), "=&v"(r[3][1]), "=&v"(r[4][0]), "=&v"(r[4][1]), "=&v"(r[5][0]), "=&v"(r[5][1]),
+                   "=&v"(r[6][0]), "=&v"(r[6][1]), "=&v"(r[7][0]), "=&v"(r[7][1])
+                 : "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(a[4]), "v"(a[5]), "v"(a[6]), "v"(a[7]), "n"(OFF));
+}
+
+// V^T of one tile as operands (rows at vt): of O^T tile n and key group kc, a lane's 8
+// values of one dimension, the keys of scores 8 kc .. 8 kc + 7.
+template <int D, int COLS>
+struct KaValuesOf {
+    using T = Ka<_Float16, D, COLS>;
+    static constexpr int KC = T::NS / 8;
+    ka_h8 v[T::NT][KC];
+    __device__ __forceinline__ void read(uint32_t vt, uint32_t vx) {
+        vx = ka_opaque(vx);
+        vt += (uint32_t)(uintptr_t)(ka_lds_c*)ka_lds;
+        // 16 lanes read 16 dimensions of 4 keys. 32 columns: an operand's second 4 keys are 8 rows on, with another
+        // swizzle, the second key group 16; 16 columns: the second 4 keys 16 rows on
+        constexpr int B = COLS == 32 ? 2 : 1;
+        uint32_t a[T::NT * B];
+        ka_p4 r[T::NT * B][2];
+#pragma unroll
+        for (int n = 0; n < T::NT; n++)
+#pragma unroll
+            for (int b = 0; b < B; b++)
+                a[n * B + b] = (vx ^ (T::flip(COLS / 8 * n) ^ (b << 4))) + vt + T::block(COLS / 8 * n) + 8 * b * 128;
+        ka_read_tr<16 * 128>(a, r);
+#pragma unroll
+        for (int n = 0; n < T::NT; n++)
+#pragma unroll
+            for (int kc = 0; kc < KC; kc++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    v[n][kc][e] = (_Float16)(B == 2 ? r[2 * n][kc] : r[n][0])[e];
+                    v[n][kc][4 + e] = (_Float16)(B == 2 ? r[2 * n + 1][kc] : r[n][1])[e];
+                }
+    }
+};
 
 // Whether any row of a tile of V holds inf or NaN.
 template <typename KT, int D, int COLS>
@@ -454,9 +503,11 @@ template <typename KT, int D, int COLS, int XP>
 __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], uint32_t vt,
                                           uint32_t vx, int part, bool odd, int t0, int limit) {
     using T = Ka<KT, D, COLS>;
-    vx = ka_opaque(vx);
+    KaValuesOf<D, T::F16 ? COLS : 16> vs;
+    if constexpr (T::F16) vs.read(vt, vx);
+    else vx = ka_opaque(vx);
     auto row = [&](int e, int half) {      // fp32: 4 dimensions of the key of score e
-        return ka_read<ka_f4>((vx ^ ((4 * e ^ 16 * half) << 4)) + vt + e * T::RB);
+        return ka_read<ka_f4>((vx ^ ((e & 2) << 5)) + vt + T::block(16 * half) + e * 128);
     };
     auto product = [&](auto finite) {
         if constexpr (T::F16) {
@@ -469,19 +520,16 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p
                     w[0][e] = hi;
                     if constexpr (XP == 2) w[XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
                 }
-                ka_h8 v[T::NT];
 #pragma unroll
-                for (int n = 0; n < T::NT; n++) v[n] = ka_vt<D, COLS>(vt, vx, n, kc);
-                if constexpr (!decltype(finite)::value) {
+                for (int n = 0; n < T::NT; n++) {
+                    ka_h8 v = vs.v[n][kc];
+                    if constexpr (!decltype(finite)::value) {
 #pragma unroll
-                    for (int n = 0; n < T::NT; n++)
+                        for (int e = 0; e < 8; e++) v[e] = fabsf((float)v[e]) <= 65504.f ? v[e] : (_Float16)0;
+                    }
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[n][e] = fabsf((float)v[n][e]) <= 65504.f ? v[n][e] : (_Float16)0;
+                    for (int w2 = 0; w2 < XP; w2++) x.o[n] = T::mfma(v, w[w2], x.o[n]);
                 }
-#pragma unroll
-                for (int part2 = 0; part2 < XP; part2++)
-#pragma unroll
-                    for (int n = 0; n < T::NT; n++) x.o[n] = T::mfma(v[n], w[part2], x.o[n]);
             }
         } else {
 #pragma unroll
@@ -513,9 +561,9 @@ __device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p
             auto is = [&](float f) { return kind == 2 ? f != f : f == what; };
             auto sees = [&](int e) { return t0 + T::key(e, part) < limit; };
             if constexpr (T::F16) {
-#pragma unroll 1
+#pragma unroll
                 for (int kc = 0; kc < T::NS / 8; kc++) {
-                    const ka_h8 v = ka_vt<D, COLS>(vt, vx, n, kc);
+                    const ka_h8 v = vs.v[n][kc];
                     ka_h8 k, w;
 #pragma unroll
                     for (int e = 0; e < 8; e++) {
@@ -718,31 +766,35 @@ struct KaWalk {
     const char *kb, *vb;
     char *kt, *vt;
     int tiles, per_page, lg, mask;
-    uint32_t next;                         // cache row of this lane's key of the next tile
-    int64_t off[T::NI];
+    int page, pos;                         // this lane's key of the next tile: its page's id, unchecked, and its row there
+    int64_t off[T::NB];
     bool bad = false;
 
     // (keys behind the last one re-read it)
-    __device__ uint32_t key_row(const KaArgs& a, const KaItem& it, int j, int lane) {
+    __device__ void look_up(const KaItem& it, int j, int lane) {
         const int t = min(it.k0 + min(j, tiles - 1) * T::KEYS + lane % T::KEYS, it.k1 - 1);
-        int page = it.table[t >> lg];
-        if (page < 0 || page >= a.c.n_pages) {
-            bad = true;
-            page = 0;
-        }
-        return (uint32_t)page * (uint32_t)per_page + (uint32_t)(t & mask);
+        page = it.table[t >> lg];
+        pos = t & mask;
     }
-    __device__ void offsets(int lane) {
+    // Where this lane's 16 bytes of each 8 rows are: rows lane / 8 of them.
+    __device__ void offsets(const KaArgs& a, int lane) {
+        const bool ok = page >= 0 && page < a.c.n_pages;
+        bad |= !ok;
+        const uint32_t row = (uint32_t)(ok ? page : 0) * (uint32_t)per_page + (uint32_t)pos;
+        int r[T::NB];
 #pragma unroll
-        for (int i = 0; i < T::NI; i++) {
-            const int r = T::RPI * i + lane / T::SL;
-            off[i] = (int64_t)(uint32_t)__shfl((int)next, r, 64) * T::RB + (((lane % T::SL) ^ T::swz(r)) << 4);
-        }
+        for (int i = 0; i < T::NB; i++) r[i] = __shfl((int)row, 8 * i + lane / 8, 64);
+#pragma unroll
+        for (int i = 0; i < T::NB; i++)
+            off[i] = (int64_t)(uint32_t)r[i] * T::RB + (((lane & 7) ^ T::swz(8 * i + lane / 8)) << 4);
     }
     __device__ void copy(const char* from, char* to) {
 #pragma unroll
-        for (int i = 0; i < T::NI; i++)
-            __builtin_amdgcn_global_load_lds((const void*)(from + off[i]), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
+        for (int i = 0; i < T::NB; i++)
+#pragma unroll
+            for (int cb = 0; cb < T::CB; cb++)
+                __builtin_amdgcn_global_load_lds((const void*)(from + off[i] + 128 * cb),
+                                                 (ka_lds_t*)(to + cb * T::BLOCK + i * 1024), 16, 0, 0);
     }
     // The first tile's copies, if the wave has one.
     __device__ void begin(const KaArgs& a, const KaItem& it, char* mine, int w, int lane) {
@@ -755,10 +807,9 @@ struct KaWalk {
         vt = mine + T::TILE;
         tiles = (it.k1 - it.k0 + T::KEYS - 1) / T::KEYS;
         if (w >= tiles) return;
-        next = key_row(a, it, w, lane);
-        const uint32_t then = key_row(a, it, w + 4, lane);
-        offsets(lane);
-        next = then;
+        look_up(it, w, lane);
+        offsets(a, lane);
+        look_up(it, w + 4, lane);
         copy(kb, kt);
         copy(vb, vt);
     }
@@ -782,9 +833,9 @@ struct KaWalk {
             ka_scores<KT, D, KA_COLS, XP>(k, q, s);
             ka_wait_reads();
             if (more) {
-                offsets(lane);
+                offsets(a, lane);
                 copy(kb, kt);
-                next = key_row(a, it, j + 8, lane);
+                look_up(it, j + 8, lane);      // (used in the next round: not waited for here)
             }
             ka_reference<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
             ka_weights<KT, D, KA_COLS>(x, s, q.cs);
@@ -871,7 +922,7 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
 
     const char* kb = ka_base<T::RB>(a, it.g);
     const char* vb = kb + ka_plane<T::RB>(a);
-    constexpr int STAGE = 2 * KA_WIDE_KEYS * T::RB, PW = 8 / T::RPI;    // copies of a wave: PW of K, PW of V
+    constexpr int STAGE = 2 * KA_WIDE_KEYS * T::RB, PW = T::CB;        // copies of a wave: PW of K, PW of V
     const int chunk = (KA_WIDE_PAGES - 1) * min(c.page_size, 1 << 16) / KA_WIDE_KEYS * KA_WIDE_KEYS;
     for (int k0 = it.k0; k0 < it.k1; k0 += chunk) {    // as many keys as page ids fit
         const int k1 = min(it.k1 - k0, chunk) + k0, p0 = k0 >> lg, np = ((k1 - 1) >> lg) - p0 + 1;
@@ -885,16 +936,17 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
             pages[i] = page;
         }
         __syncthreads();
-        // stage s: its rows 8 w .. 8 w + 7 (keys behind the last one re-read it)
+        // stage s: its rows 8 w .. 8 w + 7 (keys behind the last one re-read it), those of tile w / 4
         auto copy = [&](int s) {
-            char* to = lds + (s % KA_STAGES) * STAGE + 8 * w * T::RB;
+            const int t = min(k0 + s * KA_WIDE_KEYS + 8 * w + lane / 8, k1 - 1);
+            const uint32_t at = (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
+            const int64_t off = (int64_t)at * T::RB + (((lane & 7) ^ T::swz(8 * cg + lane / 8)) << 4);
+            char* to = lds + (s % KA_STAGES) * STAGE + kg * T::TILE + cg * 1024;
 #pragma unroll
-            for (int i = 0; i < PW; i++) {
-                const int rr = 8 * w + T::RPI * i + lane / T::SL, t = min(k0 + s * KA_WIDE_KEYS + rr, k1 - 1);
-                const uint32_t at = (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
-                const int64_t off = (int64_t)at * T::RB + (((lane % T::SL) ^ T::swz(rr)) << 4);
-                __builtin_amdgcn_global_load_lds((const void*)(kb + off), (ka_lds_t*)(to + i * 1024), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void*)(vb + off), (ka_lds_t*)(to + KA_WIDE_KEYS * T::RB + i * 1024), 16, 0, 0);
+            for (int cb = 0; cb < T::CB; cb++) {
+                __builtin_amdgcn_global_load_lds((const void*)(kb + off + 128 * cb), (ka_lds_t*)(to + cb * T::BLOCK), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const void*)(vb + off + 128 * cb),
+                                                 (ka_lds_t*)(to + KA_WIDE_KEYS * T::RB + cb * T::BLOCK), 16, 0, 0);
             }
         };
         const int stages = (k1 - k0 + KA_WIDE_KEYS - 1) / KA_WIDE_KEYS;
