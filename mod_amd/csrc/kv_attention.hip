@@ -4,19 +4,19 @@
 // The keys fall in two parts: the prefix that all sequences have in common, whose
 // columns (a column is one (query, head) pair) are those of the whole batch, and
 // the tails, one per sequence. Both are cut into items of a few columns and a run
-// of keys, one launch computes all of them, each item's (max, sum, weighted sum)
-// goes to a workspace, and a second launch joins a column's items.
+// of keys, each item's (max, sum, weighted sum) goes to a workspace, and a last
+// launch joins a column's items.
 //
 // Scores and weighted sums are contractions on the matrix cores, formed
 // transposed, S^T = K Q^T and O^T = V^T P^T, as in attention.hip: a column is held
 // by lanes c and c + 32, its softmax is arithmetic inside them, and the
 // accumulator registers of S^T are, after the exp, operand registers of O^T.
-//   fp16 cache: v_mfma_f32_32x32x16_f16. K is read from LDS as operands, V
+//   fp16 cache: v_mfma_f32_16x16x32_f16 or 32x32x16. K is read from LDS as operands, V
 //     through the transposing LDS read (a lane gets one dimension of 4 keys).
 //     fp16 queries: one part of q, weights rounded to fp16 (their sum is not).
 //     fp32 queries: q and the weights as two fp16 parts each, 22 bits, q scaled
 //     to a fixed exponent per column first (exact).
-//   fp32 cache: v_mfma_f32_32x32x2_f32.
+//   fp32 cache: v_mfma_f32_16x16x4_f32.
 // K and V come by direct global -> LDS copies: page ids only change addresses,
 // and any mix of pages in a tile costs the same.
 #include "gemm_core.hpp"
@@ -38,16 +38,24 @@ struct KaArgs {
     void* out;
     int64_t q_stride, out_stride;
     int layer, n, shared, rows, H, G;
+    uint32_t g_magic;        // floor(2^32 / G) + 1, 0 for 1
     float scale;
     bool q16;
     // items of the matrix core kernels
     int pre_items, pre_tiles, pre_splits, pre_keys;   // workgroups; column tiles; runs of keys, keys of each
     int tail_tiles, tail_runs, max_runs;              // column tiles; runs of all requests that are aimed at, and of one
+    int tail_items;                                   // (run, column tile, kv head)
     bool direct;                                      // one item per column: it writes out itself
     float* part_o;                                    // [pre_splits + max_runs][rows * H][D]
     float* part_ml;                                   // [..][rows * H][2]
     int* part_n;                                      // [rows]: tail runs, 0 for a row that is written already
 };
+
+// Column / G.
+__device__ __forceinline__ int ka_div(const KaArgs& a, int col) {
+    const int r = a.g_magic ? (int)__umulhi((uint32_t)col, a.g_magic) : col;     // at most one too large
+    return r - (r * a.G > col);
+}
 
 // Rows of request i, kept inside q whatever row_start holds.
 __device__ __forceinline__ void ka_rows(const KaArgs& a, int i, int& r0, int& r1) {
@@ -398,7 +406,6 @@ struct KaValuesOf {
     ka_h8 v[T::NT][KC];
     __device__ __forceinline__ void read(uint32_t vt, uint32_t vx) {
         vx = ka_opaque(vx);
-        vt += (uint32_t)(uintptr_t)(ka_lds_c*)ka_lds;
         // 16 lanes read 16 dimensions of 4 keys. 32 columns: an operand's second 4 keys are 8 rows on, with another
         // swizzle, the second key group 16; 16 columns: the second 4 keys 16 rows on
         constexpr int B = COLS == 32 ? 2 : 1;
@@ -409,6 +416,8 @@ struct KaValuesOf {
 #pragma unroll
             for (int b = 0; b < B; b++)
                 a[n * B + b] = (vx ^ (T::flip(COLS / 8 * n) ^ (b << 4))) + vt + T::block(COLS / 8 * n) + 8 * b * 128;
+#pragma unroll
+        for (int i = 0; i < T::NT * B; i++) a[i] += (uint32_t)(uintptr_t)(ka_lds_c*)ka_lds;
         ka_read_tr<16 * 128>(a, r);
 #pragma unroll
         for (int n = 0; n < T::NT; n++)
@@ -421,23 +430,6 @@ struct KaValuesOf {
                 }
     }
 };
-
-// Whether any row of a tile of V holds inf or NaN.
-template <typename KT, int D, int COLS>
-__device__ __forceinline__ bool ka_odd(const char* vt, int lane) {
-    bool odd = false;
-#pragma unroll 1
-    for (int u = lane; u < Ka<KT, D, COLS>::TILE / 16; u += 64) {
-        const uint4 x = *(const uint4*)(vt + 16 * u);
-        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (sizeof(KT) == 2) odd |= (w[e] & 0x7c00u) == 0x7c00u || (w[e] & 0x7c000000u) == 0x7c000000u;
-            else odd |= (w[e] & 0x7f800000u) == 0x7f800000u;
-        }
-    }
-    return __any(odd);
-}
 
 // A column's running softmax: (reference, sum) in base 2, O^T.
 template <typename KT, int D, int COLS>
@@ -452,23 +444,27 @@ struct KaAcc {
     }
 };
 
-// Scores -> weights (in s), and the running reference and sum, in two steps: the
-// reference, then the exponentials. The tile's keys from t0; edge (wave-uniform):
-// some column does not see all of them.
+// Scores -> weights (in s), and the running reference and sum, in steps. The tile's
+// keys from t0; edge (wave-uniform): some column does not see all of them.
+//   1. what a column does not see is -inf; its maximum
 template <typename KT, int D, int COLS>
-__device__ __forceinline__ void ka_reference(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs, int t0,
-                                             int limit, bool edge, int part) {
+__device__ __forceinline__ void ka_mask(int t0, int limit, int part, float (&s)[Ka<KT, D, COLS>::NS]) {
     using T = Ka<KT, D, COLS>;
-    if (edge) {
-        const int left = ka_opaque(limit - t0 - T::key(0, part));      // (in this branch alone, not hoisted out of it)
+    const int left = ka_opaque(limit - t0 - T::key(0, part));
 #pragma unroll
-        for (int e = 0; e < T::NS; e++) s[e] = T::key(e, 0) < left ? s[e] : -INFINITY;
-    }
+    for (int e = 0; e < T::NS; e++) s[e] = T::key(e, 0) < left ? s[e] : -INFINITY;
+}
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ float ka_top(const float (&s)[Ka<KT, D, COLS>::NS], float cs, int t0, int limit) {
     float top = s[0];
 #pragma unroll
-    for (int e = 1; e < T::NS; e++) top = fmaxf(top, s[e]);
-    // (a score of -inf, and one times no scale, are no numbers to compare with)
-    top = ka_max<COLS>(fmaxf(top * cs, t0 < limit ? KA_SEEN : -FLT_MAX));
+    for (int e = 1; e < Ka<KT, D, COLS>::NS; e++) top = fmaxf(top, s[e]);
+    return ka_max<COLS>(fmaxf(top * cs, t0 < limit ? KA_SEEN : -FLT_MAX));
+}
+//   2. the reference, where the maximum has grown enough
+template <typename KT, int D, int COLS>
+__device__ __forceinline__ void ka_follow(KaAcc<KT, D, COLS>& x, float top) {
+    using T = Ka<KT, D, COLS>;
     if (__any(top > x.m + KA_SLACK)) {
         const float m = fmaxf(x.m, top), corr = __builtin_amdgcn_exp2f(x.m - m);
         x.l *= corr;
@@ -479,6 +475,7 @@ __device__ __forceinline__ void ka_reference(KaAcc<KT, D, COLS>& x, float (&s)[K
         x.m = m;
     }
 }
+//   3. the weights
 template <typename KT, int D, int COLS>
 __device__ __forceinline__ void ka_weights(KaAcc<KT, D, COLS>& x, float (&s)[Ka<KT, D, COLS>::NS], float cs) {
     using T = Ka<KT, D, COLS>;
@@ -496,93 +493,84 @@ __device__ __forceinline__ void ka_weights(KaAcc<KT, D, COLS>& x, float (&s)[Ka<
     x.l += sum[0];
 }
 
-// O^T += V^T P^T over one tile. `odd`: V holds inf or NaN and some column does not
-// see all keys: 0 * inf would make those columns NaN, so inf and NaN are taken out of
-// the product and added where a column sees them (their weights are positive).
+// O^T += V^T P^T over one tile (fp16: operands vs; fp32: rows at vt). In a tile that
+// some column does not see all of (edge), a value of inf or NaN would make that column
+// NaN, 0 * inf: such values are left out, and true is returned (in every lane): ka_mend
+// adds them to the columns that see them.
 template <typename KT, int D, int COLS, int XP>
-__device__ __forceinline__ void ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], uint32_t vt,
-                                          uint32_t vx, int part, bool odd, int t0, int limit) {
+__device__ __forceinline__ bool ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS],
+                                          KaValuesOf<D, COLS>& vs, uint32_t vt, uint32_t vx, bool edge) {
     using T = Ka<KT, D, COLS>;
-    KaValuesOf<D, T::F16 ? COLS : 16> vs;
-    if constexpr (T::F16) vs.read(vt, vx);
-    else vx = ka_opaque(vx);
-    auto row = [&](int e, int half) {      // fp32: 4 dimensions of the key of score e
-        return ka_read<ka_f4>((vx ^ ((e & 2) << 5)) + vt + T::block(16 * half) + e * 128);
-    };
-    auto product = [&](auto finite) {
-        if constexpr (T::F16) {
+    bool odd = false;
+    if constexpr (T::F16) {
+        constexpr int KC = KaValuesOf<D, COLS>::KC;
+        if (edge) {
+            ka_h8 z = {0, 0, 0, 0, 0, 0, 0, 0};        // stays 0, but for inf and NaN
 #pragma unroll
-            for (int kc = 0; kc < T::NS / 8; kc++) {
-                ka_h8 w[XP];
+            for (int n = 0; n < T::NT; n++)
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const _Float16 hi = (_Float16)p[8 * kc + e];
-                    w[0][e] = hi;
-                    if constexpr (XP == 2) w[XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
-                }
+                for (int kc = 0; kc < KC; kc++) z = vs.v[n][kc] * (_Float16)0 + z;
+            bool any = false;
 #pragma unroll
-                for (int n = 0; n < T::NT; n++) {
-                    ka_h8 v = vs.v[n][kc];
-                    if constexpr (!decltype(finite)::value) {
+            for (int e = 0; e < 8; e++) any |= z[e] != z[e];
+            odd = __any(any);
+            if (odd) {
 #pragma unroll
-                        for (int e = 0; e < 8; e++) v[e] = fabsf((float)v[e]) <= 65504.f ? v[e] : (_Float16)0;
-                    }
+                for (int n = 0; n < T::NT; n++)
 #pragma unroll
-                    for (int w2 = 0; w2 < XP; w2++) x.o[n] = T::mfma(v, w[w2], x.o[n]);
-                }
+                    for (int kc = 0; kc < KC; kc++)
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const _Float16 v = vs.v[n][kc][e];
+                            vs.v[n][kc][e] = v * (_Float16)0 == (_Float16)0 ? v : (_Float16)0;
+                        }
             }
-        } else {
+        }
+#pragma unroll
+        for (int kc = 0; kc < KC; kc++) {
+            ka_h8 w[XP];
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const _Float16 hi = (_Float16)p[8 * kc + e];
+                w[0][e] = hi;
+                if constexpr (XP == 2) w[XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
+            }
+#pragma unroll
+            for (int n = 0; n < T::NT; n++)
+#pragma unroll
+                for (int i = 0; i < XP; i++) x.o[n] = T::mfma(vs.v[n][kc], w[i], x.o[n]);
+        }
+    } else {
+        vx = ka_opaque(vx);
+        ka_f4 v[T::NS][T::NT / 4];             // 4 dimensions of the key of each score
+#pragma unroll
+        for (int e = 0; e < T::NS; e++)
+#pragma unroll
+            for (int half = 0; half < T::NT / 4; half++)
+                v[e][half] = ka_read<ka_f4>((vx ^ ((e & 2) << 5)) + vt + T::block(16 * half) + e * 128);
+        if (edge) {
+            ka_f4 z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int e = 0; e < T::NS; e++)
 #pragma unroll
-                for (int half = 0; half < T::NT / 4; half++) {
-                    ka_f4 v = row(e, half);
-#pragma unroll
-                    for (int n = 0; n < 4; n++) {
-                        if constexpr (!decltype(finite)::value) v[n] = fabsf(v[n]) <= FLT_MAX ? v[n] : 0.f;
-                        ka_f4& o = x.o[4 * half + n];
-                        o = __builtin_amdgcn_mfma_f32_16x16x4f32(v[n], p[e], o, 0, 0, 0);
-                    }
-                }
-        }
-    };
-    if (!odd) {
-        product(std::true_type{});
-        return;
-    }
-    product(std::false_type{});
-    // how many +inf, -inf and NaN each (dimension, column) sees
-#pragma unroll
-    for (int n = 0; n < T::NT; n++) {
-#pragma unroll 1
-        for (int kind = 0; kind < 3; kind++) {
-            const float what = kind == 0 ? INFINITY : kind == 1 ? -INFINITY : NAN;
-            typename T::Acc c = T::zero();
-            auto is = [&](float f) { return kind == 2 ? f != f : f == what; };
-            auto sees = [&](int e) { return t0 + T::key(e, part) < limit; };
-            if constexpr (T::F16) {
-#pragma unroll
-                for (int kc = 0; kc < T::NS / 8; kc++) {
-                    const ka_h8 v = vs.v[n][kc];
-                    ka_h8 k, w;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        k[e] = is((float)v[e]) ? (_Float16)1 : (_Float16)0;
-                        w[e] = sees(8 * kc + e) ? (_Float16)1 : (_Float16)0;
-                    }
-                    c = T::mfma(k, w, c);
-                }
-            } else {
+                for (int half = 0; half < T::NT / 4; half++) z = v[e][half] * 0.f + z;
+            odd = __any(!((z[0] + z[1]) + (z[2] + z[3]) == 0.f));
+            if (odd) {
 #pragma unroll
                 for (int e = 0; e < T::NS; e++)
-                    c = __builtin_amdgcn_mfma_f32_16x16x4f32(is(row(e, n >> 2)[n & 3]) ? 1.f : 0.f, sees(e) ? 1.f : 0.f, c,
-                                                             0, 0, 0);
-            }
 #pragma unroll
-            for (int e = 0; e < T::E; e++)
-                if (c[e] > 0.5f) x.o[n][e] += what;
+                    for (int half = 0; half < T::NT / 4; half++)
+#pragma unroll
+                        for (int n = 0; n < 4; n++) v[e][half][n] = fabsf(v[e][half][n]) <= FLT_MAX ? v[e][half][n] : 0.f;
+            }
         }
+#pragma unroll
+        for (int e = 0; e < T::NS; e++)
+#pragma unroll
+            for (int n = 0; n < T::NT; n++)
+                x.o[n] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e][n >> 2][n & 3], p[e], x.o[n], 0, 0, 0);
     }
+    return odd;
 }
 
 // A lane's part of an accumulated column, times f, into LDS (column's row at `to`),
@@ -627,7 +615,7 @@ __device__ __forceinline__ void ka_out(const KaArgs& a, int D, int row, int head
     }
 }
 __device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it, int col, int d, ka_f4 v, float m, float l) {
-    const int r = col / a.G, row = it.row0 + r, head = it.g * a.G + col - r * a.G;
+    const int r = ka_div(a, col), row = it.row0 + r, head = it.g * a.G + col - r * a.G;
     if (it.direct) {
         v = v / l;
         if (m == -FLT_MAX && l == 0.f) v = ka_f4{0.f, 0.f, 0.f, 0.f};     // sees no key
@@ -664,14 +652,13 @@ __device__ __forceinline__ int ka_scan(int v, int* red, int& total) {
 
 // Which tail items there are: the tails are cut into runs of about equal length,
 // however uneven they are (every request with rows has at least one). By the whole
-// workgroup; it gets the request, run and geometry of run number `run` (two of them
-// for two groups), false if there are fewer.
+// workgroup; it gets the request, run and geometry of run number `run` (request -1 if
+// there are fewer).
 struct KaRun {
     int i, z, runs, per;     // request, run of it, runs of it, rounds of KA_ROUND keys of a run
     int r0, r1, s, L;        // rows, sequence, its length (-1: none such)
 };
-template <int GROUPS>
-__device__ __forceinline__ void ka_runs(const KaArgs& a, const int (&run)[GROUPS], KaRun* found, int* red) {
+__device__ __forceinline__ void ka_runs(const KaArgs& a, int run, KaRun& found, int* red) {
     const int tid = threadIdx.x, threads = blockDim.x;
     KaRun r{};
     auto rounds = [&](int i) {
@@ -683,7 +670,7 @@ __device__ __forceinline__ void ka_runs(const KaArgs& a, const int (&run)[GROUPS
         if (r.r1 <= r.r0) return 0;
         return r.L <= a.shared ? 1 : (r.L - a.shared + KA_ROUND - 1) / KA_ROUND;
     };
-    if (tid < GROUPS) found[tid].i = -1;
+    if (tid == 0) found.i = -1;
     int n = rounds(tid), total, sum;
     ka_scan(n, red, total);
     for (int i0 = threads; i0 < a.n; i0 += threads) {
@@ -698,12 +685,10 @@ __device__ __forceinline__ void ka_runs(const KaArgs& a, const int (&run)[GROUPS
         r.runs = (n + r.per - 1) / r.per;
         const int at = before + ka_scan(r.runs, red, sum);
         before += sum;
-#pragma unroll
-        for (int k = 0; k < GROUPS; k++)
-            if (run[k] >= at && run[k] < at + r.runs) {
-                r.z = run[k] - at;
-                found[k] = r;
-            }
+        if (run >= at && run < at + r.runs) {
+            r.z = run - at;
+            found = r;
+        }
     }
     __syncthreads();
 }
@@ -714,11 +699,12 @@ __device__ __forceinline__ void ka_limits(const KaArgs& a, int first, int* limit
     for (int i = threadIdx.x; i < N; i += blockDim.x) limit[i] = -1;
     __syncthreads();
     for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
+        const int s = a.seq[i];            // (with its rows, not behind them)
         int r0, r1;
         ka_rows(a, i, r0, r1);
         const int lo = max(r0, first), hi = min(r1, first + N);
         if (lo >= hi) continue;
-        const int L = kv_seq_len(a.c, a.seq[i]);
+        const int L = kv_seq_len(a.c, s);
         if (L < 0) continue;
         for (int row = lo; row < hi; row++) limit[row - first] = max(L - (r1 - row) + 1, 0);
     }
@@ -742,11 +728,33 @@ __device__ __forceinline__ int64_t ka_plane(const KaArgs& a) {
     return (int64_t)a.c.n_pages * a.c.n_kv_heads * a.c.page_size * RB;
 }
 
+// inf and NaN values that ka_values left out, added to 4 dimensions from d of column
+// `col` (of the item) with limit `limit`, out of the keys from `from` on.
+template <typename KT, int D>
+__device__ __forceinline__ void ka_mend(const KaArgs& a, const KaItem& it, int from, int limit, int d, ka_f4& v) {
+    const pio_kv_cache& c = a.c;
+    constexpr int RB = D * (int)sizeof(KT);
+    const int lg = kv_log2(c.page_size);
+    const KT* vb = (const KT*)(ka_base<RB>(a, it.g) + ka_plane<RB>(a));
+    for (int t = max(from, it.k0); t < min(limit, it.k1); t++) {
+        const int page = it.table[t >> lg];
+        if (page < 0 || page >= c.n_pages) continue;
+        const KT* r = vb + ((int64_t)page * c.n_kv_heads * c.page_size + (t & (c.page_size - 1))) * D + d;
+        for (int e = 0; e < 4; e++)
+            if (!(fabsf((float)r[e]) <= FLT_MAX)) v[e] += (float)r[e];
+    }
+}
+// Keys of its run that a column with row r (of the item) sees; limits: of a prefix's rows from `first`.
+__device__ __forceinline__ int ka_limit(const KaItem& it, const int* limits, int first, int r) {
+    const int n = limits ? limits[r - first] : it.first_limit + r;
+    return limits && n < 0 ? it.k1 : min(n, it.k1);     // (a row that no request has: anything)
+}
+
 // ---- narrow items: 4 waves, 16 columns, every 4th tile of the keys each, from a
 // piece of LDS of the wave's own (one tile of K, one of V). The next K tile is
 // copied during this one's softmax and product with V, the next V tile during the
 // next scores. No barriers: a wave waits for its own copies.
-constexpr int KA_COLS = 16;
+constexpr int KA_COLS = 16, KA_WAVES = 4;
 
 template <int N>
 __device__ __forceinline__ void ka_wait_copies() {
@@ -768,7 +776,7 @@ struct KaWalk {
     int tiles, per_page, lg, mask;
     int page, pos;                         // this lane's key of the next tile: its page's id, unchecked, and its row there
     int64_t off[T::NB];
-    bool bad = false;
+    bool bad = false, odd = false;
 
     // (keys behind the last one re-read it)
     __device__ void look_up(const KaItem& it, int j, int lane) {
@@ -809,7 +817,7 @@ struct KaWalk {
         if (w >= tiles) return;
         look_up(it, w, lane);
         offsets(a, lane);
-        look_up(it, w + 4, lane);
+        look_up(it, w + KA_WAVES, lane);
         copy(kb, kt);
         copy(vb, vt);
     }
@@ -823,9 +831,9 @@ struct KaWalk {
         const int least = ka_wave_min(limit);
         const uint32_t kx = ka_kx<KT, D, KA_COLS>(lane), vx = ka_vx<KT, D, KA_COLS>(lane);
         ka_wait_copies<0>();               // the query too: below only copies and one page id are counted
-        for (int j = w; j < tiles; j += 4) {
+        for (int j = w; j < tiles; j += KA_WAVES) {
             const int t0 = it.k0 + j * T::KEYS;
-            const bool more = j + 4 < tiles, edge = t0 + T::KEYS > least;
+            const bool more = j + KA_WAVES < tiles, edge = t0 + T::KEYS > least;
             ka_wait_copies<T::NI>();
             float s[T::NS];
             KaKeysOf<KT, D, KA_COLS> k;
@@ -835,14 +843,16 @@ struct KaWalk {
             if (more) {
                 offsets(a, lane);
                 copy(kb, kt);
-                look_up(it, j + 8, lane);      // (used in the next round: not waited for here)
+                look_up(it, j + 2 * KA_WAVES, lane);      // (used in the next round: not waited for here)
             }
-            ka_reference<KT, D, KA_COLS>(x, s, q.cs, t0, limit, edge, part);
+            if (edge) ka_mask<KT, D, KA_COLS>(t0, limit, part, s);
+            ka_follow<KT, D, KA_COLS>(x, ka_top<KT, D, KA_COLS>(s, q.cs, t0, limit));
             ka_weights<KT, D, KA_COLS>(x, s, q.cs);
             if (more) ka_wait_copies<T::NI + 1>();
             else ka_wait_copies<0>();
-            const bool odd = edge && ka_odd<KT, D, KA_COLS>(vt, lane);
-            ka_values<KT, D, KA_COLS, XP>(x, s, ka_addr(vt), vx, part, odd, t0, limit);
+            KaValuesOf<D, KA_COLS> vs;
+            if constexpr (T::F16) vs.read(ka_addr(vt), vx);
+            odd |= ka_values<KT, D, KA_COLS, XP>(x, s, vs, ka_addr(vt), vx, edge);
             ka_wait_reads();
             if (more) copy(vb, vt);
         }
@@ -850,15 +860,16 @@ struct KaWalk {
 };
 
 template <typename KT, int D>
-constexpr size_t ka_group_bytes() {
+constexpr size_t ka_narrow_bytes() {
     using T = Ka<KT, D, KA_COLS>;
-    return std::max<size_t>(4 * 2 * T::TILE, (size_t)4 * KA_COLS * T::OP * 4);
+    return std::max<size_t>(KA_WAVES * 2 * T::TILE, (size_t)KA_WAVES * KA_COLS * T::OP * 4);
 }
 
-// A group's 16 columns from c0 joined over its 4 waves and written.
+// An item's 16 columns from c0 joined over its waves and written.
 template <typename KT, int D>
 __device__ __forceinline__ void ka_join(const KaArgs& a, const KaItem& it, KaAcc<KT, D, KA_COLS>& x, char* lds,
-                                        float (*ml)[KA_COLS][2], int w, int lane, bool bad, int c0, bool on) {
+                                        float (*ml)[KA_COLS][2], int w, int lane, bool bad, bool odd, int c0,
+                                        const int* limits) {
     using T = Ka<KT, D, KA_COLS>;
     const int col = lane % KA_COLS, part = lane / KA_COLS;
     x.l += __shfl_xor(x.l, 32, 64);
@@ -868,36 +879,60 @@ __device__ __forceinline__ void ka_join(const KaArgs& a, const KaItem& it, KaAcc
         ml[w][col][0] = x.m;
         ml[w][col][1] = x.l;
     }
-    __syncthreads();                       // and every wave is done with its tiles
+    odd = __syncthreads_or(odd);           // and every wave is done with its tiles
     float mx = ml[0][col][0];
 #pragma unroll
-    for (int i = 1; i < 4; i++) mx = fmaxf(mx, ml[i][col][0]);
+    for (int i = 1; i < KA_WAVES; i++) mx = fmaxf(mx, ml[i][col][0]);
     ka_spill<KT, D, KA_COLS, false>(x, __builtin_amdgcn_exp2f(x.m - mx), (float*)lds + (w * KA_COLS + col) * T::OP, part);
     __syncthreads();
-    if (!on) return;
-    for (int i = w * 64 + lane; i < min(KA_COLS, it.ncols - c0) * (D / 4); i += 256) {
+    for (int i = w * 64 + lane; i < min(KA_COLS, it.ncols - c0) * (D / 4); i += 64 * KA_WAVES) {
         const int c = i / (D / 4), d = (i % (D / 4)) * 4;
         float m = ml[0][c][0], l = 0.f;
 #pragma unroll
-        for (int k = 1; k < 4; k++) m = fmaxf(m, ml[k][c][0]);
+        for (int k = 1; k < KA_WAVES; k++) m = fmaxf(m, ml[k][c][0]);
         ka_f4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < KA_WAVES; k++) {
             v += *(const ka_f4*)((const float*)lds + (k * KA_COLS + c) * T::OP + d);
             l += ml[k][c][1] * __builtin_amdgcn_exp2f(ml[k][c][0] - m);
+        }
+        if (odd) {
+            const int first = ka_div(a, c0);
+            ka_mend<KT, D>(a, it, limits ? it.k0 : it.first_limit + first - T::KEYS, ka_limit(it, limits, first, ka_div(a, c0 + c)), d, v);
         }
         ka_emit(a, D, it, c0 + c, d, v, m, l);
     }
 }
 
-// ---- wide items: 8 waves, 128 columns, 4 tiles of 32 by waves w % 4, the two halves
-// of every 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in
-// LDS that all waves copy together: K and V cross from L2 once for 128 columns.
+// A narrow item; limits: of a prefix's rows, from c0 / G.
+template <typename KT, int D, int XP>
+__device__ __forceinline__ void ka_narrow(const KaArgs& a, const KaItem& it, float (*ml)[KA_COLS][2], int* limits, int c0,
+                                          int w, int lane) {
+    using T = Ka<KT, D, KA_COLS>;
+    KaAcc<KT, D, KA_COLS> acc;
+    acc.clear();
+    KaWalk<KT, D> walk;
+    walk.begin(a, it, ka_lds + w * 2 * T::TILE, w, lane);
+    if (limits) ka_limits(a, ka_div(a, c0), limits, KA_COLS);     // under the first copies' way
+    const int col = c0 + lane % KA_COLS;
+    const bool has = col < it.ncols;
+    const int r = has ? ka_div(a, col) : 0, head = it.g * a.G + (has ? col - r * a.G : 0);
+    const int limit = has ? ka_limit(it, limits, ka_div(a, c0), r) : it.k1;
+    walk.template run<XP>(a, it, w, lane, limit, it.row0 + r, head, has, acc);
+    const bool bad = __any(it.bad || walk.bad);
+    if (bad && lane == 0) atomicOr(a.c.work, KV_BAD);
+    ka_join<KT, D>(a, it, acc, ka_lds, ml, w, lane, bad, walk.odd, c0, limits);
+}
+
+// ---- wide items: 8 waves, 128 columns: 4 tiles of 32 by waves w % 4, the halves of every
+// 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in LDS that the
+// waves copy together, so that they cross from L2 once for 128 columns. (4 waves of 64
+// columns with all registers of a SIMD each moved their accumulators between register
+// files; the second half's waves half a stage behind the first's: neither was faster.)
 constexpr int KA_WIDE_COLS = 128, KA_WIDE_KEYS = 64, KA_STAGES = 4, KA_WIDE_PAGES = 4096;
 template <int D>
 constexpr size_t ka_wide_bytes() {
-    return std::max<size_t>({(size_t)KA_STAGES * 2 * KA_WIDE_KEYS * D * 2, (size_t)KA_WIDE_COLS * (D + 4) * 4,
-                             2 * ka_group_bytes<_Float16, D>()});
+    return std::max<size_t>((size_t)KA_STAGES * 2 * KA_WIDE_KEYS * D * 2, (size_t)KA_WIDE_COLS * (D + 4) * 4);
 }
 
 template <int D, int XP>
@@ -909,26 +944,28 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), cg = w & 3, kg = w >> 2;
     const int col = lane & 31, h = lane >> 5;
     const int lg = kv_log2(c.page_size), mask = c.page_size - 1, per_page = c.n_kv_heads * c.page_size;
-    const int c0 = base + cg * 32;
-    const bool has = c0 + col < it.ncols;
-    const int r = has ? (c0 + col) / a.G : 0, row = it.row0 + r, head = it.g * a.G + (has ? (c0 + col) - r * a.G : 0);
-    int limit = it.k1, least = 0;
+    const int first = ka_div(a, base), cc = base + cg * 32 + col;
+    const bool has = cc < it.ncols;
+    const int r = has ? ka_div(a, cc) : 0, head = it.g * a.G + (has ? cc - r * a.G : 0);
     KaQ<KT, D, 32, XP> q;
-    if constexpr (XP == 1) ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
     KaAcc<KT, D, 32> x;
     x.clear();
-    bool bad = it.bad;
+    int limit = it.k1, least = it.k1;
+    bool bad = it.bad, odd = false;
     const uint32_t kx = ka_kx<KT, D, 32>(lane), vx = ka_vx<KT, D, 32>(lane);
 
     const char* kb = ka_base<T::RB>(a, it.g);
     const char* vb = kb + ka_plane<T::RB>(a);
     constexpr int STAGE = 2 * KA_WIDE_KEYS * T::RB, PW = T::CB;        // copies of a wave: PW of K, PW of V
-    const int chunk = (KA_WIDE_PAGES - 1) * min(c.page_size, 1 << 16) / KA_WIDE_KEYS * KA_WIDE_KEYS;
+    const int chunk = (KA_WIDE_PAGES - 1) * c.page_size / KA_WIDE_KEYS * KA_WIDE_KEYS;
     for (int k0 = it.k0; k0 < it.k1; k0 += chunk) {    // as many keys as page ids fit
         const int k1 = min(it.k1 - k0, chunk) + k0, p0 = k0 >> lg, np = ((k1 - 1) >> lg) - p0 + 1;
+        int page = tid < np ? it.table[p0 + tid] : 0;
         if (k0 != it.k0) __syncthreads();
+        // under its way; limits: of the rows from `first` (prefix), else by first_limit
+        else if (limits) ka_limits(a, first, limits, KA_WIDE_COLS);
         for (int i = tid; i < np; i += 512) {
-            int page = it.table[p0 + i];
+            if (i != tid) page = it.table[p0 + i];
             if (page < 0 || page >= c.n_pages) {
                 bad = true;
                 page = 0;
@@ -954,14 +991,9 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
 #pragma unroll
         for (int s = 0; s < KA_STAGES - 1; s++) copy(s);
         if (k0 == it.k0) {
-            // under the first copies' way; limits: of the rows from base / G (prefix), else by first_limit
-            if (limits) ka_limits(a, base / a.G, limits, KA_WIDE_COLS);
-            if (has) {
-                const int n = limits ? limits[r - base / a.G] : it.first_limit + r;
-                if (!limits || n >= 0) limit = min(n, it.k1);
-            }
+            if (has) limit = ka_limit(it, limits, first, r);
             least = ka_wave_min(limit);
-            if constexpr (XP == 2) ka_load_q<KT, D, 32, XP>(a, row, head, has, h, q);
+            ka_load_q<KT, D, 32, XP>(a, it.row0 + r, head, has, h, q);
             ka_wait_copies<0>();           // q is here: the waits below count copies alone
         }
         // The scores run one stage ahead of the softmax: their products fill the matrix cores
@@ -986,7 +1018,8 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
             // (a chunk's end is not the item's: keys behind it come with the next chunk)
             const int end = min(limit, k1);
             const bool edge = t0 + T::KEYS > min(least, k1);
-            ka_reference<KT, D, 32>(x, sc, q.cs, t0, end, edge, h);
+            if (edge) ka_mask<KT, D, 32>(t0, end, h, sc);
+            ka_follow<KT, D, 32>(x, ka_top<KT, D, 32>(sc, q.cs, t0, end));
             ka_weights<KT, D, 32>(x, sc, q.cs);
             if constexpr (AHEAD) {
                 ka_scores<KT, D, 32, XP>(k, q, next);
@@ -997,8 +1030,9 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
                 }
             }
             const uint32_t vt = tile(s) + KA_WIDE_KEYS * T::RB;
-            const bool odd = edge && ka_odd<KT, D, 32>(lds + vt, lane);
-            ka_values<KT, D, 32, XP>(x, sc, vt, vx, h, odd, t0, end);
+            KaValuesOf<D, 32> v;
+            v.read(vt, vx);
+            odd |= ka_values<KT, D, 32, XP>(x, sc, v, vt, vx, edge);
             if constexpr (AHEAD) {
 #pragma unroll
                 for (int e = 0; e < T::NS; e++) sc[e] = next[e];
@@ -1012,21 +1046,32 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
         ml[w][col][0] = x.m;
         ml[w][col][1] = x.l;
     }
-    const bool any_bad = __syncthreads_or(bad);        // and every copy has landed, every stage is read
+    const bool any_bad = __syncthreads_or(bad);        // and every stage is read
+    odd = __syncthreads_or(odd);
     if (any_bad && tid == 0) atomicOr(c.work, KV_BAD);
-    const float mx = fmaxf(ml[cg][col][0], ml[cg + 4][col][0]), f = __builtin_amdgcn_exp2f(x.m - mx);
+    const float f = __builtin_amdgcn_exp2f(x.m - fmaxf(ml[cg][col][0], ml[cg + 4][col][0]));
     float* ob = (float*)lds + (cg * 32 + col) * T::OP;
     if (kg) ka_spill<KT, D, 32, false>(x, f, ob, h);
     __syncthreads();
     if (!kg) ka_spill<KT, D, 32, true>(x, f, ob, h);
     __syncthreads();
-    for (int i = tid; i < min(KA_WIDE_COLS, it.ncols - base) * (D / 4); i += 512) {
+    const int out = min(KA_WIDE_COLS, it.ncols - base) * (D / 4);
+    auto emit = [&](int i, bool mend) {
         const int cc = i / (D / 4), d = (i % (D / 4)) * 4;
         const float m0 = ml[cc >> 5][cc & 31][0], m1 = ml[4 + (cc >> 5)][cc & 31][0], m = fmaxf(m0, m1);
         float l = ml[cc >> 5][cc & 31][1] * __builtin_amdgcn_exp2f(m0 - m) +
                   ml[4 + (cc >> 5)][cc & 31][1] * __builtin_amdgcn_exp2f(m1 - m);
         if (any_bad) l = NAN;
-        ka_emit(a, D, it, base + cc, d, *(const ka_f4*)((const float*)lds + cc * T::OP + d), m, l);
+        ka_f4 v = *(const ka_f4*)((const float*)lds + cc * T::OP + d);
+        if (mend)
+            ka_mend<KT, D>(a, it, limits ? it.k0 : it.first_limit + first - T::KEYS, ka_limit(it, limits, first, ka_div(a, base + cc)), d, v);
+        ka_emit(a, D, it, base + cc, d, v, m, l);
+    };
+    if (odd) {
+        for (int i = tid; i < out; i += 512) emit(i, true);
+    } else {
+#pragma unroll 4
+        for (int i = tid; i < out; i += 512) emit(i, false);
     }
 }
 
@@ -1067,88 +1112,44 @@ __device__ __forceinline__ bool ka_tail(const KaArgs& a, KaItem& it, const KaRun
     return true;
 }
 
-// Workgroups: the prefix's items, then the tails'.
-//   WIDE 0: 4 waves, narrow items
-//   WIDE 1: 8 waves, wide prefix items, narrow tail items (two to a workgroup)
-//   WIDE 2: 8 waves, wide items
+// The prefix's items, then the tails'.
+//   WIDE 0: narrow items, workgroups of 4 waves
+//   WIDE 1: wide items of the prefix alone, workgroups of 8 waves
+//   WIDE 2: wide items, workgroups of 8 waves
 template <typename KT, int D, int XP, int WIDE>
 __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
-    constexpr int GROUPS = WIDE == 1 ? 2 : 1;
+    constexpr int WAVES = WIDE ? 8 : KA_WAVES;
     __shared__ float ml[WIDE ? 8 * 32 * 2 : 4 * KA_COLS * 2];
     __shared__ int limits[WIDE ? KA_WIDE_COLS : KA_COLS];
-    const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3;
-    const bool prefix = (int)blockIdx.x < a.pre_items;
+    __shared__ KaRun found;
+    __shared__ int red[WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    float (*gml)[KA_COLS][2] = (float (*)[KA_COLS][2])ml;
     KaItem it;
-    int ct = 0, step = 1;                  // first column tile, tiles to the next
-    if (prefix) {
+    int ct;
+    if (WIDE == 1 || (int)blockIdx.x < a.pre_items) {
         if (!ka_prefix(a, it, ct)) return;
-        step = INT_MAX / 256;              // one only
-        if constexpr (WIDE) {
+        if constexpr (WIDE)
             ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, limits, ct * KA_WIDE_COLS);
-            return;
-        }
-    }
-    bool live = true;
-    if (!prefix) {
-        // (run, column tile, kv head)
-        __shared__ KaRun found[GROUPS];
-        __shared__ int red[8];
-        const int grp = GROUPS == 2 ? w8 >> 2 : 0, per_run = a.tail_tiles * a.c.n_kv_heads;
-        const int item0 = ((int)blockIdx.x - a.pre_items) * GROUPS, item = item0 + grp;
-        int run[GROUPS];
-#pragma unroll
-        for (int k = 0; k < GROUPS; k++) run[k] = (item0 + k) / per_run;
-        ka_runs<GROUPS>(a, run, found, red);
-        const int in_run = item - (GROUPS == 2 && grp ? run[GROUPS - 1] : run[0]) * per_run;
-        ct = in_run / a.c.n_kv_heads;
-        step = a.tail_tiles;
-        const KaRun r = found[grp];
-        live = ka_tail(a, it, r, in_run - ct * a.c.n_kv_heads);
-        if (live && !a.direct && it.g == 0 && ct == 0 && r.z == 0)
-            for (int i = tid & 255; i < it.ncols / a.G; i += 256) a.part_n[it.row0 + i] = it.direct ? 0 : r.runs;
-    }
-    if constexpr (WIDE == 2) {
-        // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
-        for (int base = ct * KA_WIDE_COLS; live && base < it.ncols; base += step * KA_WIDE_COLS) {
-            __syncthreads();
-            ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, nullptr, base);
-        }
+        else
+            ka_narrow<KT, D, XP>(a, it, gml, limits, ct * KA_COLS, w, lane);
     } else {
-        const int grp = GROUPS == 2 ? w8 >> 2 : 0;
-        char* lds = ka_lds + grp * ka_group_bytes<KT, D>();
-        float (*gml)[KA_COLS][2] = (float (*)[KA_COLS][2])ml + 4 * grp;
-        const int ct1 = live ? (it.ncols + KA_COLS - 1) / KA_COLS : 0;
-        int rounds = prefix ? 1 : ct < ct1 ? (ct1 - ct + step - 1) / step : 0;
-        if constexpr (GROUPS == 2) {       // both groups make as many rounds, for the barriers
-            __shared__ int most[2];
-            if ((tid & 255) == 0) most[grp] = rounds;
-            __syncthreads();
-            rounds = max(most[0], most[1]);
-        }
-        for (int r = 0; r < rounds; r++) {
-            if (r) __syncthreads();        // the last round's output is out of LDS
-            const int c0 = (ct + r * step) * KA_COLS, col = c0 + lane % KA_COLS;
-            const bool on = live && c0 < it.ncols;
-            bool bad = it.bad;
-            KaAcc<KT, D, KA_COLS> acc;
-            acc.clear();
-            const bool walks = on && it.k0 < it.k1;
-            KaWalk<KT, D> walk;
-            if (walks) walk.begin(a, it, lds + w * 2 * Ka<KT, D, KA_COLS>::TILE, w, lane);
-            if (WIDE == 0 && prefix) ka_limits(a, c0 / a.G, limits, KA_COLS);
-            if (walks) {
-                const bool has = col < it.ncols;
-                const int q = has ? col / a.G : 0, head = it.g * a.G + (has ? col - q * a.G : 0);
-                int limit = it.k1;
-                if (has) {
-                    const int n = prefix ? limits[q - c0 / a.G] : it.first_limit + q;
-                    if (!prefix || n >= 0) limit = min(n, it.k1);
-                }
-                walk.template run<XP>(a, it, w, lane, limit, it.row0 + q, head, has, acc);
-                bad |= walk.bad;
-            }
-            if (on && __any(bad) && lane == 0) atomicOr(a.c.work, KV_BAD);
-            ka_join<KT, D>(a, it, acc, lds, gml, w, lane, bad, c0, on);
+        const int per_run = a.tail_tiles * a.c.n_kv_heads, item = (int)blockIdx.x - a.pre_items;
+        const int run = item / per_run, in_run = item - run * per_run, g = in_run % a.c.n_kv_heads;
+        ct = in_run / a.c.n_kv_heads;
+        ka_runs(a, run, found, red);
+        const KaRun r = found;
+        if (!ka_tail(a, it, r, g)) return;
+        if (!a.direct && g == 0 && ct == 0 && r.z == 0)
+            for (int i = tid; i < r.r1 - r.r0; i += 64 * WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
+        // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
+        constexpr int COLS = WIDE == 2 ? KA_WIDE_COLS : KA_COLS;
+        for (int c0 = ct * COLS; c0 < it.ncols; c0 += a.tail_tiles * COLS) {
+            if constexpr (WIDE == 2)
+                ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, nullptr, c0);
+            else
+                ka_narrow<KT, D, XP>(a, it, gml, nullptr, c0, w, lane);
+            __syncthreads();               // its output is out of LDS
         }
     }
 }
@@ -1205,14 +1206,17 @@ __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
 
 template <typename KT, int D, int XP, int WIDE>
 static int ka_launch(const KaArgs& a, hipStream_t st) {
-    constexpr int GROUPS = WIDE == 1 ? 2 : 1;
-    size_t lds = ka_group_bytes<KT, D>();
+    size_t lds = ka_narrow_bytes<KT, D>();
     if constexpr (WIDE) lds = ka_wide_bytes<D>() + KA_WIDE_PAGES * sizeof(int);
-    // the aimed at runs, and up to one more for each request
-    const int64_t tails = (int64_t)(a.direct ? a.n : a.n + a.tail_runs) * a.c.n_kv_heads * a.tail_tiles;
     PIO_TRY((allow_lds<ka_kernel<KT, D, XP, WIDE>>(lds)));
-    ka_kernel<KT, D, XP, WIDE><<<(unsigned)(a.pre_items + (tails + GROUPS - 1) / GROUPS), WIDE ? 512 : 256, lds, st>>>(a);
+    ka_kernel<KT, D, XP, WIDE><<<a.pre_items + (WIDE == 1 ? 0 : a.tail_items), WIDE ? 512 : 256, lds, st>>>(a);
     PIO_LAUNCHED();
+    if constexpr (WIDE == 1) {
+        // the tails on their own: narrow workgroups beside wide ones would be one to a CU
+        KaArgs t = a;
+        t.pre_items = 0;
+        return ka_launch<KT, D, XP, 0>(t, st);
+    }
     if (!a.direct) {
         constexpr int GRP = 1024 / D;
         const int cols = a.rows * a.H;
@@ -1240,28 +1244,26 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
     const bool f16 = a.c.kv_dtype == PIO_F16;
     const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
-    const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : a.shared > 0 && cols > 64 ? 1 : 0;
+    // A wide kernel for the prefix reads it once for 128 columns, but comes on top of the tails', some
+    // 10 us: 512 columns x 4 kv heads x 128 dimensions over 4,096 tokens 39 us (narrow 32), over 8,192
+    // 42 (43), over 16,000 50 (65); 256 x 8 x 64 over 8,000 30 (26), over 32,000 52 (73).
+    const bool long_prefix = cols > 64 && (double)cols * Hk * a.c.head_dim * a.shared >= 0x1p31;
+    const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : long_prefix ? 1 : 0;
     a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
     const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
     PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
     // tails: as many runs as the device holds at once, in all and of one request (up to one
-    // more for each request comes on top)
-    const int groups = wide == 2 ? cus : 2 * cus;
+    // more for each request comes on top; where workgroups are one to a CU that would be a second round)
+    const int64_t runs = (wide == 2 ? cus : 2 * cus) / ((int64_t)Hk * a.tail_tiles);
+    a.tail_runs = (int)std::max<int64_t>({1, runs - (wide == 2 ? a.n : 0), runs / 2});
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    const int64_t runs = groups / ((int64_t)Hk * a.tail_tiles);
-    // (with 8 waves a workgroup, those beyond one a CU wait for a second round)
-    a.tail_runs = (int)std::max<int64_t>({1, runs - (wide ? a.n : 0), runs / 2});
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND)});
     a.direct = a.shared == 0 && a.max_runs == 1;
+    a.tail_items = (int)(items + (a.direct ? 0 : (int64_t)a.tail_runs * Hk * a.tail_tiles));
     if (a.shared > 0) {
         // prefix: as many items as the device holds at once, each of at least KA_ROUND keys
         const int width = wide ? KA_WIDE_COLS : KA_COLS;
-        int at_once = wide ? cus : 2 * cus;
-        if (wide == 1) {
-            // CUs kept free for the tails, 5 us a workgroup of them beside the prefix's time at 700 TFLOP/s
-            const double pre_us = 4.0 * a.c.head_dim * a.H * a.rows * a.shared * (a.q16 ? 1 : 2) / 700e6;
-            at_once -= (int)std::min<double>(cus / 3, items / 2 * 5.0 / pre_us);
-        }
+        const int at_once = wide ? cus : 2 * cus;
         a.pre_tiles = ceil_div(cols, width);
         const int64_t splits = std::max<int64_t>(1, at_once / std::max<int64_t>(1, (int64_t)Hk * a.pre_tiles));
         a.pre_keys = ceil_div(ceil_div(a.shared, std::min<int64_t>(splits, a.shared)), KA_ROUND) * KA_ROUND;
@@ -1323,6 +1325,7 @@ PIO_EXPORT int pio_kv_attention(const pio_kv_cache* c, int layer, const int32_t*
     a.rows = rows;
     a.H = n_heads;
     a.G = n_heads / c->n_kv_heads;
+    a.g_magic = a.G > 1 ? (uint32_t)((1ull << 32) / a.G + 1) : 0;
     a.scale = scale;
     a.q16 = dtype == PIO_F16;
     hipStream_t st = pick_stream(stream);

@@ -373,6 +373,40 @@ def test_attention_masked_places(torch, ops, kv, x, D):
     ops.kv_status(p.c)
 
 
+@pytest.mark.parametrize("D,Hk,shared,x", [(128, 2, 12301, "float16"), (128, 2, 12301, "float32"),
+                                           (64, 4, 24100, "float16")])
+def test_attention_long_prefix(torch, ops, D, Hk, shared, x):
+    """A prefix long enough for the kernel that reads it once for 128 columns. Rows that
+    stand inside it, and an infinite value that those rows do not see yet."""
+    _say(f"long prefix D{D} {shared} {x}")
+    rng = np.random.default_rng(13)
+    n, page, H = 44, 32, 32
+    tails = [1 + (7 * i) % 60 for i in range(n)]
+    p = Pair(torch, ops, 1, Hk, D, page, -(-shared // page) + 3 * n + 2, n + 1, -(-shared // page) + 3, "float16",
+             fill=np.nan)
+    _prefix(p, rng, n, shared, tails)
+    seq = [1 + int(i) for i in rng.permutation(n)]
+    counts = [1 + (s % 2) for s in seq]
+    counts[seq.index(1)] = 4                        # of 1 own token: three rows stand in the prefix
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+    q = rng.standard_normal((int(start[-1]), H, D)).astype(x)
+    ref = p.ref.attention(0, seq, start, q, D ** -0.5, np.zeros(q.shape))
+    tol = _tolerance(p, 0, seq, start, q, D ** -0.5, x == "float16")
+    got = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, 2)
+    err = np.abs(got.astype(np.float64) - ref).max()
+    _say(f"  {err:.2e} of {tol:.2e}")
+    assert err <= tol
+    pos = shared - 2                                # seen by all rows but the first one's first
+    for i in range(n + 1):                          # (in a page that ends behind the prefix: one for each sequence)
+        p.kv[0, 1, int(p.ref.table[i, pos // page]), :, pos % page] = np.inf
+    got = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, 4)
+    first = int(start[seq.index(1)])
+    assert np.abs(got[first].astype(np.float64) - ref[first]).max() <= tol
+    for r in set(range(len(q))) - {first}:
+        assert np.all(got[r] == np.inf)
+    ops.kv_status(p.c)
+
+
 def test_attention_large_scores(torch, ops):
     """Scores far apart and far from zero; a softmax that picks one key; queries
     beyond the fp16 range over an fp16 cache."""
