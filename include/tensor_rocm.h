@@ -416,7 +416,7 @@ int pio_kv_attention(const pio_kv_cache* cache, int layer, const int32_t* seq, c
  *   accepted  int32 [n]: drafted tokens accepted
  *   tokens    int32 [rows]: the accepted ones, the drawn one, then -1
  *   rejected  int32 [n] or null: drafted tokens not accepted (for pio_kv_drop)
- * A request without rows gets accepted 0. `rows` bounds row_start. */
+ * A request without rows gets accepted 0. `rows` bounds row_start; vocab up to 2^30. */
 int pio_verify_draft(const void* target, int64_t target_stride, const void* draft, int64_t draft_stride, int dtype,
                      const int32_t* ids, const float* u, const float* u_next, const int32_t* row_start, int n,
                      int rows, int vocab, int32_t* accepted, int32_t* tokens, int32_t* rejected, void* stream);

@@ -96,10 +96,11 @@ __device__ __forceinline__ int kv_scan(int v, int* red, int& total) {
     return before + x - v;
 }
 
-// Page counts of KV_SCAN consecutive pages from p0 (-1 behind the last page).
-__device__ __forceinline__ void kv_load_refs(const pio_kv_cache& c, int64_t p0, int (&r)[KV_SCAN]) {
+// Page counts of SCAN consecutive pages from p0 (-1 behind the last page).
+template <int SCAN>
+__device__ __forceinline__ void kv_load_refs(const pio_kv_cache& c, int64_t p0, int (&r)[SCAN]) {
 #pragma unroll
-    for (int i = 0; i < KV_SCAN; i++) r[i] = p0 + i < c.n_pages ? c.refs[p0 + i] : -1;
+    for (int i = 0; i < SCAN; i++) r[i] = p0 + i < c.n_pages ? c.refs[p0 + i] : -1;
 }
 
 // ------------------------------------------------------------------ init ----
@@ -113,13 +114,21 @@ __global__ __launch_bounds__(KV_COPY) void kv_init_kernel(pio_kv_cache c) {
 }
 
 // --------------------------------------------------------------- reserve ----
-// One workgroup. off[i]: pages that the requests before i take; held[i]: pages
-// that request i's sequence has, doubled, plus one if its last is copied.
+// One workgroup: a chain of waits, for the requests, their lengths, their last pages
+// and those pages' counts; the counts that free pages are found by are loaded first.
+// SCAN pages to a thread and step: 1 where one step then holds all pages, as its code is
+// the shorter (a plan over 1024 pages or fewer runs each instruction once).
+// off[i]: pages that the requests before i take; held[i]: pages that request i's
+// sequence has, doubled, plus one if its last is copied.
+constexpr int KV_LIST = 2048;          // free pages listed in LDS (in remap, if more are needed)
+template <int SCAN>
 __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c, const int32_t* __restrict__ seq,
                                                                  const int32_t* __restrict__ count, int n) {
-    __shared__ int off[PIO_KV_MAX_REQUESTS], held[PIO_KV_MAX_REQUESTS], red[KV_PLAN / 64], bad, pairs;
+    __shared__ int off[PIO_KV_MAX_REQUESTS], held[PIO_KV_MAX_REQUESTS], list[KV_LIST], red[KV_PLAN / 64], bad, pairs;
     const KvWork w = kv_work(c);
     const int tid = threadIdx.x, lg = kv_log2(c.page_size);
+    int r[SCAN];
+    kv_load_refs<SCAN>(c, (int64_t)tid * SCAN, r);
     if (tid == 0) bad = pairs = 0;
     for (int i = tid; i < n; i += KV_PLAN)
         if (kv_seq_ok(c, seq[i])) w.mark[seq[i]] = i;
@@ -131,7 +140,11 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
         if (i < n) {
             const int s = seq[i], k = count[i];
             int L = -1;
-            if (kv_seq_ok(c, s) && w.mark[s] == i) L = kv_seq_len(c, s);
+            if (kv_seq_ok(c, s)) {
+                const int named = w.mark[s];
+                L = kv_seq_len(c, s);
+                if (named != i) L = -1;
+            }
             if (L < 0 || k < 0) {
                 wrong = KV_BAD;
             } else if ((int64_t)L + k > (int64_t)c.max_pages * c.page_size) {
@@ -160,16 +173,20 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
     // the lowest free pages, as many as are needed
     int found = 0;
     if (!bad && total <= c.n_pages) {
-        for (int64_t p0 = 0; p0 < c.n_pages && found < total; p0 += KV_PLAN * KV_SCAN) {
-            int r[KV_SCAN], free = 0, sum;
-            kv_load_refs(c, p0 + (int64_t)tid * KV_SCAN, r);
+        for (int64_t p0 = 0; p0 < c.n_pages && found < total; p0 += KV_PLAN * SCAN) {
+            int free = 0, sum;
+            if (p0) kv_load_refs<SCAN>(c, p0 + (int64_t)tid * SCAN, r);
 #pragma unroll
-            for (int j = 0; j < KV_SCAN; j++) free += r[j] == 0;
+            for (int j = 0; j < SCAN; j++) free += r[j] == 0;
             int at = found + kv_scan(free, red, sum);
 #pragma unroll
-            for (int j = 0; j < KV_SCAN; j++)
+            for (int j = 0; j < SCAN; j++)
                 if (r[j] == 0) {
-                    if (at < total) w.remap[at] = (int)(p0 + (int64_t)tid * KV_SCAN + j);
+                    const int page = (int)(p0 + (int64_t)tid * SCAN + j);
+                    if (at < total) {
+                        if (total <= KV_LIST) list[at] = page;
+                        else w.remap[at] = page;
+                    }
                     at++;
                 }
             found += sum;
@@ -191,7 +208,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
             if (off[mid] <= k) lo = mid;
             else hi = mid - 1;
         }
-        const int s = seq[lo], h = held[lo] >> 1, copy = held[lo] & 1, j = k - off[lo], page = w.remap[k];
+        const int s = seq[lo], h = held[lo] >> 1, copy = held[lo] & 1, j = k - off[lo];
+        const int page = total <= KV_LIST ? list[k] : w.remap[k];
         int32_t* row = c.table + (int64_t)s * c.max_pages;
         c.refs[page] = 1;
         if (copy && j == 0) {
@@ -211,33 +229,47 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 }
 
 // ------------------------------------------------------------- page copy ----
-// Pairs of the plan: the first rows of each head, in every layer's k and v. A
-// plane of a pair (layer, k or v) is n_kv_heads runs of rows * head_dim elements.
+// Pairs of the plan: the first rows of each head, in every layer's k and v; a workgroup
+// takes a plane (layer, k or v) of a pair, n_kv_heads runs of rows * head_dim elements.
+// Bytes bound it: each thread has KV_DEEP loads in flight before its first store.
 // tables: also rewrites the tables by remap and moves the pages' counts (compact).
+constexpr int KV_DEEP = 4;
 __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int tables) {
     const KvWork w = kv_work(c);
-    const int pairs = *w.pairs_n, planes = 2 * c.n_layers;
+    const int pairs = *w.pairs_n, planes = 2 * c.n_layers, tid = threadIdx.x;
     const int esz = c.kv_dtype == PIO_F32 ? 4 : 2;
     const int64_t head_b = (int64_t)c.page_size * c.head_dim * esz, page_b = head_b * c.n_kv_heads;
-    for (int64_t item = blockIdx.x; item < (int64_t)pairs * planes; item += gridDim.x) {
-        const int pair = (int)(item / planes), plane = (int)(item - (int64_t)pair * planes);
+    const int pitch = (int)(head_b / 16);
+    for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
         const int from = w.pairs[3 * pair], to = w.pairs[3 * pair + 1], rows = w.pairs[3 * pair + 2];
-        const uint4* src = (const uint4*)((const char*)c.kv + ((int64_t)plane * c.n_pages + from) * page_b);
-        uint4* dst = (uint4*)((char*)c.kv + ((int64_t)plane * c.n_pages + to) * page_b);
-        const int run = rows * c.head_dim * esz / 16, pitch = (int)(head_b / 16);
-        const int all = run * c.n_kv_heads;
-        for (int u = threadIdx.x; u < all; u += KV_COPY) {
-            const int h = u / run, at = h * pitch + u - h * run;
-            dst[at] = src[at];
+        const int run = rows * c.head_dim * esz / 16, all = run * c.n_kv_heads;
+        const uint32_t magic = run > 1 ? 0xffffffffu / run + 1 : 0;     // u / run, or one more
+        auto at = [&](int u) {
+            if (run == pitch) return u;
+            int h = magic ? (int)__umulhi((uint32_t)u, magic) : u;
+            h -= h * run > u;
+            return h * pitch + u - h * run;
+        };
+        for (int plane = blockIdx.x; plane < planes; plane += gridDim.x) {
+            const uint4* src = (const uint4*)((const char*)c.kv + ((int64_t)plane * c.n_pages + from) * page_b);
+            uint4* dst = (uint4*)((char*)c.kv + ((int64_t)plane * c.n_pages + to) * page_b);
+            for (int u0 = tid; u0 < all; u0 += KV_DEEP * KV_COPY) {
+                uint4 x[KV_DEEP];
+#pragma unroll
+                for (int i = 0; i < KV_DEEP; i++) x[i] = src[at(min(u0 + i * KV_COPY, all - 1))];
+#pragma unroll
+                for (int i = 0; i < KV_DEEP; i++)
+                    if (u0 + i * KV_COPY < all) dst[at(u0 + i * KV_COPY)] = x[i];
+            }
         }
-        if (tables && plane == 0 && threadIdx.x == 0) {
+        if (tables && blockIdx.x == 0 && tid == 0) {
             c.refs[to] = c.refs[from];
             c.refs[from] = 0;
         }
     }
     if (tables && pairs > 0) {
-        const int64_t cells = (int64_t)c.max_seqs * c.max_pages;
-        for (int64_t i = (int64_t)blockIdx.x * KV_COPY + threadIdx.x; i < cells; i += (int64_t)gridDim.x * KV_COPY) {
+        const int64_t cells = (int64_t)c.max_seqs * c.max_pages, step = (int64_t)gridDim.x * gridDim.y * KV_COPY;
+        for (int64_t i = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * KV_COPY + tid; i < cells; i += step) {
             const int p = c.table[i];
             if (p >= 0 && p < c.n_pages) c.table[i] = w.remap[p];
         }
@@ -245,15 +277,41 @@ __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int ta
 }
 
 static int kv_copy(const pio_kv_cache& c, int64_t most_pairs, bool tables, hipStream_t st) {
-    const int64_t items = most_pairs * 2 * c.n_layers;
+    // a workgroup to each plane of a pair, up to some rounds of the whole device
+    const int planes = (int)std::min<int64_t>(2 * (int64_t)c.n_layers, 4096);
     const int64_t cells = tables ? ((int64_t)c.max_seqs * c.max_pages + KV_COPY - 1) / KV_COPY : 0;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(2048, std::max(items, cells)));
+    const int64_t most = std::max(most_pairs, std::min<int64_t>(2048, cells) / planes);
+    const dim3 grid(planes, (unsigned)std::max<int64_t>(1, std::min<int64_t>(most, 16384 / planes)));
     kv_copy_kernel<<<grid, KV_COPY, 0, st>>>(c, tables);
     PIO_LAUNCHED();
     return PIO_OK;
 }
 
 // --------------------------------------------------------------- compact ----
+// The k-th free page below the number of pages in use takes the k-th page in use from
+// there on. Up to KV_PLAN pages: a page to a thread, and live[k] the k-th in use.
+__global__ __launch_bounds__(KV_PLAN) void kv_compact_few_kernel(pio_kv_cache c) {
+    __shared__ int red[KV_PLAN / 64], live[KV_PLAN], below;
+    const KvWork w = kv_work(c);
+    const int p = threadIdx.x;
+    int r[1], used;
+    kv_load_refs<1>(c, p, r);
+    const bool in_use = r[0] > 0;
+    const int before = kv_scan(in_use, red, used);
+    if (in_use) live[before] = p;
+    if (p == min(used, KV_PLAN - 1)) below = before;       // in use below `used`
+    __syncthreads();
+    if (p < c.n_pages && !(in_use && p >= used)) w.remap[p] = p;
+    if (p < used && !in_use) {
+        const int k = p - before, from = live[below + k];
+        w.pairs[3 * k] = from;
+        w.pairs[3 * k + 1] = p;
+        w.pairs[3 * k + 2] = c.page_size;
+        w.remap[from] = p;
+    }
+    if (p == 0) *w.pairs_n = used == KV_PLAN ? 0 : used - below;
+}
+// Any number of pages, in steps.
 __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c) {
     __shared__ int red[KV_PLAN / 64];
     const KvWork w = kv_work(c);
@@ -262,18 +320,17 @@ __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c
     int used = 0, r[KV_SCAN];
     for (int64_t p0 = 0; p0 < c.n_pages; p0 += STEP) {
         int live = 0, sum;
-        kv_load_refs(c, p0 + (int64_t)tid * KV_SCAN, r);
+        kv_load_refs<KV_SCAN>(c, p0 + (int64_t)tid * KV_SCAN, r);
 #pragma unroll
         for (int j = 0; j < KV_SCAN; j++) live += r[j] > 0;
         kv_scan(live, red, sum);
         used += sum;
     }
-    // the k-th free page below `used` takes the k-th page in use from there on
     int holes = 0, movers = 0;
     for (int64_t p0 = 0; p0 < c.n_pages; p0 += STEP) {
         const int64_t base = p0 + (int64_t)tid * KV_SCAN;
         int hole = 0, mover = 0, sum;
-        kv_load_refs(c, base, r);
+        kv_load_refs<KV_SCAN>(c, base, r);
 #pragma unroll
         for (int j = 0; j < KV_SCAN; j++) {
             hole += base + j < used && r[j] <= 0;
@@ -443,7 +500,8 @@ PIO_EXPORT int pio_kv_reserve(const pio_kv_cache* c, const int32_t* seq, const i
     PIO_TRY(kv_requests(c, seq, count, n, "pio_kv_reserve"));
     if (n == 0) return PIO_OK;
     hipStream_t st = pick_stream(stream);
-    kv_reserve_plan_kernel<<<1, KV_PLAN, 0, st>>>(*c, seq, count, n);
+    if (c->n_pages <= KV_PLAN) kv_reserve_plan_kernel<1><<<1, KV_PLAN, 0, st>>>(*c, seq, count, n);
+    else kv_reserve_plan_kernel<KV_SCAN><<<1, KV_PLAN, 0, st>>>(*c, seq, count, n);
     PIO_LAUNCHED();
     return kv_copy(*c, n, false, st);
 }
@@ -506,7 +564,8 @@ PIO_EXPORT int pio_kv_drop(const pio_kv_cache* c, const int32_t* seq, const int3
 PIO_EXPORT int pio_kv_compact(const pio_kv_cache* c, void* stream) {
     PIO_TRY(kv_check(c, "pio_kv_compact"));
     hipStream_t st = pick_stream(stream);
-    kv_compact_plan_kernel<<<1, KV_PLAN, 0, st>>>(*c);
+    if (c->n_pages <= KV_PLAN) kv_compact_few_kernel<<<1, KV_PLAN, 0, st>>>(*c);
+    else kv_compact_plan_kernel<<<1, KV_PLAN, 0, st>>>(*c);
     PIO_LAUNCHED();
     return kv_copy(*c, c->n_pages / 2, true, st);
 }

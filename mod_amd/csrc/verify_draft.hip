@@ -162,30 +162,60 @@ __global__ __launch_bounds__(VD_THREADS) void vd_sum_kernel(VdArgs a) {
     }
 }
 
+// Of the workgroup's threads in order: the first one's `first` that is not INT_MAX (its
+// `at` in *before), and the last one's `some` that is not -1.
+struct VdPlace {
+    int first, last;
+    double before;
+};
+__device__ __forceinline__ VdPlace vd_place(int first, double at, int some, VdPlace* sh) {
+    const int wv = threadIdx.x >> 6;
+    const uint64_t f = __ballot(first != INT_MAX), l = __ballot(some >= 0);
+    VdPlace p;
+    p.first = f ? __shfl(first, __ffsll((unsigned long long)f) - 1, 64) : INT_MAX;
+    p.before = f ? __shfl(at, __ffsll((unsigned long long)f) - 1, 64) : 0.0;
+    p.last = l ? __shfl(some, 63 - __clzll((long long)l), 64) : -1;
+    if ((threadIdx.x & 63) == 0) sh[wv] = p;
+    __syncthreads();
+    p = sh[0];
+    for (int k = 1; k < VD_WAVES; k++) {
+        if (p.first == INT_MAX) {
+            p.first = sh[k].first;
+            p.before = sh[k].before;
+        }
+        p.last = max(p.last, sh[k].last);
+    }
+    return p;
+}
+
 // Second launch, one workgroup per request: the unit whose weights reach u_next *
-// total, and the token in it.
+// total, and the token in it. A chain of waits: what a request is and its sums, the
+// unit's weights; each thread has a few units in order, so that one scan gives both
+// the total and where it is reached.
 template <typename PT>
 __global__ __launch_bounds__(VD_THREADS) void vd_pick_kernel(VdArgs a) {
-    __shared__ int unit, place, last;
-    __shared__ double red[VD_WAVES], before_unit;
+    __shared__ VdPlace sh[2][VD_WAVES];
+    __shared__ double red[VD_WAVES];
     const int i = blockIdx.x, tid = threadIdx.x;
+    const int per = (a.units + VD_THREADS - 1) / VD_THREADS, first = min(tid * per, a.units), end = min(first + per, a.units);
+    double* sums = a.sums + (int64_t)i * a.units;
     VdRow r;
-    const int r0 = min(max(a.row_start[i], 0), a.rows), r1 = min(max(a.row_start[i + 1], r0), a.rows);
+    // (a request without rows has no sums: they are read all the same, with the rest)
+    const int s0 = a.row_start[i], s1 = a.row_start[i + 1];
+    r.accepted = a.accepted[i];
+    const double drawn = (double)a.u_next[i];
+    double mine = 0.0;
+    for (int u = first; u < end; u++) mine += sums[u];
+    const int r0 = min(max(s0, 0), a.rows), r1 = min(max(s1, r0), a.rows);
     if (r1 <= r0) return;
     r.first = r0;
     r.count = r1 - r0;
-    r.accepted = a.accepted[i];
     r.row = r0 + r.accepted;
     r.rejects = r.accepted < r.count - 1;
     const int id = r.rejects ? a.ids[r.row] : -1;
-    double* sums = a.sums + (int64_t)i * a.units;
     bool difference = r.rejects;
-    double total;
-    for (;;) {
-        double x = 0.0;
-        for (int u = tid; u < a.units; u += VD_THREADS) x += sums[u];
-        total = vd_block_sum(x, red);
-        if (total > 0.0 || !difference) break;
+    double total, base = vd_block_scan(mine, red, total);
+    if (!(total > 0.0) && difference) {
         // nothing is left of the target above the draft: the target's own weights
         difference = false;
         for (int u = 0; u < a.units; u++) {
@@ -195,55 +225,47 @@ __global__ __launch_bounds__(VD_THREADS) void vd_pick_kernel(VdArgs a) {
             if (tid == 0) sums[u] = s;
         }
         __syncthreads();
+        mine = 0.0;
+        for (int u = first; u < end; u++) mine += sums[u];
+        base = vd_block_scan(mine, red, total);
     }
-    if (tid == 0) {
-        unit = INT_MAX;
-        last = -1;
-        place = INT_MAX;
-    }
-    __syncthreads();
-    const double bar = (double)a.u_next[i] * total;
-    double before = 0.0;
-    for (int u0 = 0; u0 < a.units; u0 += VD_THREADS) {
-        const int u = u0 + tid;
-        const double s = u < a.units ? sums[u] : 0.0;
-        double all;
-        const double base = before + vd_block_scan(s, red, all);
+    const double bar = drawn * total;
+    int some = -1, found = INT_MAX;
+    double at = base, before = 0.0;
+    for (int u = first; u < end; u++) {
+        const double s = per == 1 ? mine : sums[u];
         if (s > 0.0) {
-            atomicMax(&last, u);
-            if (base + s > bar) atomicMin(&unit, u);
+            some = u;
+            if (found == INT_MAX && at + s > bar) {
+                found = u;
+                before = at;
+            }
         }
-        __syncthreads();
-        if (unit == u) before_unit = base;
-        if (unit != INT_MAX) break;
-        before += all;
+        at += s;
     }
-    __syncthreads();
+    const VdPlace unit = vd_place(found, before, some, sh[0]);
     // rounding (or u_next = 1) left none: the last one with a weight
-    const bool over = unit != INT_MAX;
-    const int u = over ? unit : last;
+    const bool over = unit.first != INT_MAX;
+    const int u = over ? unit.first : unit.last;
+    int token = -1;
     if (u >= 0) {
         double w[8], all;
         const int v = u * VD_UNIT + 8 * tid;
         vd_weights<PT>(a, r, id, difference, v, w);
-        double sum = (over ? before_unit : 0.0) + vd_block_scan(vd_sum8(w), red, all);
-        __syncthreads();
-        if (tid == 0) last = -1;
-        __syncthreads();
-        int some = -1, first = INT_MAX;
+        double sum = (over ? unit.before : 0.0) + vd_block_scan(vd_sum8(w), red, all);
+        int some = -1, found = INT_MAX;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             sum += w[e];
             if (w[e] > 0.0) {
                 some = v + e;
-                if (over && sum > bar) first = min(first, v + e);
+                if (over && sum > bar) found = min(found, v + e);
             }
         }
-        if (some >= 0) atomicMax(&last, some);
-        if (first != INT_MAX) atomicMin(&place, first);
-        __syncthreads();
+        const VdPlace place = vd_place(found, 0.0, some, sh[1]);
+        token = place.first != INT_MAX ? place.first : place.last;
     }
-    if (tid == 0) a.tokens[r.row] = place != INT_MAX ? place : last;
+    if (tid == 0) a.tokens[r.row] = token;
 }
 
 }  // namespace pio
@@ -257,6 +279,7 @@ PIO_EXPORT int pio_verify_draft(const void* target, int64_t target_stride, const
     const char* nm = "pio_verify_draft";
     PIO_REQUIRE(dtype == PIO_F32 || dtype == PIO_F16, "%s: dtype %d (fp32 or fp16)", nm, dtype);
     PIO_REQUIRE(n >= 0 && rows >= 0 && vocab > 0, "%s: %d requests, %d rows, vocabulary of %d", nm, n, rows, vocab);
+    PIO_REQUIRE(vocab <= 1 << 30, "%s: a vocabulary of over 2^30", nm);
     if (n == 0) return PIO_OK;
     PIO_REQUIRE(row_start && accepted && u_next, "%s: null pointer", nm);
     PIO_REQUIRE(rows == 0 || (target && ids && u && tokens), "%s: null pointer", nm);

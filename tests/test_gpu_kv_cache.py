@@ -14,6 +14,8 @@ of v rows). With u = 2^-24 (half a step of fp32) and smax the largest |score|:
   - fp32 queries over an fp16 cache: queries and weights are two fp16 parts,
     each pair off by at most 2^-22: 2^-22 of sum |q k| in a score, 2^-22 of the
     weights (fp16 outputs of any path are rounded, 2^-11)."""
+import collections
+
 import numpy as np
 import pytest
 
@@ -48,6 +50,7 @@ class Pair:
         if fill is not None:
             self.ref.kv[:] = fill
         self.kv = torch.from_numpy(self.ref.kv.copy()).cuda()
+        self.kept = collections.deque(maxlen=64)
         self.table = torch.full((seqs, width), 77, dtype=torch.int32, device="cuda")
         self.lens = torch.full((seqs,), 77, dtype=torch.int32, device="cuda")
         self.refs = torch.full((pages,), 77, dtype=torch.int32, device="cuda")
@@ -56,12 +59,12 @@ class Pair:
         ops.kv_init(self.c)
 
     def ints(self, v):
-        t = self.t.tensor([int(x) for x in v], dtype=self.t.int32, device="cuda")
-        self.t.cuda.synchronize()
-        return t
+        return self.dev(np.array([int(x) for x in v], np.int32))
 
     def dev(self, a):
         t = self.t.from_numpy(np.ascontiguousarray(a)).cuda()
+        # kept until the kernels that read it are done: the next ones wait for the device too
+        self.kept.append(t)
         self.t.cuda.synchronize()
         return t
 
@@ -228,6 +231,32 @@ def test_many_pages_and_requests(torch, ops):
     p.same()
     p.drop([int(s) for s in rng.permutation(4100)[:3000]])
     p.compact()
+    p.same()
+    ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("pages", [1, 3, 1023, 1024, 1025])
+def test_plans_at_their_steps(torch, ops, pages):
+    """Caches of one page to a thread and of one more; every page in use, and one free."""
+    rng = np.random.default_rng(pages)
+    p = Pair(torch, ops, 1, 1, 8, 2, pages, 70, 600)
+    p.add(rng, [0], [min(2 * pages, 1200)])
+    if pages > 600:
+        p.add(rng, [1], [2 * (pages - 600)])
+    assert np.all(p.ref.refs == 1)
+    p.compact()
+    p.same()
+    ops.kv_reserve(p.c, p.ints([2]), p.ints([1]), 1)
+    p.same()
+    with pytest.raises(ops.RocmError, match="too few free pages"):
+        ops.kv_status(p.c)
+    p.drop([0], [min(2 * pages, 1200) // 2])
+    p.add(rng, list(range(2, 70, 5)), [2 if pages > 600 else 0] * 14)
+    p.drop([0])
+    p.same()
+    p.compact()
+    p.same()
+    p.add(rng, [0], [min(2 * int((p.ref.refs == 0).sum()), 1200)])
     p.same()
     ops.kv_status(p.c)
 
@@ -513,3 +542,173 @@ def test_attention_far_pages(torch, ops):
         ref = torch.matmul(torch.softmax(s, 2), vv).transpose(0, 1)
         # |score| < 6, sum |q k| scale < 12: 2 (4 u sqrt(128) 7 + 12 / 2^22) + 48 u + 2^-22 = 4.7e-5
         assert float((out[a:b].double() - ref).abs().max()) < 4.7e-5 * float(v.abs().max())
+
+
+# -------------------------------------------------------------- as one step ---
+@pytest.mark.parametrize("dtype,x", [("float32", "float32"), ("float16", "float32"), ("float16", "float16")])
+def test_speculative_serving(torch, ops, dtype, x):
+    """All calls as a server makes them. A prompt that all requests share; in each step every
+    request's pending token and a few drafted ones join the cache, are attended to in every layer,
+    verified, and those that were refused go again, by counts that never leave the device.
+    Requests end and new ones begin from the prompt; the pages are compacted as it goes on."""
+    rng = np.random.default_rng(21)
+    layers, H, Hk, D, V, n, prompt = 2, 8, 4, 64, 3001, 6, 45
+    p = Pair(torch, ops, layers, Hk, D, 16, 64, n + 3, 12, dtype, fill=np.nan)
+    p.add(rng, [0], [prompt])
+    live = list(range(1, n + 1))
+    p.fork([0] * n, live)
+    head = torch.randn(H * D, V, device="cuda")
+    taken = 0
+    for step in range(14):
+        _say(f"step {step}")
+        counts = [int(c) for c in rng.integers(1, 6, len(live))]
+        start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+        rows = int(start[-1])
+        p.add(rng, live, counts, x)
+        for layer in range(layers):
+            q = rng.standard_normal((rows, H, D)).astype(x)
+            ref = p.ref.attention(layer, live, start, q, D ** -0.5, np.zeros(q.shape))
+            got = _attend(p, torch, ops, layer, live, start, q, D ** -0.5, prompt, 5)
+            tol = _tolerance(p, layer, live, start, q, D ** -0.5, x == "float16")
+            assert np.abs(got.astype(np.float64) - ref).max() <= tol
+        hidden = torch.from_numpy(got).cuda().float().reshape(rows, H * D)
+        target = torch.softmax(hidden @ head, 1)
+        draft = torch.softmax((hidden + 0.02 * torch.randn_like(hidden)) @ head, 1)
+        ids = torch.multinomial(draft, 1).reshape(rows).int()
+        u, u_next = torch.rand(rows, device="cuda"), torch.rand(len(live), device="cuda")
+        i32 = dict(dtype=torch.int32, device="cuda")
+        accepted, tokens, rejected = torch.empty(len(live), **i32), torch.empty(rows, **i32), torch.empty(len(live), **i32)
+        torch.cuda.synchronize()
+        ops.verify_draft(target, draft, ids, u, u_next, p.ints(start), len(live), rows, V, accepted, tokens, rejected)
+        ops.kv_drop(p.c, p.ints(live), rejected, len(live))
+        ref = kv_ref.verify(*(t.cpu().numpy() for t in (target, draft, ids, u, u_next)), start)
+        torch.cuda.synchronize()
+        for a, b in zip((accepted, tokens, rejected), ref):
+            assert np.array_equal(a.cpu().numpy(), b)
+        assert p.ref.drop(live, [int(r) for r in ref[2]]) == []
+        taken += int(np.sum(ref[0]))
+        p.same()
+        if step % 3 == 2:                           # two requests end, one begins
+            gone = [live.pop(int(rng.integers(len(live)))) for _ in range(2)]
+            p.drop(gone)
+            free = next(s for s in range(1, n + 3) if p.ref.lens[s] == 0)
+            p.fork([0], [free])
+            live.append(free)
+        if step % 4 == 3:
+            p.compact()
+            p.same()
+    assert 0 < taken
+    ops.kv_status(p.c)
+
+
+class Step:
+    """A step with inputs at fixed places, for graphs: every call of the cache and the verification."""
+
+    def __init__(self, torch, ops, seed, dtype="float16"):
+        self.t, self.ops = torch, ops
+        rng = np.random.default_rng(seed)
+        self.p = p = Pair(torch, ops, 2, 4, 64, 16, 80, 10, 20, dtype, fill=0)
+        p.add(rng, [0], [70])
+        p.fork([0] * 5, [1, 2, 3, 4, 5])
+        self.n, self.rows, self.V = 5, 13, 4099
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.seq, self.start = torch.tensor([3, 1, 5, 2, 4], **i32), torch.tensor([0, 3, 4, 8, 10, 13], **i32)
+        self.count, self.last = torch.tensor([3, 1, 4, 2, 3], **i32), torch.tensor([9], **i32)
+        self.zero = torch.tensor([0], **i32)
+        self.q = torch.empty(13, 8, 64, device="cuda")
+        self.k, self.v = torch.empty(2, 13, 256, device="cuda"), torch.empty(2, 13, 256, device="cuda")
+        self.out = torch.empty(2, 13, 8, 64, device="cuda")
+        self.target, self.draft = torch.empty(13, 4099, device="cuda"), torch.empty(13, 4099, device="cuda")
+        self.u, self.u_next = torch.empty(13, device="cuda"), torch.empty(5, device="cuda")
+        self.ids = torch.empty(13, **i32)
+        self.accepted, self.tokens, self.rejected = torch.empty(5, **i32), torch.empty(13, **i32), torch.empty(5, **i32)
+        self.g = g
+        torch.cuda.synchronize()
+
+    def fill(self):
+        """New inputs (the device is waited for before and after)."""
+        t = self.t
+        t.cuda.synchronize()
+        for a in (self.q, self.k, self.v):
+            a.copy_(t.randn(a.shape, device="cuda", generator=self.g))
+        logits = 3 * t.randn(self.target.shape, device="cuda", generator=self.g)
+        self.target.copy_(t.softmax(logits, 1))
+        self.draft.copy_(t.softmax(logits + 0.3 * t.randn(logits.shape, device="cuda", generator=self.g), 1))
+        self.ids.copy_(t.multinomial(self.draft, 1, generator=self.g).reshape(13))
+        for a in (self.u, self.u_next):
+            a.copy_(t.rand(a.shape, device="cuda", generator=self.g))
+        t.cuda.synchronize()
+
+    def run(self, stream=None):
+        o, c = self.ops, self.p.c
+        o.kv_reserve(c, self.seq, self.count, 5, stream=stream)
+        o.kv_write(c, 0, 2, self.seq, self.start, 5, self.k, self.v, 13, stream=stream)
+        for layer in range(2):
+            o.kv_attention(c, layer, self.seq, self.start, 5, self.q, self.out[layer], 13, 8, 0.125, shared=70, max_rows=4,
+                           stream=stream)
+        o.verify_draft(self.target, self.draft, self.ids, self.u, self.u_next, self.start, 5, 13, self.V, self.accepted,
+                       self.tokens, self.rejected, stream=stream)
+        o.kv_drop(c, self.seq, self.rejected, 5, stream=stream)
+        o.kv_fork(c, self.seq, self.last, 1, stream=stream)     # a copy of the first request, and gone again
+        o.kv_drop(c, self.last, None, 1, stream=stream)
+        o.kv_compact(c, stream=stream)
+
+    def state(self):
+        self.t.cuda.synchronize()
+        p = self.p
+        return [a.clone() for a in (p.table, p.lens, p.refs, self.out, self.accepted, self.tokens, self.rejected)]
+
+
+def _alike(torch, a, b):
+    for x, y in zip(a.state(), b.state()):
+        assert torch.equal(x, y)
+    # a page that no sequence holds may differ
+    held = a.p.refs.bool()
+    assert torch.equal(a.p.kv[:, :, held], b.p.kv[:, :, held])
+
+
+def test_captured_step(torch, ops):
+    """A step captured by the library's own graph, its first call included, replayed with new inputs
+    and eager work between, against the same steps run one call after the other."""
+    from mod_amd import backend
+    eager, captured = Step(torch, ops, 5), Step(torch, ops, 5)
+    graph = backend.HIPGraph()
+    graph.capture_begin()
+    captured.run()
+    graph.capture_end()
+    for i in range(6):
+        _say(f"replay {i}")
+        for s in (eager, captured):
+            s.fill()
+        graph.replay()
+        eager.run()
+        _alike(torch, eager, captured)
+        torch.randn(1 << 20, device="cuda").sum().item()
+    for s in (eager, captured):
+        ops.kv_status(s.p.c)
+
+
+def test_two_graphs_and_streams(torch, ops):
+    """Two captured steps of two caches, replayed at once on two streams, against eager steps."""
+    eager = [Step(torch, ops, 6), Step(torch, ops, 7)]
+    captured = [Step(torch, ops, 6), Step(torch, ops, 7)]
+    streams, graphs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for s, st in zip(captured, streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            s.run(stream=st)
+        graphs.append(g)
+    for i in range(5):
+        _say(f"replay {i}")
+        for s in eager + captured:
+            s.fill()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        for s in eager:
+            s.run()
+        for a, b in zip(eager, captured):
+            _alike(torch, a, b)
+    for s, st in zip(eager + captured, [None, None] + streams):
+        ops.kv_status(s.p.c, stream=st)

@@ -170,3 +170,16 @@ def test_long_window(torch, ops):
         q = np.where(np.arange(k)[:, None] == stop, 1.0, p * 0.5).astype(np.float32)
         got = _check(torch, ops, p, q, rng.integers(0, V, k), u, rng.random(1), [0, k])
         assert got[0][0] == min(stop, k - 1)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_large_vocabulary(torch, ops, dtype):
+    """More units of the vocabulary than a workgroup has threads; nothing left of the target above the draft there."""
+    rng = np.random.default_rng(4)
+    V = 600001
+    p, q = _probs(rng, 6, V, dtype, 1.0), _probs(rng, 6, V, dtype, 1.0)
+    ids = rng.integers(0, V, 6)
+    for un in (0.0, 0.37, 1.0):
+        _check(torch, ops, p, q, ids, np.ones(6), np.full(3, un), [0, 1, 4, 6])
+    got = _check(torch, ops, p, p, ids, np.ones(6), rng.random(3), [0, 1, 4, 6])
+    assert np.all(got[0] == 0) and np.all(got[1][[0, 1, 4]] >= 0)

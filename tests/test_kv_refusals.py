@@ -98,6 +98,7 @@ def test_attention(change, error):
 
 @pytest.mark.parametrize("change,error", [
     (dict(dtype=2), "dtype"), (dict(n=-1), "requests"), (dict(rows=-1), "rows"), (dict(vocab=0), "vocabulary"),
+    (dict(vocab=(1 << 30) + 1), "vocabulary"),
     (dict(target=None), "null"), (dict(ids=None), "null"), (dict(u=None), "null"), (dict(u_next=None), "null"),
     (dict(start=None), "null"), (dict(accepted=None), "null"), (dict(tokens=None), "null"),
     (dict(target_stride=99), "strides"), (dict(draft_stride=99), "strides"), (dict(target=66), "unaligned"),
