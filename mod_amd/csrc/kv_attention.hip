@@ -23,6 +23,7 @@
 #include "kv_pages.hpp"
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <float.h>
 #include <type_traits>
@@ -43,7 +44,9 @@ struct KaArgs {
     bool q16;
     // items of the matrix core kernels
     int pre_items, pre_tiles, pre_splits, pre_keys;   // workgroups; column tiles; runs of keys, keys of each
-    int tail_tiles, tail_runs, max_runs;              // column tiles; runs of all requests that are aimed at, and of one
+    int tail_tiles, tail_runs, max_runs;              // column tiles; the most runs beside one for each request, and of one
+    int slots;                                        // items that the device holds at once
+    float pre_work;                                   // rounds of keys that the prefix's items cost
     int tail_items;                                   // (run, column tile, kv head)
     bool direct;                                      // one item per column: it writes out itself
     float* part_o;                                    // [pre_splits + max_runs][rows * H][D]
@@ -628,6 +631,16 @@ __device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it
 }
 
 constexpr int KA_ROUND = 128;          // keys that runs are multiples of
+// An item costs its rounds of keys and this many more (its requests, pages, first copies; its
+// join and output): 12,000 clocks beside 3,400 of a round.
+constexpr float KA_FIXED = 3.5f;
+// Rounds of keys for each of the runs that `rounds` are cut into, if every run is an item in
+// each of `units` places and all else costs `work`: the longest item, KA_FIXED + r, takes as
+// long as the device's share of all work.
+__device__ __forceinline__ float ka_cut(float rounds, float units, float work, float slots) {
+    const float d = (work + units * rounds) / slots - KA_FIXED;
+    return 0.5f * (d + sqrtf(d * d + 4.f * KA_FIXED * units / slots * rounds));
+}
 
 // Sum over the workgroup's threads before this one, and over all.
 __device__ __forceinline__ int ka_scan(int v, int* red, int& total) {
@@ -677,12 +690,20 @@ __device__ __forceinline__ void ka_runs(const KaArgs& a, int run, KaRun& found, 
         ka_scan(rounds(i0 + tid), red, sum);
         total += min(sum, INT_MAX - total);
     }
-    const int most = max(1, (int)(((int64_t)total + a.tail_runs - 1) / a.tail_runs));
+    const float units = a.c.n_kv_heads * a.tail_tiles;
+    // runs that balance the items, or of KA_FIXED rounds: the last items to start should be short ones
+    // (and at most tail_runs more runs than requests)
+    const float cut = fmaxf(fmaxf(1.f, (float)total / a.tail_runs),
+                            fminf(KA_FIXED, ka_cut(total, units, a.pre_work + a.n * units * KA_FIXED, a.slots)));
     int before = 0;
     for (int i0 = 0; i0 < a.n; i0 += threads) {
         if (a.n > threads) n = rounds(i0 + tid);
-        r.per = max(most, (n + a.max_runs - 1) / a.max_runs);
-        r.runs = (n + r.per - 1) / r.per;
+        r.per = r.runs = 0;
+        if (n > 0) {
+            r.runs = min(max(1, (int)(n / cut + 0.5f)), a.max_runs);
+            r.per = (n + r.runs - 1) / r.runs;
+            r.runs = (n + r.per - 1) / r.per;
+        }
         const int at = before + ka_scan(r.runs, red, sum);
         before += sum;
         if (run >= at && run < at + r.runs) {
@@ -933,6 +954,11 @@ constexpr int KA_WIDE_COLS = 128, KA_WIDE_KEYS = 64, KA_STAGES = 4, KA_WIDE_PAGE
 template <int D>
 constexpr size_t ka_wide_bytes() {
     return std::max<size_t>((size_t)KA_STAGES * 2 * KA_WIDE_KEYS * D * 2, (size_t)KA_WIDE_COLS * (D + 4) * 4);
+}
+
+template <int D>
+constexpr size_t ka_wide_lds() {
+    return ka_wide_bytes<D>() + KA_WIDE_PAGES * sizeof(int);
 }
 
 template <int D, int XP>
@@ -1207,7 +1233,7 @@ __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
 template <typename KT, int D, int XP, int WIDE>
 static int ka_launch(const KaArgs& a, hipStream_t st) {
     size_t lds = ka_narrow_bytes<KT, D>();
-    if constexpr (WIDE) lds = ka_wide_bytes<D>() + KA_WIDE_PAGES * sizeof(int);
+    if constexpr (WIDE) lds = ka_wide_lds<D>();
     PIO_TRY((allow_lds<ka_kernel<KT, D, XP, WIDE>>(lds)));
     ka_kernel<KT, D, XP, WIDE><<<a.pre_items + (WIDE == 1 ? 0 : a.tail_items), WIDE ? 512 : 256, lds, st>>>(a);
     PIO_LAUNCHED();
@@ -1239,6 +1265,26 @@ static int ka_route(const KaArgs& a, int wide, hipStream_t st) {
     return a.q16 ? ka_route16<D, 1>(a, wide, st) : ka_route16<D, 2>(a, wide, st);
 }
 
+// Workgroups of the tails' kernel that a CU holds.
+template <typename KT, int D, int XP, int WIDE>
+static int ka_held_by(int& held) {
+    static std::atomic<int> known{0};
+    held = known.load(std::memory_order_relaxed);
+    if (held) return PIO_OK;
+    const size_t lds = WIDE ? ka_wide_lds<D>() : ka_narrow_bytes<KT, D>();
+    PIO_TRY((allow_lds<ka_kernel<KT, D, XP, WIDE>>(lds)));
+    PIO_HIP(hipOccupancyMaxActiveBlocksPerMultiprocessor(&held, ka_kernel<KT, D, XP, WIDE>, WIDE ? 512 : 256, lds));
+    held = std::max(held, 1);
+    known.store(held, std::memory_order_relaxed);
+    return PIO_OK;
+}
+template <int D>
+static int ka_held(const KaArgs& a, bool wide, int& held) {
+    if (a.c.kv_dtype == PIO_F32) return ka_held_by<float, D, 1, 0>(held);
+    if (wide) return a.q16 ? ka_held_by<_Float16, D, 1, 2>(held) : ka_held_by<_Float16, D, 2, 2>(held);
+    return a.q16 ? ka_held_by<_Float16, D, 1, 0>(held) : ka_held_by<_Float16, D, 2, 0>(held);
+}
+
 // Items for the matrix core kernels.
 static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
@@ -1247,27 +1293,32 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     // A wide kernel for the prefix reads it once for 128 columns, but comes on top of the tails', some
     // 10 us: 512 columns x 4 kv heads x 128 dimensions over 4,096 tokens 39 us (narrow 32), over 8,192
     // 42 (43), over 16,000 50 (65); 256 x 8 x 64 over 8,000 30 (26), over 32,000 52 (73).
-    const bool long_prefix = cols > 64 && (double)cols * Hk * a.c.head_dim * a.shared >= 0x1p31;
+    const bool long_prefix = cols > 64 && (double)cols * Hk * a.c.head_dim * a.shared >= 0x1.8p30;
     const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : long_prefix ? 1 : 0;
     a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
     const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
     PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
-    // tails: as many runs as the device holds at once, in all and of one request (up to one
-    // more for each request comes on top; where workgroups are one to a CU that would be a second round)
-    const int64_t runs = (wide == 2 ? cus : 2 * cus) / ((int64_t)Hk * a.tail_tiles);
-    a.tail_runs = (int)std::max<int64_t>({1, runs - (wide == 2 ? a.n : 0), runs / 2});
+    // Runs. The lengths of the tails are not known here: a short prefix gets a quarter of the device,
+    // a longer one up to all of it in runs of 8 rounds or more, and the tails are cut for what is there
+    // by the kernel (ka_runs). 32 sequences behind 2,039 tokens 17 us, where both are cut to
+    // fill the device on their own 24 us.
+    int held = 1;
+    PIO_TRY(a.c.head_dim == 128 ? ka_held<128>(a, wide == 2, held) : ka_held<64>(a, wide == 2, held));
+    a.slots = cus * held;
+    const int64_t units = (int64_t)Hk * a.tail_tiles;
+    a.tail_runs = (int)std::max<int64_t>(1, (wide == 2 ? cus / 2 : 2 * cus) / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND)});
     a.direct = a.shared == 0 && a.max_runs == 1;
-    a.tail_items = (int)(items + (a.direct ? 0 : (int64_t)a.tail_runs * Hk * a.tail_tiles));
+    a.tail_items = (int)(items + (a.direct ? 0 : (int64_t)a.tail_runs * units));
     if (a.shared > 0) {
-        // prefix: as many items as the device holds at once, each of at least KA_ROUND keys
-        const int width = wide ? KA_WIDE_COLS : KA_COLS;
-        const int at_once = wide ? cus : 2 * cus;
-        a.pre_tiles = ceil_div(cols, width);
-        const int64_t splits = std::max<int64_t>(1, at_once / std::max<int64_t>(1, (int64_t)Hk * a.pre_tiles));
-        a.pre_keys = ceil_div(ceil_div(a.shared, std::min<int64_t>(splits, a.shared)), KA_ROUND) * KA_ROUND;
+        a.pre_tiles = ceil_div(cols, wide ? KA_WIDE_COLS : KA_COLS);
+        const int64_t pre_units = (int64_t)Hk * a.pre_tiles, rounds = ceil_div(a.shared, KA_ROUND), at_once = wide ? cus : 2 * cus;
+        const int64_t most = at_once / pre_units;
+        const int64_t splits = std::max<int64_t>({1, most / 4, wide == 1 ? most : std::min(rounds / 8, most)});
+        a.pre_keys = (int)ceil_div(rounds, std::min(splits, rounds)) * KA_ROUND;
         a.pre_splits = ceil_div(a.shared, a.pre_keys);
+        if (wide != 1) a.pre_work = (float)pre_units * (a.pre_splits * KA_FIXED + rounds);
         const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
         PIO_REQUIRE(pre <= INT_MAX / 2, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)pre;
