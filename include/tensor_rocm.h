@@ -363,7 +363,7 @@ int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t*
  * `layers` layers from `layer`. k and v [layers][rows][n_kv_heads * head_dim]
  * with rows `row_stride` and layers `layer_stride` elements apart (each a
  * multiple of 8, or 0 for dense rows / layers), fp32|fp16, rounded to the
- * cache's type, 16-byte aligned. row_start int32 [n + 1], ascending; rows at
+ * cache's type, 16-byte aligned, each sequence once, fewer than 2^24 rows. row_start int32 [n + 1], ascending; rows at
  * and behind row_start[n] are not read. */
 int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
                  int n, const void* k, const void* v, int dtype, int rows, int64_t row_stride,
@@ -388,7 +388,7 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * common system prompt, say; 0: none): they are read through the table row of
  * seq[0], once for all queries. q and out fp32|fp16 [rows, n_heads, head_dim],
  * rows q_stride / out_stride elements apart (multiples of 8), 16-byte aligned;
- * out may be q. max_rows: the most queries that one sequence has (larger ones
+ * out may be q (at one stride). max_rows: the most queries that one sequence has (larger ones
  * are served too, but slower). A sequence id or a page outside the cache gives
  * NaN rows. Products and sums in fp32: of fp16 queries over an fp16 cache on
  * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32

@@ -25,6 +25,7 @@
 #include <algorithm>
 #include <atomic>
 #include <climits>
+#include <cmath>
 #include <float.h>
 #include <type_traits>
 
@@ -1297,7 +1298,7 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : long_prefix ? 1 : 0;
     a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
     const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
-    PIO_REQUIRE(items <= INT_MAX / 64, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
+    PIO_REQUIRE(items <= 1 << 22, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
     // Runs. The lengths of the tails are not known here: a short prefix gets a quarter of the device,
     // a longer one up to all of it in runs of 8 rounds or more, and the tails are cut for what is there
     // by the kernel (ka_runs). 32 sequences behind 2,039 tokens 17 us, where both are cut to
@@ -1308,7 +1309,9 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int64_t units = (int64_t)Hk * a.tail_tiles;
     a.tail_runs = (int)std::max<int64_t>(1, (wide == 2 ? cus / 2 : 2 * cus) / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND)});
+    // (and no more than 256 MB of the workspace: many requests fill the device without)
+    const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
+    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
     a.direct = a.shared == 0 && a.max_runs == 1;
     a.tail_items = (int)(items + (a.direct ? 0 : (int64_t)a.tail_runs * units));
     if (a.shared > 0) {
@@ -1320,7 +1323,7 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
         a.pre_splits = ceil_div(a.shared, a.pre_keys);
         if (wide != 1) a.pre_work = (float)pre_units * (a.pre_splits * KA_FIXED + rounds);
         const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
-        PIO_REQUIRE(pre <= INT_MAX / 2, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
+        PIO_REQUIRE(pre <= 1 << 22, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)pre;
     }
     Scratch ws;
@@ -1361,7 +1364,11 @@ PIO_EXPORT int pio_kv_attention(const pio_kv_cache* c, int layer, const int32_t*
                 "%s: strides %lld, %lld (multiples of 8, rows of %lld)", nm, (long long)q_stride, (long long)out_stride,
                 (long long)width);
     PIO_REQUIRE(aligned16(q) && aligned16(out), "%s: q or out not 16-byte aligned", nm);
-    PIO_REQUIRE((int64_t)rows * n_heads <= INT_MAX, "%s: too many rows", nm);
+    PIO_REQUIRE(out != q || q_stride == out_stride, "%s: out is q, at another stride", nm);
+    // (a grid has fewer than 2^32 threads: the join's 8 columns to a workgroup, the simple kernel's one)
+    const bool matrix = c->head_dim == 128 || c->head_dim == 64;
+    PIO_REQUIRE((int64_t)rows * n_heads < (matrix ? 1 << 26 : 1 << 24), "%s: too many rows", nm);
+    PIO_REQUIRE(std::isfinite(scale), "%s: scale %g", nm, (double)scale);
     KaArgs a{};
     a.c = *c;
     a.seq = seq;
@@ -1380,7 +1387,7 @@ PIO_EXPORT int pio_kv_attention(const pio_kv_cache* c, int layer, const int32_t*
     a.scale = scale;
     a.q16 = dtype == PIO_F16;
     hipStream_t st = pick_stream(stream);
-    if (c->head_dim == 128 || c->head_dim == 64) return ka_matrix(a, max_rows, st);
+    if (matrix) return ka_matrix(a, max_rows, st);
     if (c->kv_dtype == PIO_F32) ka_simple_kernel<float><<<rows * n_heads, KA_THREADS, 0, st>>>(a);
     else ka_simple_kernel<_Float16><<<rows * n_heads, KA_THREADS, 0, st>>>(a);
     PIO_LAUNCHED();

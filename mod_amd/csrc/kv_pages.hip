@@ -514,7 +514,7 @@ PIO_EXPORT int pio_kv_write(const pio_kv_cache* c, int layer, int layers, const 
     PIO_REQUIRE(layer >= 0 && layers >= 0 && layers <= c->n_layers - layer, "%s: layers %d + %d of %d", nm, layer, layers,
                 c->n_layers);
     PIO_REQUIRE(dtype == PIO_F32 || dtype == PIO_F16, "%s: dtype %d (fp32 or fp16)", nm, dtype);
-    PIO_REQUIRE(rows >= 0, "%s: %d rows", nm, rows);
+    PIO_REQUIRE(rows >= 0 && rows < 1 << 24, "%s: %d rows (fewer than 2^24)", nm, rows);    // (2^32 threads of a grid)
     if (n == 0 || rows == 0 || layers == 0) return PIO_OK;
     PIO_REQUIRE(k && v, "%s: null k or v", nm);
     PIO_REQUIRE(aligned16(k) && aligned16(v), "%s: k or v not 16-byte aligned", nm);

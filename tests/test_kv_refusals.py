@@ -86,7 +86,8 @@ def test_write(change, error):
     (dict(heads=6), "heads"), (dict(max_rows=0), "max_rows"), (dict(q=None), "null"), (dict(out=None), "null"),
     (dict(seq=None), "null"), (dict(start=None), "null"), (dict(q=72), "16-byte"), (dict(out=8), "16-byte"),
     (dict(seq=66), "4-byte"), (dict(q_stride=500), "strides"), (dict(out_stride=504), "strides"),
-    (dict(rows=1 << 29), "too many rows")])
+    (dict(rows=1 << 29), "too many rows"), (dict(rows=1 << 23), "too many rows"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"), (dict(out_stride=520), "another stride")])
 def test_attention(change, error):
     from mod_amd import ops
     f = dict(layer=0, seq=64, start=64, n=1, shared=0, q=64, out=64, dtype=0, rows=4, heads=8, q_stride=0, out_stride=0,
