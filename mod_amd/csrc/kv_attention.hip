@@ -237,8 +237,13 @@ struct KaQ<float, D, COLS, 1> {
 // Maximum over the parts of a column.
 template <int COLS>
 __device__ __forceinline__ float ka_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 32, 64));
-    if constexpr (COLS == 16) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    // (the halves of the wave swapped, then neighbouring rows of 16 lanes: no trip through LDS)
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    if constexpr (COLS == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
     return v;
 }
 
@@ -497,53 +502,81 @@ __device__ __forceinline__ void ka_weights(KaAcc<KT, D, COLS>& x, float (&s)[Ka<
     x.l += sum[0];
 }
 
-// O^T += V^T P^T over one tile (fp16: operands vs; fp32: rows at vt). In a tile that
-// some column does not see all of (edge), a value of inf or NaN would make that column
-// NaN, 0 * inf: such values are left out, and true is returned (in every lane): ka_mend
-// adds them to the columns that see them.
-template <typename KT, int D, int COLS, int XP>
-__device__ __forceinline__ bool ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS],
-                                          KaValuesOf<D, COLS>& vs, uint32_t vt, uint32_t vx, bool edge) {
-    using T = Ka<KT, D, COLS>;
-    bool odd = false;
-    if constexpr (T::F16) {
-        constexpr int KC = KaValuesOf<D, COLS>::KC;
-        if (edge) {
-            ka_h8 z = {0, 0, 0, 0, 0, 0, 0, 0};        // stays 0, but for inf and NaN
+// fp16 weights as operands, in XP parts.
+template <int D, int COLS, int XP>
+struct KaWeights {
+    static constexpr int KC = KaValuesOf<D, COLS>::KC;
+    ka_h8 w[KC][XP];
+    __device__ __forceinline__ void pack(const float (&p)[8 * KC]) {
 #pragma unroll
-            for (int n = 0; n < T::NT; n++)
-#pragma unroll
-                for (int kc = 0; kc < KC; kc++) z = vs.v[n][kc] * (_Float16)0 + z;
-            bool any = false;
-#pragma unroll
-            for (int e = 0; e < 8; e++) any |= z[e] != z[e];
-            odd = __any(any);
-            if (odd) {
-#pragma unroll
-                for (int n = 0; n < T::NT; n++)
-#pragma unroll
-                    for (int kc = 0; kc < KC; kc++)
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            const _Float16 v = vs.v[n][kc][e];
-                            vs.v[n][kc][e] = v * (_Float16)0 == (_Float16)0 ? v : (_Float16)0;
-                        }
-            }
-        }
-#pragma unroll
-        for (int kc = 0; kc < KC; kc++) {
-            ka_h8 w[XP];
+        for (int kc = 0; kc < KC; kc++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const _Float16 hi = (_Float16)p[8 * kc + e];
-                w[0][e] = hi;
-                if constexpr (XP == 2) w[XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
+                w[kc][0][e] = hi;
+                if constexpr (XP == 2) w[kc][XP - 1][e] = (_Float16)(p[8 * kc + e] - (float)hi);
             }
+    }
+    // computed where this stands: the compiler would sink it behind the next branch
+    __device__ __forceinline__ void here() {
 #pragma unroll
-            for (int n = 0; n < T::NT; n++)
+        for (int kc = 0; kc < KC; kc++)
 #pragma unroll
-                for (int i = 0; i < XP; i++) x.o[n] = T::mfma(vs.v[n][kc], w[i], x.o[n]);
-        }
+            for (int i = 0; i < XP; i++) asm volatile("" : "+v"(w[kc][i]));
+    }
+};
+
+// O^T += V^T P^T over one tile. In a tile that some column does not see all of, a value
+// of inf or NaN would make that column NaN, 0 * inf: such values are left out (ka_finite,
+// for fp16; it returns whether there were any, in every lane), and ka_mend adds them to
+// the columns that see them.
+template <int D, int COLS>
+__device__ __forceinline__ bool ka_finite(KaValuesOf<D, COLS>& vs) {
+    using T = Ka<_Float16, D, COLS>;
+    constexpr int KC = KaValuesOf<D, COLS>::KC;
+    ka_h8 z = {0, 0, 0, 0, 0, 0, 0, 0};        // stays 0, but for inf and NaN
+#pragma unroll
+    for (int n = 0; n < T::NT; n++)
+#pragma unroll
+        for (int kc = 0; kc < KC; kc++) z = vs.v[n][kc] * (_Float16)0 + z;
+    bool any = false;
+#pragma unroll
+    for (int e = 0; e < 8; e++) any |= z[e] != z[e];
+    if (!__any(any)) return false;
+#pragma unroll
+    for (int n = 0; n < T::NT; n++)
+#pragma unroll
+        for (int kc = 0; kc < KC; kc++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const _Float16 v = vs.v[n][kc][e];
+                vs.v[n][kc][e] = v * (_Float16)0 == (_Float16)0 ? v : (_Float16)0;
+            }
+    return true;
+}
+template <int D, int COLS, int XP>
+__device__ __forceinline__ void ka_product(KaAcc<_Float16, D, COLS>& x, const KaWeights<D, COLS, XP>& w,
+                                           const KaValuesOf<D, COLS>& vs) {
+    using T = Ka<_Float16, D, COLS>;
+#pragma unroll
+    for (int kc = 0; kc < KaValuesOf<D, COLS>::KC; kc++)
+#pragma unroll
+        for (int n = 0; n < T::NT; n++)
+#pragma unroll
+            for (int i = 0; i < XP; i++) x.o[n] = T::mfma(vs.v[n][kc], w.w[kc][i], x.o[n]);
+}
+template <typename KT, int D, int COLS, int XP>
+__device__ __forceinline__ bool ka_values(KaAcc<KT, D, COLS>& x, const float (&p)[Ka<KT, D, COLS>::NS], uint32_t vt,
+                                          uint32_t vx, bool edge) {
+    using T = Ka<KT, D, COLS>;
+    bool odd = false;
+    if constexpr (T::F16) {
+        KaValuesOf<D, COLS> vs;
+        vs.read(vt, vx);
+        if (edge) odd = ka_finite<D, COLS>(vs);
+        KaWeights<D, COLS, XP> w;
+        w.pack(p);
+        ka_product<D, COLS, XP>(x, w, vs);
     } else {
         vx = ka_opaque(vx);
         ka_f4 v[T::NS][T::NT / 4];             // 4 dimensions of the key of each score
@@ -872,9 +905,7 @@ struct KaWalk {
             ka_weights<KT, D, KA_COLS>(x, s, q.cs);
             if (more) ka_wait_copies<T::NI + 1>();
             else ka_wait_copies<0>();
-            KaValuesOf<D, KA_COLS> vs;
-            if constexpr (T::F16) vs.read(ka_addr(vt), vx);
-            odd |= ka_values<KT, D, KA_COLS, XP>(x, s, vs, ka_addr(vt), vx, edge);
+            odd |= ka_values<KT, D, KA_COLS, XP>(x, s, ka_addr(vt), vx, edge);
             ka_wait_reads();
             if (more) copy(vb, vt);
         }
@@ -1001,68 +1032,100 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
         }
         __syncthreads();
         // stage s: its rows 8 w .. 8 w + 7 (keys behind the last one re-read it), those of tile w / 4
-        auto copy = [&](int s) {
+        auto place = [&](int s) {
             const int t = min(k0 + s * KA_WIDE_KEYS + 8 * w + lane / 8, k1 - 1);
-            const uint32_t at = (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
-            const int64_t off = (int64_t)at * T::RB + (((lane & 7) ^ T::swz(8 * cg + lane / 8)) << 4);
-            char* to = lds + (s % KA_STAGES) * STAGE + kg * T::TILE + cg * 1024;
+            return (uint32_t)pages[(t >> lg) - p0] * (uint32_t)per_page + (uint32_t)(t & mask);
+        };
+        auto copy = [&](int s, uint32_t at, int kind) {        // K (0) or V (1)
+            const char* from = (kind ? vb : kb) + (int64_t)at * T::RB + (((lane & 7) ^ T::swz(8 * cg + lane / 8)) << 4);
+            char* to = lds + (s % KA_STAGES) * STAGE + kind * KA_WIDE_KEYS * T::RB + kg * T::TILE + cg * 1024;
 #pragma unroll
-            for (int cb = 0; cb < T::CB; cb++) {
-                __builtin_amdgcn_global_load_lds((const void*)(kb + off + 128 * cb), (ka_lds_t*)(to + cb * T::BLOCK), 16, 0, 0);
-                __builtin_amdgcn_global_load_lds((const void*)(vb + off + 128 * cb),
-                                                 (ka_lds_t*)(to + KA_WIDE_KEYS * T::RB + cb * T::BLOCK), 16, 0, 0);
-            }
+            for (int cb = 0; cb < T::CB; cb++)
+                __builtin_amdgcn_global_load_lds((const void*)(from + 128 * cb), (ka_lds_t*)(to + cb * T::BLOCK), 16, 0, 0);
         };
         const int stages = (k1 - k0 + KA_WIDE_KEYS - 1) / KA_WIDE_KEYS;
         ka_wait_copies<0>();
 #pragma unroll
-        for (int s = 0; s < KA_STAGES - 1; s++) copy(s);
+        for (int s = 0; s < KA_STAGES - 1; s++) {
+            copy(s, place(s), 0);
+            copy(s, place(s), 1);
+        }
+        // The scores run one stage ahead of the softmax: their products fill the matrix cores
+        // while the exponentials fill the VALU. (A workgroup's waves pass the barriers together,
+        // and so do not cover each other.) Two parts of 128 dimensions leave no registers for it.
+        constexpr bool AHEAD = XP == 1 || D < 128;
+        uint32_t at = place(3);
+        if constexpr (AHEAD) copy(3, at, 0);
         if (k0 == it.k0) {
             if (has) limit = ka_limit(it, limits, first, r);
             least = ka_wave_min(limit);
             ka_load_q<KT, D, 32, XP>(a, it.row0 + r, head, has, h, q);
             ka_wait_copies<0>();           // q is here: the waits below count copies alone
         }
-        // The scores run one stage ahead of the softmax: their products fill the matrix cores
-        // while the exponentials fill the VALU. (A workgroup's waves pass the barriers together,
-        // and so do not cover each other.) Two parts of 128 dimensions leave no registers for it.
-        constexpr bool AHEAD = XP == 1 || D < 128;
+        const int end = min(limit, k1);    // (a chunk's end is not the item's: keys behind it come with the next chunk)
         auto tile = [&](int s) { return ka_addr(lds + (s % KA_STAGES) * STAGE + kg * T::TILE); };
+        auto first_key = [&](int s) { return k0 + s * KA_WIDE_KEYS + kg * T::KEYS; };
+        auto edge = [&](int s) { return first_key(s) + T::KEYS > min(least, k1); };
         KaKeysOf<KT, D, 32> k;
-        float sc[T::NS], next[T::NS];
+        KaValuesOf<D, 32> v;
+        KaWeights<D, 32, XP> wt;
+        float sc[T::NS], top;
+        auto masked_top = [&](int s) {
+            if (edge(s)) ka_mask<KT, D, 32>(first_key(s), end, h, sc);
+            top = ka_top<KT, D, 32>(sc, q.cs, first_key(s), end);
+        };
         if constexpr (AHEAD) {
-            stage_barrier<(KA_STAGES - 2) * 2 * PW>();
+            // K of stage s + 2 is read into registers beside the products of stage s with V, so that LDS
+            // and the matrix cores work at one time. So K's places are free two stages before V's.
+            uint32_t at1 = place(4), at2 = place(5);
+            stage_barrier<0>();
             k.read(tile(0), kx);
             ka_scores<KT, D, 32, XP>(k, q, sc);
-        }
-        for (int s = 0; s < stages; s++) {
-            stage_barrier<(KA_STAGES - (AHEAD ? 3 : 2)) * 2 * PW>();
-            // into the stage that every wave has read before this barrier; past the end the last key again
-            copy(s + KA_STAGES - 1);
-            k.read(tile(AHEAD ? s + 1 : s), kx);
-            if constexpr (!AHEAD) ka_scores<KT, D, 32, XP>(k, q, sc);
-            const int t0 = k0 + s * KA_WIDE_KEYS + kg * T::KEYS;
-            // (a chunk's end is not the item's: keys behind it come with the next chunk)
-            const int end = min(limit, k1);
-            const bool edge = t0 + T::KEYS > min(least, k1);
-            if (edge) ka_mask<KT, D, 32>(t0, end, h, sc);
-            ka_follow<KT, D, 32>(x, ka_top<KT, D, 32>(sc, q.cs, t0, end));
-            ka_weights<KT, D, 32>(x, sc, q.cs);
-            if constexpr (AHEAD) {
+            masked_top(0);
+            k.read(tile(1), kx);
+            stage_barrier<0>();
+            copy(4, at1, 0);
+            for (int s = 0; s < stages; s++) {
+                // K of stage s + 2 and V of stage s have landed; read by all: K up to s + 1, V up to s - 1
+                stage_barrier<4 * PW>();
+                copy(s + 5, at2, 0);               // (past the end the last key again)
+                copy(s + 3, at, 1);
+                ka_follow<KT, D, 32>(x, top);
+                const uint32_t vt = tile(s) + KA_WIDE_KEYS * T::RB;
+                v.read(vt, vx);
+                if (edge(s)) odd |= ka_finite<D, 32>(v);
+                float next[T::NS];
+                ka_weights<KT, D, 32>(x, sc, q.cs);
+                wt.pack(sc);
                 ka_scores<KT, D, 32, XP>(k, q, next);
 #pragma unroll
                 for (int i = 0; i < T::QC * XP; i++) {
                     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                   // a product
                     __builtin_amdgcn_sched_group_barrier(0x402, 64 / (T::QC * XP), 0);   // its share of the VALU's work
                 }
-            }
-            const uint32_t vt = tile(s) + KA_WIDE_KEYS * T::RB;
-            KaValuesOf<D, 32> v;
-            v.read(vt, vx);
-            odd |= ka_values<KT, D, 32, XP>(x, sc, v, vt, vx, edge);
-            if constexpr (AHEAD) {
+                wt.here();
 #pragma unroll
                 for (int e = 0; e < T::NS; e++) sc[e] = next[e];
+                k.read(tile(s + 2), kx);
+                ka_product<D, 32, XP>(x, wt, v);
+                at = at1;
+                at1 = at2;
+                at2 = place(s + 6);
+                masked_top(s + 1);
+            }
+        } else {
+            for (int s = 0; s < stages; s++) {
+                stage_barrier<(KA_STAGES - 2) * 2 * PW>();
+                k.read(tile(s), kx);
+                // into the stage that every wave has read before this barrier
+                copy(s + 3, at, 0);
+                copy(s + 3, at, 1);
+                ka_scores<KT, D, 32, XP>(k, q, sc);
+                masked_top(s);
+                ka_follow<KT, D, 32>(x, top);
+                ka_weights<KT, D, 32>(x, sc, q.cs);
+                odd |= ka_values<KT, D, 32, XP>(x, sc, tile(s) + KA_WIDE_KEYS * T::RB, vx, edge(s));
+                at = place(s + 4);
             }
         }
     }
