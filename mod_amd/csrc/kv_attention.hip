@@ -71,12 +71,15 @@ __device__ __forceinline__ float ka_q(const KaArgs& a, int64_t at) {
     return a.q16 ? (float)((const _Float16*)a.q)[at] : ((const float*)a.q)[at];
 }
 
-// One workgroup per (row, head): 256 keys at a time, a thread for each key's
-// score, then a thread for each dimension of the weighted sum.
+// Head dimensions other than 64 and 128. One workgroup per (row, head): 256 keys at a time,
+// a thread for each key's score, then a thread for each dimension of the weighted sum, bound
+// by the waits for a row of K and for KA_DEEP values. 32 sequences of 2,040 to 2,700 tokens, 16 heads of
+// 256: 210 us (one value at a time, K 16 bytes at a time: 860).
+constexpr int KA_DEEP = 16;
 template <typename KT>
 __global__ __launch_bounds__(KA_THREADS) void ka_simple_kernel(KaArgs a) {
     __shared__ float qs[256], ps[KA_THREADS], red[4];
-    __shared__ const KT* vrow[KA_THREADS];
+    __shared__ int64_t vrow[KA_THREADS];       // where a key's value is, -1: nowhere
     __shared__ int req, count0;
     const pio_kv_cache& c = a.c;
     const int tid = threadIdx.x, row = blockIdx.x / a.H, h = blockIdx.x - row * a.H, g = h / a.G, D = c.head_dim;
@@ -104,7 +107,7 @@ __global__ __launch_bounds__(KA_THREADS) void ka_simple_kernel(KaArgs a) {
     for (int t0 = 0; t0 < limit && !bad; t0 += KA_THREADS) {
         const int t = t0 + tid;
         float sc = -INFINITY;
-        const KT* vr = nullptr;
+        int64_t vr = -1;
         int wrong = 0;
         if (t < limit) {
             const int page = c.table[(int64_t)(t < a.shared ? s0 : s) * c.max_pages + (t >> lg)];
@@ -113,14 +116,18 @@ __global__ __launch_bounds__(KA_THREADS) void ka_simple_kernel(KaArgs a) {
             } else {
                 const int64_t at = page * page_e + (int64_t)(t & (c.page_size - 1)) * D;
                 float d = 0.f;
-                for (int e = 0; e < D; e += 8) {
-                    float x[8];
-                    load8<KT>(kb + at + e, x);
+                for (int e0 = 0; e0 < D; e0 += 32) {           // whole lines of a row at once
+                    float x[4][8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) d = fmaf(x[j], qs[e + j], d);
+                    for (int i = 0; i < 4; i++) load8<KT>(kb + at + min(e0 + 8 * i, D - 8), x[i]);
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (e0 + 8 * i < D) d = fmaf(x[i][j], qs[e0 + 8 * i + j], d);
                 }
                 sc = d * a.scale;
-                vr = vb + at;
+                vr = at;
             }
         }
         vrow[tid] = vr;
@@ -128,16 +135,24 @@ __global__ __launch_bounds__(KA_THREADS) void ka_simple_kernel(KaArgs a) {
         if ((tid & 63) == 0) red[tid >> 6] = mt;
         __syncthreads();
         mt = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-        ps[tid] = vr ? expf(sc - mt) : 0.f;
+        ps[tid] = vr >= 0 ? expf(sc - mt) : 0.f;
         const float corr = expf(m - mt);
         m = mt;
         o *= corr;
         l *= corr;
         __syncthreads();
         const int keys = min(KA_THREADS, limit - t0);
-        for (int u = 0; u < keys; u++) {
-            l += ps[u];
-            if (tid < D && vrow[u]) o = fmaf(ps[u], (float)vrow[u][tid], o);
+        for (int u0 = 0; u0 < keys; u0 += KA_DEEP) {      // (a key behind the last one has no row and weight 0)
+            float x[KA_DEEP];
+#pragma unroll
+            for (int i = 0; i < KA_DEEP; i++) x[i] = (float)vb[max(vrow[u0 + i], (int64_t)0) + min(tid, D - 1)];
+#pragma unroll
+            for (int i = 0; i < KA_DEEP; i++) x[i] = vrow[u0 + i] >= 0 ? x[i] : 0.f;
+#pragma unroll
+            for (int i = 0; i < KA_DEEP; i++) {
+                l += ps[u0 + i];
+                o = fmaf(ps[u0 + i], x[i], o);
+            }
         }
         bad = __syncthreads_or(wrong);
     }
@@ -809,6 +824,11 @@ __device__ __forceinline__ int ka_limit(const KaItem& it, const int* limits, int
 // piece of LDS of the wave's own (one tile of K, one of V). The next K tile is
 // copied during this one's softmax and product with V, the next V tile during the
 // next scores. No barriers: a wave waits for its own copies.
+//   16 columns and not 32: few queries to a request leave the rest of a tile empty, and the
+// 16 x 16 products read K and V at the same rate. Two workgroups to a CU (64 KB of LDS each at
+// fp16 x 128). Long tails are bound by HBM: 8 sequences of 20,000 tokens (8 kv heads x 128,
+// fp16) 24.4 us, 4.1 TB/s; short ones by an item's chain of waits (its requests, a page, K, the
+// join), some 12,000 clocks: 32 sequences behind 2,039 tokens 14.8 us, 2.1 TB/s.
 constexpr int KA_COLS = 16, KA_WAVES = 4;
 
 template <int N>
@@ -979,9 +999,13 @@ __device__ __forceinline__ void ka_narrow(const KaArgs& a, const KaItem& it, flo
 
 // ---- wide items: 8 waves, 128 columns: 4 tiles of 32 by waves w % 4, the halves of every
 // 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in LDS that the
-// waves copy together, so that they cross from L2 once for 128 columns. (4 waves of 64
-// columns with all registers of a SIMD each moved their accumulators between register
-// files; the second half's waves half a stage behind the first's: neither was faster.)
+// waves copy together, so that they cross from L2 once for 128 columns. Bound by the waves'
+// own work between two barriers, 2,700 clocks a stage: the matrix cores have 1,024 of it, the
+// VALU 1,600, LDS 1,300. 512 columns over 32,000 tokens (4 kv heads x 128): 54 us, 620 TFLOP/s,
+// 10 of it an item's first and last 20,000 clocks; 4 x as many columns 700 TFLOP/s. Tried
+// and no faster: 4 waves of 64 columns with all registers of a SIMD each (the accumulators move
+// between register files), the second half's waves half a stage behind the first's, products
+// and exponentials interleaved by hand.
 constexpr int KA_WIDE_COLS = 128, KA_WIDE_KEYS = 64, KA_STAGES = 4, KA_WIDE_PAGES = 4096;
 template <int D>
 constexpr size_t ka_wide_bytes() {
@@ -1246,7 +1270,8 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
 
 // A column's items joined: D / 4 lanes have its dimensions, Z groups of them take
 // every Z-th item, all loads of a few in flight together. Z = 8: few columns, where
-// latency counts; Z = 1: 8 (16) columns to a workgroup.
+// latency counts (1,024 columns of 5 items 4 us); Z = 1: 8 (16) columns to a workgroup
+// (6,752 of 4 items 5.5 us, 3.6 TB/s).
 template <int D, int Z>
 __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
     constexpr int TPC = D / 4, GRP = 256 / TPC, COLS = GRP / Z;

@@ -233,6 +233,10 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 // takes a plane (layer, k or v) of a pair, n_kv_heads runs of rows * head_dim elements.
 // Bytes bound it: each thread has KV_DEEP loads in flight before its first store.
 // tables: also rewrites the tables by remap and moves the pages' counts (compact).
+//   Whole pages (84 of 16 x 8 x 128 fp16 in 56 planes, half of them moved): 42 us, 3.6 TB/s.
+// 5 rows of 16 (64 pages in 56 planes): 31 us at 2 TB/s, since rows at the head of 4 KB runs
+// fall on few of the memory's channels; several planes to a workgroup, and pages before planes
+// in the grid's order, changed neither.
 constexpr int KV_DEEP = 4;
 __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int tables) {
     const KvWork w = kv_work(c);
@@ -359,7 +363,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c
 
 // ----------------------------------------------------------------- write ----
 // A workgroup takes one row through a few layers: it finds the row's request,
-// then moves k and v in pieces of 8 elements.
+// then moves k and v in pieces of 8 elements. Bytes bound it: 336 rows of 28 layers,
+// fp32 to fp16, 31 us, 3.6 TB/s.
 template <typename XT, typename KT>
 __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int layer, int layers,
                                                           const int32_t* __restrict__ seq,
