@@ -231,13 +231,10 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 // ------------------------------------------------------------- page copy ----
 // Pairs of the plan: the first rows of each head, in every layer's k and v; a workgroup
 // takes a plane (layer, k or v) of a pair, n_kv_heads runs of rows * head_dim elements.
-// Bytes bound it: each thread has KV_DEEP loads in flight before its first store.
 // tables: also rewrites the tables by remap and moves the pages' counts (compact).
-//   Whole pages (84 of 16 x 8 x 128 fp16 in 56 planes, half of them moved): 42 us, 3.6 TB/s.
-// 5 rows of 16 (64 pages in 56 planes): 31 us at 2 TB/s, since rows at the head of 4 KB runs
-// fall on few of the memory's channels; several planes to a workgroup, and pages before planes
-// in the grid's order, changed neither.
-constexpr int KV_DEEP = 4;
+//   Bytes bound it, from memory: 84 whole pages of 16 x 8 x 128 fp16 in 56 planes, half of
+// them moved, 35 us, 4.3 TB/s; 5 rows of 16 of 64 pages 19 us. One load of a thread at a
+// time: with 4 in flight before the first store, 4 KB apart, 42 and 31 us.
 __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int tables) {
     const KvWork w = kv_work(c);
     const int pairs = *w.pairs_n, planes = 2 * c.n_layers, tid = threadIdx.x;
@@ -257,14 +254,8 @@ __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int ta
         for (int plane = blockIdx.x; plane < planes; plane += gridDim.x) {
             const uint4* src = (const uint4*)((const char*)c.kv + ((int64_t)plane * c.n_pages + from) * page_b);
             uint4* dst = (uint4*)((char*)c.kv + ((int64_t)plane * c.n_pages + to) * page_b);
-            for (int u0 = tid; u0 < all; u0 += KV_DEEP * KV_COPY) {
-                uint4 x[KV_DEEP];
-#pragma unroll
-                for (int i = 0; i < KV_DEEP; i++) x[i] = src[at(min(u0 + i * KV_COPY, all - 1))];
-#pragma unroll
-                for (int i = 0; i < KV_DEEP; i++)
-                    if (u0 + i * KV_COPY < all) dst[at(u0 + i * KV_COPY)] = x[i];
-            }
+#pragma unroll 1
+            for (int u = tid; u < all; u += KV_COPY) dst[at(u)] = src[at(u)];
         }
         if (tables && blockIdx.x == 0 && tid == 0) {
             c.refs[to] = c.refs[from];
