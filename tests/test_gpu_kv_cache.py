@@ -436,6 +436,59 @@ def test_attention_long_prefix(torch, ops, D, Hk, shared, x):
     ops.kv_status(p.c)
 
 
+@pytest.mark.parametrize("H,rows,kv,x", [(2, 1, "float16", "float32"), (8, 5, "float16", "float16"),
+                                         (2, 2, "float32", "float32")])
+def test_attention_many_requests(torch, ops, H, rows, kv, x):
+    """More requests than a workgroup has threads, most of them short, some without rows."""
+    _say(f"many requests H{H} {kv} {x}")
+    rng = np.random.default_rng(14)
+    n = 700
+    p = Pair(torch, ops, 1, 1, 64, 16, 2 * n + 100, n + 1, 60, kv, fill=np.nan)
+    tails = [int(t) for t in rng.integers(1, 20, n)]
+    tails[5], tails[n - 2] = 400, 700
+    _prefix(p, rng, n, 21, tails)
+    seq = [1 + int(i) for i in rng.permutation(n)]
+    start = np.concatenate([[0], np.cumsum([0 if s % 9 == 0 else rows for s in seq])]).astype(int)
+    q = rng.standard_normal((int(start[-1]), H, 64)).astype(x)
+    ref = p.ref.attention(0, seq, start, q, 0.125, np.zeros(q.shape))
+    tol = _tolerance(p, 0, seq, start, q, 0.125, x == "float16")
+    for shared in (21, 0):
+        got = _attend(p, torch, ops, 0, seq, start, q, 0.125, shared, rows)
+        assert np.abs(got.astype(np.float64) - ref).max() <= tol
+    ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("page", [1, 2])
+def test_attention_many_pages_of_an_item(torch, ops, page):
+    """Items of more pages than their ids fit into LDS at once: 33,000 tokens in pages of one, and in fewer."""
+    tokens, Hk, G, D, rows = 33000, 16, 3, 64, 11
+    pages = tokens // page + 4
+    i32 = dict(dtype=torch.int32, device="cuda")
+    kv = torch.full((1, 2, pages, Hk, page, D), float("nan"), dtype=torch.float16, device="cuda")
+    c = ops.KvCache(kv, torch.empty(1, pages, **i32), torch.empty(1, **i32), torch.empty(pages, **i32))
+    seq, start, count = torch.zeros(1, **i32), torch.tensor([0, rows], **i32), torch.tensor([tokens], **i32)
+    all_rows = torch.tensor([0, tokens], **i32)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    k, v = (torch.randn(1, tokens, Hk * D, device="cuda", generator=g).half() for _ in range(2))
+    q = torch.randn(rows, Hk * G, D, device="cuda", generator=g).half()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    ops.kv_init(c)
+    ops.kv_reserve(c, seq, count, 1)
+    ops.kv_write(c, 0, 1, seq, all_rows, 1, k, v, tokens)
+    ops.kv_attention(c, 0, seq, start, 1, q, out, rows, Hk * G, 0.125, max_rows=rows)
+    ops.kv_status(c)
+    kk, vv = (t.reshape(tokens, Hk, D).double().transpose(0, 1).contiguous() for t in (k, v))
+    qq = q.double().reshape(rows, Hk, G, D).permute(1, 2, 0, 3).reshape(Hk, G * rows, D).contiguous()
+    s = torch.matmul(qq, kk.transpose(1, 2).contiguous()).reshape(Hk, G, rows, tokens) * 0.125
+    late = torch.arange(tokens, device="cuda") > tokens - rows + torch.arange(rows, device="cuda")[:, None]
+    w = torch.softmax(s.masked_fill(late, -torch.inf), 3).reshape(Hk, G * rows, tokens)
+    ref = torch.matmul(w, vv).reshape(Hk, G, rows, D).permute(2, 0, 1, 3).reshape(rows, Hk * G, D)
+    # |score| < 8: 2 es + 8 u + 4 u sqrt(33000) = 7.4e-5, and the weights' 2^-11 as a random walk is
+    # less than 2^-11 itself; the output's 2^-11
+    assert float((out.double() - ref).abs().max()) <= (7.4e-5 + 2.0 ** -11) * float(v.abs().max()) + 2.0 ** -11 * float(ref.abs().max())
+
+
 def test_attention_large_scores(torch, ops):
     """Scores far apart and far from zero; a softmax that picks one key; queries
     beyond the fp16 range over an fp16 cache."""

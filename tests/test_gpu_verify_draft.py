@@ -183,3 +183,14 @@ def test_large_vocabulary(torch, ops, dtype):
         _check(torch, ops, p, q, ids, np.ones(6), np.full(3, un), [0, 1, 4, 6])
     got = _check(torch, ops, p, p, ids, np.ones(6), rng.random(3), [0, 1, 4, 6])
     assert np.all(got[0] == 0) and np.all(got[1][[0, 1, 4]] >= 0)
+
+
+def test_many_requests(torch, ops):
+    """More requests than one dimension of a grid has."""
+    rng = np.random.default_rng(5)
+    n, V = 70000, 6
+    counts = rng.integers(0, 3, n)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    rows = int(start[-1])
+    p, q = _probs(rng, rows, V, np.float32, 1.0), _probs(rng, rows, V, np.float32, 1.0)
+    _check(torch, ops, p, q, rng.integers(0, V, rows), rng.random(rows), rng.random(n), start)
