@@ -342,6 +342,13 @@ typedef struct {
 
 /* Bytes of `work` (0 for a struct that no call would take). */
 size_t pio_kv_work_bytes(const pio_kv_cache* cache);
+/* Zeroed memory for `work`, on `device`: into cache->work, and back from there.
+ * It is no part of the allocator's pool or cache. pio_kv_work_destroy waits for
+ * all work of the device, whichever streams the cache's calls ran on; graphs that
+ * hold such calls may not be replayed behind it. A caller may just as well bring
+ * zeroed memory of their own, and keep it until those are done. */
+int pio_kv_work_create(pio_kv_cache* cache, int device);
+void pio_kv_work_destroy(pio_kv_cache* cache, int device);
 /* Empties the cache: no sequence holds a page. The pages' contents stay. */
 int pio_kv_init(const pio_kv_cache* cache, void* stream);
 /* Waits for `stream` and reports what the kernels of the calls before found

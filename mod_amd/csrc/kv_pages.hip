@@ -237,12 +237,16 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 // time: with 4 in flight before the first store, 4 KB apart, 42 and 31 us.
 __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int tables) {
     const KvWork w = kv_work(c);
-    const int pairs = *w.pairs_n, planes = 2 * c.n_layers, tid = threadIdx.x;
+    const int pairs = min(*w.pairs_n, c.n_pages), planes = 2 * c.n_layers, tid = threadIdx.x;
     const int esz = c.kv_dtype == PIO_F32 ? 4 : 2;
     const int64_t head_b = (int64_t)c.page_size * c.head_dim * esz, page_b = head_b * c.n_kv_heads;
     const int pitch = (int)(head_b / 16);
     for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
         const int from = w.pairs[3 * pair], to = w.pairs[3 * pair + 1], rows = w.pairs[3 * pair + 2];
+        // (a plan that something else wrote over may not lead out of the cache)
+        if ((unsigned)from >= (unsigned)c.n_pages || (unsigned)to >= (unsigned)c.n_pages ||
+            (unsigned)rows > (unsigned)c.page_size)
+            continue;
         const int run = rows * c.head_dim * esz / 16, all = run * c.n_kv_heads;
         const uint32_t magic = run > 1 ? 0xffffffffu / run + 1 : 0;     // u / run, or one more
         auto at = [&](int u) {
@@ -464,6 +468,22 @@ using namespace pio;
 PIO_EXPORT size_t pio_kv_work_bytes(const pio_kv_cache* c) {
     if (!c || c->max_seqs <= 0 || c->n_pages <= 0) return 0;
     return kv_work_ints(*c) * sizeof(int32_t);
+}
+
+PIO_EXPORT int pio_kv_work_create(pio_kv_cache* c, int device) {
+    PIO_REQUIRE(c, "pio_kv_work_create: null cache");
+    c->work = nullptr;
+    const size_t bytes = pio_kv_work_bytes(c);
+    PIO_REQUIRE(bytes, "pio_kv_work_create: empty cache dimension");
+    PIO_REQUIRE(device >= 0, "pio_kv_work_create: device %d", device);
+    PIO_REQUIRE(!capture_id(current_stream()), "pio_kv_work_create: the stream is capturing");
+    return device_own((void**)&c->work, bytes, device);
+}
+
+PIO_EXPORT void pio_kv_work_destroy(pio_kv_cache* c, int device) {
+    if (!c || !c->work) return;
+    device_disown(c->work, device);
+    c->work = nullptr;
 }
 
 PIO_EXPORT int pio_kv_init(const pio_kv_cache* c, void* stream) {

@@ -91,6 +91,11 @@ int device_alloc(void** p, size_t bytes, hipStream_t stream = nullptr);
 // Back to the cache (a no-op for pool memory). A block whose stream is
 // capturing is parked with the capture instead: the graph keeps using it.
 void device_free(void* p);
+// Zeroed memory of its owner alone, outside the cache and the pool, for state
+// that calls on any stream use: device_disown waits for all of the device's work
+// before it goes. (The current stream may not be capturing for device_own.)
+int device_own(void** p, size_t bytes, int dev);
+void device_disown(void* p, int dev);
 // Drains `s`, releases the blocks cached for it and retires its cache id; call
 // before destroying a stream the library created.
 void release_stream(hipStream_t s);

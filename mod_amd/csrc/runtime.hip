@@ -251,6 +251,52 @@ void device_free(void* p) {
     cache_block_locked(a, p, l);
 }
 
+int device_own(void** out, size_t bytes, int dev) {
+    *out = nullptr;
+    RelaxedCapture relaxed;
+    int cur = 0;
+    PIO_HIP(hipGetDevice(&cur));
+    if (dev != cur && hipSetDevice(dev) != hipSuccess) {
+        (void)hipGetLastError();
+        return set_error(PIO_ERR_INVALID, "no device %d", dev);
+    }
+    hipError_t e = hipMalloc(out, bytes);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        tensor_empty_cache();
+        e = hipMalloc(out, bytes);
+    }
+    int status = PIO_OK;
+    if (e != hipSuccess) {
+        *out = nullptr;
+        status = set_error(PIO_ERR_OOM, "hipMalloc(%zu) failed on device %d: %s", bytes, dev, hipGetErrorString(e));
+    } else {
+        const hipStream_t s = current_stream();
+        e = hipMemsetAsync(*out, 0, bytes, s);
+        if (e == hipSuccess) e = hipStreamSynchronize(s);
+        if (e != hipSuccess) {
+            (void)hipFree(*out);
+            *out = nullptr;
+            status = set_error(PIO_ERR_HIP, "clearing %zu bytes failed: %s", bytes, hipGetErrorString(e));
+        }
+    }
+    (void)hipGetLastError();
+    if (dev != cur) (void)hipSetDevice(cur);
+    return status;
+}
+
+void device_disown(void* p, int dev) {
+    if (!p) return;
+    RelaxedCapture relaxed;
+    int cur = 0;
+    (void)hipGetDevice(&cur);
+    if (dev != cur) (void)hipSetDevice(dev);
+    // hipFree waits for the device; hipDeviceSynchronize would end a capture of any other stream
+    (void)hipFree(p);
+    (void)hipGetLastError();
+    if (dev != cur) (void)hipSetDevice(cur);
+}
+
 unsigned long long capture_id(hipStream_t s) {
     hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
     unsigned long long cid = 0;

@@ -157,6 +157,8 @@ SIGNATURES: dict[str, tuple] = {
     "pio_moe_w8a8": (_i, [_vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i,
                           _vp, _vp]),
     "pio_kv_work_bytes": (_sz, [_cp]),
+    "pio_kv_work_create": (_i, [_cp, _i]),
+    "pio_kv_work_destroy": (None, [_cp, _i]),
     "pio_kv_init": (_i, [_cp, _vp]),
     "pio_kv_status": (_i, [_cp, _vp]),
     "pio_kv_reserve": (_i, [_cp, _vp, _vp, _i, _vp]),
@@ -331,7 +333,8 @@ class KvCache:
     pages of a sequence], lens [sequences] and refs [pages] int32, all dense on
     one device (torch or backend tensors; kept alive by this object). The plans'
     workspace is allocated here, and the tables are taken as they are: kv_init
-    empties a new cache."""
+    empties a new cache. The object has to live as long as the graphs that its
+    calls were captured into; when it goes it waits for the device."""
 
     def __init__(self, kv, table, lens, refs):
         if len(kv.shape) != 6 or kv.shape[1] != 2:
@@ -354,24 +357,21 @@ class KvCache:
         self.tensors = (kv, table, lens, refs)
         self.c = CKvCache(_ptr(kv), _ptr(table), _ptr(lens), _ptr(refs), None, _dt(kv), L, heads, dim, page, pages,
                           seqs, width)
-        words = lib.pio_kv_work_bytes(ctypes.byref(self.c)) // 4
-        self._work = lib.create_tensor_typed((ctypes.c_int * 1)(words), 1,
-                                             int(device.split(":")[1]) if ":" in device else 0, I32)
-        if not self._work:
-            raise RocmError(f"KvCache: {last_error()}")
-        zero = (ctypes.c_int * words)()
-        check(lib.tensor_load_bytes_status(self._work, zero, 4 * words), "KvCache")
-        self.c.work = ctypes.cast(self._work.contents.data, ctypes.c_void_p).value
+        self.device = int(device.split(":")[1]) if ":" in device else 0
         self.ref = ctypes.byref(self.c)
+        check(lib.pio_kv_work_create(self.ref, self.device), "KvCache")
+
+    def close(self) -> None:
+        """Waits for the device and frees the workspace; no call may follow, nor a replay of a graph that holds one."""
+        if getattr(self, "ref", None) is not None:
+            lib.pio_kv_work_destroy(self.ref, self.device)
+            self.ref = None
 
     def __del__(self):
-        h = getattr(self, "_work", None)
-        if h:
-            try:
-                lib.free_tensor(h)
-            except Exception:
-                pass
-            self._work = None
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def kv_init(cache: KvCache, stream=None) -> None:
