@@ -315,7 +315,7 @@ int pio_moe_w8a8(const void* x, int x_dtype, const float* logits, const int8_t* 
  *   table  int32 [max_seqs][max_pages]  page ids of each sequence, -1 behind its last
  *   lens   int32 [max_seqs]             tokens of each sequence
  *   refs   int32 [n_pages]              table entries that hold each page, 0 = free
- *   work   int32, pio_kv_work_bytes()   plans of the calls below and their status
+ *   work   int32, pio_kv_work_bytes()   plans of the calls below and their status; zeroed, or pio_kv_init
  * Sequences may share pages (pio_kv_fork). page_size is a power of two from 1 to
  * 1024, head_dim a multiple of 8 up to 256; kv is 16-byte aligned, table rows
  * and the other arrays 4-byte. The lists of sequence ids and counts are int32
@@ -363,7 +363,12 @@ int pio_kv_status(const pio_kv_cache* cache, void* stream);
  * another table entry holds as well, the sequence gets a copy of it first: the
  * rows in use, in every layer (two requests that share such a page each get
  * one). All or nothing: if any request is refused, or the free pages do not
- * suffice, no request is served. */
+ * suffice, no request is served. Behind a refused call its sequences are held up:
+ * pio_kv_write and pio_kv_drop with counts leave them as they are, so that a step's
+ * calls need not wait for its outcome (the attention and verification of such a
+ * step mean nothing: ask pio_kv_status before their results are used). That ends
+ * with pio_kv_status, with a pio_kv_reserve that serves the sequence, and with its
+ * end (pio_kv_drop without counts, pio_kv_fork onto it). */
 int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t* count, int n, void* stream);
 /* Keys and values of each sequence's last tokens: rows row_start[i] ..
  * row_start[i + 1] - 1 of k and v become the last positions of seq[i], in

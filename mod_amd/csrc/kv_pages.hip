@@ -22,12 +22,15 @@ constexpr int KV_SCAN = 16;            // page counts per thread and step of a p
 //   mark [max_seqs]        request that names a sequence
 //   pairs [n_pages][3]     (from, to, rows of each head)
 //   remap [n_pages]        free pages (reserve) / new page of each old one (compact)
+//   held_up [max_seqs]     1: the last reserve that names a sequence was refused
+// A step's calls follow each other without the host, so those behind a refused reserve have
+// to find out on the device: its tokens are not there to be written or dropped.
 constexpr int KV_HEAD = 16;
 static inline size_t kv_work_ints(const pio_kv_cache& c) {
-    return KV_HEAD + (size_t)c.max_seqs + 4 * (size_t)c.n_pages;
+    return KV_HEAD + 2 * (size_t)c.max_seqs + 4 * (size_t)c.n_pages;
 }
 struct KvWork {
-    int *status, *pairs_n, *mark, *pairs, *remap;
+    int *status, *pairs_n, *mark, *pairs, *remap, *held_up;
 };
 __host__ __device__ __forceinline__ KvWork kv_work(const pio_kv_cache& c) {
     KvWork w;
@@ -36,6 +39,7 @@ __host__ __device__ __forceinline__ KvWork kv_work(const pio_kv_cache& c) {
     w.mark = c.work + KV_HEAD;
     w.pairs = w.mark + c.max_seqs;
     w.remap = w.pairs + 3 * (int64_t)c.n_pages;
+    w.held_up = w.remap + c.n_pages;
     return w;
 }
 
@@ -108,9 +112,19 @@ __global__ __launch_bounds__(KV_COPY) void kv_init_kernel(pio_kv_cache c) {
     const int64_t cells = (int64_t)c.max_seqs * c.max_pages;
     const int64_t at = (int64_t)blockIdx.x * KV_COPY + threadIdx.x, step = (int64_t)gridDim.x * KV_COPY;
     for (int64_t i = at; i < cells; i += step) c.table[i] = -1;
-    for (int64_t i = at; i < c.max_seqs; i += step) c.lens[i] = 0;
+    for (int64_t i = at; i < c.max_seqs; i += step) {
+        c.lens[i] = 0;
+        kv_work(c).held_up[i] = 0;
+    }
     for (int64_t i = at; i < c.n_pages; i += step) c.refs[i] = 0;
     if (at < 2) c.work[at] = 0;
+}
+// What was refused is known (pio_kv_status).
+__global__ __launch_bounds__(KV_COPY) void kv_settle_kernel(pio_kv_cache c) {
+    const KvWork w = kv_work(c);
+    const int at = blockIdx.x * KV_COPY + threadIdx.x;
+    if (at == 0) *w.status = 0;
+    for (int i = at; i < c.max_seqs; i += gridDim.x * KV_COPY) w.held_up[i] = 0;
 }
 
 // --------------------------------------------------------------- reserve ----
@@ -193,6 +207,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
         }
     }
     if (bad || found < total) {
+        for (int i = tid; i < n; i += KV_PLAN)
+            if (kv_seq_ok(c, seq[i])) w.held_up[seq[i]] = 1;
         if (tid == 0) {
             *w.pairs_n = 0;
             atomicOr(w.status, bad ? bad : KV_FULL);
@@ -224,7 +240,10 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
         }
     }
     __syncthreads();
-    for (int i = tid; i < n; i += KV_PLAN) c.lens[seq[i]] += count[i];
+    for (int i = tid; i < n; i += KV_PLAN) {
+        c.lens[seq[i]] += count[i];
+        w.held_up[seq[i]] = 0;
+    }
     if (tid == 0) *w.pairs_n = pairs;
 }
 
@@ -376,6 +395,7 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         const int s = seq[i];
         int page = -1, pos = -1;
         if (kv_seq_ok(c, s)) {
+            if (kv_work(c).held_up[s]) continue;           // its tokens have no room: reported by the reserve
             pos = kv_seq_len(c, s) - (r1 - row);
             if (pos >= 0) page = c.table[(int64_t)s * c.max_pages + (pos >> lg)];
         }
@@ -387,7 +407,7 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         }
     }
     __syncthreads();
-    if (where[0] < 0) return;          // behind the last request, or refused above
+    if (where[0] < 0) return;          // behind the last request, without room, or refused above
     const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8;
     const int64_t head = (int64_t)c.page_size * c.head_dim, plane = head * c.n_kv_heads * c.n_pages;
     KT* base = (KT*)c.kv + head * c.n_kv_heads * where[0] + (int64_t)where[1] * c.head_dim;
@@ -433,7 +453,10 @@ __global__ __launch_bounds__(KV_COPY) void kv_fork_kernel(pio_kv_cache c, const 
         if (p >= 0 && p < c.n_pages) atomicAdd(&c.refs[p], 1);
         else atomicOr(kv_work(c).status, KV_BAD);
     }
-    if (tid == 0) c.lens[d] = L;
+    if (tid == 0) {
+        c.lens[d] = L;
+        kv_work(c).held_up[d] = 0;     // a new sequence
+    }
 }
 
 __global__ __launch_bounds__(KV_COPY) void kv_drop_kernel(pio_kv_cache c, const int32_t* __restrict__ seq,
@@ -449,6 +472,7 @@ __global__ __launch_bounds__(KV_COPY) void kv_drop_kernel(pio_kv_cache c, const 
         if (tid == 0) atomicOr(kv_work(c).status, KV_BAD);
         return;
     }
+    if (count && kv_work(c).held_up[s]) return;            // the tokens that it would take back never came
     const int left = L > k ? L - k : 0, p1 = kv_pages_of(L, lg);
     __syncthreads();                   // every thread has read the length
     for (int j = kv_pages_of(left, lg) + tid; j < p1; j += KV_COPY) {
@@ -458,7 +482,10 @@ __global__ __launch_bounds__(KV_COPY) void kv_drop_kernel(pio_kv_cache c, const 
         if (p >= 0 && p < c.n_pages) atomicAdd(&c.refs[p], -1);
         else atomicOr(kv_work(c).status, KV_BAD);
     }
-    if (tid == 0) c.lens[s] = left;
+    if (tid == 0) {
+        c.lens[s] = left;
+        if (!count) kv_work(c).held_up[s] = 0;
+    }
 }
 
 }  // namespace pio
@@ -500,11 +527,11 @@ PIO_EXPORT int pio_kv_status(const pio_kv_cache* c, void* stream) {
     hipStream_t st = pick_stream(stream);
     PIO_REQUIRE(!capture_id(st), "pio_kv_status: the stream is capturing (it cannot be waited for)");
     int bits = 0;
-    const int none = 0;
     PIO_HIP(hipMemcpyAsync(&bits, c->work, sizeof(int), hipMemcpyDeviceToHost, st));
     PIO_HIP(hipStreamSynchronize(st));
     if (!bits) return PIO_OK;
-    PIO_HIP(hipMemcpyAsync(c->work, &none, sizeof(int), hipMemcpyHostToDevice, st));
+    kv_settle_kernel<<<std::min(ceil_div(c->max_seqs, KV_COPY), 1024), KV_COPY, 0, st>>>(*c);
+    PIO_LAUNCHED();
     PIO_HIP(hipStreamSynchronize(st));
     if (bits & KV_BAD)
         return set_error(PIO_ERR_INVALID, "kv cache: a call named a sequence, count or page that it does not have, one "

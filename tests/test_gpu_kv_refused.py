@@ -1,0 +1,149 @@
+"""The paged cache where a call is refused on the device, or part of what it reads
+is outside the cache: nothing but the refused request changes, and only rows that
+see what is wrong are NaN. Pages, tables, lengths and counts are held to equality,
+attention to the bounds derived in test_gpu_kv_cache.py."""
+import numpy as np
+import pytest
+
+from oracle import kv_ref
+from test_gpu_kv_cache import Pair, _say, _tolerance
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch(torch_dev):
+    import torch
+    return torch
+
+
+@pytest.fixture(scope="module")
+def ops(torch_dev):
+    from mod_amd import ops
+    return ops
+
+
+def _rows(rng, p, n):
+    """Keys and values of n rows in all layers."""
+    shape = (p.ref.kv.shape[0], n, p.ref.kv.shape[3], p.ref.kv.shape[5])
+    return [rng.standard_normal(shape).astype(np.float32) for _ in range(2)]
+
+
+def _write(p, rng, seq, count, known=True):
+    """The last count[i] tokens of seq[i] written, in the oracle too where `known`."""
+    start = np.concatenate([[0], np.cumsum(count)]).astype(int)
+    k, v = _rows(rng, p, int(start[-1]))
+    p.ops.kv_write(p.c, 0, k.shape[0], p.ints(seq), p.ints(start), len(seq), p.dev(k), p.dev(v), k.shape[1])
+    if known:
+        p.ref.write(0, list(seq), start, k, v)
+
+
+# ------------------------------------------------------- a reserve is refused ---
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("tokens", [32, 37])
+def test_refused_step_changes_nothing(torch, ops, dtype, tokens):
+    """A step whose reserve finds too few pages: its writes would fall onto tokens that the sequences
+    have, in pages that they share, and its drop onto tokens that they keep."""
+    _say(f"refused step {dtype} {tokens}")
+    rng = np.random.default_rng(tokens)
+    p = Pair(torch, ops, 2, 2, 64, 16, 7, 6, 4, dtype)
+    p.add(rng, [0], [tokens])
+    p.fork([0, 0, 0, 0], [1, 2, 3, 4])
+    seq, count = [1, 2, 3], [3, 18, 40]
+    with pytest.raises(kv_ref.Refused):
+        p.ref.reserve(seq, count)
+    ops.kv_reserve(p.c, p.ints(seq), p.ints(count), 3)
+    _write(p, rng, seq, [3, 18, 1], known=False)
+    ops.kv_drop(p.c, p.ints(seq), p.ints([2, 17, 39]), 3)
+    p.same()
+    # a request that ends is dropped all the same, and one that is not of the refused step is served
+    p.drop([3])
+    p.add(rng, [4], [1])
+    _write(p, rng, [1], [1], known=False)
+    p.same()
+    with pytest.raises(ops.RocmError, match="too few free pages"):
+        ops.kv_status(p.c)
+    # once that is known, or the next reserve is served, the sequences are as any other
+    p.drop([2], [4])
+    p.same()
+    p.add(rng, [1, 2], [2, 3])
+    p.drop([1], [1])
+    p.same()
+    ops.kv_status(p.c)
+
+
+def test_next_step_is_served(torch, ops):
+    """Without a status between: the step behind a refused one is served, a slot that ends and begins
+    again is a new sequence, and a reserve of other sequences does not set the refused ones free."""
+    rng = np.random.default_rng(2)
+    p = Pair(torch, ops, 1, 2, 16, 4, 8, 6, 6)
+    p.add(rng, [0, 1, 2], [6, 3, 5])                # 5 of 8 pages
+    for seq, count in (([0, 1], [12, 8]), ([2, 2], [1, 1]), ([2], [-1])):
+        ops.kv_reserve(p.c, p.ints(seq), p.ints(count), len(seq))
+    p.add(rng, [3], [1])
+    _write(p, rng, [0, 1, 2], [1, 1, 1], known=False)
+    ops.kv_drop(p.c, p.ints([0, 1, 2]), p.ints([1, 2, 3]), 3)
+    p.same()
+    p.add(rng, [0], [3])
+    p.drop([0], [1])
+    p.same()
+    p.drop([1])
+    p.fork([0], [1])
+    p.drop([1], [4])                                # a branch from an earlier token
+    p.same()
+    with pytest.raises(ops.RocmError):
+        ops.kv_status(p.c)
+    ops.kv_reserve(p.c, p.ints([2]), p.ints([400]), 1)
+    ops.kv_init(p.c)
+    p.ref = kv_ref.Cache(1, 2, 16, 4, 8, 6, 6)
+    p.ref.kv[:] = p.kv.cpu().numpy()
+    p.add(rng, [2], [5])
+    p.drop([2], [2])
+    p.same()
+    ops.kv_status(p.c)
+
+
+def test_captured_steps_until_the_pages_run_out(torch, ops):
+    """Reserve, write, attention and a drop by counts in one graph, replayed until the pages run out and
+    beyond: from then on nothing changes, until a sequence ends and the steps are served again."""
+    rng = np.random.default_rng(3)
+    p = Pair(torch, ops, 1, 2, 64, 16, 9, 5, 8, "float16")
+    p.add(rng, [0], [40])
+    p.fork([0, 0], [1, 2])
+    seq, start, count, drop = p.ints([1, 2]), p.ints([0, 7, 12]), p.ints([7, 5]), p.ints([2, 1])
+    k, v = (torch.empty(1, 12, 2 * 64, device="cuda") for _ in range(2))
+    q, out = torch.randn(12, 4, 64, device="cuda"), torch.empty(12, 4, 64, device="cuda")
+    st, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        ops.kv_reserve(p.c, seq, count, 2, stream=st)
+        ops.kv_write(p.c, 0, 1, seq, start, 2, k, v, 12, stream=st)
+        ops.kv_attention(p.c, 0, seq, start, 2, q, out, 12, 4, 0.125, shared=40, max_rows=7, stream=st)
+        ops.kv_drop(p.c, seq, drop, 2, stream=st)
+    refused = 0
+    for i in range(14):
+        _say(f"replay {i}")
+        kk, vv = (rng.standard_normal((1, 12, 2, 64)).astype(np.float32) for _ in range(2))
+        k.copy_(torch.from_numpy(kk).reshape(1, 12, 128)), v.copy_(torch.from_numpy(vv).reshape(1, 12, 128))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graph.replay()
+        torch.cuda.synchronize()
+        try:
+            p.ref.reserve([1, 2], [7, 5])
+        except kv_ref.Refused:
+            refused += 1
+            p.same()
+            if refused == 3:                        # the two that ran out end, and begin again
+                with pytest.raises(ops.RocmError, match="too few free pages"):
+                    ops.kv_status(p.c, stream=st)
+                p.drop([1, 2])
+                p.fork([0, 0], [1, 2])
+            continue
+        p.ref.write(0, [1, 2], [0, 7, 12], kk, vv)
+        ref = p.ref.attention(0, [1, 2], [0, 7, 12], q.cpu().numpy(), 0.125, np.zeros((12, 4, 64)))
+        tol = _tolerance(p, 0, [1, 2], [0, 7, 12], q.cpu().numpy(), 0.125, False)
+        assert np.abs(out.cpu().numpy() - ref).max() <= tol
+        assert p.ref.drop([1, 2], [2, 1]) == []
+        p.same()
+    assert 3 <= refused <= 8
