@@ -355,7 +355,7 @@ int pio_kv_init(const pio_kv_cache* cache, void* stream);
  * wrong since the last pio_kv_status: PIO_OK, PIO_ERR_OOM (a pio_kv_reserve
  * found too few free pages or too short table rows) or PIO_ERR_INVALID (bad
  * sequence id, count or page, one sequence twice, a fork onto a sequence that
- * is not empty). */
+ * is not empty, a write into a page that several table entries hold). */
 int pio_kv_status(const pio_kv_cache* cache, void* stream);
 /* Room for count[i] more tokens of sequence seq[i], i < n: the pages it needs
  * join its table row, the lowest free ones in the order of the requests, and
@@ -376,7 +376,9 @@ int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t*
  * with rows `row_stride` and layers `layer_stride` elements apart (each a
  * multiple of 8, or 0 for dense rows / layers), fp32|fp16, rounded to the
  * cache's type, 16-byte aligned, each sequence once, fewer than 2^24 rows. row_start int32 [n + 1], ascending; rows at
- * and behind row_start[n] are not read. */
+ * and behind row_start[n] are not read. A row whose page another table entry holds
+ * as well is refused, the others are written: pio_kv_reserve gives new tokens pages
+ * of their own, and what sequences share is written in all layers before the fork. */
 int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
                  int n, const void* k, const void* v, int dtype, int rows, int64_t row_stride,
                  int64_t layer_stride, void* stream);

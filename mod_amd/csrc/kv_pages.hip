@@ -399,7 +399,8 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
             pos = kv_seq_len(c, s) - (r1 - row);
             if (pos >= 0) page = c.table[(int64_t)s * c.max_pages + (pos >> lg)];
         }
-        if (page < 0 || page >= c.n_pages) {
+        // (a page that another table entry holds too is not this sequence's to change)
+        if (page < 0 || page >= c.n_pages || c.refs[page] > 1) {
             atomicOr(kv_work(c).status, KV_BAD);
         } else {
             where[0] = page;
@@ -535,7 +536,8 @@ PIO_EXPORT int pio_kv_status(const pio_kv_cache* c, void* stream) {
     PIO_HIP(hipStreamSynchronize(st));
     if (bits & KV_BAD)
         return set_error(PIO_ERR_INVALID, "kv cache: a call named a sequence, count or page that it does not have, one "
-                                          "sequence twice, or forked onto a sequence that is not empty");
+                                          "sequence twice, forked onto a sequence that is not empty, or wrote "
+                                          "into a page that several sequences hold");
     return set_error(PIO_ERR_OOM, "kv cache: pio_kv_reserve found too few free pages or too short table rows");
 }
 

@@ -147,3 +147,36 @@ def test_captured_steps_until_the_pages_run_out(torch, ops):
         assert p.ref.drop([1, 2], [2, 1]) == []
         p.same()
     assert 3 <= refused <= 8
+
+
+# -------------------------------------------------------------- shared pages ---
+def test_write_into_shared_pages_is_refused(torch, ops):
+    """Rows that fall into pages of another table entry: a fork without room of its own, a request that
+    rewrites tokens which it shares. The rows of the same call in pages of their own are written."""
+    rng = np.random.default_rng(5)
+    p = Pair(torch, ops, 2, 1, 16, 4, 20, 5, 6)
+    p.add(rng, [0, 3], [10, 6])
+    p.fork([0], [1])
+    _write(p, rng, [1], [1], known=False)           # nothing of its own yet
+    p.same()
+    with pytest.raises(ops.RocmError):
+        ops.kv_status(p.c)
+    p.reserve([1, 0], [3, 0])
+    start = [0, 5, 8]                               # tokens 8 and on are in its own copy; tokens 0 .. 7 are common
+    k, v = _rows(rng, p, 8)
+    ops.kv_write(p.c, 0, 2, p.ints([1, 3]), p.ints(start), 2, p.dev(k), p.dev(v), 8)
+    p.ref.write(0, [1], [0, 5], k[:, :5], v[:, :5])
+    p.ref.write(0, [3], [0, 3], k[:, 5:], v[:, 5:])
+    p.same()
+    ops.kv_status(p.c)
+    k, v = _rows(rng, p, 9)
+    before = p.ref.kv.copy()
+    ops.kv_write(p.c, 0, 2, p.ints([1, 3]), p.ints([0, 7, 9]), 2, p.dev(k), p.dev(v), 9)
+    p.ref.write(0, [1], [0, 7], k[:, :7], v[:, :7])
+    for t in (6, 7):                                # common tokens: left as they were
+        page = int(p.ref.table[1, t // 4])
+        p.ref.kv[:, :, page, :, t % 4] = before[:, :, page, :, t % 4]
+    p.ref.write(0, [3], [0, 2], k[:, 7:], v[:, 7:])
+    p.same()
+    with pytest.raises(ops.RocmError):
+        ops.kv_status(p.c)
