@@ -375,7 +375,8 @@ int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t*
  * `layers` layers from `layer`. k and v [layers][rows][n_kv_heads * head_dim]
  * with rows `row_stride` and layers `layer_stride` elements apart (each a
  * multiple of 8, or 0 for dense rows / layers), fp32|fp16, rounded to the
- * cache's type, 16-byte aligned, each sequence once, fewer than 2^24 rows. row_start int32 [n + 1], ascending; rows at
+ * cache's type, 16-byte aligned, fewer than 2^24 rows; of requests with rows for one
+ * sequence the first is served. row_start int32 [n + 1], ascending; rows at
  * and behind row_start[n] are not read. A row whose page another table entry holds
  * as well is refused, the others are written: pio_kv_reserve gives new tokens pages
  * of their own, and what sequences share is written in all layers before the fork. */

@@ -385,30 +385,47 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
                                                           const int32_t* __restrict__ row_start, int n,
                                                           const XT* __restrict__ k, const XT* __restrict__ v,
                                                           int64_t row_stride, int64_t layer_stride, int per_block) {
-    __shared__ int where[2];           // page, row in it
+    __shared__ int found, named, where[2];     // the row's request, its sequence; page, row in it
     const int row = blockIdx.x, tid = threadIdx.x, lg = kv_log2(c.page_size);
-    if (tid == 0) where[0] = -1;
+    if (tid == 0) found = where[0] = -1;
     __syncthreads();
+    int s = -1, back = 0, first = -1;          // (first: what thread tid's first request with rows names)
     for (int i = tid; i < n; i += KV_COPY) {
-        const int r0 = row_start[i], r1 = row_start[i + 1];
+        const int r0 = row_start[i], r1 = row_start[i + 1], si = seq[i];
+        if (i == tid && r1 > r0) first = si;
         if (row < r0 || row >= r1) continue;
-        const int s = seq[i];
+        found = i;
+        named = s = si;
+        back = r1 - row;
+    }
+    __syncthreads();
+    const int req = found;
+    if (req < 0) return;               // behind the last request
+    if (tid == req % KV_COPY) {
         int page = -1, pos = -1;
+        bool held_up = false;
         if (kv_seq_ok(c, s)) {
-            if (kv_work(c).held_up[s]) continue;           // its tokens have no room: reported by the reserve
-            pos = kv_seq_len(c, s) - (r1 - row);
+            held_up = kv_work(c).held_up[s];               // its tokens have no room: reported by the reserve
+            pos = kv_seq_len(c, s) - back;
             if (pos >= 0) page = c.table[(int64_t)s * c.max_pages + (pos >> lg)];
         }
         // (a page that another table entry holds too is not this sequence's to change)
-        if (page < 0 || page >= c.n_pages || c.refs[page] > 1) {
+        if (held_up) {
+        } else if (page < 0 || page >= c.n_pages || c.refs[page] > 1) {
             atomicOr(kv_work(c).status, KV_BAD);
         } else {
             where[0] = page;
             where[1] = pos & (c.page_size - 1);
         }
     }
-    __syncthreads();
-    if (where[0] < 0) return;          // behind the last request, without room, or refused above
+    // a sequence that an earlier request with rows names is left to that one
+    int twice = tid < req && first == named;
+    for (int i = tid + KV_COPY; i < req; i += KV_COPY) twice |= seq[i] == named && row_start[i + 1] > row_start[i];
+    if (__syncthreads_or(twice)) {
+        if (tid == 0) atomicOr(kv_work(c).status, KV_BAD);
+        return;
+    }
+    if (where[0] < 0) return;          // without room, or refused above
     const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8;
     const int64_t head = (int64_t)c.page_size * c.head_dim, plane = head * c.n_kv_heads * c.n_pages;
     KT* base = (KT*)c.kv + head * c.n_kv_heads * where[0] + (int64_t)where[1] * c.head_dim;

@@ -180,3 +180,21 @@ def test_write_into_shared_pages_is_refused(torch, ops):
     p.same()
     with pytest.raises(ops.RocmError):
         ops.kv_status(p.c)
+
+
+def test_write_of_one_sequence_twice(torch, ops):
+    """The first of two requests for a sequence is carried out, the other refused; one without rows is none."""
+    rng = np.random.default_rng(6)
+    p = Pair(torch, ops, 1, 2, 32, 4, 400, 400, 6)
+    p.add(rng, list(range(300)), [4] * 300)
+    seq, start = list(range(300)) + [7, 9], list(range(301)) + [301, 301]
+    k, v = _rows(rng, p, 301)
+    ops.kv_write(p.c, 0, 1, p.ints(seq), p.ints(start), 302, p.dev(k), p.dev(v), 301)
+    p.ref.write(0, seq[:300], start[:301], k, v)
+    p.same()
+    with pytest.raises(ops.RocmError, match="twice"):
+        ops.kv_status(p.c)
+    ops.kv_write(p.c, 0, 1, p.ints([7, 9, 9]), p.ints([0, 2, 2, 5]), 3, p.dev(k), p.dev(v), 5)
+    p.ref.write(0, [7, 9], [0, 2, 5], k, v)
+    p.same()
+    ops.kv_status(p.c)
