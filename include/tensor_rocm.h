@@ -387,7 +387,8 @@ int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t
  * empty and may not be a source of the same call; a source may come often. */
 int pio_kv_fork(const pio_kv_cache* cache, const int32_t* src, const int32_t* dst, int n, void* stream);
 /* The last count[i] tokens of seq[i] go (all of them where it has fewer, or
- * where count is null); pages that no table entry holds any longer are free. */
+ * where count is null); pages that no table entry holds any longer are free. A
+ * page id outside the cache goes like any other, and is reported. */
 int pio_kv_drop(const pio_kv_cache* cache, const int32_t* seq, const int32_t* count, int n, void* stream);
 /* Moves the pages in use to the lowest slots (the k-th page in use behind them
  * to the k-th free one among them) and rewrites the tables. */

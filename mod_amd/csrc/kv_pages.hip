@@ -454,22 +454,25 @@ __global__ __launch_bounds__(KV_COPY) void kv_fork_kernel(pio_kv_cache c, const 
     const int s = src[i], d = dst[i];
     int bad = !kv_seq_ok(c, s) || !kv_seq_ok(c, d);
     for (int j = tid; j < n; j += KV_COPY) bad |= src[j] == d || (j < i && dst[j] == d);
-    int L = 0;
+    int L = 0, pages = 0, first = 0;
     if (kv_seq_ok(c, s) && kv_seq_ok(c, d)) {
+        const int32_t* row = c.table + (int64_t)s * c.max_pages;
+        if (tid < c.max_pages) first = row[tid];       // beside the length, not behind it
         L = kv_seq_len(c, s);
         // a target that an earlier request names is refused above, whatever its length is by now
         bad |= L < 0 || c.lens[d] != 0;
+        pages = L < 0 ? 0 : kv_pages_of(L, lg);
+        bad |= tid < pages && (first < 0 || first >= c.n_pages);
+        for (int j = tid + KV_COPY; j < pages; j += KV_COPY) bad |= row[j] < 0 || row[j] >= c.n_pages;
     }
     if (__syncthreads_or(bad)) {
         if (tid == 0) atomicOr(kv_work(c).status, KV_BAD);
         return;
     }
-    const int pages = kv_pages_of(L, lg);
     for (int j = tid; j < pages; j += KV_COPY) {
-        const int p = c.table[(int64_t)s * c.max_pages + j];
+        const int p = j == tid ? first : c.table[(int64_t)s * c.max_pages + j];
         c.table[(int64_t)d * c.max_pages + j] = p;
-        if (p >= 0 && p < c.n_pages) atomicAdd(&c.refs[p], 1);
-        else atomicOr(kv_work(c).status, KV_BAD);
+        atomicAdd(&c.refs[p], 1);
     }
     if (tid == 0) {
         c.lens[d] = L;

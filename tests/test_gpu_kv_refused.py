@@ -198,3 +198,23 @@ def test_write_of_one_sequence_twice(torch, ops):
     p.ref.write(0, [7, 9], [0, 2, 5], k, v)
     p.same()
     ops.kv_status(p.c)
+
+
+def test_fork_of_a_bad_page(torch, ops):
+    """A source whose table row holds a page outside the cache is refused, and the target stays empty."""
+    rng = np.random.default_rng(7)
+    p = Pair(torch, ops, 1, 1, 8, 1, 700, 6, 600)
+    p.add(rng, [0, 1], [560, 3])
+    for at, page in ((0, -1), (3, 700), (559, 1 << 30)):
+        p.table[0, at] = page
+        ops.kv_fork(p.c, p.ints([0, 1]), p.ints([2, 3]), 2)
+        torch.cuda.synchronize()
+        p.table[0, at] = int(p.ref.table[0, at])
+        p.ref.fork([1], [3])
+        p.same()
+        with pytest.raises(ops.RocmError):
+            ops.kv_status(p.c)
+        p.drop([3])
+    assert p.fork([0, 1], [2, 3]) == []
+    p.same()
+    ops.kv_status(p.c)
