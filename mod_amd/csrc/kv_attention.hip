@@ -99,7 +99,8 @@ __global__ __launch_bounds__(KA_THREADS) void ka_simple_kernel(KaArgs a) {
     if (req < 0) return;
     const int s = a.seq[req], s0 = a.seq[0], L = kv_seq_len(c, s);
     const int limit = L - count0 + 1;
-    int bad = L < 0 || kv_seq_len(c, s0) < 0;     // the same in every thread, always
+    // the same in every thread, always; of seq[0] only the table row counts, and only where tokens are shared
+    int bad = L < 0 || (a.shared > 0 && (s0 < 0 || s0 >= c.max_seqs));
     const int64_t head = (int64_t)c.page_size * D, page_e = head * c.n_kv_heads;
     const KT* kb = (const KT*)c.kv + (int64_t)(2 * a.layer) * c.n_pages * page_e + g * head;
     const KT* vb = kb + (int64_t)c.n_pages * page_e;

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 from oracle import kv_ref
-from test_gpu_kv_cache import Pair, _say, _tolerance
+from test_gpu_kv_cache import Pair, _attend, _prefix, _say, _tolerance
 
 pytestmark = pytest.mark.gpu
 
@@ -218,3 +218,31 @@ def test_fork_of_a_bad_page(torch, ops):
     assert p.fork([0, 1], [2, 3]) == []
     p.same()
     ops.kv_status(p.c)
+
+
+# ----------------------------------------------------------------- attention ---
+@pytest.mark.parametrize("kv", ["float32", "float16"])
+@pytest.mark.parametrize("D", [40, 64, 128, 256])
+def test_attention_bad_id_first(torch, ops, D, kv):
+    """A bad id at the head of the list, as of a slot without a request. Where nothing is shared, only its
+    own rows are NaN; where something is, the rows have no prefix to read."""
+    _say(f"bad id first D{D} {kv}")
+    rng = np.random.default_rng(11)
+    p = Pair(torch, ops, 1, 2, D, 16, 20, 5, 10, kv)
+    _prefix(p, rng, 3, 40, [4, 40, 20])
+    q = rng.standard_normal((4, 4, D)).astype(np.float32)
+    start = [0, 1, 2, 3, 4]
+    good = _attend(p, torch, ops, 0, [1, 3, 2, 1], start, q, 0.125, 0, 1)
+    ops.kv_status(p.c)
+    for bad in (5, -1):
+        got = _attend(p, torch, ops, 0, [bad, 3, 2, 1], start, q, 0.125, 0, 1)
+        assert np.isnan(got[0]).all() and np.array_equal(got[1:], good[1:])
+        with pytest.raises(ops.RocmError):
+            ops.kv_status(p.c)
+        # a slot without rows is not looked at
+        got = _attend(p, torch, ops, 0, [bad, 3, 2, 1], [1, 1, 2, 3, 4], q, 0.125, 0, 1)
+        assert np.all(got[0] == 7) and np.array_equal(got[1:], good[1:])
+        ops.kv_status(p.c)
+        assert np.isnan(_attend(p, torch, ops, 0, [bad, 3, 2, 1], start, q, 0.125, 40, 1)).all()
+        with pytest.raises(ops.RocmError):
+            ops.kv_status(p.c)
