@@ -48,7 +48,7 @@ struct KaArgs {
     int tail_tiles, tail_runs, max_runs;              // column tiles; the most runs beside one for each request, and of one
     int slots;                                        // items that the device holds at once
     float pre_work;                                   // rounds of keys that the prefix's items cost
-    int tail_items;                                   // (run, column tile, kv head)
+    int tail_items;                                   // workgroups: (run, column tile, kv head), as many as there may be
     bool direct;                                      // one item per column: it writes out itself
     float* part_o;                                    // [pre_splits + max_runs][rows * H][D]
     float* part_ml;                                   // [..][rows * H][2]
@@ -714,14 +714,16 @@ __device__ __forceinline__ int ka_scan(int v, int* red, int& total) {
 }
 
 // Which tail items there are: the tails are cut into runs of about equal length,
-// however uneven they are (every request with rows has at least one). By the whole
-// workgroup; it gets the request, run and geometry of run number `run` (request -1 if
+// however uneven they are (every request with rows has at least one), and a run has the
+// column tiles of its request, at most tail_tiles. By the whole workgroup; it gets the
+// request, run and geometry of item number `unit` over all runs' tiles (request -1 if
 // there are fewer).
 struct KaRun {
     int i, z, runs, per;     // request, run of it, runs of it, rounds of KA_ROUND keys of a run
+    int ct, tiles;           // column tile, tiles of the request
     int r0, r1, s, L;        // rows, sequence, its length (-1: none such)
 };
-__device__ __forceinline__ void ka_runs(const KaArgs& a, int run, KaRun& found, int* red) {
+__device__ __forceinline__ void ka_runs(const KaArgs& a, int unit, KaRun& found, int* red, int cols) {
     const int tid = threadIdx.x, threads = blockDim.x;
     KaRun r{};
     auto rounds = [&](int i) {
@@ -748,16 +750,18 @@ __device__ __forceinline__ void ka_runs(const KaArgs& a, int run, KaRun& found, 
     int before = 0;
     for (int i0 = 0; i0 < a.n; i0 += threads) {
         if (a.n > threads) n = rounds(i0 + tid);
-        r.per = r.runs = 0;
+        r.per = r.runs = r.tiles = 0;
         if (n > 0) {
+            r.tiles = min(a.tail_tiles, ((r.r1 - r.r0) * a.G + cols - 1) / cols);
             r.runs = min(max(1, (int)(n / cut + 0.5f)), a.max_runs);
             r.per = (n + r.runs - 1) / r.runs;
             r.runs = (n + r.per - 1) / r.per;
         }
-        const int at = before + ka_scan(r.runs, red, sum);
+        const int at = before + ka_scan(r.runs * r.tiles, red, sum);
         before += sum;
-        if (run >= at && run < at + r.runs) {
-            r.z = run - at;
+        if (unit >= at && unit < at + r.runs * r.tiles) {
+            r.z = (unit - at) / r.tiles;
+            r.ct = unit - at - r.z * r.tiles;
             found = r;
         }
     }
@@ -1249,17 +1253,16 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
         else
             ka_narrow<KT, D, XP>(a, it, gml, limits, ct * KA_COLS, w, lane);
     } else {
-        const int per_run = a.tail_tiles * a.c.n_kv_heads, item = (int)blockIdx.x - a.pre_items;
-        const int run = item / per_run, in_run = item - run * per_run, g = in_run % a.c.n_kv_heads;
-        ct = in_run / a.c.n_kv_heads;
-        ka_runs(a, run, found, red);
+        constexpr int COLS = WIDE == 2 ? KA_WIDE_COLS : KA_COLS;
+        const int item = (int)blockIdx.x - a.pre_items, unit = item / a.c.n_kv_heads, g = item - unit * a.c.n_kv_heads;
+        ka_runs(a, unit, found, red, COLS);
         const KaRun r = found;
+        ct = r.ct;
         if (!ka_tail(a, it, r, g)) return;
         if (!a.direct && g == 0 && ct == 0 && r.z == 0)
             for (int i = tid; i < r.r1 - r.r0; i += 64 * WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
         // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
-        constexpr int COLS = WIDE == 2 ? KA_WIDE_COLS : KA_COLS;
-        for (int c0 = ct * COLS; c0 < it.ncols; c0 += a.tail_tiles * COLS) {
+        for (int c0 = ct * COLS; c0 < it.ncols; c0 += r.tiles * COLS) {
             if constexpr (WIDE == 2)
                 ka_wide<D, XP>(a, it, ka_lds, (int*)(ka_lds + ka_wide_bytes<D>()), (float (*)[32][2])ml, nullptr, c0);
             else
@@ -1386,8 +1389,10 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const bool long_prefix = cols > 64 && (double)cols * Hk * a.c.head_dim * a.shared >= 0x1.8p30;
     const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : long_prefix ? 1 : 0;
     a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
-    const int64_t items = (int64_t)a.n * Hk * a.tail_tiles;
-    PIO_REQUIRE(items <= 1 << 22, "pio_kv_attention: %d requests of %d rows are too many", a.n, max_rows);
+    // Items of one run to a request: all requests have max_rows rows, or one the most of them and each of
+    // the others at worst one tile that is not full.
+    PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);
+    const int64_t items = std::min((int64_t)a.n * a.tail_tiles, cols / (wide == 2 ? KA_WIDE_COLS : KA_COLS) + a.n) * Hk;
     // Runs. The lengths of the tails are not known here: a short prefix gets a quarter of the device,
     // a longer one up to all of it in runs of 8 rounds or more, and the tails are cut for what is there
     // by the kernel (ka_runs). 32 sequences behind 2,039 tokens 17 us, where both are cut to
@@ -1402,7 +1407,7 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
     a.direct = a.shared == 0 && a.max_runs == 1;
-    a.tail_items = (int)(items + (a.direct ? 0 : (int64_t)a.tail_runs * units));
+    a.tail_items = (int)(items + (a.max_runs == 1 ? 0 : (int64_t)a.tail_runs * units));
     if (a.shared > 0) {
         a.pre_tiles = ceil_div(cols, wide ? KA_WIDE_COLS : KA_COLS);
         const int64_t pre_units = (int64_t)Hk * a.pre_tiles, rounds = ceil_div(a.shared, KA_ROUND), at_once = wide ? cus : 2 * cus;
@@ -1415,6 +1420,9 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
         PIO_REQUIRE(pre <= 1 << 22, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)pre;
     }
+    // (a grid has fewer than 2^32 threads)
+    PIO_REQUIRE(((int64_t)a.pre_items + a.tail_items) * (wide ? 512 : 256) < (int64_t)1 << 32,
+                "pio_kv_attention: %d requests and %d rows are too many", a.n, a.rows);
     Scratch ws;
     if (!a.direct) {
         const size_t parts = (size_t)(a.pre_splits + a.max_runs) * a.rows * a.H;

@@ -246,3 +246,58 @@ def test_attention_bad_id_first(torch, ops, D, kv):
         assert np.isnan(_attend(p, torch, ops, 0, [bad, 3, 2, 1], start, q, 0.125, 40, 1)).all()
         with pytest.raises(ops.RocmError):
             ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("n,Hk,D,rows,kv,x", [(4096, 32, 64, 4200, "float16", "float16"),
+                                              (1024, 16, 64, 5000, "float32", "float32")])
+def test_attention_one_long_window_among_many(torch, ops, n, Hk, D, rows, kv, x):
+    """A prompt in a batch of single tokens, with the right max_rows: n x kv heads x column tiles of the
+    longest window are more items than a launch has."""
+    _say(f"one long window among {n} {kv}")
+    rng = np.random.default_rng(15)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    long = n // 3
+    counts = np.ones(n, int)
+    counts[long] = rows
+    lens = rng.integers(1, 12, n)
+    lens[long] = rows + 30
+    start = np.concatenate([[0], np.cumsum(counts)])
+    all_rows = np.concatenate([[0], np.cumsum(lens)])
+    page, total, R = 8, int(lens.sum()), int(start[-1])
+    pages = int((-(-lens // page)).sum())
+    k, v = (torch.randn(1, total, Hk * D, device="cuda").to(getattr(torch, kv)) for _ in range(2))
+    cache = ops.KvCache(torch.empty(1, 2, pages, Hk, page, D, dtype=k.dtype, device="cuda"),
+                        torch.empty(n, -(-(rows + 30) // page), **i32), torch.empty(n, **i32), torch.empty(pages, **i32))
+    q = torch.randn(R, Hk, D, device="cuda").to(getattr(torch, x))
+    out = torch.full_like(q, 7)
+    seq, dstart = torch.arange(n, **i32), torch.from_numpy(start).to(**i32)
+    dlens, dall = torch.from_numpy(lens).to(**i32), torch.from_numpy(all_rows).to(**i32)
+    torch.cuda.synchronize()
+    ops.kv_init(cache)
+    ops.kv_reserve(cache, seq, dlens, n)
+    ops.kv_write(cache, 0, 1, seq, dall, n, k, v, total)
+    ops.kv_attention(cache, 0, seq, dstart, n, q, out, R, Hk, 0.125, max_rows=rows)
+    ops.kv_status(cache)
+    # |score| < 8 over up to 5,030 keys: 2 es + 8 u + 4 u sqrt(T), es = 4 u sqrt(64) 9
+    u = 2.0 ** -24
+    far = 2 * 4 * u * 8 * 9 + 8 * u + 4 * u * np.sqrt(rows + 30) + (2.0 ** -11 if x == "float16" else 0.0)
+    vmax = float(v.abs().max())
+    tol = vmax * (far + (2.0 ** -11 if x == "float16" else 0.0))
+    for i in [0, 1, long - 1, long, long + 1, n - 1]:
+        a, b, c, d = int(start[i]), int(start[i + 1]), int(all_rows[i]), int(all_rows[i + 1])
+        late = torch.arange(d - c, device="cuda") > (d - c) - (b - a) + torch.arange(b - a, device="cuda")[:, None]
+        for h in range(0, Hk, 5):
+            kk, vv = (t[0, c:d, h * D:(h + 1) * D].double() for t in (k, v))
+            s = (torch.mm(q[a:b, h].double(), kk.T.contiguous()) * 0.125).masked_fill(late, -torch.inf)
+            ref = torch.mm(torch.softmax(s, 1), vv)
+            assert float((out[a:b, h].double() - ref).abs().max()) <= tol
+    # every other request has one row: the mean over its keys by their weights, all at once
+    ones = [i for i in range(n) if i != long]
+    at = torch.from_numpy(start[:-1][ones]).cuda()
+    width = torch.arange(11, device="cuda")
+    key = torch.from_numpy(all_rows[:-1][ones]).cuda()[:, None] + width
+    dead = width >= torch.from_numpy(lens[ones]).cuda()[:, None]
+    kk, vv = (t[0][key.clamp(max=total - 1)].reshape(len(ones), 11, Hk, D).double() for t in (k, v))
+    s = ((kk * q[at].double()[:, None]).sum(3) * 0.125).masked_fill(dead[:, :, None], -torch.inf)
+    ref = (torch.softmax(s, 1)[..., None] * vv).sum(1)
+    assert float((out[at].double() - ref).abs().max()) <= tol
