@@ -405,8 +405,9 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * seq[0], once for all queries. q and out fp32|fp16 [rows, n_heads, head_dim],
  * rows q_stride / out_stride elements apart (multiples of 8), 16-byte aligned;
  * out may be q (at one stride). max_rows: the most queries that one sequence has (larger ones
- * are served too, but slower). A sequence id or a page outside the cache gives
- * NaN rows. Products and sums in fp32: of fp16 queries over an fp16 cache on
+ * are served too, but slower). A sequence id outside the cache gives
+ * NaN rows, seq[0] to all of them where tokens are shared; a page outside it to
+ * the rows that see its keys. Products and sums in fp32: of fp16 queries over an fp16 cache on
  * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32
  * queries over an fp16 cache with queries and weights as two fp16 parts each;
  * over an fp32 cache on the fp32 matrix cores. */

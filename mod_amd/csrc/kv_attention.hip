@@ -854,21 +854,21 @@ struct KaWalk {
     const char *kb, *vb;
     char *kt, *vt;
     int tiles, per_page, lg, mask;
-    int page, pos;                         // this lane's key of the next tile: its page's id, unchecked, and its row there
+    int page, key;                         // this lane's key of the next tile, and its page's id, unchecked
     int64_t off[T::NB];
-    bool bad = false, odd = false;
+    int bad_at = INT_MAX;                  // first key of this lane in a page outside the cache
+    bool odd = false;
 
     // (keys behind the last one re-read it)
     __device__ void look_up(const KaItem& it, int j, int lane) {
-        const int t = min(it.k0 + min(j, tiles - 1) * T::KEYS + lane % T::KEYS, it.k1 - 1);
-        page = it.table[t >> lg];
-        pos = t & mask;
+        key = min(it.k0 + min(j, tiles - 1) * T::KEYS + lane % T::KEYS, it.k1 - 1);
+        page = it.table[key >> lg];
     }
     // Where this lane's 16 bytes of each 8 rows are: rows lane / 8 of them.
     __device__ void offsets(const KaArgs& a, int lane) {
         const bool ok = page >= 0 && page < a.c.n_pages;
-        bad |= !ok;
-        const uint32_t row = (uint32_t)(ok ? page : 0) * (uint32_t)per_page + (uint32_t)pos;
+        bad_at = ok ? bad_at : min(bad_at, key);
+        const uint32_t row = (uint32_t)(ok ? page : 0) * (uint32_t)per_page + (uint32_t)(key & mask);
         int r[T::NB];
 #pragma unroll
         for (int i = 0; i < T::NB; i++) r[i] = __shfl((int)row, 8 * i + lane / 8, 64);
@@ -952,7 +952,7 @@ __device__ __forceinline__ void ka_join(const KaArgs& a, const KaItem& it, KaAcc
     const int col = lane % KA_COLS, part = lane / KA_COLS;
     x.l += __shfl_xor(x.l, 32, 64);
     x.l += __shfl_xor(x.l, 16, 64);
-    if (__any(bad)) x.l = NAN;
+    if (bad) x.l = NAN;
     if (part == 0) {
         ml[w][col][0] = x.m;
         ml[w][col][1] = x.l;
@@ -997,8 +997,14 @@ __device__ __forceinline__ void ka_narrow(const KaArgs& a, const KaItem& it, flo
     const int r = has ? ka_div(a, col) : 0, head = it.g * a.G + (has ? col - r * a.G : 0);
     const int limit = has ? ka_limit(it, limits, ka_div(a, c0), r) : it.k1;
     walk.template run<XP>(a, it, w, lane, limit, it.row0 + r, head, has, acc);
-    const bool bad = __any(it.bad || walk.bad);
-    if (bad && lane == 0) atomicOr(a.c.work, KV_BAD);
+    // a page outside the cache: NaN for the columns that see its keys
+    bool bad = it.bad, told = it.bad;
+    if (__any(walk.bad_at != INT_MAX)) {
+        const int first_bad = ka_wave_min(walk.bad_at);
+        bad |= limit > first_bad;
+        told |= has && (limits ? limits[r - ka_div(a, c0)] : it.first_limit + r) > first_bad;    // (a row without a request: -1)
+    }
+    if (told) atomicOr(a.c.work, KV_BAD);
     ka_join<KT, D>(a, it, acc, ka_lds, ml, w, lane, bad, walk.odd, c0, limits);
 }
 
@@ -1038,7 +1044,8 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
     KaAcc<KT, D, 32> x;
     x.clear();
     int limit = it.k1, least = it.k1;
-    bool bad = it.bad, odd = false;
+    int bad_at = it.bad ? INT_MIN : INT_MAX;       // first key in a page outside the cache
+    bool odd = false;
     const uint32_t kx = ka_kx<KT, D, 32>(lane), vx = ka_vx<KT, D, 32>(lane);
 
     const char* kb = ka_base<T::RB>(a, it.g);
@@ -1054,7 +1061,7 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
         for (int i = tid; i < np; i += 512) {
             if (i != tid) page = it.table[p0 + i];
             if (page < 0 || page >= c.n_pages) {
-                bad = true;
+                bad_at = min(bad_at, max(k0, (p0 + i) << lg));
                 page = 0;
             }
             pages[i] = page;
@@ -1165,9 +1172,19 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
         ml[w][col][0] = x.m;
         ml[w][col][1] = x.l;
     }
-    const bool any_bad = __syncthreads_or(bad);        // and every stage is read
+    const bool any_bad = __syncthreads_or(bad_at != INT_MAX);      // and every stage is read
     odd = __syncthreads_or(odd);
-    if (any_bad && tid == 0) atomicOr(c.work, KV_BAD);
+    if (any_bad) {                         // NaN for the columns that see it
+        if (tid == 0) pages[0] = INT_MAX;
+        __syncthreads();
+        atomicMin(pages, bad_at);
+        __syncthreads();
+        bad_at = pages[0];
+        if (tid < min(KA_WIDE_COLS, it.ncols - base)) {
+            const int row = ka_div(a, base + tid);
+            if ((limits ? limits[row - first] : it.first_limit + row) > bad_at) atomicOr(c.work, KV_BAD);   // (a row without a request: -1)
+        }
+    }
     const float f = __builtin_amdgcn_exp2f(x.m - fmaxf(ml[cg][col][0], ml[cg + 4][col][0]));
     float* ob = (float*)lds + (cg * 32 + col) * T::OP;
     if (kg) ka_spill<KT, D, 32, false>(x, f, ob, h);
@@ -1180,7 +1197,7 @@ __device__ __forceinline__ void ka_wide(const KaArgs& a, const KaItem& it, char*
         const float m0 = ml[cc >> 5][cc & 31][0], m1 = ml[4 + (cc >> 5)][cc & 31][0], m = fmaxf(m0, m1);
         float l = ml[cc >> 5][cc & 31][1] * __builtin_amdgcn_exp2f(m0 - m) +
                   ml[4 + (cc >> 5)][cc & 31][1] * __builtin_amdgcn_exp2f(m1 - m);
-        if (any_bad) l = NAN;
+        if (any_bad && ka_limit(it, limits, first, ka_div(a, base + cc)) > bad_at) l = NAN;
         ka_f4 v = *(const ka_f4*)((const float*)lds + cc * T::OP + d);
         if (mend)
             ka_mend<KT, D>(a, it, limits ? it.k0 : it.first_limit + first - T::KEYS, ka_limit(it, limits, first, ka_div(a, base + cc)), d, v);

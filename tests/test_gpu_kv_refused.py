@@ -301,3 +301,45 @@ def test_attention_one_long_window_among_many(torch, ops, n, Hk, D, rows, kv, x)
     s = ((kk * q[at].double()[:, None]).sum(3) * 0.125).masked_fill(dead[:, :, None], -torch.inf)
     ref = (torch.softmax(s, 1)[..., None] * vv).sum(1)
     assert float((out[at].double() - ref).abs().max()) <= tol
+
+
+@pytest.mark.parametrize("kv,x", [("float32", "float32"), ("float16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("D,window", [(64, 1), (128, 3), (128, 40), (40, 3)])
+def test_attention_bad_page_of_the_prefix(torch, ops, kv, x, D, window):
+    """A page outside the cache in the table row that the common tokens are read through: the rows that see
+    it are NaN and it is reported; rows that stand before it are what they are, and nothing is reported
+    where no row sees it."""
+    _say(f"bad page of the prefix D{D} window {window} {kv} {x}")
+    rng = np.random.default_rng(12)
+    p = Pair(torch, ops, 1, 1, D, 16, 40, 6, 20, kv, fill=np.nan)
+    _prefix(p, rng, 4, 150, [4, 60, 41, 50])
+    p.drop([2, 3], [150, 186])                      # 60 and 5 tokens are left of these
+    seq, counts = [1, 2, 3, 4], [min(window, 4), window, min(window, 9), window]
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+    q = rng.standard_normal((int(start[-1]), 4, D)).astype(x)
+    ref = p.ref.attention(0, seq, start, q, 0.1, np.zeros(q.shape))
+    tol = _tolerance(p, 0, seq, start, q, 0.1, x == "float16")
+    limit = np.concatenate([int(p.ref.lens[s]) - n + 1 + np.arange(n) for s, n in zip(seq, counts)])
+    shared = 150
+    good = _attend(p, torch, ops, 0, seq, start, q, 0.1, shared, window)
+    assert np.abs(good.astype(np.float64) - ref).max() <= tol
+    ops.kv_status(p.c)
+    for at, page in ((4, 40), (3, -1), (2, 1 << 30), (0, -5)):        # (its first token is 64, 48, 32, 0)
+        was = int(p.table[1, at])
+        p.table[1, at] = page
+        got = _attend(p, torch, ops, 0, seq, start, q, 0.1, shared, window)
+        sees = limit > 16 * at
+        assert np.isnan(got[sees]).all()
+        assert np.abs(got[~sees].astype(np.float64) - ref[~sees]).max(initial=0) <= tol
+        with pytest.raises(ops.RocmError):
+            ops.kv_status(p.c)
+        # the short ones alone, behind the first one's table row, whose own rows are left out
+        short = [int(start[1])] + [int(v) for v in start[1:4]]
+        got = _attend(p, torch, ops, 0, seq[:3], short, q, 0.1, shared, window)
+        for r in range(int(start[1]), int(start[3])):
+            assert np.isnan(got[r]).all() if sees[r] else np.abs(got[r].astype(np.float64) - ref[r]).max() <= tol
+        if sees[start[1]:start[3]].any():
+            with pytest.raises(ops.RocmError):
+                ops.kv_status(p.c)
+        ops.kv_status(p.c)
+        p.table[1, at] = was
