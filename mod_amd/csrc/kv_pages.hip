@@ -401,6 +401,14 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
     __syncthreads();
     const int req = found;
     if (req < 0) return;               // behind the last request
+    const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8;
+    const int l0 = blockIdx.y * per_block, l1 = min(layers, l0 + per_block);
+    auto from = [&](int l, int u) {
+        const int kind = u >= width;
+        return (kind ? v : k) + l * layer_stride + row * row_stride + 8 * (u - kind * width);
+    };
+    float x[8];
+    if (tid < 2 * width) load8<XT>(from(l0, tid), x);      // under the way of the checks below
     if (tid == req % KV_COPY) {
         int page = -1, pos = -1;
         bool held_up = false;
@@ -426,15 +434,12 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         return;
     }
     if (where[0] < 0) return;          // without room, or refused above
-    const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8;
     const int64_t head = (int64_t)c.page_size * c.head_dim, plane = head * c.n_kv_heads * c.n_pages;
     KT* base = (KT*)c.kv + head * c.n_kv_heads * where[0] + (int64_t)where[1] * c.head_dim;
-    const int l1 = min(layers, (int)(blockIdx.y + 1) * per_block);
-    for (int l = blockIdx.y * per_block; l < l1; l++) {
+    for (int l = l0; l < l1; l++) {
         for (int u = tid; u < 2 * width; u += KV_COPY) {
             const int kind = u >= width, e = u - kind * width, h = e / per_head;
-            float x[8];
-            load8<XT>((kind ? v : k) + l * layer_stride + row * row_stride + 8 * e, x);
+            if (l != l0 || u != tid) load8<XT>(from(l, u), x);
             KT* to = base + (2 * (layer + l) + kind) * plane + h * head + 8 * (e - h * per_head);
             __attribute__((aligned(16))) KT y[8];
 #pragma unroll
