@@ -327,6 +327,25 @@ def moe_w8a8(x, logits, w_gu, s_gu, w_down, s_down, out, T: int, H: int, I: int,
                            _ptr(workspace), _stream(stream)), "pio_moe_w8a8")
 
 
+def _list(x, name: str, code: int = I32) -> int | None:
+    """Device pointer of a list that the library reads as int32 (or `code`); raw pointers are taken as they are."""
+    if x is None or type(x) is int:
+        return x
+    try:
+        if _dtype_seen[x.dtype] == code:
+            p = x.data_ptr()
+            return p if type(p) is int else int(p)
+    except (KeyError, TypeError, AttributeError):    # not seen yet, without a hash, without a dtype
+        pass
+    try:
+        right = _dt(x, code) == code
+    except TypeError:                                # a type that no call takes
+        right = False
+    if not right:
+        raise TypeError(f"{name} must be {'int32' if code == I32 else 'float32'}, not {x.dtype}")
+    return _ptr(x)
+
+
 class KvCache:
     """A paged key / value cache over memory that the caller owns: kv
     [layers, 2, pages, kv heads, page size, head dim] fp32 | fp16, table [sequences,
@@ -384,22 +403,24 @@ def kv_status(cache: KvCache, stream=None) -> None:
 
 
 def kv_reserve(cache: KvCache, seq, count, n: int, stream=None) -> None:
-    check(lib.pio_kv_reserve(cache.ref, _ptr(seq), _ptr(count), n, _stream(stream)), "pio_kv_reserve")
+    check(lib.pio_kv_reserve(cache.ref, _list(seq, "seq"), _list(count, "count"), n, _stream(stream)), "pio_kv_reserve")
 
 
 def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, row_stride: int = 0,
              layer_stride: int = 0, stream=None) -> None:
-    check(lib.pio_kv_write(cache.ref, layer, layers, _ptr(seq), _ptr(row_start), n, _ptr(k), _ptr(v), _dt(k), rows,
-                           row_stride, layer_stride, _stream(stream)), "pio_kv_write")
+    if _dt(k) != _dt(v):
+        raise TypeError("kv_write: k and v differ in dtype")
+    check(lib.pio_kv_write(cache.ref, layer, layers, _list(seq, "seq"), _list(row_start, "row_start"), n, _ptr(k), _ptr(v),
+                           _dt(k), rows, row_stride, layer_stride, _stream(stream)), "pio_kv_write")
 
 
 def kv_fork(cache: KvCache, src, dst, n: int, stream=None) -> None:
-    check(lib.pio_kv_fork(cache.ref, _ptr(src), _ptr(dst), n, _stream(stream)), "pio_kv_fork")
+    check(lib.pio_kv_fork(cache.ref, _list(src, "src"), _list(dst, "dst"), n, _stream(stream)), "pio_kv_fork")
 
 
 def kv_drop(cache: KvCache, seq, count, n: int, stream=None) -> None:
     """count None: all tokens of each sequence."""
-    check(lib.pio_kv_drop(cache.ref, _ptr(seq), _ptr(count), n, _stream(stream)), "pio_kv_drop")
+    check(lib.pio_kv_drop(cache.ref, _list(seq, "seq"), _list(count, "count"), n, _stream(stream)), "pio_kv_drop")
 
 
 def kv_compact(cache: KvCache, stream=None) -> None:
@@ -412,8 +433,8 @@ def kv_attention(cache: KvCache, layer: int, seq, row_start, n: int, q, out, row
     tokens are common to the batch and read once."""
     if _dt(q) != _dt(out):
         raise TypeError("kv_attention: q and out differ in dtype")
-    check(lib.pio_kv_attention(cache.ref, layer, _ptr(seq), _ptr(row_start), n, shared, _ptr(q), _ptr(out), _dt(q),
-                               rows, n_heads, q_stride, out_stride, max_rows, scale, _stream(stream)),
+    check(lib.pio_kv_attention(cache.ref, layer, _list(seq, "seq"), _list(row_start, "row_start"), n, shared, _ptr(q),
+                               _ptr(out), _dt(q), rows, n_heads, q_stride, out_stride, max_rows, scale, _stream(stream)),
           "pio_kv_attention")
 
 
@@ -422,9 +443,10 @@ def verify_draft(target, draft, ids, u, u_next, row_start, n: int, rows: int, vo
     """draft None: the drafted tokens were certain."""
     if draft is not None and _dt(draft) != _dt(target):
         raise TypeError("verify_draft: target and draft differ in dtype")
-    check(lib.pio_verify_draft(_ptr(target), target_stride, _ptr(draft), draft_stride, _dt(target), _ptr(ids), _ptr(u),
-                               _ptr(u_next), _ptr(row_start), n, rows, vocab, _ptr(accepted), _ptr(tokens),
-                               _ptr(rejected), _stream(stream)), "pio_verify_draft")
+    check(lib.pio_verify_draft(_ptr(target), target_stride, _ptr(draft), draft_stride, _dt(target), _list(ids, "ids"),
+                               _list(u, "u", F32), _list(u_next, "u_next", F32), _list(row_start, "row_start"), n, rows,
+                               vocab, _list(accepted, "accepted"), _list(tokens, "tokens"), _list(rejected, "rejected"),
+                               _stream(stream)), "pio_verify_draft")
 
 
 def pool_stats() -> dict:

@@ -70,3 +70,30 @@ def test_workspace_refusals():
     assert ops.lib.pio_kv_work_create(ctypes.byref(c), -1) == ops.ERR_INVALID and "device" in ops.last_error()
     ops.lib.pio_kv_work_destroy(None, 0)
     ops.lib.pio_kv_work_destroy(ctypes.byref(c), 0)
+
+
+def test_lists_and_types():
+    """What the library reads as int32 or fp32 is that type, and k and v are of one."""
+    from mod_amd import ops
+    i, wrong = torch.zeros(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int64)
+    f, half = torch.zeros(8), torch.zeros(8).half()
+
+    class Cache:
+        ref = None
+    c = Cache()
+    for bad in (lambda: ops.kv_reserve(c, wrong, i, 1), lambda: ops.kv_reserve(c, i, wrong, 1),
+                lambda: ops.kv_fork(c, wrong, i, 1), lambda: ops.kv_fork(c, i, wrong, 1),
+                lambda: ops.kv_drop(c, wrong, None, 1), lambda: ops.kv_drop(c, i, wrong, 1),
+                lambda: ops.kv_write(c, 0, 1, wrong, i, 1, f, f, 1), lambda: ops.kv_write(c, 0, 1, i, wrong, 1, f, f, 1),
+                lambda: ops.kv_write(c, 0, 1, i, i, 1, f, half, 1),
+                lambda: ops.kv_attention(c, 0, wrong, i, 1, f, f, 1, 8, 1.0),
+                lambda: ops.kv_attention(c, 0, i, wrong, 1, f, f, 1, 8, 1.0),
+                lambda: ops.verify_draft(f, None, wrong, f, f, i, 1, 1, 8, i, i),
+                lambda: ops.verify_draft(f, None, i, half, f, i, 1, 1, 8, i, i),
+                lambda: ops.verify_draft(f, None, i, f, half, i, 1, 1, 8, i, i),
+                lambda: ops.verify_draft(f, None, i, f, f, wrong, 1, 1, 8, i, i),
+                lambda: ops.verify_draft(f, None, i, f, f, i, 1, 1, 8, wrong, i),
+                lambda: ops.verify_draft(f, None, i, f, f, i, 1, 1, 8, i, wrong),
+                lambda: ops.verify_draft(f, None, i, f, f, i, 1, 1, 8, i, i, wrong)):
+        with pytest.raises(TypeError, match="must be|differ"):
+            bad()
