@@ -410,7 +410,11 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * the rows that see its keys. Products and sums in fp32: of fp16 queries over an fp16 cache on
  * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32
  * queries over an fp16 cache with queries and weights as two fp16 parts each;
- * over an fp32 cache on the fp32 matrix cores. */
+ * over an fp32 cache on the fp32 matrix cores. Where head_dim is 64 or 128 the
+ * parts of a row that are computed apart (runs of its own tokens, of the shared
+ * ones) meet in a workspace, rows * n_heads * (head_dim + 2) * 4 bytes each: up to
+ * 256 MB for its own tokens or one part, whichever is more, and the shared ones'
+ * on top (one part where rows are many). */
 int pio_kv_attention(const pio_kv_cache* cache, int layer, const int32_t* seq, const int32_t* row_start, int n,
                      int shared, const void* q, void* out, int dtype, int rows, int n_heads, int64_t q_stride,
                      int64_t out_stride, int max_rows, float scale, void* stream);

@@ -1401,9 +1401,17 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const bool f16 = a.c.kv_dtype == PIO_F16;
     const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
     // A wide kernel for the prefix reads it once for 128 columns, but comes on top of the tails', some
-    // 10 us: 512 columns x 4 kv heads x 128 dimensions over 4,096 tokens 39 us (narrow 32), over 8,192
-    // 42 (43), over 16,000 50 (65); 256 x 8 x 64 over 8,000 30 (26), over 32,000 52 (73).
+    // 10 us. fp16 queries, 512 columns x 4 kv heads x 128 dimensions over 4,000 tokens 36 us (narrow 28),
+    // over 8,000 39 (39), over 16,000 45 (58), over 32,000 64 (94); 128 x 8 x 64 over 16,000 30 (24), over
+    // 32,000 36 (37). fp32 queries, whose wide kernel spills registers, even out at more than this: 512
+    // x 4 x 128 over 8,000 49 (42), over 16,000 64 (64), over 32,000 93 (108).
     const bool long_prefix = cols > 64 && (double)cols * Hk * a.c.head_dim * a.shared >= 0x1.8p30;
+    // Wide items for tails of more than 32 columns, which pays where there is much to read for many of them:
+    // 8 heads to each of 4 kv heads of 128, fp16 queries, a prompt of 1,000 tokens 37 us (narrow 67), 48
+    // windows of 8 behind 8,000 tokens 99 (121), of 5 behind 2,000 41 (52), 16 windows of 5 over 3,000 own
+    // tokens 41 (44); and costs up to twice as much where there is little (the tails' lengths are not known
+    // here): 16 windows of 16 over 300 own tokens 23 (16), one of 8 over 4,000 19 (13); fp32 queries 35 (18),
+    // 25 (14), the prompt 56 (77), the windows behind 8,000 144 (161).
     const int wide = !f16 ? 0 : tail_cols > 32 ? 2 : long_prefix ? 1 : 0;
     a.tail_tiles = ceil_div(tail_cols, wide == 2 ? KA_WIDE_COLS : KA_COLS);
     // Items of one run to a request: all requests have max_rows rows, or one the most of them and each of
@@ -1420,7 +1428,10 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int64_t units = (int64_t)Hk * a.tail_tiles;
     a.tail_runs = (int)std::max<int64_t>(1, (wide == 2 ? cus / 2 : 2 * cus) / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    // (and no more than 256 MB of the workspace: many requests fill the device without)
+    // At most 32 to a request: one of 100,000 tokens over 4 kv heads of 128 takes 38 us (with 128 runs 41),
+    // over one kv head 34 (20). And no more than 256 MB of partial results hold, as many rows fill the
+    // device without; one there is whatever its size, and the prefix's runs come on top: rows x heads x
+    // (D + 2) x 4 bytes for each.
     const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 32, ceil_div(longest, KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
     a.direct = a.shared == 0 && a.max_runs == 1;
