@@ -68,3 +68,39 @@ def test_close_while_another_stream_captures(torch, ops):
         torch.cuda.synchronize()
         assert int(lens[1]) == 3 * (i + 1)
     ops.kv_status(c)
+
+
+def test_open_while_another_stream_captures(torch, ops):
+    """A handle opened while torch captures a graph on a stream of its own works, and the graph too."""
+    c, (kv, table, lens, refs) = _open(torch, ops)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    one, three = torch.tensor([1], **i32), torch.tensor([3], **i32)
+    more = (torch.zeros(1, 2, 6, 1, 4, 8, device="cuda"), torch.full((4, 6), -1, **i32), torch.zeros(4, **i32),
+            torch.zeros(6, **i32))
+    graph, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=st):
+        ops.kv_reserve(c, one, three, 1, stream=st)
+        other = ops.KvCache(*more)
+    for i in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int(lens[1]) == 3 * (i + 1)
+    ops.kv_reserve(other, one, three, 1)
+    ops.kv_status(other)
+    assert more[2].tolist() == [0, 3, 0, 0]
+    ops.kv_status(c)
+
+
+def test_open_in_the_captured_stream_is_refused(torch, ops):
+    """The workspace is cleared by work that is waited for, which the library's own capture cannot record."""
+    from mod_amd import backend
+    c, t = _open(torch, ops)
+    graph = backend.HIPGraph()
+    torch.cuda.synchronize()
+    graph.capture_begin()
+    ops.kv_fork(c, t[2], t[2], 0)
+    with pytest.raises(ops.RocmError, match="capturing"):
+        ops.KvCache(*t)
+    graph.capture_end()
+    ops.kv_status(c)
