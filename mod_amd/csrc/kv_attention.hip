@@ -833,7 +833,7 @@ __device__ __forceinline__ int ka_limit(const KaItem& it, const int* limits, int
 // 16 x 16 products read K and V at the same rate. Two workgroups to a CU (64 KB of LDS each at
 // fp16 x 128). Long tails are bound by HBM: 8 sequences of 20,000 tokens (8 kv heads x 128,
 // fp16) 24.4 us, 4.1 TB/s; short ones by an item's chain of waits (its requests, a page, K, the
-// join), some 12,000 clocks: 32 sequences behind 2,039 tokens 14.8 us, 2.1 TB/s.
+// join), some 12,000 clocks: 32 sequences behind 2,039 tokens 15.3 us, 2.1 TB/s.
 constexpr int KA_COLS = 16, KA_WAVES = 4;
 
 template <int N>
@@ -1012,7 +1012,7 @@ __device__ __forceinline__ void ka_narrow(const KaArgs& a, const KaItem& it, flo
 // 64 keys by waves w / 4. K and V of 64 keys are one of KA_STAGES stages in LDS that the
 // waves copy together, so that they cross from L2 once for 128 columns. Bound by the waves'
 // own work between two barriers, 2,700 clocks a stage: the matrix cores have 1,024 of it, the
-// VALU 1,600, LDS 1,300. 512 columns over 32,000 tokens (4 kv heads x 128): 54 us, 620 TFLOP/s,
+// VALU 1,600, LDS 1,300. 512 columns over 32,000 tokens (4 kv heads x 128): 53 us, 630 TFLOP/s,
 // 10 of it an item's first and last 20,000 clocks; 4 x as many columns 700 TFLOP/s. Tried
 // and no faster: 4 waves of 64 columns with all registers of a SIMD each (the accumulators move
 // between register files), the second half's waves half a stage behind the first's, products
@@ -1292,7 +1292,7 @@ __global__ __launch_bounds__(WIDE ? 512 : 256, 2) void ka_kernel(KaArgs a) {
 // A column's items joined: D / 4 lanes have its dimensions, Z groups of them take
 // every Z-th item, all loads of a few in flight together. Z = 8: few columns, where
 // latency counts (1,024 columns of 5 items 4 us); Z = 1: 8 (16) columns to a workgroup
-// (6,752 of 4 items 5.5 us, 3.6 TB/s).
+// (6,752 of 4 items 5.7 us, 3.5 TB/s).
 template <int D, int Z>
 __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
     constexpr int TPC = D / 4, GRP = 256 / TPC, COLS = GRP / Z;

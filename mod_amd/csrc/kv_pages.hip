@@ -378,7 +378,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c
 // ----------------------------------------------------------------- write ----
 // A workgroup takes one row through a few layers: it finds the row's request,
 // then moves k and v in pieces of 8 elements. Bytes bound it: 336 rows of 28 layers,
-// fp32 to fp16, 31 us, 3.6 TB/s.
+// fp32 to fp16, 32 us, 3.5 TB/s; few rows, the chain of loads that says where a row goes
+// and whether it may: 8 rows of one layer 4.3 us, 3.6 without its checks.
 template <typename XT, typename KT>
 __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int layer, int layers,
                                                           const int32_t* __restrict__ seq,

@@ -403,11 +403,14 @@ def kv_status(cache: KvCache, stream=None) -> None:
 
 
 def kv_reserve(cache: KvCache, seq, count, n: int, stream=None) -> None:
+    """Room for count[i] more tokens of seq[i], all or nothing. Behind a refused call kv_write and kv_drop by
+    counts leave its sequences alone, until kv_status, a reserve that serves them, or their end."""
     check(lib.pio_kv_reserve(cache.ref, _list(seq, "seq"), _list(count, "count"), n, _stream(stream)), "pio_kv_reserve")
 
 
 def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, row_stride: int = 0,
              layer_stride: int = 0, stream=None) -> None:
+    """The last tokens of each sequence, in pages that no other sequence holds."""
     if _dt(k) != _dt(v):
         raise TypeError("kv_write: k and v differ in dtype")
     check(lib.pio_kv_write(cache.ref, layer, layers, _list(seq, "seq"), _list(row_start, "row_start"), n, _ptr(k), _ptr(v),
