@@ -327,15 +327,18 @@ def moe_w8a8(x, logits, w_gu, s_gu, w_down, s_down, out, T: int, H: int, I: int,
                            _ptr(workspace), _stream(stream)), "pio_moe_w8a8")
 
 
+_list_dtype: dict = {I32: _MISSING, F32: _MISSING}     # of the last list of each type
+
+
 def _list(x, name: str, code: int = I32) -> int | None:
     """Device pointer of a list that the library reads as int32 (or `code`); raw pointers are taken as they are."""
     if x is None or type(x) is int:
         return x
     try:
-        if _dtype_seen[x.dtype] == code:
+        if x.dtype is _list_dtype[code]:             # as the last one's: a torch dtype is one object
             p = x.data_ptr()
             return p if type(p) is int else int(p)
-    except (KeyError, TypeError, AttributeError):    # not seen yet, without a hash, without a dtype
+    except AttributeError:                           # without a dtype
         pass
     try:
         right = _dt(x, code) == code
@@ -343,6 +346,7 @@ def _list(x, name: str, code: int = I32) -> int | None:
         right = False
     if not right:
         raise TypeError(f"{name} must be {'int32' if code == I32 else 'float32'}, not {x.dtype}")
+    _list_dtype[code] = getattr(x, "dtype", _MISSING)
     return _ptr(x)
 
 
@@ -411,10 +415,11 @@ def kv_reserve(cache: KvCache, seq, count, n: int, stream=None) -> None:
 def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, row_stride: int = 0,
              layer_stride: int = 0, stream=None) -> None:
     """The last tokens of each sequence, in pages that no other sequence holds."""
-    if _dt(k) != _dt(v):
+    dt = _dt(k)
+    if _dt(v) != dt:
         raise TypeError("kv_write: k and v differ in dtype")
     check(lib.pio_kv_write(cache.ref, layer, layers, _list(seq, "seq"), _list(row_start, "row_start"), n, _ptr(k), _ptr(v),
-                           _dt(k), rows, row_stride, layer_stride, _stream(stream)), "pio_kv_write")
+                           dt, rows, row_stride, layer_stride, _stream(stream)), "pio_kv_write")
 
 
 def kv_fork(cache: KvCache, src, dst, n: int, stream=None) -> None:
@@ -434,19 +439,21 @@ def kv_attention(cache: KvCache, layer: int, seq, row_start, n: int, q, out, row
                  shared: int = 0, max_rows: int = 1, q_stride: int = 0, out_stride: int = 0, stream=None) -> None:
     """out[r, h] = softmax(scale q[r, h] k^T) v, causal, over each sequence's pages; the first `shared`
     tokens are common to the batch and read once."""
-    if _dt(q) != _dt(out):
+    dt = _dt(q)
+    if _dt(out) != dt:
         raise TypeError("kv_attention: q and out differ in dtype")
     check(lib.pio_kv_attention(cache.ref, layer, _list(seq, "seq"), _list(row_start, "row_start"), n, shared, _ptr(q),
-                               _ptr(out), _dt(q), rows, n_heads, q_stride, out_stride, max_rows, scale, _stream(stream)),
+                               _ptr(out), dt, rows, n_heads, q_stride, out_stride, max_rows, scale, _stream(stream)),
           "pio_kv_attention")
 
 
 def verify_draft(target, draft, ids, u, u_next, row_start, n: int, rows: int, vocab: int, accepted, tokens,
                  rejected=None, target_stride: int = 0, draft_stride: int = 0, stream=None) -> None:
     """draft None: the drafted tokens were certain."""
-    if draft is not None and _dt(draft) != _dt(target):
+    dt = _dt(target)
+    if draft is not None and _dt(draft) != dt:
         raise TypeError("verify_draft: target and draft differ in dtype")
-    check(lib.pio_verify_draft(_ptr(target), target_stride, _ptr(draft), draft_stride, _dt(target), _list(ids, "ids"),
+    check(lib.pio_verify_draft(_ptr(target), target_stride, _ptr(draft), draft_stride, dt, _list(ids, "ids"),
                                _list(u, "u", F32), _list(u_next, "u_next", F32), _list(row_start, "row_start"), n, rows,
                                vocab, _list(accepted, "accepted"), _list(tokens, "tokens"), _list(rejected, "rejected"),
                                _stream(stream)), "pio_verify_draft")
