@@ -53,6 +53,7 @@ enum {
     PIO_F16 = 1,
     PIO_I8 = 2,
     PIO_I32 = 3,
+    PIO_MX4 = 4,            /* paged caches only: 4 bits a value, see pio_kv_cache */
 };
 
 /* Status codes returned by every `int` entry point. */
@@ -311,14 +312,14 @@ int pio_moe_w8a8(const void* x, int x_dtype, const float* logits, const int8_t* 
  *
  * The caller owns the memory; all of it is on the device, so that a step's
  * calls can be captured into a HIP graph and need no host round trip:
- *   kv     fp32|fp16 [n_layers][2 (k, v)][n_pages][n_kv_heads][page_size][head_dim]
+ *   kv     fp32|fp16 [n_layers][2 (k, v)][n_pages][n_kv_heads][page_size][head_dim], or 4 bits, below
  *   table  int32 [max_seqs][max_pages]  page ids of each sequence, -1 behind its last
  *   lens   int32 [max_seqs]             tokens of each sequence
  *   refs   int32 [n_pages]              table entries that hold each page, 0 = free
  *   work   int32, pio_kv_work_bytes()   plans of the calls below and their status; zeroed, or pio_kv_init
  * Sequences may share pages (pio_kv_fork). page_size is a power of two from 1 to
- * 1024, head_dim a multiple of 8 up to 256; kv is 16-byte aligned, table rows
- * and the other arrays 4-byte. The lists of sequence ids and counts are int32
+ * 1024, head_dim a multiple of 8 up to 256 (4 bits: from 16, and of 32); kv is
+ * 16-byte aligned, table rows and the other arrays 4-byte. The lists of sequence ids and counts are int32
  * on the device as well. Calls on one cache are ordered by the caller (one
  * stream, or events): each reads what the one before it left.
  *
@@ -327,6 +328,19 @@ int pio_moe_w8a8(const void* x, int x_dtype, const float* logits, const int8_t* 
  * checked by the kernels: such a request changes nothing, and
  * pio_kv_status reports it. At most 2^20 pages, sequences and pages a sequence, 2^28
  * tokens a sequence.
+ *
+ * 4 bits (kv_dtype PIO_MX4): 32 neighbouring values of a token's head share a power
+ * of two, 2^e, and each is +- 0, 0.5, 1, 1.5, 2, 3, 4 or 6 times it, the operand
+ * type of the scaled matrix instructions. e is the least with max |x| < 7 * 2^e,
+ * so that no value is off by more than half a step, within -23 .. 13 (all values
+ * are fp16 numbers; those beyond 7 * 2^13 become 6 * 2^13); a value goes to the
+ * nearest, ties to the even code. A block of 32 that holds an inf or a NaN is NaN.
+ *   kv     bytes [n_layers][2 (k, v)][n_pages][n_kv_heads][page_size * 17 * head_dim / 32]:
+ *          of a (page, kv head) the codes [page_size][head_dim / 2], two to a byte, the even
+ *          dimension in the low half (sign, 2 bits of exponent, 1 of mantissa), then the
+ *          scales [head_dim / 32][page_size], a byte each: e + 127, 104 to 140; 255 is NaN.
+ * Other scale bytes may lie behind a sequence's last token; among its tokens they
+ * make the results of rows that see them undefined.
  * ------------------------------------------------------------------------- */
 typedef struct {
     void* kv;
@@ -375,7 +389,7 @@ int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t*
  * `layers` layers from `layer`. k and v [layers][rows][n_kv_heads * head_dim]
  * with rows `row_stride` and layers `layer_stride` elements apart (each a
  * multiple of 8, or 0 for dense rows / layers), fp32|fp16, rounded to the
- * cache's type, 16-byte aligned, fewer than 2^24 rows; of requests with rows for one
+ * cache's type (quantised, in 4 bits), 16-byte aligned, fewer than 2^24 rows; of requests with rows for one
  * sequence the first is served. row_start int32 [n + 1], ascending; rows at
  * and behind row_start[n] are not read. A row whose page another table entry holds
  * as well is refused, the others are written: pio_kv_reserve gives new tokens pages
@@ -383,6 +397,16 @@ int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t*
 int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
                  int n, const void* k, const void* v, int dtype, int rows, int64_t row_stride,
                  int64_t layer_stride, void* stream);
+/* Tokens out of the cache: rows row_start[i] .. row_start[i + 1] - 1 of k and v
+ * become the keys and values of seq[i]'s tokens from first[i] on (its last ones,
+ * where first is null), in `layers` layers from `layer`; the layouts and limits are
+ * pio_kv_write's, and rows and layers may not overlap. fp32|fp16, rounded to
+ * it from an fp32 cache. A row whose sequence, token or page is not there becomes NaN, and
+ * pio_kv_status reports it; rows at and behind row_start[n] are left as they are. One
+ * sequence may come often. */
+int pio_kv_read(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
+                const int32_t* first, int n, void* k, void* v, int dtype, int rows, int64_t row_stride,
+                int64_t layer_stride, void* stream);
 /* dst[i] becomes a copy of src[i] that shares all its pages. dst[i] must be
  * empty and may not be a source of the same call; a source may come often. */
 int pio_kv_fork(const pio_kv_cache* cache, const int32_t* src, const int32_t* dst, int n, void* stream);
@@ -410,7 +434,10 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * the rows that see its keys. Products and sums in fp32: of fp16 queries over an fp16 cache on
  * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32
  * queries over an fp16 cache with queries and weights as two fp16 parts each;
- * over an fp32 cache on the fp32 matrix cores. Where head_dim is 64 or 128 the
+ * over an fp32 cache on the fp32 matrix cores. Over a cache of 4 bits the keys are
+ * operands of the scaled matrix cores as they lie there and the queries the sum of 3 (fp16) or
+ * 5 (fp32) parts of 6 bits, exact to 2^-13 (2^-23) of the largest of 32 dimensions; the values
+ * are exact in fp16, the weights as over an fp16 cache. Where head_dim is 64 or 128 the
  * parts of a row that are computed apart (runs of its own tokens, of the shared
  * ones) meet in a workspace, rows * n_heads * (head_dim + 2) * 4 bytes each: up to
  * 256 MB for its own tokens or one part, whichever is more, and the shared ones'

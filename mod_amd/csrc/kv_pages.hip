@@ -11,6 +11,8 @@
 
 #include <algorithm>
 #include <climits>
+#include <cmath>
+#include <type_traits>
 
 namespace pio {
 
@@ -46,14 +48,16 @@ __host__ __device__ __forceinline__ KvWork kv_work(const pio_kv_cache& c) {
 int kv_check(const pio_kv_cache* c, const char* what) {
     PIO_REQUIRE(c, "%s: null cache", what);
     PIO_REQUIRE(c->kv && c->table && c->lens && c->refs && c->work, "%s: null pointer in the cache", what);
-    PIO_REQUIRE(c->kv_dtype == PIO_F32 || c->kv_dtype == PIO_F16, "%s: cache dtype %d (fp32 or fp16)", what,
-                c->kv_dtype);
+    PIO_REQUIRE(c->kv_dtype == PIO_F32 || c->kv_dtype == PIO_F16 || c->kv_dtype == PIO_MX4,
+                "%s: cache dtype %d (fp32, fp16 or 4 bits)", what, c->kv_dtype);
     PIO_REQUIRE(c->n_layers > 0 && c->n_kv_heads > 0 && c->n_pages > 0 && c->max_seqs > 0 && c->max_pages > 0,
                 "%s: empty cache dimension", what);
     PIO_REQUIRE(c->head_dim >= 8 && c->head_dim <= 256 && c->head_dim % 8 == 0,
                 "%s: head_dim %d (a multiple of 8 up to 256)", what, c->head_dim);
     PIO_REQUIRE(c->page_size >= 1 && c->page_size <= 1024 && (c->page_size & (c->page_size - 1)) == 0,
                 "%s: page_size %d (a power of two up to 1024)", what, c->page_size);
+    PIO_REQUIRE(c->kv_dtype != PIO_MX4 || (c->head_dim % 32 == 0 && c->page_size >= 16),
+                "%s: 4 bits, head_dim %d, page_size %d (a multiple of 32, from 16)", what, c->head_dim, c->page_size);
     // positions, and the pages or rounds of keys that 1024 requests need, are counted in 32 bits
     PIO_REQUIRE((int64_t)c->max_pages * c->page_size <= 1 << 28, "%s: table rows of over 2^28 positions", what);
     PIO_REQUIRE(c->n_pages <= 1 << 20 && c->max_seqs <= 1 << 20 && c->max_pages <= 1 << 20,
@@ -248,7 +252,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 }
 
 // ------------------------------------------------------------- page copy ----
-// Pairs of the plan: the first rows of each head, in every layer's k and v; a workgroup
+// Pairs of the plan: the first rows of each head (of a cache of 4 bits, whose scales lie
+// behind a page's codes, the whole page), in every layer's k and v; a workgroup
 // takes a plane (layer, k or v) of a pair, n_kv_heads runs of rows * head_dim elements.
 // tables: also rewrites the tables by remap and moves the pages' counts (compact).
 //   Bytes bound it, from memory: 84 whole pages of 16 x 8 x 128 fp16 in 56 planes, half of
@@ -257,8 +262,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_reserve_plan_kernel(pio_kv_cache c
 __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int tables) {
     const KvWork w = kv_work(c);
     const int pairs = min(*w.pairs_n, c.n_pages), planes = 2 * c.n_layers, tid = threadIdx.x;
-    const int esz = c.kv_dtype == PIO_F32 ? 4 : 2;
-    const int64_t head_b = (int64_t)c.page_size * c.head_dim * esz, page_b = head_b * c.n_kv_heads;
+    const int token_b = kv_token_bytes(c);
+    const int64_t head_b = (int64_t)c.page_size * token_b, page_b = head_b * c.n_kv_heads;
     const int pitch = (int)(head_b / 16);
     for (int pair = blockIdx.y; pair < pairs; pair += gridDim.y) {
         const int from = w.pairs[3 * pair], to = w.pairs[3 * pair + 1], rows = w.pairs[3 * pair + 2];
@@ -266,7 +271,7 @@ __global__ __launch_bounds__(KV_COPY) void kv_copy_kernel(pio_kv_cache c, int ta
         if ((unsigned)from >= (unsigned)c.n_pages || (unsigned)to >= (unsigned)c.n_pages ||
             (unsigned)rows > (unsigned)c.page_size)
             continue;
-        const int run = rows * c.head_dim * esz / 16, all = run * c.n_kv_heads;
+        const int run = c.kv_dtype == PIO_MX4 ? pitch : rows * token_b / 16, all = run * c.n_kv_heads;
         const uint32_t magic = run > 1 ? 0xffffffffu / run + 1 : 0;     // u / run, or one more
         auto at = [&](int u) {
             if (run == pitch) return u;
@@ -379,7 +384,8 @@ __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c
 // A workgroup takes one row through a few layers: it finds the row's request,
 // then moves k and v in pieces of 8 elements. Bytes bound it: 336 rows of 28 layers,
 // fp32 to fp16, 32 us, 3.5 TB/s; few rows, the chain of loads that says where a row goes
-// and whether it may: 8 rows of one layer 4.3 us, 3.6 without its checks.
+// and whether it may: 8 rows of one layer 4.3 us, 3.6 without its checks. In 4 bits the four
+// threads of a block of 32 values share its largest magnitude.
 template <typename XT, typename KT>
 __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int layer, int layers,
                                                           const int32_t* __restrict__ seq,
@@ -435,18 +441,93 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         return;
     }
     if (where[0] < 0) return;          // without room, or refused above
-    const int64_t head = (int64_t)c.page_size * c.head_dim, plane = head * c.n_kv_heads * c.n_pages;
-    KT* base = (KT*)c.kv + head * c.n_kv_heads * where[0] + (int64_t)where[1] * c.head_dim;
+    if constexpr (std::is_same_v<KT, KvMx4>) {
+        const int64_t head = (int64_t)c.page_size * kv_token_bytes(c), plane = head * c.n_kv_heads * c.n_pages;
+        char* base = (char*)c.kv + head * c.n_kv_heads * where[0];
+        for (int l = l0; l < l1; l++) {
+            for (int u = tid; u < 2 * width; u += KV_COPY) {       // (all four threads of a block, or none)
+                const int kind = u >= width, e = u - kind * width, h = e / per_head, piece = e - h * per_head;
+                if (l != l0 || u != tid) load8<XT>(from(l, u), x);
+                uint32_t most = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+                most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, DPP_XOR1, 0xF, 0xF, false));
+                most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, DPP_XOR2, 0xF, 0xF, false));
+                const int scale = kv_mx4_scale(most);
+                char* to = base + (2 * (layer + l) + kind) * plane + h * head;
+                *(uint32_t*)(to + where[1] * (c.head_dim / 2) + 4 * piece) = kv_mx4_codes(x, scale);
+                if ((piece & 3) == 0)
+                    to[c.page_size * (c.head_dim / 2 + (piece >> 2)) + where[1]] = (char)scale;
+            }
+        }
+    } else {
+        const int64_t head = (int64_t)c.page_size * c.head_dim, plane = head * c.n_kv_heads * c.n_pages;
+        KT* base = (KT*)c.kv + head * c.n_kv_heads * where[0] + (int64_t)where[1] * c.head_dim;
+        for (int l = l0; l < l1; l++) {
+            for (int u = tid; u < 2 * width; u += KV_COPY) {
+                const int kind = u >= width, e = u - kind * width, h = e / per_head;
+                if (l != l0 || u != tid) load8<XT>(from(l, u), x);
+                KT* to = base + (2 * (layer + l) + kind) * plane + h * head + 8 * (e - h * per_head);
+                __attribute__((aligned(16))) KT y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = from_f32<KT>(x[j]);   // to nearest, ties to even
+#pragma unroll
+                for (int j = 0; j < (int)sizeof(KT) / 2; j++) ((uint4*)to)[j] = ((const uint4*)y)[j];
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ read ----
+// The way back: a workgroup takes one row through a few layers, in pieces of 8 elements.
+template <typename KT, typename YT>
+__global__ __launch_bounds__(KV_COPY) void kv_read_kernel(pio_kv_cache c, int layer, int layers,
+                                                         const int32_t* __restrict__ seq,
+                                                         const int32_t* __restrict__ row_start,
+                                                         const int32_t* __restrict__ first, int n, YT* __restrict__ k,
+                                                         YT* __restrict__ v, int64_t row_stride, int64_t layer_stride,
+                                                         int per_block) {
+    __shared__ int where[3];                   // page, row in it; whether a request has the row
+    const int row = blockIdx.x, tid = threadIdx.x, lg = kv_log2(c.page_size);
+    if (tid == 0) where[0] = where[2] = -1;
+    __syncthreads();
+    for (int i = tid; i < n; i += KV_COPY) {
+        const int r0 = row_start[i], r1 = row_start[i + 1];
+        if (row < r0 || row >= r1) continue;
+        const int s = seq[i], L = kv_seq_len(c, s);
+        const int64_t pos = first ? first[i] + ((int64_t)row - r0) : L - ((int64_t)r1 - row);
+        const int page = pos >= 0 && pos < L ? c.table[(int64_t)s * c.max_pages + (pos >> lg)] : -1;
+        if (page >= 0 && page < c.n_pages) {
+            where[0] = page;
+            where[1] = (int)(pos & (c.page_size - 1));
+        } else {
+            atomicOr(kv_work(c).status, KV_BAD);
+        }
+        where[2] = i;
+    }
+    __syncthreads();
+    if (where[2] < 0) return;          // behind the last request
+    const bool there = where[0] >= 0;
+    const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8, at = there ? where[1] : 0;
+    const int64_t head = (int64_t)c.page_size * kv_token_bytes(c), plane = head * c.n_kv_heads * c.n_pages;
+    const char* base = (const char*)c.kv + head * c.n_kv_heads * (there ? where[0] : 0);
+    const int l0 = blockIdx.y * per_block, l1 = min(layers, l0 + per_block);
     for (int l = l0; l < l1; l++) {
         for (int u = tid; u < 2 * width; u += KV_COPY) {
-            const int kind = u >= width, e = u - kind * width, h = e / per_head;
-            if (l != l0 || u != tid) load8<XT>(from(l, u), x);
-            KT* to = base + (2 * (layer + l) + kind) * plane + h * head + 8 * (e - h * per_head);
-            __attribute__((aligned(16))) KT y[8];
+            const int kind = u >= width, e = u - kind * width, h = e / per_head, piece = e - h * per_head;
+            const char* from = base + (2 * (layer + l) + kind) * plane + h * head;
+            float x[8];
+            if constexpr (std::is_same_v<KT, KvMx4>)
+                kv_mx4_widen(*(const uint32_t*)(from + at * (c.head_dim / 2) + 4 * piece),
+                             (uint8_t)from[c.page_size * (c.head_dim / 2 + (piece >> 2)) + at], x);
+            else
+                load8<KT>((const KT*)from + (int64_t)at * c.head_dim + 8 * piece, x);
+            __attribute__((aligned(16))) YT y[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = from_f32<KT>(x[j]);   // to nearest, ties to even
+            for (int j = 0; j < 8; j++) y[j] = from_f32<YT>(there ? x[j] : NAN);
+            YT* to = (kind ? v : k) + l * layer_stride + row * row_stride + 8 * e;
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(KT) / 2; j++) ((uint4*)to)[j] = ((const uint4*)y)[j];
+            for (int j = 0; j < (int)sizeof(YT) / 2; j++) ((uint4*)to)[j] = ((const uint4*)y)[j];
         }
     }
 }
@@ -605,12 +686,61 @@ PIO_EXPORT int pio_kv_write(const pio_kv_cache* c, int layer, int layers, const 
                                                      row_stride, layer_stride, per_block)
     if (dtype == PIO_F32) {
         if (c->kv_dtype == PIO_F32) KV_WRITE(float, float);
-        else KV_WRITE(float, _Float16);
+        else if (c->kv_dtype == PIO_F16) KV_WRITE(float, _Float16);
+        else KV_WRITE(float, KvMx4);
     } else {
         if (c->kv_dtype == PIO_F32) KV_WRITE(_Float16, float);
-        else KV_WRITE(_Float16, _Float16);
+        else if (c->kv_dtype == PIO_F16) KV_WRITE(_Float16, _Float16);
+        else KV_WRITE(_Float16, KvMx4);
     }
 #undef KV_WRITE
+    PIO_LAUNCHED();
+    return PIO_OK;
+}
+
+PIO_EXPORT int pio_kv_read(const pio_kv_cache* c, int layer, int layers, const int32_t* seq, const int32_t* row_start,
+                           const int32_t* first, int n, void* k, void* v, int dtype, int rows, int64_t row_stride,
+                           int64_t layer_stride, void* stream) {
+    const char* nm = "pio_kv_read";
+    PIO_TRY(kv_check(c, nm));
+    PIO_REQUIRE(n >= 0 && n <= PIO_KV_MAX_REQUESTS, "%s: %d requests (0..%d)", nm, n, PIO_KV_MAX_REQUESTS);
+    PIO_REQUIRE(n == 0 || (seq && row_start), "%s: null request list", nm);
+    for (const int32_t* p : {seq, row_start, first})
+        PIO_REQUIRE(((uintptr_t)p & 3u) == 0, "%s: request list not 4-byte aligned", nm);
+    PIO_REQUIRE(layer >= 0 && layers >= 0 && layers <= c->n_layers - layer, "%s: layers %d + %d of %d", nm, layer, layers,
+                c->n_layers);
+    PIO_REQUIRE(dtype == PIO_F32 || dtype == PIO_F16, "%s: dtype %d (fp32 or fp16)", nm, dtype);
+    PIO_REQUIRE(rows >= 0 && rows < 1 << 24, "%s: %d rows (fewer than 2^24)", nm, rows);    // (2^32 threads of a grid)
+    if (n == 0 || rows == 0 || layers == 0) return PIO_OK;
+    PIO_REQUIRE(k && v && k != v, "%s: null k or v, or both the same", nm);
+    PIO_REQUIRE(aligned16(k) && aligned16(v), "%s: k or v not 16-byte aligned", nm);
+    const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
+    if (row_stride == 0) row_stride = width;
+    if (layer_stride == 0) layer_stride = (int64_t)rows * row_stride;
+    PIO_REQUIRE(row_stride % 8 == 0 && layer_stride % 8 == 0 && row_stride >= width && layer_stride >= 0,
+                "%s: strides %lld, %lld (multiples of 8, rows of %lld)", nm, (long long)row_stride,
+                (long long)layer_stride, (long long)width);
+    // one layer behind the other, or one row's layers behind the other's
+    PIO_REQUIRE(layers == 1 || (layer_stride >= width && ((layer_stride - width) / row_stride >= rows - 1 ||
+                                                          (row_stride - width) / layer_stride >= layers - 1)),
+                "%s: strides %lld, %lld: rows or layers overlap", nm, (long long)row_stride, (long long)layer_stride);
+    const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>(layers, (int64_t)rows * layers / 2048));
+    const dim3 grid(rows, ceil_div(layers, per_block));
+    PIO_REQUIRE(grid.y <= 65535, "%s: too many layers", nm);
+    hipStream_t st = pick_stream(stream);
+#define KV_READ(KT, YT)                                                                                              \
+    kv_read_kernel<KT, YT><<<grid, KV_COPY, 0, st>>>(*c, layer, layers, seq, row_start, first, n, (YT*)k, (YT*)v, \
+                                                    row_stride, layer_stride, per_block)
+    if (dtype == PIO_F32) {
+        if (c->kv_dtype == PIO_F32) KV_READ(float, float);
+        else if (c->kv_dtype == PIO_F16) KV_READ(_Float16, float);
+        else KV_READ(KvMx4, float);
+    } else {
+        if (c->kv_dtype == PIO_F32) KV_READ(float, _Float16);
+        else if (c->kv_dtype == PIO_F16) KV_READ(_Float16, _Float16);
+        else KV_READ(KvMx4, _Float16);
+    }
+#undef KV_READ
     PIO_LAUNCHED();
     return PIO_OK;
 }

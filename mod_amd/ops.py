@@ -24,6 +24,7 @@ from pathlib import Path
 from .build_ops import LIB_PATH
 
 F32, F16, I8, I32 = 0, 1, 2, 3
+MX4 = 4                  # of a KvCache only
 OK, ERR_INVALID, ERR_HIP, ERR_OOM, ERR_UNSUPPORTED = 0, -1, -2, -3, -4
 
 _DTYPE_CODES = {"float32": F32, "float16": F16, "int8": I8, "int32": I32}
@@ -163,6 +164,7 @@ SIGNATURES: dict[str, tuple] = {
     "pio_kv_status": (_i, [_cp, _vp]),
     "pio_kv_reserve": (_i, [_cp, _vp, _vp, _i, _vp]),
     "pio_kv_write": (_i, [_cp, _i, _i, _vp, _vp, _i, _vp, _vp, _i, _i, _i64, _i64, _vp]),
+    "pio_kv_read": (_i, [_cp, _i, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _i64, _i64, _vp]),
     "pio_kv_fork": (_i, [_cp, _vp, _vp, _i, _vp]),
     "pio_kv_drop": (_i, [_cp, _vp, _vp, _i, _vp]),
     "pio_kv_compact": (_i, [_cp, _vp]),
@@ -352,7 +354,9 @@ def _list(x, name: str, code: int = I32) -> int | None:
 
 class KvCache:
     """A paged key / value cache over memory that the caller owns: kv
-    [layers, 2, pages, kv heads, page size, head dim] fp32 | fp16, table [sequences,
+    [layers, 2, pages, kv heads, page size, head dim] fp32 | fp16, or uint8 with a last
+    dimension of 17 * head dim / 32 for a cache of 4 bits (include/tensor_rocm.h: what
+    its bytes are; kv_write and kv_read go between it and numbers), table [sequences,
     pages of a sequence], lens [sequences] and refs [pages] int32, all dense on
     one device (torch or backend tensors; kept alive by this object). The plans'
     workspace is allocated here, and the tables are taken as they are: kv_init
@@ -377,9 +381,14 @@ class KvCache:
         device = str(kv.device)
         if device.split(":")[0] not in ("cuda", "rocm"):
             raise ValueError(f"KvCache: the cache is on {device}, not on a GPU")
+        dtype = MX4 if str(kv.dtype).replace("torch.", "") == "uint8" else _dt(kv)
+        if dtype == MX4:
+            if dim % 17:
+                raise ValueError(f"KvCache: 4 bits with a last dimension of {dim}, not 17 * head dim / 32")
+            dim = dim // 17 * 32
         self.tensors = (kv, table, lens, refs)
-        self.c = CKvCache(_ptr(kv), _ptr(table), _ptr(lens), _ptr(refs), None, _dt(kv), L, heads, dim, page, pages,
-                          seqs, width)
+        self.c = CKvCache(_ptr(kv), _ptr(table), _ptr(lens), _ptr(refs), None, dtype, L, heads, dim, page, pages, seqs,
+                          width)
         self.device = int(device.split(":")[1]) if ":" in device else 0
         self.ref = ctypes.byref(self.c)
         check(lib.pio_kv_work_create(self.ref, self.device), "KvCache")
@@ -420,6 +429,16 @@ def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k,
         raise TypeError("kv_write: k and v differ in dtype")
     check(lib.pio_kv_write(cache.ref, layer, layers, _list(seq, "seq"), _list(row_start, "row_start"), n, _ptr(k), _ptr(v),
                            dt, rows, row_stride, layer_stride, _stream(stream)), "pio_kv_write")
+
+
+def kv_read(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, first=None,
+            row_stride: int = 0, layer_stride: int = 0, stream=None) -> None:
+    """Each sequence's tokens from first[i] on (None: its last ones) into k and v, as kv_write takes them."""
+    dt = _dt(k)
+    if _dt(v) != dt:
+        raise TypeError("kv_read: k and v differ in dtype")
+    check(lib.pio_kv_read(cache.ref, layer, layers, _list(seq, "seq"), _list(row_start, "row_start"), _list(first, "first"),
+                          n, _ptr(k), _ptr(v), dt, rows, row_stride, layer_stride, _stream(stream)), "pio_kv_read")
 
 
 def kv_fork(cache: KvCache, src, dst, n: int, stream=None) -> None:

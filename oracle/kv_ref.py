@@ -2,8 +2,8 @@
 drafted tokens -- TEST INFRASTRUCTURE ONLY.
 
 Plain Python and numpy, request by request and token by token, from the
-definitions in include/tensor_rocm.h; attention and the verification's sums in
-float64. No counterpart in the reference (its paged attention kernel is never
+definitions in include/tensor_rocm.h (caches of fp32, fp16 and 4 bits); attention
+and the verification's sums in float64. No counterpart in the reference (its paged attention kernel is never
 launched, tensor_ops_cuda.cu:582-618): parity unpinned, checked against closed
 forms in tests/test_oracle_kv.py."""
 from __future__ import annotations
@@ -24,6 +24,9 @@ class Cache:
         self.lens = np.zeros(seqs, np.int32)
         self.refs = np.zeros(pages, np.int32)
         self.P = page
+
+    def _copy(self, kv, old, new, rows):
+        kv[:, :, new, :, :rows] = kv[:, :, old, :, :rows]
 
     def _count(self, n):
         return -(-int(n) // self.P)
@@ -55,7 +58,7 @@ class Cache:
                 refs[table[s, j]] = 1
             lens[s] = L + k
         for old, new, rows in copies:
-            kv[:, :, new, :, :rows] = kv[:, :, old, :, :rows]
+            self._copy(kv, old, new, rows)
         self.table, self.lens, self.refs = table, lens, refs
 
     def write(self, layer, seq, row_start, k, v):
@@ -136,6 +139,82 @@ class Cache:
                     p = np.exp(sc - sc.max(1, keepdims=True))
                     out[r] = np.einsum("ht,thd->hd", p / p.sum(1, keepdims=True), v)
         return out
+
+
+MX4_VALUES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+
+
+def mx4_encode(x):
+    """Codes [.., D] 0 .. 15 and scale bytes [.., D / 32] of x [.., D], by trying every power of two and every value."""
+    x = np.asarray(x, np.float64)
+    x = x.reshape(*x.shape[:-1], -1, 32)
+    most = np.abs(x).max(-1)
+    fine = np.isfinite(x).all(-1)
+    most, x = np.where(fine, most, 0.0), np.where(fine[..., None], x, 0.0)
+    e = np.full(most.shape, 13)
+    for power in range(12, -24, -1):
+        e = np.where(most < 7 * 2.0 ** power, power, e)
+    y = np.minimum(np.abs(x) / 2.0 ** e[..., None], 7.0)
+    code, best = np.zeros(x.shape, np.uint8), np.full(x.shape, np.inf)
+    for c in (0, 2, 4, 6, 1, 3, 5, 7):              # ties to the even code: it comes first
+        off = np.abs(y - MX4_VALUES[c])
+        code, best = np.where(off < best, c, code), np.minimum(off, best)
+    code = np.where(np.signbit(x) & (x != 0), code + 8, code).astype(np.uint8)
+    return code.reshape(*x.shape[:-2], -1), np.where(fine, e + 127, 255).astype(np.uint8)
+
+
+def mx4_decode(code, scale):
+    """Values [.., D] of codes [.., D] and scale bytes [.., D / 32]."""
+    v = np.where(code & 8, -1.0, 1.0) * MX4_VALUES[code & 7]
+    unit = np.where(scale == 255, np.nan, 2.0 ** (scale.astype(np.float64) - 127))
+    return v * np.repeat(unit, 32, -1)
+
+
+class Cache4(Cache):
+    """A cache of 4 bits: kv uint8 [layers, 2, pages, heads, page, 17 dim / 32], of each (page, head) the packed
+    codes [page, dim / 2], then the scales [dim / 32, page]."""
+
+    def __init__(self, layers, heads, dim, page, pages, seqs, width):
+        super().__init__(layers, heads, dim // 32 * 17, page, pages, seqs, width, np.uint8)
+        self.D = dim
+
+    def blocks(self):
+        """Codes [.., page, D / 2] and scales [.., D / 32, page], views of kv."""
+        flat = self.kv.reshape(*self.kv.shape[:4], -1)
+        n = self.P * self.D // 2
+        return (flat[..., :n].reshape(*flat.shape[:4], self.P, self.D // 2),
+                flat[..., n:].reshape(*flat.shape[:4], self.D // 32, self.P))
+
+    def _copy(self, kv, old, new, rows):
+        kv[:, :, new] = kv[:, :, old]               # the whole page
+
+    def put(self, layer, kind, page, at, x):
+        """Token `at` of a page of one layer's k or v: x [heads, D]."""
+        codes, scales = self.blocks()
+        code, scale = mx4_encode(x)
+        codes[layer, kind, page, :, at] = code[:, 0::2] | code[:, 1::2] << 4
+        scales[layer, kind, page, :, :, at] = scale
+
+    def write(self, layer, seq, row_start, k, v):
+        for i, s in enumerate(seq):
+            n = row_start[i + 1] - row_start[i]
+            for r in range(row_start[i], row_start[i + 1]):
+                pos = int(self.lens[s]) - n + r - row_start[i]
+                for l in range(k.shape[0]):
+                    for kind, x in enumerate((k, v)):
+                        self.put(layer + l, kind, self.table[s, pos // self.P], pos % self.P, x[l, r])
+
+    def values(self):
+        """All that the cache holds, [layers, 2, pages, heads, page, D]."""
+        codes, scales = self.blocks()
+        code = np.stack([codes & 15, codes >> 4], -1).reshape(*codes.shape[:-1], self.D)
+        return mx4_decode(code, np.swapaxes(scales, -1, -2))
+
+    def rows(self, layer, s, upto):
+        t = np.arange(upto)
+        page = self.table[s, t // self.P]
+        v = self.values() if upto else np.zeros((layer + 1, 2, 1, self.kv.shape[3], self.P, self.D))
+        return v[layer, 0, page, :, t % self.P], v[layer, 1, page, :, t % self.P]
 
 
 def verify(target, draft, ids, u, u_next, row_start):
