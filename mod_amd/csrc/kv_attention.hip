@@ -129,11 +129,6 @@ typedef __fp16 ka_p4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) void ka_lds_t;
 typedef __attribute__((address_space(3))) ka_p4 ka_lds_p4;
 
-// A column's reference (the exponent that its weights are relative to) follows its
-// maximum only when that has grown by KA_SLACK: rescaling O^T for every new maximum of 32
-// columns cost as much as a tile's exponentials. fp16 weights are held times 2^10, so that they
-// stay below 2^15, and are normal numbers down to 2^-24 of the reference.
-constexpr float KA_LIFT = 10.f, KA_SLACK = 5.f;
 constexpr int KA_Q_EXP = 12;     // fp32 queries over an fp16 cache: the column's largest is 2^12 .. 2^13
 
 // A tile of keys x COLS columns (16 or 32) on v_mfma_*_COLSxCOLS: lane l holds
@@ -1090,6 +1085,10 @@ static int ka_held(const KaArgs& a, bool wide, int& held) {
     return a.q16 ? ka_held_by<_Float16, D, 1, 0>(held) : ka_held_by<_Float16, D, 2, 0>(held);
 }
 
+// An item costs its rounds of keys and this many more (its requests, pages, first copies; its
+// join and output): 12,000 clocks beside 3,400 of a round.
+constexpr float KA_FIXED = 3.5f;
+
 // Items for the matrix core kernels.
 static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
@@ -1138,7 +1137,7 @@ static int ka_matrix(KaArgs& a, int max_rows, hipStream_t st) {
         const int64_t splits = std::max<int64_t>({1, most / 4, wide == 1 ? most : std::min(rounds / 8, most)});
         a.pre_keys = (int)ceil_div(rounds, std::min(splits, rounds)) * KA_ROUND;
         a.pre_splits = ceil_div(a.shared, a.pre_keys);
-        if (wide != 1) a.pre_work = (float)pre_units * (a.pre_splits * KA_FIXED + rounds);
+        if (wide != 1) a.pre_work = (float)pre_units * (a.pre_splits * a.fixed + rounds);
         const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
         PIO_REQUIRE(pre <= 1 << 22, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)pre;
@@ -1190,6 +1189,7 @@ PIO_EXPORT int pio_kv_attention(const pio_kv_cache* c, int layer, const int32_t*
     PIO_REQUIRE((int64_t)rows * n_heads < (matrix ? 1 << 26 : 1 << 24), "%s: too many rows", nm);
     PIO_REQUIRE(std::isfinite(scale), "%s: scale %g", nm, (double)scale);
     KaArgs a{};
+    a.fixed = KA_FIXED;
     a.c = *c;
     a.seq = seq;
     a.row_start = row_start;

@@ -25,6 +25,7 @@ struct KaArgs {
     // items of the matrix core kernels
     int pre_items, pre_tiles, pre_splits, pre_keys;   // workgroups; column tiles; runs of keys, keys of each
     int tail_tiles, tail_runs, max_runs;              // column tiles; the most runs beside one for each request, and of one
+    float fixed;                                      // rounds of keys that an item costs besides its own
     int slots;                                        // items that the device holds at once
     float pre_work;                                   // rounds of keys that the prefix's items cost
     int tail_items;                                   // workgroups: (run, column tile, kv head), as many as there may be
@@ -59,6 +60,11 @@ typedef float ka_f2 __attribute__((ext_vector_type(2)));
 typedef _Float16 ka_h8 __attribute__((ext_vector_type(8)));
 
 constexpr float KA_LOG2E = 1.44269504088896340736f;
+// A column's reference (the exponent that its weights are relative to) follows its
+// maximum only when that has grown by KA_SLACK: rescaling O^T for every new maximum of 32
+// columns cost as much as a tile's exponentials. fp16 weights are held times 2^10, so that they
+// stay below 2^15, and are normal numbers down to 2^-24 of the reference.
+constexpr float KA_LIFT = 10.f, KA_SLACK = 5.f;
 // Least maximum of a column that sees a key; one that sees none keeps -FLT_MAX.
 constexpr float KA_SEEN = -3.4e38f;
 
@@ -113,15 +119,12 @@ __device__ __forceinline__ void ka_emit(const KaArgs& a, int D, const KaItem& it
 }
 
 constexpr int KA_ROUND = 128;          // keys that runs are multiples of
-// An item costs its rounds of keys and this many more (its requests, pages, first copies; its
-// join and output): 12,000 clocks beside 3,400 of a round.
-constexpr float KA_FIXED = 3.5f;
 // Rounds of keys for each of the runs that `rounds` are cut into, if every run is an item in
-// each of `units` places and all else costs `work`: the longest item, KA_FIXED + r, takes as
+// each of `units` places and all else costs `work`: the longest item, fixed + r, takes as
 // long as the device's share of all work.
-__device__ __forceinline__ float ka_cut(float rounds, float units, float work, float slots) {
-    const float d = (work + units * rounds) / slots - KA_FIXED;
-    return 0.5f * (d + sqrtf(d * d + 4.f * KA_FIXED * units / slots * rounds));
+__device__ __forceinline__ float ka_cut(float rounds, float units, float work, float slots, float fixed) {
+    const float d = (work + units * rounds) / slots - fixed;
+    return 0.5f * (d + sqrtf(d * d + 4.f * fixed * units / slots * rounds));
 }
 
 // Sum over the workgroup's threads before this one, and over all.
@@ -175,10 +178,10 @@ __device__ __forceinline__ void ka_runs(const KaArgs& a, int unit, KaRun& found,
         total += min(sum, INT_MAX - total);
     }
     const float units = a.c.n_kv_heads * a.tail_tiles;
-    // runs that balance the items, or of KA_FIXED rounds: the last items to start should be short ones
+    // runs that balance the items, or of as many rounds as an item costs besides: the last items to start should be short ones
     // (and at most tail_runs more runs than requests)
     const float cut = fmaxf(fmaxf(1.f, (float)total / a.tail_runs),
-                            fminf(KA_FIXED, ka_cut(total, units, a.pre_work + a.n * units * KA_FIXED, a.slots)));
+                            fminf(a.fixed, ka_cut(total, units, a.pre_work + a.n * units * a.fixed, a.slots, a.fixed)));
     int before = 0;
     for (int i0 = 0; i0 < a.n; i0 += threads) {
         if (a.n > threads) n = rounds(i0 + tid);

@@ -2,7 +2,9 @@
 //   out[r, h] = sum_t softmax_t(q[r, h] . k[t] * scale) v[t].
 #include "kv_attention.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace pio {
 
@@ -108,7 +110,487 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
     if (bad && tid == 0) atomicOr(c.work, KV_BAD);
 }
 
+// ------------------------------------------------- the matrix core kernels ----
+// Items (kv_attention.hpp) of 16 * NC columns by 4 waves; each wave takes every 4th tile of 32 keys on its own,
+// K and V straight from memory into registers, the next tile under the way of this one's products. No LDS until
+// the waves' sums meet.
+//   S^T = K Q^T on v_mfma_scale_f32_16x16x128: 16 keys are one operand as they lie in memory, lane l the 16
+//     bytes of key row l % 16 and dimensions 32 (l / 16) .. + 31, whose scale byte is the operand's own. Queries
+//     are parts of 6 bits (e2m3), each of a scale of its own: a part holds 32 dimensions to within a 30th of the
+//     largest, and the next part the rest. 6-bit operands run at the rate of 4-bit ones, twice that of 8 bits.
+//     64 dimensions are half of an operand's depth: its halves are two parts of the query, the keys in both.
+//   O^T = V^T P^T on v_mfma_f32_16x16x32_f16. Lane l reads the codes of 8 keys and dimensions D / 16 (l % 16) ..,
+//     and widens each key's to fp16 under its scale, exactly: two keys' halves side by side are the operand, so
+//     V is turned inside a lane. Row i of O^T tile n is dimension (D / 16) i + n.
+//   Row 4 q + e of the t-th 16 keys is key 8 q + 4 t + e, so that a lane's 8 scores are the 8 keys of its part
+//     q = l / 16 of the weights' operand, neighbours on one page, whose scales are 8 bytes in a row.
+typedef int ka4_i8 __attribute__((ext_vector_type(8)));
+typedef uint32_t ka4_u6 __attribute__((ext_vector_type(6)));
+typedef float ka4_v32 __attribute__((ext_vector_type(32)));
+typedef _Float16 ka4_h2 __attribute__((ext_vector_type(2)));
+
+constexpr int KA4_TILE = 32, KA4_WAVES = 4;
+
+// X16: fp16 queries, 3 parts and weights in fp16; else 5 parts, and weights as two fp16 parts.
+template <int D, bool X16>
+struct Ka4 {
+    static constexpr int PARTS = X16 ? 3 : 5, XP = X16 ? 1 : 2;
+    static constexpr int QM = D == 128 ? PARTS : (PARTS + 1) / 2;      // products of a score
+    static constexpr int NT = D / 16, RB = D / 2;                      // O^T tiles; bytes of a row's codes
+    static constexpr int OP = D + 4;                                   // LDS pitch of a column's output (floats)
+};
+
+// The conversions between 32 floats (the even ones in a, the odd ones in b) and 6-bit codes write
+// their result while they still read: the builtins do not say so, and the registers may overlap.
+__device__ __forceinline__ ka4_u6 ka4_to6(const ka_v16& a, const ka_v16& b, float scale) {
+    ka4_u6 r;
+    asm("v_cvt_scalef32_2xpk16_fp6_f32 %0, %1, %2, %3\n s_nop 1" : "=&v"(r) : "v"(a), "v"(b), "v"(scale));
+    return r;
+}
+__device__ __forceinline__ ka4_v32 ka4_from6(const ka4_u6& c, float scale) {
+    ka4_v32 r;
+    asm("v_cvt_scalef32_pk32_f32_fp6 %0, %1, %2\n s_nop 1" : "=&v"(r) : "v"(c), "v"(scale));
+    return r;
+}
+
+// A column's query times scale * log2(e), so that a score is the exponent of its weight as it comes: lane l has
+// 32 dimensions of column l % 16.
+template <int D, bool X16>
+struct Ka4Q {
+    ka4_u6 p[Ka4<D, X16>::QM];
+    int e[Ka4<D, X16>::QM];
+};
+template <int D, bool X16>
+__device__ __forceinline__ void ka4_load_q(const KaArgs& a, int row, int head, bool live, int part, Ka4Q<D, X16>& q) {
+    using T = Ka4<D, X16>;
+    const int64_t at = (live ? row * a.q_stride + (int64_t)head * D : 0) + 32 * (D == 128 ? part : part & 1);
+    const int half = D == 128 ? 0 : part >> 1;         // 64 dimensions: which parts this half of the operand has
+    const float scale = a.scale * KA_LOG2E;
+    ka_v16 xa, xb;
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float x[8];
+        if constexpr (X16) load8<_Float16>((const _Float16*)a.q + at + 8 * i, x);
+        else load8<float>((const float*)a.q + at + 8 * i, x);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            x[j] *= scale;
+            most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
+            (j & 1 ? xb : xa)[4 * i + j / 2] = x[j];
+        }
+    }
+    const bool odd = most >= 0x7f800000u;              // inf or NaN: a NaN scale makes the column's scores NaN
+    if (!live || odd) {
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) xa[i] = xb[i] = 0.f;
+    }
+    // the least power of two (a byte of exponent) that the largest is below 7.5 of, with what rounds up to 8; a
+    // part's rest is at most a quarter of its step's unit, or an eighth from the second part on: 4 and 5 bits
+    const int first = (int)((most + 0x100000u) >> 23) - 2;
+#pragma unroll
+    for (int p = 0; p < T::PARTS; p++) {
+        int e = max(first - (p ? 5 * p - 1 : 0), 1);
+        const float unit = __uint_as_float((uint32_t)e << 23);
+        const ka4_u6 c = ka4_to6(xa, xb, unit);
+        if (live && odd) e = KV_MX4_NAN;
+        if constexpr (D == 128) {
+            q.p[p] = c;
+            q.e[p] = e;
+        } else if (p % 2 == 0) {
+            q.p[p / 2] = c;
+            q.e[p / 2] = e;
+            if (half && p == T::PARTS - 1) q.p[p / 2] = ka4_u6{0, 0, 0, 0, 0, 0};
+        } else if (half) {
+            q.p[p / 2] = c;
+            q.e[p / 2] = e;
+        }
+        if (p + 1 < T::PARTS) {
+            const ka4_v32 y = ka4_from6(c, unit);
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                xa[i] -= y[2 * i];
+                xb[i] -= y[2 * i + 1];
+            }
+        }
+    }
+}
+
+// A column's running softmax: (reference, sum) in base 2, O^T.
+template <int D>
+struct Ka4Acc {
+    float m, l;
+    ka_f4 o[D / 16];
+    __device__ void clear() {
+        m = -FLT_MAX;
+        l = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 16; n++) o[n] = ka_f4{0.f, 0.f, 0.f, 0.f};
+    }
+};
+
+// A lane's share of 32 keys and values.
+template <int D>
+struct Ka4Keys {
+    uint4 k[2];
+    int ks[2];
+    uint32_t v[8];
+    uint2 vs;
+};
+
+template <int D, bool X16, int NC>
+struct Ka4Walk {
+    using T = Ka4<D, X16>;
+    const char *kb, *vb;
+    uint32_t page_b;
+    int first, tiles, lo, hi, lg, mask, codes;     // keys from `first`; first and last group of 8 keys; bytes of codes
+    int kg, vg, kid, vid;                          // this lane's groups of 8 keys of the next tile, their pages
+    int bad_at = INT_MAX;                          // first key of this lane in a page outside the cache
+    bool odd = false;
+    Ka4Keys<D> next;
+
+    // (groups outside the item's keys: the nearest inside)
+    __device__ void look_up(const KaItem& it, int j, int lane) {
+        const int t0 = first + min(j, tiles - 1) * KA4_TILE;
+        kg = min(max(t0 + 8 * ((lane & 15) >> 2), lo), hi);
+        vg = min(max(t0 + 8 * (lane >> 4), lo), hi);
+        kid = it.table[kg >> lg];
+        vid = it.table[vg >> lg];
+    }
+    __device__ void load(const KaArgs& a, const KaItem& it, int lane) {
+        const bool ok = (unsigned)kid < (unsigned)a.c.n_pages;
+        bad_at = ok ? bad_at : min(bad_at, max(kg, it.k0));
+        const char* k = kb + (uint64_t)(ok ? (uint32_t)kid : 0u) * page_b;
+        const char* v = vb + (uint64_t)((unsigned)vid < (unsigned)a.c.n_pages ? (uint32_t)vid : 0u) * page_b;
+        const int kt = (kg & mask) + (lane & 3), vt = vg & mask, part = lane >> 4, i = lane & 15;
+        const int kblock = D == 128 ? part : part & 1;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            next.k[t] = *(const uint4*)(k + (kt + 4 * t) * T::RB + 16 * kblock);
+            next.ks[t] = *(const uint8_t*)(k + codes + (kblock << lg) + kt + 4 * t);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if constexpr (D == 128) next.v[j] = *(const uint32_t*)(v + (vt + j) * T::RB + 4 * i);
+            else next.v[j] = *(const uint16_t*)(v + (vt + j) * T::RB + 2 * i);
+        }
+        next.vs = *(const uint2*)(v + codes + (((D / 16 * i) >> 5) << lg) + vt);
+    }
+    // The first tile's loads, if the wave has one.
+    __device__ void begin(const KaArgs& a, const KaItem& it, int w, int lane) {
+        const pio_kv_cache& c = a.c;
+        lg = kv_log2(c.page_size);
+        mask = c.page_size - 1;
+        codes = c.page_size * T::RB;
+        const int64_t head = (int64_t)c.page_size * (D / 32 * 17);
+        page_b = (uint32_t)(head * c.n_kv_heads);
+        kb = (const char*)c.kv + (int64_t)2 * a.layer * c.n_pages * page_b + it.g * head;
+        vb = kb + (int64_t)c.n_pages * page_b;
+        first = it.k0 & -KA4_TILE;
+        lo = it.k0 & -8;
+        hi = (it.k1 - 1) & -8;
+        tiles = it.k1 > it.k0 ? (it.k1 - first + KA4_TILE - 1) / KA4_TILE : 0;
+        if (w >= tiles) return;
+        look_up(it, w, lane);
+        load(a, it, lane);
+        look_up(it, w + KA4_WAVES, lane);
+    }
+    __device__ void run(const KaArgs& a, const KaItem& it, int w, int lane, const Ka4Q<D, X16> (&q)[NC],
+                        const int (&limit)[NC], Ka4Acc<D> (&x)[NC]) {
+        const int part = lane >> 4;
+        int least = limit[0];
+#pragma unroll
+        for (int c = 1; c < NC; c++) least = min(least, limit[c]);
+        least = ka_wave_min(least);
+        for (int j = w; j < tiles; j += KA4_WAVES) {
+            const int t0 = first + j * KA4_TILE, key0 = t0 + 8 * part;
+            const bool edge = t0 < it.k0 || t0 + KA4_TILE > least;
+            Ka4Keys<D> now = next;
+            if (j + KA4_WAVES < tiles) {
+                load(a, it, lane);
+                look_up(it, j + 2 * KA4_WAVES, lane);
+            }
+            if (edge) {
+                // A value that some column does not see must not reach it, 0 * NaN: NaN blocks are left out (ka4_mend
+                // adds them to the columns that see them), and whatever lies outside the item's keys
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    uint32_t& word = i < 4 ? now.vs.x : now.vs.y;
+                    const uint32_t byte = word >> 8 * (i & 3) & 255u;
+                    const bool in = key0 + i >= it.k0 && key0 + i < it.k1, wrong = byte > KV_MX4_MOST;
+                    odd |= in && wrong;
+                    if (!in || wrong) word &= ~(255u << 8 * (i & 3));
+                }
+            }
+            ka_h8 wt[NC][T::XP];
+#pragma unroll
+            for (int c = 0; c < NC; c++) {
+                float s[8];
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    const ka4_i8 k = {(int)now.k[t].x, (int)now.k[t].y, (int)now.k[t].z, (int)now.k[t].w, 0, 0, 0, 0};
+                    ka_f4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int m = T::QM - 1; m >= 0; m--) {         // the small parts first
+                        const ka4_u6& p = q[c].p[m];
+                        const ka4_i8 qm = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
+                        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qm, acc, 4, 2, 0, now.ks[t], 0, q[c].e[m]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e];
+                }
+                if (edge) {
+                    const int end = limit[c] - key0, begin = it.k0 - key0;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) s[i] = i < end && i >= begin ? s[i] : -INFINITY;
+                }
+                float top = s[0];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
+                top = ka_max<16>(fmaxf(top, max(t0, it.k0) < limit[c] ? KA_SEEN : -FLT_MAX));
+                if (__any(top > x[c].m + KA_SLACK)) {
+                    const float m = fmaxf(x[c].m, top), corr = __builtin_amdgcn_exp2f(x[c].m - m);
+                    x[c].l *= corr;
+#pragma unroll
+                    for (int n = 0; n < T::NT; n++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[c].o[n][e] *= corr;
+                    x[c].m = m;
+                }
+                const float base = x[c].m - KA_LIFT;       // (behind a score beyond 2^24 the weights stay below 2^15)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    s[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                    const _Float16 hi = (_Float16)s[i];
+                    wt[c][0][i] = hi;
+                    if constexpr (T::XP == 2) wt[c][T::XP - 1][i] = (_Float16)(s[i] - (float)hi);
+                }
+                x[c].l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+            }
+            float vs[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) vs[i] = __uint_as_float(((i < 4 ? now.vs.x : now.vs.y) >> 8 * (i & 3) & 255u) << 23);
+            auto pair = [&](auto byte) {
+                constexpr int B = decltype(byte)::value;
+                ka_h8 v0, v1;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const ka4_h2 y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(now.v[i], vs[i], B);
+                    v0[i] = y[0];
+                    v1[i] = y[1];
+                }
+#pragma unroll
+                for (int c = 0; c < NC; c++)
+#pragma unroll
+                    for (int k = 0; k < T::XP; k++) {
+                        x[c].o[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wt[c][k], x[c].o[2 * B], 0, 0, 0);
+                        x[c].o[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wt[c][k], x[c].o[2 * B + 1], 0, 0, 0);
+                    }
+            };
+            pair(std::integral_constant<int, 0>{});
+            pair(std::integral_constant<int, 1>{});
+            if constexpr (D == 128) {
+                pair(std::integral_constant<int, 2>{});
+                pair(std::integral_constant<int, 3>{});
+            }
+        }
+    }
+};
+
+// NaN value blocks that the walk left out, added to 4 dimensions from d of a column that sees the keys up to `limit`.
+template <int D>
+__device__ __forceinline__ void ka4_mend(const KaArgs& a, const KaItem& it, int limit, int d, ka_f4& v) {
+    const pio_kv_cache& c = a.c;
+    const int lg = kv_log2(c.page_size);
+    const int64_t head = (int64_t)c.page_size * (D / 32 * 17), page_b = head * c.n_kv_heads;
+    const uint8_t* vb = (const uint8_t*)c.kv + (int64_t)(2 * a.layer + 1) * c.n_pages * page_b + it.g * head +
+                        c.page_size * (D / 2 + d / 32);
+    for (int t = it.k0; t < min(limit, it.k1); t++) {
+        const int page = it.table[t >> lg];
+        if (page < 0 || page >= c.n_pages) continue;
+        if (vb[page * page_b + (t & (c.page_size - 1))] > KV_MX4_MOST) v = ka_f4{NAN, NAN, NAN, NAN};
+    }
+}
+
+// An item's columns from c0 joined over its waves and written, 16 at a time.
+template <int D, bool X16, int NC>
+__device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, float* lds, float (*ml)[16][2], int* limits,
+                                         int c0, int w, int lane) {
+    using T = Ka4<D, X16>;
+    Ka4Walk<D, X16, NC> walk;
+    walk.begin(a, it, w, lane);
+    const int first = ka_div(a, c0);
+    if (limits) ka_limits(a, first, limits, 16 * NC);      // under the first loads' way
+    Ka4Q<D, X16> q[NC];
+    Ka4Acc<D> x[NC];
+    int limit[NC], sees[NC];                               // in this item; at all (-1: no such column or row)
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int col = c0 + 16 * c + (lane & 15);
+        const bool has = col < it.ncols;
+        const int r = has ? ka_div(a, col) : 0, head = it.g * a.G + (has ? col - r * a.G : 0);
+        limit[c] = has ? ka_limit(it, limits, first, r) : it.k1;
+        sees[c] = !has ? -1 : limits ? limits[r - first] : it.first_limit + r;
+        x[c].clear();
+        if (w < walk.tiles) ka4_load_q<D, X16>(a, it.row0 + r, head, has, lane >> 4, q[c]);
+    }
+    walk.run(a, it, w, lane, q, limit, x);
+    // a page outside the cache: NaN for the columns that see its keys
+    int bad_at = INT_MAX;
+    if (__any(walk.bad_at != INT_MAX)) bad_at = ka_wave_min(walk.bad_at);
+    bool told = it.bad;
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        told |= sees[c] > bad_at;
+        x[c].l += __shfl_xor(x[c].l, 32, 64);
+        x[c].l += __shfl_xor(x[c].l, 16, 64);
+        if (it.bad || limit[c] > bad_at) x[c].l = NAN;
+    }
+    if (told) atomicOr(a.c.work, KV_BAD);
+    const bool odd = __syncthreads_or(walk.odd);
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        if (c && c0 + 16 * c >= it.ncols) break;
+        if (c) __syncthreads();                            // the last columns are out of LDS
+        const int col = lane & 15, part = lane >> 4;
+        if (part == 0) {
+            ml[w][col][0] = x[c].m;
+            ml[w][col][1] = x[c].l;
+        }
+        __syncthreads();
+        float mx = ml[0][col][0];
+#pragma unroll
+        for (int i = 1; i < KA4_WAVES; i++) mx = fmaxf(mx, ml[i][col][0]);
+        const float f = __builtin_amdgcn_exp2f(x[c].m - mx);
+        float* to = lds + (w * 16 + col) * T::OP;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int n = 0; n < T::NT; n += 4) {
+                ka_f4 v;
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[k] = x[c].o[n + k][e] * f;
+                *(ka_f4*)(to + T::NT * (4 * part + e) + n) = v;
+            }
+        __syncthreads();
+        for (int i = w * 64 + lane; i < min(16, it.ncols - c0 - 16 * c) * (D / 4); i += 64 * KA4_WAVES) {
+            const int cc = i / (D / 4), d = (i % (D / 4)) * 4, at = c0 + 16 * c + cc;
+            float m = ml[0][cc][0], l = 0.f;
+#pragma unroll
+            for (int k = 1; k < KA4_WAVES; k++) m = fmaxf(m, ml[k][cc][0]);
+            ka_f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KA4_WAVES; k++) {
+                v += *(const ka_f4*)(lds + (k * 16 + cc) * T::OP + d);
+                l += ml[k][cc][1] * __builtin_amdgcn_exp2f(ml[k][cc][0] - m);
+            }
+            if (odd) ka4_mend<D>(a, it, ka_limit(it, limits, first, ka_div(a, at)), d, v);
+            ka_emit(a, D, it, at, d, v, m, l);
+        }
+    }
+}
+
+// The prefix's items, then the tails'.
+template <int D, bool X16, int NC>
+__global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void ka4_kernel(KaArgs a) {
+    __shared__ __attribute__((aligned(16))) float lds[KA4_WAVES * 16 * Ka4<D, X16>::OP];
+    __shared__ float ml[KA4_WAVES][16][2];
+    __shared__ int limits[16 * NC];
+    __shared__ KaRun found;
+    __shared__ int red[KA4_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    constexpr int COLS = 16 * NC;
+    KaItem it;
+    int ct;
+    if ((int)blockIdx.x < a.pre_items) {
+        if (ka_prefix(a, it, ct)) ka4_item<D, X16, NC>(a, it, lds, ml, limits, ct * COLS, w, lane);
+        return;
+    }
+    const int item = (int)blockIdx.x - a.pre_items, unit = item / a.c.n_kv_heads, g = item - unit * a.c.n_kv_heads;
+    ka_runs(a, unit, found, red, COLS);
+    const KaRun r = found;
+    if (!ka_tail(a, it, r, g)) return;
+    if (!a.direct && g == 0 && r.ct == 0 && r.z == 0)
+        for (int i = tid; i < r.r1 - r.r0; i += 64 * KA4_WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
+    // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
+    for (int c0 = r.ct * COLS; c0 < it.ncols; c0 += r.tiles * COLS) {
+        ka4_item<D, X16, NC>(a, it, lds, ml, nullptr, c0, w, lane);
+        __syncthreads();                                   // its output is out of LDS
+    }
+}
+
+template <int D, bool X16, int NC>
+static int ka4_launch(const KaArgs& a, hipStream_t st) {
+    ka4_kernel<D, X16, NC><<<a.pre_items + a.tail_items, 256, 0, st>>>(a);
+    PIO_LAUNCHED();
+    return PIO_OK;
+}
+template <int D>
+static int ka4_route(const KaArgs& a, int nc, hipStream_t st) {
+    if (a.q16) return nc == 1 ? ka4_launch<D, true, 1>(a, st) : ka4_launch<D, true, 2>(a, st);
+    return nc == 1 ? ka4_launch<D, false, 1>(a, st) : ka4_launch<D, false, 2>(a, st);
+}
+template <int D>
+static int ka4_join(const KaArgs& a, hipStream_t st) {
+    constexpr int GRP = 1024 / D;
+    const int cols = a.rows * a.H;
+    if (cols <= 2048) ka_merge_kernel<D, 8><<<ceil_div(cols, GRP / 8), 256, 0, st>>>(a);
+    else ka_merge_kernel<D, 1><<<ceil_div(cols, GRP), 256, 0, st>>>(a);
+    PIO_LAUNCHED();
+    return PIO_OK;
+}
+
+// An item costs its rounds of keys and this many more.
+constexpr float KA4_FIXED = 8.f;
+
+// Items for the matrix core kernels.
+static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
+    const int Hk = a.c.n_kv_heads, cus = 256;
+    const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
+    a.fixed = KA4_FIXED;
+    const int nc = tail_cols > 16 ? 2 : 1, width = 16 * nc, held = nc == 1 ? 3 : 2;
+    a.tail_tiles = ceil_div(tail_cols, width);
+    PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);
+    const int64_t items = std::min((int64_t)a.n * a.tail_tiles, cols / width + a.n) * Hk;
+    a.slots = cus * held;
+    const int64_t units = (int64_t)Hk * a.tail_tiles;
+    a.tail_runs = (int)std::max<int64_t>(1, a.slots / units);
+    const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
+    const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
+    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 64, ceil_div(longest, KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
+    a.direct = a.shared == 0 && a.max_runs == 1;
+    a.tail_items = (int)(items + (a.max_runs == 1 ? 0 : (int64_t)a.tail_runs * units));
+    if (a.shared > 0) {
+        a.pre_tiles = ceil_div(cols, width);
+        const int64_t pre_units = (int64_t)Hk * a.pre_tiles, rounds = ceil_div(a.shared, KA_ROUND);
+        const int64_t most = a.slots / pre_units;
+        const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most)});
+        a.pre_keys = (int)ceil_div(rounds, std::min(splits, rounds)) * KA_ROUND;
+        a.pre_splits = ceil_div(a.shared, a.pre_keys);
+        a.pre_work = (float)pre_units * (a.pre_splits * a.fixed + rounds);
+        const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
+        PIO_REQUIRE(pre <= 1 << 22, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
+        a.pre_items = (int)pre;
+    }
+    // (a grid has fewer than 2^32 threads)
+    PIO_REQUIRE(((int64_t)a.pre_items + a.tail_items) * 256 < (int64_t)1 << 32,
+                "pio_kv_attention: %d requests and %d rows are too many", a.n, a.rows);
+    Scratch ws;
+    if (!a.direct) {
+        const size_t parts = (size_t)(a.pre_splits + a.max_runs) * a.rows * a.H;
+        PIO_TRY(ws.get(parts * (a.c.head_dim + 2) * sizeof(float) + a.rows * sizeof(int), st));
+        a.part_o = (float*)ws.ptr;
+        a.part_ml = a.part_o + parts * a.c.head_dim;
+        a.part_n = (int*)(a.part_ml + 2 * parts);
+    }
+    PIO_TRY(a.c.head_dim == 128 ? ka4_route<128>(a, nc, st) : ka4_route<64>(a, nc, st));
+    if (a.direct) return PIO_OK;
+    return a.c.head_dim == 128 ? ka4_join<128>(a, st) : ka4_join<64>(a, st);
+}
+
 int ka4_attention(KaArgs& a, int max_rows, hipStream_t st) {
+    if (a.c.head_dim == 128 || a.c.head_dim == 64) return ka4_matrix(a, max_rows, st);
     PIO_REQUIRE((int64_t)a.rows * a.H < 1 << 24, "pio_kv_attention: too many rows");
     ka4_simple_kernel<<<a.rows * a.H, KA_THREADS, 0, st>>>(a);
     PIO_LAUNCHED();
