@@ -160,25 +160,33 @@ struct Ka4Q {
     ka4_u6 p[Ka4<D, X16>::QM];
     int e[Ka4<D, X16>::QM];
 };
+// Its elements as they lie in memory, loaded ahead of the keys (waits for loads are in order).
+template <bool X16>
+struct Ka4Raw {
+    uint4 u[X16 ? 4 : 8];
+};
 template <int D, bool X16>
-__device__ __forceinline__ void ka4_load_q(const KaArgs& a, int row, int head, bool live, int part, Ka4Q<D, X16>& q) {
-    using T = Ka4<D, X16>;
+__device__ __forceinline__ void ka4_raw_q(const KaArgs& a, int row, int head, bool live, int part, Ka4Raw<X16>& raw) {
     const int64_t at = (live ? row * a.q_stride + (int64_t)head * D : 0) + 32 * (D == 128 ? part : part & 1);
+    const uint4* from = (const uint4*)((const char*)a.q + at * (X16 ? 2 : 4));
+#pragma unroll
+    for (int i = 0; i < (X16 ? 4 : 8); i++) raw.u[i] = from[i];
+}
+template <int D, bool X16>
+__device__ __forceinline__ void ka4_set_q(const KaArgs& a, const Ka4Raw<X16>& raw, bool live, int part, Ka4Q<D, X16>& q) {
+    using T = Ka4<D, X16>;
     const int half = D == 128 ? 0 : part >> 1;         // 64 dimensions: which parts this half of the operand has
     const float scale = a.scale * KA_LOG2E;
     ka_v16 xa, xb;
     uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float x[8];
-        if constexpr (X16) load8<_Float16>((const _Float16*)a.q + at + 8 * i, x);
-        else load8<float>((const float*)a.q + at + 8 * i, x);
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            x[j] *= scale;
-            most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
-            (j & 1 ? xb : xa)[4 * i + j / 2] = x[j];
-        }
+    for (int i = 0; i < 32; i++) {
+        float x;
+        if constexpr (X16) x = (float)__builtin_bit_cast(ka_h8, raw.u[i / 8])[i % 8];
+        else x = __builtin_bit_cast(ka_f4, raw.u[i / 4])[i % 4];
+        x *= scale;
+        most = max(most, __float_as_uint(x) & 0x7fffffffu);
+        (i & 1 ? xb : xa)[i / 2] = x;
     }
     const bool odd = most >= 0x7f800000u;              // inf or NaN: a NaN scale makes the column's scores NaN
     if (!live || odd) {
@@ -217,21 +225,22 @@ __device__ __forceinline__ void ka4_load_q(const KaArgs& a, int row, int head, b
     }
 }
 
-// A column's running softmax: (reference, sum) in base 2, O^T.
+// A column's running softmax. `ref`: minus its reference, plus KA_LIFT, in all elements: the products of a score
+// start there, and give the exponent of its weight. l: the sum of the weights, which the matrix cores add up too
+// (of the rounded weights, as O^T is), in all elements.
 template <int D>
 struct Ka4Acc {
-    float m, l;
-    ka_f4 o[D / 16];
+    float m;                       // the reference; -FLT_MAX: saw no key
+    ka_f4 ref, l, o[D / 16];
     __device__ void clear() {
         m = -FLT_MAX;
-        l = 0.f;
+        ref = l = ka_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < D / 16; n++) o[n] = ka_f4{0.f, 0.f, 0.f, 0.f};
     }
 };
 
 // A lane's share of 32 keys and values.
-template <int D>
 struct Ka4Keys {
     uint4 k[2];
     int ks[2];
@@ -242,74 +251,93 @@ struct Ka4Keys {
 template <int D, bool X16, int NC>
 struct Ka4Walk {
     using T = Ka4<D, X16>;
+    typedef const __attribute__((address_space(4))) int32_t* Table;    // (the same for the wave: a scalar load)
     const char *kb, *vb;
     uint32_t page_b;
-    int first, tiles, lo, hi, lg, mask, codes;     // keys from `first`; first and last group of 8 keys; bytes of codes
-    int kg, vg, kid, vid;                          // this lane's groups of 8 keys of the next tile, their pages
-    int bad_at = INT_MAX;                          // first key of this lane in a page outside the cache
+    uint32_t ko, kso, vo, vso;                     // this lane's offsets from a tile's first row
+    int first, tiles, lo, hi, lg, mask;            // keys from `first`; first and last page of the table row
+    int id[2], at[2];                              // pages of the next tile's halves, rows in them
+    int bad_at = INT_MAX;                          // first key in a page outside the cache
     bool odd = false;
-    Ka4Keys<D> next;
+    Ka4Keys next;
 
-    // (groups outside the item's keys: the nearest inside)
-    __device__ void look_up(const KaItem& it, int j, int lane) {
-        const int t0 = first + min(j, tiles - 1) * KA4_TILE;
-        kg = min(max(t0 + 8 * ((lane & 15) >> 2), lo), hi);
-        vg = min(max(t0 + 8 * (lane >> 4), lo), hi);
-        kid = it.table[kg >> lg];
-        vid = it.table[vg >> lg];
+    // Pages of 16 keys or more: the halves of a tile have one each (a half outside the item's keys: the nearest).
+    __device__ void look_up(const KaItem& it, int j) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int t = first + min(j, tiles - 1) * KA4_TILE + 16 * h;
+            at[h] = t & mask;
+            id[h] = ((Table)(uintptr_t)it.table)[min(max(t >> lg, lo), hi)];
+        }
     }
-    __device__ void load(const KaArgs& a, const KaItem& it, int lane) {
-        const bool ok = (unsigned)kid < (unsigned)a.c.n_pages;
-        bad_at = ok ? bad_at : min(bad_at, max(kg, it.k0));
-        const char* k = kb + (uint64_t)(ok ? (uint32_t)kid : 0u) * page_b;
-        const char* v = vb + (uint64_t)((unsigned)vid < (unsigned)a.c.n_pages ? (uint32_t)vid : 0u) * page_b;
-        const int kt = (kg & mask) + (lane & 3), vt = vg & mask, part = lane >> 4, i = lane & 15;
-        const int kblock = D == 128 ? part : part & 1;
+    __device__ void load(const KaArgs& a, const KaItem& it, int j, int lane) {
+        const char *k[2], *v[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const bool ok = (unsigned)id[h] < (unsigned)a.c.n_pages;
+            const int t = min(max(first + j * KA4_TILE + 16 * h, it.k0), it.k1 - 1);
+            bad_at = ok ? bad_at : min(bad_at, max(t & -16, it.k0));
+            const uint64_t page = (uint64_t)(ok ? (uint32_t)id[h] : 0u) * page_b;
+            k[h] = kb + page;
+            v[h] = vb + page;
+        }
+        const bool kh = lane & 8, vh = lane & 32;
+        const char *kp = kh ? k[1] : k[0], *vp = vh ? v[1] : v[0];
+        const uint32_t kt = kh ? at[1] : at[0], vt = vh ? at[1] : at[0];
+        const char *kr = kp + (kt * T::RB + ko), *ks = kp + (kt + kso);
+        const char *vr = vp + (vt * T::RB + vo), *vs = vp + (vt + vso);
 #pragma unroll
         for (int t = 0; t < 2; t++) {
-            next.k[t] = *(const uint4*)(k + (kt + 4 * t) * T::RB + 16 * kblock);
-            next.ks[t] = *(const uint8_t*)(k + codes + (kblock << lg) + kt + 4 * t);
+            next.k[t] = *(const uint4*)(kr + 4 * t * T::RB);
+            next.ks[t] = *(const uint8_t*)(ks + 4 * t);
         }
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if constexpr (D == 128) next.v[j] = *(const uint32_t*)(v + (vt + j) * T::RB + 4 * i);
-            else next.v[j] = *(const uint16_t*)(v + (vt + j) * T::RB + 2 * i);
+        for (int i = 0; i < 8; i++) {
+            if constexpr (D == 128) next.v[i] = *(const uint32_t*)(vr + i * T::RB);
+            else next.v[i] = *(const uint16_t*)(vr + i * T::RB);
         }
-        next.vs = *(const uint2*)(v + codes + (((D / 16 * i) >> 5) << lg) + vt);
+        next.vs = *(const uint2*)vs;
     }
     // The first tile's loads, if the wave has one.
     __device__ void begin(const KaArgs& a, const KaItem& it, int w, int lane) {
         const pio_kv_cache& c = a.c;
         lg = kv_log2(c.page_size);
         mask = c.page_size - 1;
-        codes = c.page_size * T::RB;
         const int64_t head = (int64_t)c.page_size * (D / 32 * 17);
         page_b = (uint32_t)(head * c.n_kv_heads);
         kb = (const char*)c.kv + (int64_t)2 * a.layer * c.n_pages * page_b + it.g * head;
         vb = kb + (int64_t)c.n_pages * page_b;
         first = it.k0 & -KA4_TILE;
-        lo = it.k0 & -8;
-        hi = (it.k1 - 1) & -8;
+        lo = it.k0 >> lg;
+        hi = max(it.k1 - 1, 0) >> lg;
         tiles = it.k1 > it.k0 ? (it.k1 - first + KA4_TILE - 1) / KA4_TILE : 0;
         if (w >= tiles) return;
-        look_up(it, w, lane);
-        load(a, it, lane);
-        look_up(it, w + KA4_WAVES, lane);
+        look_up(it, w);
+        const uint32_t r = lane & 15, part = lane >> 4, kblock = D == 128 ? part : part & 1;
+        const uint32_t kt = (8 * (r >> 2) + (r & 3)) & 15, vt = 8 * (part & 1), codes = c.page_size * T::RB;
+        ko = kt * T::RB + 16 * kblock;
+        kso = codes + (kblock << lg) + kt;
+        vo = vt * T::RB + D / 32 * r;
+        vso = codes + ((D / 16 * r >> 5) << lg) + vt;
+        load(a, it, w, lane);
+        look_up(it, w + KA4_WAVES);
     }
     __device__ void run(const KaArgs& a, const KaItem& it, int w, int lane, const Ka4Q<D, X16> (&q)[NC],
                         const int (&limit)[NC], Ka4Acc<D> (&x)[NC]) {
         const int part = lane >> 4;
+        const _Float16 one = (_Float16)1.f;
+        const ka_h8 ones = {one, one, one, one, one, one, one, one};
         int least = limit[0];
 #pragma unroll
         for (int c = 1; c < NC; c++) least = min(least, limit[c]);
-        least = ka_wave_min(least);
+        least = __builtin_amdgcn_readfirstlane(ka_wave_min(least));
         for (int j = w; j < tiles; j += KA4_WAVES) {
             const int t0 = first + j * KA4_TILE, key0 = t0 + 8 * part;
             const bool edge = t0 < it.k0 || t0 + KA4_TILE > least;
-            Ka4Keys<D> now = next;
+            Ka4Keys now = next;
             if (j + KA4_WAVES < tiles) {
-                load(a, it, lane);
-                look_up(it, j + 2 * KA4_WAVES, lane);
+                load(a, it, j + KA4_WAVES, lane);
+                look_up(it, j + 2 * KA4_WAVES);
             }
             if (edge) {
                 // A value that some column does not see must not reach it, 0 * NaN: NaN blocks are left out (ka4_mend
@@ -330,7 +358,7 @@ struct Ka4Walk {
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     const ka4_i8 k = {(int)now.k[t].x, (int)now.k[t].y, (int)now.k[t].z, (int)now.k[t].w, 0, 0, 0, 0};
-                    ka_f4 acc = {0.f, 0.f, 0.f, 0.f};
+                    ka_f4 acc = x[c].ref;
 #pragma unroll
                     for (int m = T::QM - 1; m >= 0; m--) {         // the small parts first
                         const ka4_u6& p = q[c].p[m];
@@ -348,25 +376,32 @@ struct Ka4Walk {
                 float top = s[0];
 #pragma unroll
                 for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
-                top = ka_max<16>(fmaxf(top, max(t0, it.k0) < limit[c] ? KA_SEEN : -FLT_MAX));
-                if (__any(top > x[c].m + KA_SLACK)) {
-                    const float m = fmaxf(x[c].m, top), corr = __builtin_amdgcn_exp2f(x[c].m - m);
-                    x[c].l *= corr;
+                // The reference is the wave's first tile's maximum (a column that sees no key there sees none at
+                // all), and follows where a score has grown past it
+                if (j == w || __any(top > KA_LIFT + KA_SLACK)) {
+                    top = ka_max<16>(top);
+                    const bool sees = top > KA_SEEN;
+                    const float by = j == w ? (sees ? KA_LIFT - top : 0.f) : fminf(KA_LIFT - fmaxf(top, KA_LIFT), 0.f);
+                    const float corr = __builtin_amdgcn_exp2f(by);
+                    x[c].ref += by;
+                    if (j != w) {
+                        x[c].l *= corr;
 #pragma unroll
-                    for (int n = 0; n < T::NT; n++)
+                        for (int n = 0; n < T::NT; n++) x[c].o[n] *= corr;
+                    }
+                    if (sees) x[c].m = -x[c].ref[0];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[c].o[n][e] *= corr;
-                    x[c].m = m;
+                    for (int i = 0; i < 8; i++) s[i] += by;
                 }
-                const float base = x[c].m - KA_LIFT;       // (behind a score beyond 2^24 the weights stay below 2^15)
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    s[i] = __builtin_amdgcn_exp2f(s[i] - base);
+                    s[i] = __builtin_amdgcn_exp2f(s[i]);
                     const _Float16 hi = (_Float16)s[i];
                     wt[c][0][i] = hi;
                     if constexpr (T::XP == 2) wt[c][T::XP - 1][i] = (_Float16)(s[i] - (float)hi);
                 }
-                x[c].l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+#pragma unroll
+                for (int k = 0; k < T::XP; k++) x[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wt[c][k], x[c].l, 0, 0, 0);
             }
             float vs[8];
 #pragma unroll
@@ -419,8 +454,16 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
                                          int c0, int w, int lane) {
     using T = Ka4<D, X16>;
     Ka4Walk<D, X16, NC> walk;
-    walk.begin(a, it, w, lane);
     const int first = ka_div(a, c0);
+    Ka4Raw<X16> raw[NC];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        const int col = c0 + 16 * c + (lane & 15);
+        const bool has = col < it.ncols;
+        const int r = has ? ka_div(a, col) : 0, head = it.g * a.G + (has ? col - r * a.G : 0);
+        ka4_raw_q<D, X16>(a, it.row0 + r, head, has, lane >> 4, raw[c]);
+    }
+    walk.begin(a, it, w, lane);
     if (limits) ka_limits(a, first, limits, 16 * NC);      // under the first loads' way
     Ka4Q<D, X16> q[NC];
     Ka4Acc<D> x[NC];
@@ -429,23 +472,20 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
     for (int c = 0; c < NC; c++) {
         const int col = c0 + 16 * c + (lane & 15);
         const bool has = col < it.ncols;
-        const int r = has ? ka_div(a, col) : 0, head = it.g * a.G + (has ? col - r * a.G : 0);
+        const int r = has ? ka_div(a, col) : 0;
         limit[c] = has ? ka_limit(it, limits, first, r) : it.k1;
         sees[c] = !has ? -1 : limits ? limits[r - first] : it.first_limit + r;
         x[c].clear();
-        if (w < walk.tiles) ka4_load_q<D, X16>(a, it.row0 + r, head, has, lane >> 4, q[c]);
+        ka4_set_q<D, X16>(a, raw[c], has, lane >> 4, q[c]);
     }
     walk.run(a, it, w, lane, q, limit, x);
     // a page outside the cache: NaN for the columns that see its keys
-    int bad_at = INT_MAX;
-    if (__any(walk.bad_at != INT_MAX)) bad_at = ka_wave_min(walk.bad_at);
+    const int bad_at = walk.bad_at;
     bool told = it.bad;
 #pragma unroll
     for (int c = 0; c < NC; c++) {
         told |= sees[c] > bad_at;
-        x[c].l += __shfl_xor(x[c].l, 32, 64);
-        x[c].l += __shfl_xor(x[c].l, 16, 64);
-        if (it.bad || limit[c] > bad_at) x[c].l = NAN;
+        if (it.bad || limit[c] > bad_at) x[c].l[0] = NAN;
     }
     if (told) atomicOr(a.c.work, KV_BAD);
     const bool odd = __syncthreads_or(walk.odd);
@@ -456,7 +496,7 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
         const int col = lane & 15, part = lane >> 4;
         if (part == 0) {
             ml[w][col][0] = x[c].m;
-            ml[w][col][1] = x[c].l;
+            ml[w][col][1] = x[c].l[0];
         }
         __syncthreads();
         float mx = ml[0][col][0];
@@ -491,6 +531,73 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
     }
 }
 
+// Sums over the lanes up to each.
+__device__ __forceinline__ int ka4_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);      // row_bcast 15, into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);      // row_bcast 31, into rows 2 and 3
+    return x;
+}
+
+// ka_runs for up to 64 N requests, by each wave on its own: no LDS and no barriers, and what is found is the same
+// for the wave's lanes as the compiler sees it, so that page ids are scalar loads.
+template <int N>
+__device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found, int cols) {
+    const int lane = threadIdx.x & 63;
+    int r0[N], r1[N], s[N], L[N], n[N], sum = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        const int i = min(lane + 64 * k, a.n - 1);
+        ka_rows(a, i, r0[k], r1[k]);
+        s[k] = a.seq[i];
+    }
+#pragma unroll
+    for (int k = 0; k < N; k++) L[k] = kv_seq_len(a.c, s[k]);
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        n[k] = L[k] <= a.shared ? 1 : (L[k] - a.shared + KA_ROUND - 1) / KA_ROUND;
+        if (lane + 64 * k >= a.n || r1[k] <= r0[k]) n[k] = 0;
+        sum += n[k];
+    }
+    const int total = __builtin_amdgcn_readlane(ka4_scan(sum), 63);
+    const float units = a.c.n_kv_heads * a.tail_tiles;
+    const float cut = fmaxf(fmaxf(1.f, (float)total / a.tail_runs),
+                            fminf(a.fixed, ka_cut(total, units, a.pre_work + a.n * units * a.fixed, a.slots, a.fixed)));
+    found.i = -1;
+    int before = 0;
+#pragma unroll
+    for (int k = 0; k < N; k++) {
+        int per = 1, runs = 0, tiles = 0;
+        if (n[k] > 0) {
+            tiles = min(a.tail_tiles, ((r1[k] - r0[k]) * a.G + cols - 1) / cols);
+            runs = min(max(1, (int)(n[k] / cut + 0.5f)), a.max_runs);
+            per = (n[k] + runs - 1) / runs;
+            runs = (n[k] + per - 1) / per;
+        }
+        const int mine = runs * tiles, upto = before + ka4_scan(mine);
+        const uint64_t hit = __ballot(unit >= upto - mine && unit < upto);
+        if (hit) {
+            const int l = __ffsll((unsigned long long)hit) - 1;
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            found.i = l + 64 * k;
+            found.runs = of(runs);
+            found.per = of(per);
+            found.tiles = of(tiles);
+            found.r0 = of(r0[k]);
+            found.r1 = of(r1[k]);
+            found.s = of(s[k]);
+            found.L = of(L[k]);
+            const int at = unit - of(upto - mine);
+            found.z = at / found.tiles;
+            found.ct = at - found.z * found.tiles;
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+    }
+}
+
 // The prefix's items, then the tails'.
 template <int D, bool X16, int NC>
 __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void ka4_kernel(KaArgs a) {
@@ -508,8 +615,17 @@ __global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void ka4_kernel(KaArgs a) {
         return;
     }
     const int item = (int)blockIdx.x - a.pre_items, unit = item / a.c.n_kv_heads, g = item - unit * a.c.n_kv_heads;
-    ka_runs(a, unit, found, red, COLS);
-    const KaRun r = found;
+    KaRun r;
+    if (a.n <= 64) {
+        ka4_runs<1>(a, unit, r, COLS);
+    } else if (a.n <= 256) {
+        ka4_runs<4>(a, unit, r, COLS);
+    } else {
+        ka_runs(a, unit, found, red, COLS);
+        auto same = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+        r = KaRun{same(found.i), same(found.z), same(found.runs), same(found.per), same(found.ct), same(found.tiles),
+                  same(found.r0), same(found.r1), same(found.s), same(found.L)};
+    }
     if (!ka_tail(a, it, r, g)) return;
     if (!a.direct && g == 0 && r.ct == 0 && r.z == 0)
         for (int i = tid; i < r.r1 - r.r0; i += 64 * KA4_WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
