@@ -280,21 +280,32 @@ __global__ __launch_bounds__(256) void ka_merge_kernel(KaArgs a) {
     __shared__ __attribute__((aligned(16))) float so[GRP][D];
     __shared__ float sml[GRP][2];
     const int tid = threadIdx.x, grp = tid / TPC, d = (tid % TPC) * 4, zg = grp % Z;
-    const int64_t at = (int64_t)blockIdx.x * COLS + grp / Z, step = (int64_t)a.rows * a.H;
-    const int row = at < step ? (int)(at / a.H) : a.rows, head = (int)(at - (int64_t)row * a.H);
-    const bool has = row >= a.row_start[0] && row < min(a.row_start[a.n], a.rows);
+    // (rows * H < 2^26) Which parts a column has is known later than the first ones' loads are under way: those are
+    // read whatever they hold, inside the workspace.
+    const uint32_t col = blockIdx.x * COLS + grp / Z;
+    const int64_t step = (int64_t)a.rows * a.H, at = col < step ? col : 0;
+    const int row = (int)((uint32_t)at / (uint32_t)a.H), head = (int)at - row * a.H, most = a.pre_splits + a.max_runs;
+    auto part = [&](int z) { return at + min(z, most - 1) * step; };
+    ka_f2 ml = *(const ka_f2*)(a.part_ml + 2 * part(zg));
+    ka_f4 o = *(const ka_f4*)(a.part_o + part(zg) * D + d);
+    const int runs_of = a.part_n[row];
+    const bool has = col < step && row >= a.row_start[0] && row < min(a.row_start[a.n], a.rows);
     // (0: the row's only item wrote it)
-    const int runs = has ? min(max(a.part_n[row], 0), a.max_runs) : 0, parts = runs ? a.pre_splits + runs : 0;
+    const int runs = has ? min(max(runs_of, 0), a.max_runs) : 0, parts = runs ? a.pre_splits + runs : 0;
     float m = -FLT_MAX, l = 0.f;
     ka_f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int z = zg; z < parts; z += Z) {
-        const ka_f2 ml = *(const ka_f2*)(a.part_ml + 2 * (at + z * step));
-        const ka_f4 o = *(const ka_f4*)(a.part_o + (at + z * step) * D + d);
+    auto add = [&]() {
         const float nm = fmaxf(m, ml[0]), f = __builtin_amdgcn_exp2f(m - nm), fz = __builtin_amdgcn_exp2f(ml[0] - nm);
         l = l * f + ml[1] * fz;
         v = v * f + o * fz;
         m = nm;
+    };
+    if (zg < parts) add();
+#pragma unroll 4
+    for (int z = zg + Z; z < parts; z += Z) {
+        ml = *(const ka_f2*)(a.part_ml + 2 * part(z));
+        o = *(const ka_f4*)(a.part_o + part(z) * D + d);
+        add();
     }
     if constexpr (Z > 1) {
         *(ka_f4*)&so[grp][d] = v;

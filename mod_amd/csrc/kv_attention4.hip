@@ -122,8 +122,8 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 //   O^T = V^T P^T on v_mfma_f32_16x16x32_f16. Lane l reads the codes of 8 keys and dimensions D / 16 (l % 16) ..,
 //     and widens each key's to fp16 under its scale, exactly: two keys' halves side by side are the operand, so
 //     V is turned inside a lane. Row i of O^T tile n is dimension (D / 16) i + n.
-//   Row 4 q + e of the t-th 16 keys is key 8 q + 4 t + e, so that a lane's 8 scores are the 8 keys of its part
-//     q = l / 16 of the weights' operand, neighbours on one page, whose scales are 8 bytes in a row.
+//   A lane's 8 scores are of the keys 4 q .. 4 q + 3 of either 16, q = l / 16, and those are the keys of its part of
+//     the weights' operand; V's rows are read in that order.
 typedef int ka4_i8 __attribute__((ext_vector_type(8)));
 typedef uint32_t ka4_u6 __attribute__((ext_vector_type(6)));
 typedef float ka4_v32 __attribute__((ext_vector_type(32)));
@@ -240,66 +240,84 @@ struct Ka4Acc {
     }
 };
 
-// A lane's share of 32 keys and values.
-struct Ka4Keys {
+// A lane's share of a tile's keys, and of its values.
+struct Ka4K {
     uint4 k[2];
     int ks[2];
-    uint32_t v[8];
-    uint2 vs;
+};
+struct Ka4V {
+    uint32_t v[8], vs[2];
 };
 
+// A wave's tiles, every KA4_WAVES-th. The scores run one tile ahead of the softmax, in one piece of code without
+// branches: their products fill the matrix cores while the VALU forms the weights and widens the values. K is
+// loaded two tiles ahead, V one, by turns into two sets of registers.
 template <int D, bool X16, int NC>
 struct Ka4Walk {
     using T = Ka4<D, X16>;
-    typedef const __attribute__((address_space(4))) int32_t* Table;    // (the same for the wave: a scalar load)
     const char *kb, *vb;
     uint32_t page_b;
-    uint32_t ko, kso, vo, vso;                     // this lane's offsets from a tile's first row
-    int first, tiles, lo, hi, lg, mask;            // keys from `first`; first and last page of the table row
-    int id[2], at[2];                              // pages of the next tile's halves, rows in them
+    uint32_t ko, kso, vo, vso;                     // this lane's offsets from a half tile's codes, and scales
+    int first, count, lo, hi, lg, mask;            // first key, tiles of this wave; first and last page of the table row
+    // Of the next 32 tiles to be loaded, lane l has half l % 2 of the l / 2-th (pages of 16 keys or more: a half has
+    // one; outside the item's keys, the nearest): where its codes begin, how far behind them its scales, and the page
+    // of the 32 behind
+    uint64_t off;
+    int behind, id;
     int bad_at = INT_MAX;                          // first key in a page outside the cache
     bool odd = false;
-    Ka4Keys next;
+    const char *kc[2], *vc[2];                     // halves of the next tiles of K and V to be loaded
+    int kd[2], vd[2];
+    Ka4K k0, k1;
+    Ka4V v0, v1;
 
-    // Pages of 16 keys or more: the halves of a tile have one each (a half outside the item's keys: the nearest).
-    __device__ void look_up(const KaItem& it, int j) {
+    __device__ __forceinline__ int half_of(int i, int lane) const {
+        return first + min(i + (lane >> 1), count - 1) * (KA4_WAVES * KA4_TILE) + 16 * (lane & 1);
+    }
+    __device__ __forceinline__ void look_up(const KaItem& it, int i, int lane) {
+        id = it.table[min(max(half_of(i, lane) >> lg, lo), hi)];
+    }
+    // The next tile's place: its lanes' words as scalars, so that a load is one instruction of scalars and an offset.
+    __device__ __forceinline__ void place(const KaArgs& a, const KaItem& it, int i, int lane) {
+        if ((i & 31) == 0) {
+            const int t = half_of(i, lane), at = t & mask;
+            const bool ok = (unsigned)id < (unsigned)a.c.n_pages;
+            if (__any(!ok))
+                bad_at = min(bad_at, ka_wave_min(ok ? INT_MAX : max(min(max(t, it.k0), it.k1 - 1) & -16, it.k0)));
+            off = (uint64_t)(ok ? (uint32_t)id : 0u) * page_b + at * T::RB;
+            behind = (T::RB << lg) - at * (T::RB - 1);
+            if (i + 32 < count) look_up(it, i + 32, lane);
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int t = first + min(j, tiles - 1) * KA4_TILE + 16 * h;
-            at[h] = t & mask;
-            id[h] = ((Table)(uintptr_t)it.table)[min(max(t >> lg, lo), hi)];
+            const int l = 2 * (i & 31) + h;
+            const uint64_t o = (uint32_t)__builtin_amdgcn_readlane((int)off, l) |
+                               (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), l) << 32;
+            kc[h] = kb + o;
+            vc[h] = vb + o;
+            kd[h] = vd[h] = __builtin_amdgcn_readlane(behind, l);
         }
     }
-    __device__ void load(const KaArgs& a, const KaItem& it, int j, int lane) {
-        const char *k[2], *v[2];
+    __device__ __forceinline__ void load_k(Ka4K& to) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const bool ok = (unsigned)id[h] < (unsigned)a.c.n_pages;
-            const int t = min(max(first + j * KA4_TILE + 16 * h, it.k0), it.k1 - 1);
-            bad_at = ok ? bad_at : min(bad_at, max(t & -16, it.k0));
-            const uint64_t page = (uint64_t)(ok ? (uint32_t)id[h] : 0u) * page_b;
-            k[h] = kb + page;
-            v[h] = vb + page;
+            to.k[h] = *(const uint4*)(kc[h] + ko);
+            to.ks[h] = *(const uint8_t*)(kc[h] + kd[h] + kso);
         }
-        const bool kh = lane & 8, vh = lane & 32;
-        const char *kp = kh ? k[1] : k[0], *vp = vh ? v[1] : v[0];
-        const uint32_t kt = kh ? at[1] : at[0], vt = vh ? at[1] : at[0];
-        const char *kr = kp + (kt * T::RB + ko), *ks = kp + (kt + kso);
-        const char *vr = vp + (vt * T::RB + vo), *vs = vp + (vt + vso);
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            next.k[t] = *(const uint4*)(kr + 4 * t * T::RB);
-            next.ks[t] = *(const uint8_t*)(ks + 4 * t);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            if constexpr (D == 128) next.v[i] = *(const uint32_t*)(vr + i * T::RB);
-            else next.v[i] = *(const uint16_t*)(vr + i * T::RB);
-        }
-        next.vs = *(const uint2*)vs;
     }
-    // The first tile's loads, if the wave has one.
-    __device__ void begin(const KaArgs& a, const KaItem& it, int w, int lane) {
+    __device__ __forceinline__ void load_v(Ka4V& to) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if constexpr (D == 128) to.v[4 * h + i] = *(const uint32_t*)(vc[h] + vo + i * T::RB);
+                else to.v[4 * h + i] = *(const uint16_t*)(vc[h] + vo + i * T::RB);
+            }
+            to.vs[h] = *(const uint32_t*)(vc[h] + vd[h] + vso);
+        }
+    }
+    // The first tiles' loads, if the wave has any.
+    __device__ __forceinline__ void begin(const KaArgs& a, const KaItem& it, int w, int lane) {
         const pio_kv_cache& c = a.c;
         lg = kv_log2(c.page_size);
         mask = c.page_size - 1;
@@ -307,128 +325,180 @@ struct Ka4Walk {
         page_b = (uint32_t)(head * c.n_kv_heads);
         kb = (const char*)c.kv + (int64_t)2 * a.layer * c.n_pages * page_b + it.g * head;
         vb = kb + (int64_t)c.n_pages * page_b;
-        first = it.k0 & -KA4_TILE;
+        first = (it.k0 & -KA4_TILE) + w * KA4_TILE;
         lo = it.k0 >> lg;
         hi = max(it.k1 - 1, 0) >> lg;
-        tiles = it.k1 > it.k0 ? (it.k1 - first + KA4_TILE - 1) / KA4_TILE : 0;
-        if (w >= tiles) return;
-        look_up(it, w);
+        count = it.k1 > first ? (it.k1 - first + KA4_WAVES * KA4_TILE - 1) / (KA4_WAVES * KA4_TILE) : 0;
+        if (it.k1 <= it.k0) count = 0;
+        if (count == 0) return;
+        look_up(it, 0, lane);
         const uint32_t r = lane & 15, part = lane >> 4, kblock = D == 128 ? part : part & 1;
-        const uint32_t kt = (8 * (r >> 2) + (r & 3)) & 15, vt = 8 * (part & 1), codes = c.page_size * T::RB;
-        ko = kt * T::RB + 16 * kblock;
-        kso = codes + (kblock << lg) + kt;
-        vo = vt * T::RB + D / 32 * r;
-        vso = codes + ((D / 16 * r >> 5) << lg) + vt;
-        load(a, it, w, lane);
-        look_up(it, w + KA4_WAVES);
+        ko = r * T::RB + 16 * kblock;
+        kso = (kblock << lg) + r;
+        vo = 4 * part * T::RB + D / 32 * r;
+        vso = ((D / 16 * r >> 5) << lg) + 4 * part;
+        place(a, it, 0, lane);
+        load_k(k0);
+        load_v(v0);
+        place(a, it, 1, lane);
+        load_k(k1);
     }
-    __device__ void run(const KaArgs& a, const KaItem& it, int w, int lane, const Ka4Q<D, X16> (&q)[NC],
-                        const int (&limit)[NC], Ka4Acc<D> (&x)[NC]) {
-        const int part = lane >> 4;
+
+    // Scores of 16 NC columns, exponents of weights.
+    __device__ __forceinline__ void scores(const Ka4K& k, const Ka4Q<D, X16> (&q)[NC], const Ka4Acc<D> (&x)[NC],
+                                           float (&s)[NC][8]) {
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const ka4_i8 kt = {(int)k.k[t].x, (int)k.k[t].y, (int)k.k[t].z, (int)k.k[t].w, 0, 0, 0, 0};
+                ka_f4 acc = x[c].ref;
+#pragma unroll
+                for (int m = T::QM - 1; m >= 0; m--) {             // the small parts first
+                    const ka4_u6& p = q[c].p[m];
+                    const ka4_i8 qm = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
+                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 0, q[c].e[m]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[c][4 * t + e] = acc[e];
+            }
+    }
+    // Keys of a lane's scores (from 4 part on), and the rows of its values.
+    static constexpr int key(int i) { return 16 * (i / 4) + i % 4; }
+    // What a column does not see, and the references. They are the wave's first tile's maxima (a column that sees no
+    // key there sees none at all), and follow where a score has grown past them.
+    __device__ __forceinline__ void settle(const KaItem& it, int t0, int part, bool edge, bool begin,
+                                           const int (&limit)[NC], Ka4Acc<D> (&x)[NC], float (&s)[NC][8]) {
+        if (edge) {
+            int key0 = t0 + 4 * part;
+            asm volatile("" : "+v"(key0));         // (a branch: as selects in every tile the masks cost 40 instructions)
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    s[c][i] = key0 + key(i) < limit[c] && key0 + key(i) >= it.k0 ? s[c][i] : -INFINITY;
+        }
+        float top[NC], most;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            top[c] = s[c][0];
+#pragma unroll
+            for (int i = 1; i < 8; i++) top[c] = fmaxf(top[c], s[c][i]);
+            most = c ? fmaxf(most, top[c]) : top[c];
+        }
+        if (!begin && !__any(most > KA_LIFT + KA_SLACK)) return;
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+            const float t = ka_max<16>(top[c]);
+            const bool sees = t > KA_SEEN;
+            const float by = begin ? (sees ? KA_LIFT - t : 0.f) : fminf(KA_LIFT - fmaxf(t, KA_LIFT), 0.f);
+            x[c].ref += by;
+            if (!begin) {
+                const float corr = __builtin_amdgcn_exp2f(by);
+                x[c].l *= corr;
+#pragma unroll
+                for (int n = 0; n < T::NT; n++) x[c].o[n] *= corr;
+            }
+            if (sees) x[c].m = -x[c].ref[0];
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[c][i] += by;
+        }
+    }
+    // O^T and l of one tile, of the scores s; their place then has the next tile's.
+    __device__ __forceinline__ void products(const Ka4K& k, const Ka4V& v, const Ka4Q<D, X16> (&q)[NC], Ka4Acc<D> (&x)[NC],
+                                             float (&s)[NC][8]) {
         const _Float16 one = (_Float16)1.f;
         const ka_h8 ones = {one, one, one, one, one, one, one, one};
+        float next[NC][8];
+        scores(k, q, x, next);
+        ka_h8 wt[NC][T::XP];
+#pragma unroll
+        for (int c = 0; c < NC; c++) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float w = __builtin_amdgcn_exp2f(s[c][i]);
+                const _Float16 hi = (_Float16)w;
+                wt[c][0][i] = hi;
+                if constexpr (T::XP == 2) wt[c][T::XP - 1][i] = (_Float16)(w - (float)hi);
+            }
+#pragma unroll
+            for (int p = 0; p < T::XP; p++) x[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wt[c][p], x[c].l, 0, 0, 0);
+        }
+        // (the conversions look at a scale's exponent alone: what else a shift leaves in the word does not matter)
+        float unit[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t word = v.vs[i / 4];
+            unit[i] = __uint_as_float((i & 3) == 3 ? word >> 1 : word << (23 - 8 * (i & 3)));
+        }
+        auto pair = [&](auto byte) {
+            constexpr int B = decltype(byte)::value;
+            ka_h8 a0, a1;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const ka4_h2 y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(v.v[i], unit[i], B);
+                a0[i] = y[0];
+                a1[i] = y[1];
+            }
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+#pragma unroll
+                for (int p = 0; p < T::XP; p++) {
+                    x[c].o[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, wt[c][p], x[c].o[2 * B], 0, 0, 0);
+                    x[c].o[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, wt[c][p], x[c].o[2 * B + 1], 0, 0, 0);
+                }
+        };
+        pair(std::integral_constant<int, 0>{});
+        pair(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            pair(std::integral_constant<int, 2>{});
+            pair(std::integral_constant<int, 3>{});
+        }
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int i = 0; i < 8; i++) s[c][i] = next[c][i];
+    }
+    __device__ __forceinline__ void run(const KaArgs& a, const KaItem& it, int lane, const Ka4Q<D, X16> (&q)[NC],
+                                        const int (&limit)[NC], Ka4Acc<D> (&x)[NC]) {
+        if (count == 0) return;
+        const int part = lane >> 4;
         int least = limit[0];
 #pragma unroll
         for (int c = 1; c < NC; c++) least = min(least, limit[c]);
         least = __builtin_amdgcn_readfirstlane(ka_wave_min(least));
-        for (int j = w; j < tiles; j += KA4_WAVES) {
-            const int t0 = first + j * KA4_TILE, key0 = t0 + 8 * part;
-            const bool edge = t0 < it.k0 || t0 + KA4_TILE > least;
-            Ka4Keys now = next;
-            if (j + KA4_WAVES < tiles) {
-                load(a, it, j + KA4_WAVES, lane);
-                look_up(it, j + 2 * KA4_WAVES);
-            }
-            if (edge) {
+        auto begins = [&](int i) { return first + i * (KA4_WAVES * KA4_TILE); };
+        const int whole = least >= first ? (least - first) / (KA4_WAVES * KA4_TILE) + (((least - first) & (KA4_WAVES * KA4_TILE - 1)) >= KA4_TILE) : 0;
+        const int low = first < it.k0 ? 0 : -1;
+        auto edge = [&](int i) { return i >= whole || i == low; };
+        float s[NC][8];
+        scores(k0, q, x, s);
+        settle(it, begins(0), part, edge(0), true, limit, x, s);
+        auto step = [&](int i, const Ka4K& k, Ka4K& kfree, Ka4V& v, Ka4V& vfree) {
+            // (past the end the last tile again: under a branch the waits for loads could not count these)
+            load_v(vfree);
+            place(a, it, i + 2, lane);
+            load_k(kfree);
+            if (edge(i)) {
                 // A value that some column does not see must not reach it, 0 * NaN: NaN blocks are left out (ka4_mend
                 // adds them to the columns that see them), and whatever lies outside the item's keys
+                int key0 = begins(i) + 4 * part;
+                asm volatile("" : "+v"(key0));
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    uint32_t& word = i < 4 ? now.vs.x : now.vs.y;
-                    const uint32_t byte = word >> 8 * (i & 3) & 255u;
-                    const bool in = key0 + i >= it.k0 && key0 + i < it.k1, wrong = byte > KV_MX4_MOST;
+                for (int e = 0; e < 8; e++) {
+                    uint32_t& word = v.vs[e / 4];
+                    const uint32_t byte = word >> 8 * (e & 3) & 255u;
+                    const bool in = key0 + key(e) >= it.k0 && key0 + key(e) < it.k1, wrong = byte > KV_MX4_MOST;
                     odd |= in && wrong;
-                    if (!in || wrong) word &= ~(255u << 8 * (i & 3));
+                    if (!in || wrong) word &= ~(255u << 8 * (e & 3));
                 }
             }
-            ka_h8 wt[NC][T::XP];
-#pragma unroll
-            for (int c = 0; c < NC; c++) {
-                float s[8];
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const ka4_i8 k = {(int)now.k[t].x, (int)now.k[t].y, (int)now.k[t].z, (int)now.k[t].w, 0, 0, 0, 0};
-                    ka_f4 acc = x[c].ref;
-#pragma unroll
-                    for (int m = T::QM - 1; m >= 0; m--) {         // the small parts first
-                        const ka4_u6& p = q[c].p[m];
-                        const ka4_i8 qm = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
-                        acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(k, qm, acc, 4, 2, 0, now.ks[t], 0, q[c].e[m]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 4; e++) s[4 * t + e] = acc[e];
-                }
-                if (edge) {
-                    const int end = limit[c] - key0, begin = it.k0 - key0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s[i] = i < end && i >= begin ? s[i] : -INFINITY;
-                }
-                float top = s[0];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, s[i]);
-                // The reference is the wave's first tile's maximum (a column that sees no key there sees none at
-                // all), and follows where a score has grown past it
-                if (j == w || __any(top > KA_LIFT + KA_SLACK)) {
-                    top = ka_max<16>(top);
-                    const bool sees = top > KA_SEEN;
-                    const float by = j == w ? (sees ? KA_LIFT - top : 0.f) : fminf(KA_LIFT - fmaxf(top, KA_LIFT), 0.f);
-                    const float corr = __builtin_amdgcn_exp2f(by);
-                    x[c].ref += by;
-                    if (j != w) {
-                        x[c].l *= corr;
-#pragma unroll
-                        for (int n = 0; n < T::NT; n++) x[c].o[n] *= corr;
-                    }
-                    if (sees) x[c].m = -x[c].ref[0];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s[i] += by;
-                }
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    s[i] = __builtin_amdgcn_exp2f(s[i]);
-                    const _Float16 hi = (_Float16)s[i];
-                    wt[c][0][i] = hi;
-                    if constexpr (T::XP == 2) wt[c][T::XP - 1][i] = (_Float16)(s[i] - (float)hi);
-                }
-#pragma unroll
-                for (int k = 0; k < T::XP; k++) x[c].l = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, wt[c][k], x[c].l, 0, 0, 0);
-            }
-            float vs[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) vs[i] = __uint_as_float(((i < 4 ? now.vs.x : now.vs.y) >> 8 * (i & 3) & 255u) << 23);
-            auto pair = [&](auto byte) {
-                constexpr int B = decltype(byte)::value;
-                ka_h8 v0, v1;
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const ka4_h2 y = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(now.v[i], vs[i], B);
-                    v0[i] = y[0];
-                    v1[i] = y[1];
-                }
-#pragma unroll
-                for (int c = 0; c < NC; c++)
-#pragma unroll
-                    for (int k = 0; k < T::XP; k++) {
-                        x[c].o[2 * B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, wt[c][k], x[c].o[2 * B], 0, 0, 0);
-                        x[c].o[2 * B + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, wt[c][k], x[c].o[2 * B + 1], 0, 0, 0);
-                    }
-            };
-            pair(std::integral_constant<int, 0>{});
-            pair(std::integral_constant<int, 1>{});
-            if constexpr (D == 128) {
-                pair(std::integral_constant<int, 2>{});
-                pair(std::integral_constant<int, 3>{});
-            }
+            products(k, v, q, x, s);               // (behind the last tile the scores of some tile again, unused)
+            if (i + 1 < count) settle(it, begins(i + 1), part, edge(i + 1), false, limit, x, s);
+        };
+        for (int i = 0; i < count; i += 2) {
+            step(i, k1, k0, v0, v1);
+            if (i + 1 < count) step(i + 1, k0, k1, v1, v0);
         }
     }
 };
@@ -478,7 +548,7 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
         x[c].clear();
         ka4_set_q<D, X16>(a, raw[c], has, lane >> 4, q[c]);
     }
-    walk.run(a, it, w, lane, q, limit, x);
+    walk.run(a, it, lane, q, limit, x);
     // a page outside the cache: NaN for the columns that see its keys
     const int bad_at = walk.bad_at;
     bool told = it.bad;
@@ -600,7 +670,7 @@ __device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found
 
 // The prefix's items, then the tails'.
 template <int D, bool X16, int NC>
-__global__ __launch_bounds__(256, NC == 1 ? 3 : 2) void ka4_kernel(KaArgs a) {
+__global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[KA4_WAVES * 16 * Ka4<D, X16>::OP];
     __shared__ float ml[KA4_WAVES][16][2];
     __shared__ int limits[16 * NC];
@@ -665,7 +735,7 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
     const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
     a.fixed = KA4_FIXED;
-    const int nc = tail_cols > 16 ? 2 : 1, width = 16 * nc, held = nc == 1 ? 3 : 2;
+    const int nc = tail_cols > 16 ? 2 : 1, width = 16 * nc, held = 2;
     a.tail_tiles = ceil_div(tail_cols, width);
     PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);
     const int64_t items = std::min((int64_t)a.n * a.tail_tiles, cols / width + a.n) * Hk;
