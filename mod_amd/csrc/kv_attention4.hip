@@ -125,6 +125,7 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 //   A lane's 8 scores are of the keys 4 q .. 4 q + 3 of either 16, q = l / 16, and those are the keys of its part of
 //     the weights' operand; V's rows are read in that order.
 typedef int ka4_i8 __attribute__((ext_vector_type(8)));
+typedef uint32_t ka4_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ka4_u6 __attribute__((ext_vector_type(6)));
 typedef float ka4_v32 __attribute__((ext_vector_type(32)));
 typedef _Float16 ka4_h2 __attribute__((ext_vector_type(2)));
@@ -252,7 +253,8 @@ struct Ka4V {
 // A wave's tiles, every KA4_WAVES-th. The scores run one tile ahead of the softmax, in one piece of code without
 // branches: their products fill the matrix cores while the VALU forms the weights and widens the values. K is
 // loaded two tiles ahead, V one, by turns into two sets of registers.
-template <int D, bool X16, int NC>
+// ONCE: nothing else reads these keys.
+template <int D, bool X16, int NC, bool ONCE>
 struct Ka4Walk {
     using T = Ka4<D, X16>;
     const char *kb, *vb;
@@ -301,7 +303,10 @@ struct Ka4Walk {
     __device__ __forceinline__ void load_k(Ka4K& to) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            to.k[h] = *(const uint4*)(kc[h] + ko);
+            // (past the caches where the keys are read once: 3 sequences of 120,000 36.4 us, so 32.9. V's rows, whose lines
+            // two loads share, are not: 35.1)
+            if constexpr (ONCE) to.k[h] = __builtin_bit_cast(uint4, __builtin_nontemporal_load((const ka4_u4*)(kc[h] + ko)));
+            else to.k[h] = *(const uint4*)(kc[h] + ko);
             to.ks[h] = *(const uint8_t*)(kc[h] + kd[h] + kso);
         }
     }
@@ -519,11 +524,11 @@ __device__ __forceinline__ void ka4_mend(const KaArgs& a, const KaItem& it, int 
 }
 
 // An item's columns from c0 joined over its waves and written, 16 at a time.
-template <int D, bool X16, int NC>
+template <int D, bool X16, int NC, bool ONCE>
 __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, float* lds, float (*ml)[16][2], int* limits,
                                          int c0, int w, int lane) {
     using T = Ka4<D, X16>;
-    Ka4Walk<D, X16, NC> walk;
+    Ka4Walk<D, X16, NC, ONCE> walk;
     const int first = ka_div(a, c0);
     Ka4Raw<X16> raw[NC];
 #pragma unroll
@@ -681,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
     KaItem it;
     int ct;
     if ((int)blockIdx.x < a.pre_items) {
-        if (ka_prefix(a, it, ct)) ka4_item<D, X16, NC>(a, it, lds, ml, limits, ct * COLS, w, lane);
+        if (ka_prefix(a, it, ct)) ka4_item<D, X16, NC, false>(a, it, lds, ml, limits, ct * COLS, w, lane);
         return;
     }
     const int item = (int)blockIdx.x - a.pre_items, unit = item / a.c.n_kv_heads, g = item - unit * a.c.n_kv_heads;
@@ -701,7 +706,7 @@ __global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
         for (int i = tid; i < r.r1 - r.r0; i += 64 * KA4_WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
     // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
     for (int c0 = r.ct * COLS; c0 < it.ncols; c0 += r.tiles * COLS) {
-        ka4_item<D, X16, NC>(a, it, lds, ml, nullptr, c0, w, lane);
+        ka4_item<D, X16, NC, NC == 1>(a, it, lds, ml, nullptr, c0, w, lane);
         __syncthreads();                                   // its output is out of LDS
     }
 }
@@ -728,7 +733,10 @@ static int ka4_join(const KaArgs& a, hipStream_t st) {
 }
 
 // An item costs its rounds of keys and this many more.
-constexpr float KA4_FIXED = 8.f;
+constexpr float KA4_FIXED = 4.f;
+// Rounds of a run, at least, where a table row has no more for the most runs: below, what a wave saves is
+// less than what the join costs.
+constexpr int KA4_LEAST = 4;
 
 // Items for the matrix core kernels.
 static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
@@ -744,7 +752,7 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     a.tail_runs = (int)std::max<int64_t>(1, a.slots / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
     const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
-    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 64, ceil_div(longest, KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
+    a.max_runs = (int)std::min<int64_t>({a.tail_runs, 64, ceil_div(longest, KA4_LEAST * KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
     a.direct = a.shared == 0 && a.max_runs == 1;
     a.tail_items = (int)(items + (a.max_runs == 1 ? 0 : (int64_t)a.tail_runs * units));
     if (a.shared > 0) {

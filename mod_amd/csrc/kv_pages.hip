@@ -380,6 +380,36 @@ __global__ __launch_bounds__(KV_PLAN) void kv_compact_plan_kernel(pio_kv_cache c
     if (tid == 0) *w.pairs_n = movers;
 }
 
+// Rows of a cache of 4 bits share lines (two rows' codes, all of a page's scales), and each XCD has its own L2:
+// neighbouring rows on one XCD, so that a line is read or written once. A grid's workgroups go round the XCDs.
+__device__ __forceinline__ int kv_row_of(int block, int rows) {
+    const int each = (rows + 7) >> 3, x = block & 7, full = rows & 7 ? rows & 7 : 8;     // the last XCDs have one fewer
+    return x < full ? x * each + (block >> 3) : full * each + (x - full) * (each - 1) + (block >> 3);
+}
+// Quotients by a few fixed numbers: u / run, u < 2^31.
+struct KvDiv {
+    uint32_t run, magic;
+    __device__ __forceinline__ explicit KvDiv(uint32_t run) : run(run), magic(run > 1 ? 0xffffffffu / run + 1 : 0) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t u) const {
+        uint32_t q = magic ? __umulhi(u, magic) : u;           // or one more
+        return q - (q * run > u);
+    }
+};
+// Pieces of 8 elements of a row, [layer][k, v][head]: which one `u` is.
+struct KvPiece {
+    int l, kind, e, h, piece;          // e: of the row, piece: of the head
+    __device__ __forceinline__ KvPiece(uint32_t u, const KvDiv& by_layer, const KvDiv& by_head) {
+        l = (int)by_layer(u);
+        const int in = (int)u - l * (int)by_layer.run, width = (int)by_layer.run / 2;
+        kind = in >= width;
+        e = in - kind * width;
+        h = (int)by_head((uint32_t)e);
+        piece = e - h * (int)by_head.run;
+    }
+};
+constexpr int KV_FLIGHT = 4;           // pieces of a thread in flight
+typedef uint32_t KvU4 __attribute__((ext_vector_type(4)));
+
 // ----------------------------------------------------------------- write ----
 // A workgroup takes one row through a few layers: it finds the row's request,
 // then moves k and v in pieces of 8 elements. Bytes bound it: 336 rows of 28 layers,
@@ -393,7 +423,8 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
                                                           const XT* __restrict__ k, const XT* __restrict__ v,
                                                           int64_t row_stride, int64_t layer_stride, int per_block) {
     __shared__ int found, named, where[2];     // the row's request, its sequence; page, row in it
-    const int row = blockIdx.x, tid = threadIdx.x, lg = kv_log2(c.page_size);
+    constexpr bool MX4 = std::is_same_v<KT, KvMx4>;
+    const int row = MX4 ? kv_row_of(blockIdx.x, gridDim.x) : (int)blockIdx.x, tid = threadIdx.x, lg = kv_log2(c.page_size);
     if (tid == 0) found = where[0] = -1;
     __syncthreads();
     int s = -1, back = 0, first = -1;          // (first: what thread tid's first request with rows names)
@@ -415,7 +446,24 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         return (kind ? v : k) + l * layer_stride + row * row_stride + 8 * (u - kind * width);
     };
     float x[8];
-    if (tid < 2 * width) load8<XT>(from(l0, tid), x);      // under the way of the checks below
+    const KvDiv by_layer(2 * width), by_head(per_head);
+    const int pieces = (l1 - l0) * 2 * width;
+    Raw8<XT> raw[KV_FLIGHT];
+    auto load = [&](int u0) {
+#pragma unroll
+        for (int i = 0; i < KV_FLIGHT; i++) {
+            if (u0 + i * KV_COPY >= pieces) break;
+            const KvPiece p(u0 + i * KV_COPY, by_layer, by_head);
+            // (past the caches: they are not read again, the pages are)
+            const KvU4* at = (const KvU4*)((p.kind ? v : k) + (l0 + p.l) * layer_stride + row * row_stride + 8 * p.e);
+#pragma unroll
+            for (int j = 0; j < (int)sizeof(XT) / 2; j++)
+                raw[i].u[j] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(at + j));
+        }
+    };
+    // under the way of the checks below
+    if constexpr (MX4) load(tid);
+    else if (tid < 2 * width) load8<XT>(from(l0, tid), x);
     if (tid == req % KV_COPY) {
         int page = -1, pos = -1;
         bool held_up = false;
@@ -441,23 +489,27 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
         return;
     }
     if (where[0] < 0) return;          // without room, or refused above
-    if constexpr (std::is_same_v<KT, KvMx4>) {
+    if constexpr (MX4) {
         const int64_t head = (int64_t)c.page_size * kv_token_bytes(c), plane = head * c.n_kv_heads * c.n_pages;
-        char* base = (char*)c.kv + head * c.n_kv_heads * where[0];
-        for (int l = l0; l < l1; l++) {
-            for (int u = tid; u < 2 * width; u += KV_COPY) {       // (all four threads of a block, or none)
-                const int kind = u >= width, e = u - kind * width, h = e / per_head, piece = e - h * per_head;
-                if (l != l0 || u != tid) load8<XT>(from(l, u), x);
+        char* base = (char*)c.kv + head * c.n_kv_heads * where[0] + 2 * (layer + l0) * plane;
+        for (int u0 = tid; u0 < pieces; u0 += KV_FLIGHT * KV_COPY) {
+            if (u0 != tid) load(u0);
+#pragma unroll
+            for (int i = 0; i < KV_FLIGHT; i++) {
+                const int u = u0 + i * KV_COPY;
+                if (u >= pieces) break;                            // (all four threads of a block, or none)
+                const KvPiece p(u, by_layer, by_head);
+                raw8_widen<XT>(raw[i], x);
                 uint32_t most = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(x[j]) & 0x7fffffffu);
                 most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, DPP_XOR1, 0xF, 0xF, false));
                 most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, DPP_XOR2, 0xF, 0xF, false));
                 const int scale = kv_mx4_scale(most);
-                char* to = base + (2 * (layer + l) + kind) * plane + h * head;
-                *(uint32_t*)(to + where[1] * (c.head_dim / 2) + 4 * piece) = kv_mx4_codes(x, scale);
-                if ((piece & 3) == 0)
-                    to[c.page_size * (c.head_dim / 2 + (piece >> 2)) + where[1]] = (char)scale;
+                char* to = base + (2 * p.l + p.kind) * plane + p.h * head;
+                *(uint32_t*)(to + where[1] * (c.head_dim / 2) + 4 * p.piece) = kv_mx4_codes(x, scale);
+                if ((p.piece & 3) == 0)
+                    to[c.page_size * (c.head_dim / 2 + (p.piece >> 2)) + where[1]] = (char)scale;
             }
         }
     } else {
@@ -488,14 +540,14 @@ __global__ __launch_bounds__(KV_COPY) void kv_read_kernel(pio_kv_cache c, int la
                                                          YT* __restrict__ v, int64_t row_stride, int64_t layer_stride,
                                                          int per_block) {
     __shared__ int where[3];                   // page, row in it; whether a request has the row
-    const int row = blockIdx.x, tid = threadIdx.x, lg = kv_log2(c.page_size);
+    const int row = kv_row_of(blockIdx.x, gridDim.x), tid = threadIdx.x, lg = kv_log2(c.page_size);
     if (tid == 0) where[0] = where[2] = -1;
     __syncthreads();
     for (int i = tid; i < n; i += KV_COPY) {
-        const int r0 = row_start[i], r1 = row_start[i + 1];
+        const int r0 = row_start[i], r1 = row_start[i + 1], s = seq[i], f = first ? first[i] : 0;
         if (row < r0 || row >= r1) continue;
-        const int s = seq[i], L = kv_seq_len(c, s);
-        const int64_t pos = first ? first[i] + ((int64_t)row - r0) : L - ((int64_t)r1 - row);
+        const int L = kv_seq_len(c, s);
+        const int64_t pos = first ? f + ((int64_t)row - r0) : L - ((int64_t)r1 - row);
         const int page = pos >= 0 && pos < L ? c.table[(int64_t)s * c.max_pages + (pos >> lg)] : -1;
         if (page >= 0 && page < c.n_pages) {
             where[0] = page;
@@ -508,26 +560,41 @@ __global__ __launch_bounds__(KV_COPY) void kv_read_kernel(pio_kv_cache c, int la
     __syncthreads();
     if (where[2] < 0) return;          // behind the last request
     const bool there = where[0] >= 0;
-    const int width = c.n_kv_heads * c.head_dim / 8, per_head = c.head_dim / 8, at = there ? where[1] : 0;
+    const int at = there ? where[1] : 0, l0 = blockIdx.y * per_block;
     const int64_t head = (int64_t)c.page_size * kv_token_bytes(c), plane = head * c.n_kv_heads * c.n_pages;
-    const char* base = (const char*)c.kv + head * c.n_kv_heads * (there ? where[0] : 0);
-    const int l0 = blockIdx.y * per_block, l1 = min(layers, l0 + per_block);
-    for (int l = l0; l < l1; l++) {
-        for (int u = tid; u < 2 * width; u += KV_COPY) {
-            const int kind = u >= width, e = u - kind * width, h = e / per_head, piece = e - h * per_head;
-            const char* from = base + (2 * (layer + l) + kind) * plane + h * head;
+    const char* base = (const char*)c.kv + head * c.n_kv_heads * (there ? where[0] : 0) + 2 * (layer + l0) * plane;
+    const int width = c.n_kv_heads * c.head_dim / 8, pieces = (min(layers, l0 + per_block) - l0) * 2 * width;
+    const KvDiv by_layer(2 * width), by_head(c.head_dim / 8);
+    for (int u0 = tid; u0 < pieces; u0 += KV_FLIGHT * KV_COPY) {
+        uint32_t codes[KV_FLIGHT], scale[KV_FLIGHT];
+        Raw8<KT> raw[KV_FLIGHT];
+#pragma unroll
+        for (int i = 0; i < KV_FLIGHT; i++) {
+            if (u0 + i * KV_COPY >= pieces) break;
+            const KvPiece p(u0 + i * KV_COPY, by_layer, by_head);
+            const char* from = base + (2 * p.l + p.kind) * plane + p.h * head;
+            if constexpr (std::is_same_v<KT, KvMx4>) {
+                codes[i] = *(const uint32_t*)(from + at * (c.head_dim / 2) + 4 * p.piece);
+                scale[i] = (uint8_t)from[c.page_size * (c.head_dim / 2 + (p.piece >> 2)) + at];
+            } else {
+                raw[i] = raw8_load<KT>((const KT*)from + (int64_t)at * c.head_dim + 8 * p.piece);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < KV_FLIGHT; i++) {
+            const int u = u0 + i * KV_COPY;
+            if (u >= pieces) break;
+            const KvPiece p(u, by_layer, by_head);
             float x[8];
-            if constexpr (std::is_same_v<KT, KvMx4>)
-                kv_mx4_widen(*(const uint32_t*)(from + at * (c.head_dim / 2) + 4 * piece),
-                             (uint8_t)from[c.page_size * (c.head_dim / 2 + (piece >> 2)) + at], x);
-            else
-                load8<KT>((const KT*)from + (int64_t)at * c.head_dim + 8 * piece, x);
+            if constexpr (std::is_same_v<KT, KvMx4>) kv_mx4_widen(codes[i], scale[i], x);
+            else raw8_widen<KT>(raw[i], x);
             __attribute__((aligned(16))) YT y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) y[j] = from_f32<YT>(there ? x[j] : NAN);
-            YT* to = (kind ? v : k) + l * layer_stride + row * row_stride + 8 * e;
+            // (past the caches, which have the pages to hold)
+            KvU4* to = (KvU4*)((p.kind ? v : k) + (l0 + p.l) * layer_stride + row * row_stride + 8 * p.e);
 #pragma unroll
-            for (int j = 0; j < (int)sizeof(YT) / 2; j++) ((uint4*)to)[j] = ((const uint4*)y)[j];
+            for (int j = 0; j < (int)sizeof(YT) / 2; j++) __builtin_nontemporal_store(((const KvU4*)y)[j], to + j);
         }
     }
 }
@@ -677,7 +744,7 @@ PIO_EXPORT int pio_kv_write(const pio_kv_cache* c, int layer, int layers, const 
                 "%s: strides %lld, %lld (multiples of 8, rows of %lld)", nm, (long long)row_stride,
                 (long long)layer_stride, (long long)width);
     // enough workgroups for the device, and no more: each looks its row up once
-    const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>(layers, (int64_t)rows * layers / 2048));
+    const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>({layers, (int64_t)rows * layers / (c->kv_dtype == PIO_MX4 ? 4096 : 2048), (1 << 28) / width}));
     const dim3 grid(rows, ceil_div(layers, per_block));
     PIO_REQUIRE(grid.y <= 65535, "%s: too many layers", nm);
     hipStream_t st = pick_stream(stream);
@@ -724,7 +791,7 @@ PIO_EXPORT int pio_kv_read(const pio_kv_cache* c, int layer, int layers, const i
     PIO_REQUIRE(layers == 1 || (layer_stride >= width && ((layer_stride - width) / row_stride >= rows - 1 ||
                                                           (row_stride - width) / layer_stride >= layers - 1)),
                 "%s: strides %lld, %lld: rows or layers overlap", nm, (long long)row_stride, (long long)layer_stride);
-    const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>(layers, (int64_t)rows * layers / 2048));
+    const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>({layers, (int64_t)rows * layers / 4096, (1 << 28) / width}));
     const dim3 grid(rows, ceil_div(layers, per_block));
     PIO_REQUIRE(grid.y <= 65535, "%s: too many layers", nm);
     hipStream_t st = pick_stream(stream);
