@@ -127,6 +127,9 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 typedef int ka4_i8 __attribute__((ext_vector_type(8)));
 typedef uint32_t ka4_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ka4_u6 __attribute__((ext_vector_type(6)));
+typedef const __attribute__((address_space(1))) char* Ka4At;       // (global memory, as the compiler could not tell)
+template <typename V>
+__device__ __forceinline__ V ka4_get(Ka4At p) { return *(const __attribute__((address_space(1))) V*)p; }
 typedef float ka4_v32 __attribute__((ext_vector_type(32)));
 typedef _Float16 ka4_h2 __attribute__((ext_vector_type(2)));
 
@@ -243,7 +246,7 @@ struct Ka4Acc {
 
 // A lane's share of a tile's keys, and of its values.
 struct Ka4K {
-    uint4 k[2];
+    ka4_u4 k[2];
     int ks[2];
 };
 struct Ka4V {
@@ -257,19 +260,19 @@ struct Ka4V {
 template <int D, bool X16, int NC, bool ONCE>
 struct Ka4Walk {
     using T = Ka4<D, X16>;
-    const char *kb, *vb;
+    const char* kb;
+    int64_t plane;                                 // from K to V
     uint32_t page_b;
     uint32_t ko, kso, vo, vso;                     // this lane's offsets from a half tile's codes, and scales
     int first, count, lo, hi, lg, mask;            // first key, tiles of this wave; first and last page of the table row
     // Of the next 32 tiles to be loaded, lane l has half l % 2 of the l / 2-th (pages of 16 keys or more: a half has
-    // one; outside the item's keys, the nearest): where its codes begin, how far behind them its scales, and the page
-    // of the 32 behind
-    uint64_t off;
-    int behind, id;
+    // one; outside the item's keys, the nearest): where its codes begin, and the page of the 32 behind
+    uint64_t base;
+    int id;
     int bad_at = INT_MAX;                          // first key in a page outside the cache
     bool odd = false;
-    const char *kc[2], *vc[2];                     // halves of the next tiles of K and V to be loaded
-    int kd[2], vd[2];
+    Ka4At kc[2], vc[2];                            // halves of the next tiles of K and V to be loaded: their codes,
+    int kd[2], vd[2];                              // and how far behind those their scales
     Ka4K k0, k1;
     Ka4V v0, v1;
 
@@ -279,46 +282,54 @@ struct Ka4Walk {
     __device__ __forceinline__ void look_up(const KaItem& it, int i, int lane) {
         id = it.table[min(max(half_of(i, lane) >> lg, lo), hi)];
     }
-    // The next tile's place: its lanes' words as scalars, so that a load is one instruction of scalars and an offset.
+    // The next tile's place: its lanes' words as scalars.
     __device__ __forceinline__ void place(const KaArgs& a, const KaItem& it, int i, int lane) {
         if ((i & 31) == 0) {
-            const int t = half_of(i, lane), at = t & mask;
+            const int t = half_of(i, lane);
             const bool ok = (unsigned)id < (unsigned)a.c.n_pages;
             if (__any(!ok))
                 bad_at = min(bad_at, ka_wave_min(ok ? INT_MAX : max(min(max(t, it.k0), it.k1 - 1) & -16, it.k0)));
-            off = (uint64_t)(ok ? (uint32_t)id : 0u) * page_b + at * T::RB;
-            behind = (T::RB << lg) - at * (T::RB - 1);
+            base = (uint64_t)(uintptr_t)kb + (uint64_t)(ok ? (uint32_t)id : 0u) * page_b + (t & mask) * T::RB;
             if (i + 32 < count) look_up(it, i + 32, lane);
         }
+        const int t = first + min(i, count - 1) * (KA4_WAVES * KA4_TILE);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             const int l = 2 * (i & 31) + h;
-            const uint64_t o = (uint32_t)__builtin_amdgcn_readlane((int)off, l) |
-                               (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), l) << 32;
-            kc[h] = kb + o;
-            vc[h] = vb + o;
-            kd[h] = vd[h] = __builtin_amdgcn_readlane(behind, l);
+            kc[h] = (Ka4At)(uintptr_t)((uint32_t)__builtin_amdgcn_readlane((int)base, l) |
+                                             (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(base >> 32), l) << 32);
+            vc[h] = kc[h] + plane;
+            kd[h] = vd[h] = (T::RB << lg) - ((t + 16 * h) & mask) * (T::RB - 1);
         }
     }
+    // (opaque where they are used: a load is then one instruction, of scalars and an offset)
+    __device__ __forceinline__ static uint32_t here(uint32_t offset) {
+        asm volatile("" : "+v"(offset));
+        return offset;
+    }
     __device__ __forceinline__ void load_k(Ka4K& to) {
+        const uint32_t o = here(ko);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             // (past the caches where the keys are read once: 3 sequences of 120,000 36.4 us, so 32.9. V's rows, whose lines
             // two loads share, are not: 35.1)
-            if constexpr (ONCE) to.k[h] = __builtin_bit_cast(uint4, __builtin_nontemporal_load((const ka4_u4*)(kc[h] + ko)));
-            else to.k[h] = *(const uint4*)(kc[h] + ko);
-            to.ks[h] = *(const uint8_t*)(kc[h] + kd[h] + kso);
+            if constexpr (ONCE)
+                to.k[h] = __builtin_nontemporal_load((const __attribute__((address_space(1))) ka4_u4*)(kc[h] + o));
+            else
+                to.k[h] = ka4_get<ka4_u4>(kc[h] + o);
+            to.ks[h] = ka4_get<uint8_t>(kc[h] + here(kso + kd[h]));
         }
     }
     __device__ __forceinline__ void load_v(Ka4V& to) {
+        const uint32_t o = here(vo);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if constexpr (D == 128) to.v[4 * h + i] = *(const uint32_t*)(vc[h] + vo + i * T::RB);
-                else to.v[4 * h + i] = *(const uint16_t*)(vc[h] + vo + i * T::RB);
+                if constexpr (D == 128) to.v[4 * h + i] = ka4_get<uint32_t>(vc[h] + o + i * T::RB);
+                else to.v[4 * h + i] = ka4_get<uint16_t>(vc[h] + o + i * T::RB);
             }
-            to.vs[h] = *(const uint32_t*)(vc[h] + vd[h] + vso);
+            to.vs[h] = ka4_get<uint32_t>(vc[h] + here(vso + vd[h]));
         }
     }
     // The first tiles' loads, if the wave has any.
@@ -328,8 +339,8 @@ struct Ka4Walk {
         mask = c.page_size - 1;
         const int64_t head = (int64_t)c.page_size * (D / 32 * 17);
         page_b = (uint32_t)(head * c.n_kv_heads);
-        kb = (const char*)c.kv + (int64_t)2 * a.layer * c.n_pages * page_b + it.g * head;
-        vb = kb + (int64_t)c.n_pages * page_b;
+        plane = (int64_t)c.n_pages * page_b;
+        kb = (const char*)c.kv + 2 * a.layer * plane + it.g * head;
         first = (it.k0 & -KA4_TILE) + w * KA4_TILE;
         lo = it.k0 >> lg;
         hi = max(it.k1 - 1, 0) >> lg;
@@ -356,7 +367,7 @@ struct Ka4Walk {
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int t = 0; t < 2; t++) {
-                const ka4_i8 kt = {(int)k.k[t].x, (int)k.k[t].y, (int)k.k[t].z, (int)k.k[t].w, 0, 0, 0, 0};
+                const ka4_i8 kt = {(int)k.k[t][0], (int)k.k[t][1], (int)k.k[t][2], (int)k.k[t][3], 0, 0, 0, 0};
                 ka_f4 acc = x[c].ref;
 #pragma unroll
                 for (int m = T::QM - 1; m >= 0; m--) {             // the small parts first
