@@ -748,6 +748,7 @@ constexpr float KA4_FIXED = 4.f;
 // Rounds of a run, at least, where a table row has no more for the most runs: below, what a wave saves is
 // less than what the join costs.
 constexpr int KA4_LEAST = 4;
+constexpr int KA4_RUN = 8192;
 
 // Items for the matrix core kernels.
 static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
@@ -770,7 +771,12 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
         a.pre_tiles = ceil_div(cols, width);
         const int64_t pre_units = (int64_t)Hk * a.pre_tiles, rounds = ceil_div(a.shared, KA_ROUND);
         const int64_t most = a.slots / pre_units;
-        const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most)});
+        // As many runs as fill the device, a quarter of that where the prefix is short (the tails need some of it), and
+        // none longer than KA4_RUN keys where several column tiles read them: an XCD's workgroups then stay within what
+        // its L2 holds (and no more of these than 256 MB of partial results hold). 624 columns x 4 kv heads over 96,000
+        // tokens 185 us, 240 in longer runs; over 48,000 the same, in runs of 6,144 83 -> 93.
+        const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most),
+                                                  a.pre_tiles > 1 ? std::min<int64_t>(ceil_div(a.shared, KA4_RUN), (256 << 20) / part) : 1});
         a.pre_keys = (int)ceil_div(rounds, std::min(splits, rounds)) * KA_ROUND;
         a.pre_splits = ceil_div(a.shared, a.pre_keys);
         a.pre_work = (float)pre_units * (a.pre_splits * a.fixed + rounds);

@@ -213,8 +213,13 @@ class Cache4(Cache):
     def rows(self, layer, s, upto):
         t = np.arange(upto)
         page = self.table[s, t // self.P]
-        v = self.values() if upto else np.zeros((layer + 1, 2, 1, self.kv.shape[3], self.P, self.D))
-        return v[layer, 0, page, :, t % self.P], v[layer, 1, page, :, t % self.P]
+        codes, scales = self.blocks()
+        out = []
+        for kind in range(2):
+            c = codes[layer, kind, page, :, t % self.P]
+            code = np.stack([c & 15, c >> 4], -1).reshape(*c.shape[:-1], self.D)
+            out.append(mx4_decode(code, scales[layer, kind, page, :, :, t % self.P]))
+        return tuple(out)
 
 
 def verify(target, draft, ids, u, u_next, row_start):

@@ -423,3 +423,259 @@ def test_attention_bad_pages(torch, ops, D, x):
     torch.cuda.synchronize()
     _attend(p, torch, ops, 0, [1], [0, 1], q, 0.2, 0, 1)
     ops.kv_status(p.c)
+
+
+def _bytes(rng, shape_layers, heads, dim, page, pages):
+    """Bytes of a cache of normal values, as a server's would be, without the oracle's token by token."""
+    ref = kv_ref.Cache4(shape_layers, heads, dim, page, pages, 1, 1)
+    codes, scales = ref.blocks()
+    codes[:] = rng.integers(0, 256, codes.shape)
+    scales[:] = rng.integers(120, 130, scales.shape)
+    return ref.kv
+
+
+def _held(torch, ops, rng, lens, Hk, D, page, common=0, spare=3, order=None):
+    """Sequences 0 .. n - 1 of random contents, with their first `common` pages the same."""
+    need = [-(-k // page) for k in lens]
+    pages = common + sum(max(0, k - common) for k in need) + spare
+    p = Pair4(torch, ops, 1, Hk, D, page, pages, len(lens), max(need) + 1)
+    p.ref.kv = _bytes(rng, 1, Hk, D, page, pages)
+    free = [int(x) for x in rng.permutation(pages)]
+    shared = [free.pop() for _ in range(common)]
+    for s, (k, n) in enumerate(zip(need, lens)):
+        p.ref.table[s, :k] = (shared + [free.pop() for _ in range(k - common)]) if k > common else shared[:k]
+        p.ref.lens[s] = n
+    for x in p.ref.table[p.ref.table >= 0]:
+        p.ref.refs[x] += 1
+    p.upload()
+    for dev, ref in ((p.table, p.ref.table), (p.lens, p.ref.lens), (p.refs, p.ref.refs)):
+        dev.copy_(torch.from_numpy(ref))
+    torch.cuda.synchronize()
+    return p
+
+
+def _compare(p, torch, ops, seq, counts, H, D, x, rng, shared, window, most=None):
+    """Attention of a batch against the oracle; `most`: of so many of its requests only."""
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+    q = rng.standard_normal((int(start[-1]), H, D)).astype(x)
+    got = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, window)
+    again = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, window)
+    assert np.array_equal(got, again)
+    for i in (range(len(seq)) if most is None else rng.permutation(len(seq))[:most]):
+        rows = slice(start[i], start[i + 1])
+        one = [0, counts[i]]
+        ref = p.ref.attention(0, [seq[i]], one, q[rows], D ** -0.5, np.zeros(q[rows].shape))
+        tol = _tolerance(p, 0, [seq[i]], one, q[rows], D ** -0.5, x == "float16")
+        assert np.abs(got[rows].astype(np.float64) - ref).max(initial=0) <= tol
+    ops.kv_status(p.c)
+    return q, got
+
+
+@pytest.mark.parametrize("n,x,D", [(64, "float16", 128), (65, "float32", 64), (256, "float16", 64), (257, "float32", 128),
+                                   (700, "float16", 128)])
+def test_attention_many_requests(torch, ops, n, x, D):
+    """As many requests as a wave finds on its own, and one more; ragged lengths, empty requests among them, windows
+    longer than announced."""
+    _say(f"{n} requests {x} D{D}")
+    rng = np.random.default_rng(n)
+    lens = [int(k) for k in np.exp(rng.uniform(0, np.log(600), n))]
+    p = _held(torch, ops, rng, lens, 2, D, 16)
+    seq = [int(s) for s in rng.permutation(n)]
+    counts = [int(rng.integers(0, min(4, lens[s]) + 1)) for s in seq]
+    for window in (1, 4):
+        _compare(p, torch, ops, seq, counts, 14, D, x, rng, 0, window, 60)
+
+
+@pytest.mark.parametrize("H,Hk,D,page,x,tail,window,shared", [
+    (8, 1, 128, 16, "float16", 20011, 1, 0),        # runs of one sequence, over one kv head
+    (8, 1, 128, 128, "float32", 20011, 2, 0),
+    (8, 4, 64, 64, "float16", 9973, 5, 0),
+    (16, 2, 128, 32, "float16", 37, 3, 12320),      # a long prefix of many columns
+    (16, 2, 64, 16, "float32", 700, 1, 17001),
+    (24, 2, 128, 16, "float32", 3, 7, 2999),        # rows that stand inside the prefix
+])
+def test_attention_long(torch, ops, H, Hk, D, page, x, tail, window, shared):
+    """Many tiles of a wave, more than one load of page ids holds, and runs that are joined."""
+    _say(f"long H{H}/{Hk} D{D} page {page} {x} {shared} + {tail}")
+    rng = np.random.default_rng(tail)
+    n = 1 if not shared else 12
+    lens = [shared + max(1, tail - 11 * i) for i in range(n)]
+    p = _held(torch, ops, rng, lens, Hk, D, page, shared // page)
+    if shared % page:                               # the prefix's last tokens lie in a page of each one's own
+        codes, scales = p.ref.blocks()
+        at, k = p.ref.table[:, shared // page], shared % page
+        codes, scales = codes.copy(), scales.copy()
+        for s in range(1, n):
+            codes[:, :, at[s], :, :k] = codes[:, :, at[0], :, :k]
+            scales[:, :, at[s], :, :, :k] = scales[:, :, at[0], :, :, :k]
+        p.ref.kv = np.concatenate([codes.reshape(*codes.shape[:4], -1), scales.reshape(*scales.shape[:4], -1)],
+                                  4).reshape(p.ref.kv.shape)
+        p.upload()
+    seq = [int(s) for s in rng.permutation(n)]
+    counts = [min(window, lens[s]) for s in seq]
+    q, got = _compare(p, torch, ops, seq, counts, H, D, x, rng, shared, window, 5)
+    if shared:
+        assert np.abs(_attend(p, torch, ops, 0, seq, np.concatenate([[0], np.cumsum(counts)]), q, D ** -0.5, 0, 1)
+                      .astype(np.float64) - got).max() <= 2 * _tolerance(p, 0, seq[:1], [0, 1], q[:1], D ** -0.5, x == "float16")
+
+
+def test_far_pages(torch, ops):
+    """Pages beyond 4 GB: the same tokens there and in a small cache, written, read and attended to."""
+    rng = np.random.default_rng(11)
+    Hk, D, page = 8, 128, 64
+    pages = (5 << 30) // (Hk * page * 68)           # of each of k and v
+    small = Pair4(torch, ops, 1, Hk, D, page, 8, 2, 8)
+    far = torch.empty((1, 2, pages, Hk, page, 68), dtype=torch.uint8, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, lens, refs = torch.full((2, 8), -1, **i32), torch.zeros(2, **i32), torch.ones(pages, **i32)
+    ids = [pages - 1, pages // 2, pages - 7, 3]
+    refs[ids] = 0
+    c = ops.KvCache(far, table, lens, refs)
+    n = 200
+    small.reserve([0], [n])
+    torch.cuda.synchronize()
+    ops.kv_reserve(c, small.ints([0]), small.ints([n]), 1)
+    torch.cuda.synchronize()
+    assert sorted(table[0, :4].tolist()) == sorted(ids)
+    k, v = (rng.standard_normal((1, n, Hk, D)).astype(np.float32) for _ in range(2))
+    small.write(0, [0], [0, n], k, v)
+    ops.kv_write(c, 0, 1, small.ints([0]), small.ints([0, n]), 1, small.dev(k), small.dev(v), n)
+    small.same()
+    back = small.read(0, 1, [0], [0, n], None, torch.float32)
+    kb, vb = (torch.zeros(n * Hk * D, device="cuda") for _ in range(2))
+    torch.cuda.synchronize()
+    ops.kv_read(c, 0, 1, small.ints([0]), small.ints([0, n]), 1, kb, vb, n)
+    torch.cuda.synchronize()
+    assert np.array_equal(kb.cpu().numpy(), back[0]) and np.array_equal(vb.cpu().numpy(), back[1])
+    for x in ("float32", "float16"):
+        q = rng.standard_normal((3, 16, D)).astype(x)
+        want = _attend(small, torch, ops, 0, [0], [0, 3], q, 0.1, 0, 3)
+        qd = small.dev(q)
+        out = torch.zeros_like(qd)
+        torch.cuda.synchronize()
+        ops.kv_attention(c, 0, small.ints([0]), small.ints([0, 3]), 1, qd, out, 3, 16, 0.1, max_rows=3)
+        torch.cuda.synchronize()
+        assert np.array_equal(out.cpu().numpy(), want)
+    ops.kv_status(c)
+    c.close()
+
+
+def test_refused_writes(torch, ops):
+    """What kv_write refuses of other caches it refuses here: rows in shared pages, one sequence twice, tokens that a
+    refused reserve did not make room for."""
+    rng = np.random.default_rng(12)
+    p = Pair4(torch, ops, 2, 2, 64, 16, 9, 6, 4)
+    p.add(rng, [0], [20])
+    p.fork([0], [1])
+    k, v = (p.dev(rng.standard_normal((2, 8, 2, 64)).astype(np.float32)) for _ in range(2))
+    ops.kv_write(p.c, 0, 2, p.ints([1]), p.ints([0, 4]), 1, k, v, 8)
+    p.same()
+    with pytest.raises(ops.RocmError, match="several sequences hold"):
+        ops.kv_status(p.c)
+    p.reserve([2, 3], [3, 3])
+    ops.kv_write(p.c, 0, 2, p.ints([2, 3, 2]), p.ints([0, 3, 6, 8]), 3, k, v, 8)
+    kn, vn = k.cpu().numpy(), v.cpu().numpy()
+    p.ref.write(0, [2, 3], [0, 3, 6], kn, vn)
+    p.same()
+    with pytest.raises(ops.RocmError, match="twice"):
+        ops.kv_status(p.c)
+    with pytest.raises(kv_ref.Refused):
+        p.ref.reserve([2, 4], [1, 200])
+    ops.kv_reserve(p.c, p.ints([2, 4]), p.ints([1, 200]), 2)
+    ops.kv_write(p.c, 0, 2, p.ints([2]), p.ints([0, 1]), 1, k, v, 8)
+    p.same()
+    with pytest.raises(ops.RocmError, match="too short table rows"):
+        ops.kv_status(p.c)
+
+
+def test_serving(torch, ops):
+    """Prompt, forks, steps of ragged windows over two layers, drops and compaction, as a server would."""
+    rng = np.random.default_rng(13)
+    layers, Hk, H, D, page = 2, 2, 8, 128, 16
+    p = Pair4(torch, ops, layers, Hk, D, page, 60, 9, 12)
+    p.add(rng, [0], [70])
+    p.fork([0] * 4, [1, 2, 3, 4])
+    for step in range(6):
+        seq = [int(s) for s in 1 + rng.permutation(4)]
+        count = [int(k) for k in rng.integers(1, 6, 4)]
+        p.reserve(seq, count)
+        start = np.concatenate([[0], np.cumsum(count)]).astype(int)
+        rows = int(start[-1])
+        k, v = (rng.standard_normal((layers, rows, Hk, D)).astype(np.float32) for _ in range(2))
+        for layer in range(layers):
+            p.write(layer, seq, start, k[layer:layer + 1], v[layer:layer + 1])
+            q = rng.standard_normal((rows, H, D)).astype(np.float32)
+            got = _attend(p, torch, ops, layer, seq, start, q, D ** -0.5, 70, max(count))
+            ref = p.ref.attention(layer, seq, start, q, D ** -0.5, np.zeros(q.shape))
+            assert np.abs(got - ref).max() <= _tolerance(p, layer, seq, start, q, D ** -0.5, False)
+        p.drop(seq, [int(rng.integers(0, c)) for c in count])
+        if step % 2:
+            p.compact()
+        p.same()
+    ops.kv_status(p.c)
+
+
+class Step4:
+    """One step of a server over a cache of 4 bits of its own: room, write, attention, read back, drop."""
+
+    def __init__(self, torch, ops, seed):
+        self.t, self.ops, self.rng = torch, ops, np.random.default_rng(seed)
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.kv = torch.zeros((2, 2, 40, 2, 16, 68), dtype=torch.uint8, device="cuda")
+        self.table, self.lens, self.refs = torch.full((5, 12), -1, **i32), torch.zeros(5, **i32), torch.zeros(40, **i32)
+        self.c = ops.KvCache(self.kv, self.table, self.lens, self.refs)
+        self.seq = torch.tensor([3, 0, 4], **i32)
+        self.count, self.start = torch.tensor([2, 1, 3], **i32), torch.tensor([0, 2, 3, 6], **i32)
+        self.back = torch.tensor([1, 0, 2], **i32)
+        self.k, self.v = (torch.zeros((2, 6, 2, 128), device="cuda") for _ in range(2))
+        self.q, self.out = (torch.zeros((6, 8, 128), device="cuda") for _ in range(2))
+        self.kb, self.vb = (torch.zeros((2, 6, 2, 128), device="cuda", dtype=torch.float16) for _ in range(2))
+
+    def fill(self, rng):
+        for t in (self.k, self.v, self.q):
+            t.copy_(self.t.from_numpy(rng.standard_normal(tuple(t.shape)).astype(np.float32)))
+
+    def run(self, stream=None):
+        o, c = self.ops, self.c
+        o.kv_reserve(c, self.seq, self.count, 3, stream=stream)
+        o.kv_write(c, 0, 2, self.seq, self.start, 3, self.k, self.v, 6, stream=stream)
+        o.kv_attention(c, 1, self.seq, self.start, 3, self.q, self.out, 6, 8, 0.09, max_rows=3, stream=stream)
+        o.kv_read(c, 0, 2, self.seq, self.start, 3, self.kb, self.vb, 6, stream=stream)
+        o.kv_drop(c, self.seq, self.back, 3, stream=stream)
+
+    def state(self):
+        return [t.clone() for t in (self.kv, self.table, self.lens, self.refs, self.out, self.kb, self.vb)]
+
+
+def _same_steps(torch, steps):
+    torch.cuda.synchronize()
+    first = steps[0].state()
+    for s in steps[1:]:
+        for a, b in zip(first, s.state()):
+            assert torch.equal(a, b)
+
+
+def test_captured_step(torch, ops):
+    """A step captured into a graph of torch's, replayed with new inputs between eager ones on two streams."""
+    eager, captured, other = (Step4(torch, ops, s) for s in (1, 1, 1))
+    torch.cuda.synchronize()
+    graphs, streams = [], [torch.cuda.Stream() for _ in range(2)]
+    for s, st in zip((captured, other), streams):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            s.run(st)
+        graphs.append(g)
+    torch.cuda.synchronize()
+    for step in range(12):
+        for s in (eager, captured, other):
+            s.fill(np.random.default_rng(100 + step))
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):          # at once, each with its own workspaces
+            with torch.cuda.stream(st):
+                g.replay()
+        eager.run()
+        _same_steps(torch, (eager, captured, other))
+    assert eager.lens.tolist() == [12, 0, 0, 12, 12] and float(eager.out.abs().sum()) > 0
+    for s in (eager, captured, other):
+        ops.kv_status(s.c)
+    graphs.clear()
