@@ -9,7 +9,8 @@
 namespace pio {
 
 // Head dimensions other than 64 and 128. One workgroup per (row, head): 256 keys at a time, a thread
-// for each key's score, then a thread for each dimension of the weighted sum.
+// for each key's score, then a thread for each dimension of the weighted sum, KA4_DEEP values in flight; bound by the
+// waits for them (where the matrix core kernels run, 128 dimensions: 40 sequences behind a prompt 273 us, there 15.6).
 constexpr int KA4_DEEP = 8;
 __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
     __shared__ float qs[256], ps[KA_THREADS], red[4];
@@ -122,6 +123,13 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 //   O^T = V^T P^T on v_mfma_f32_16x16x32_f16. Lane l reads the codes of 8 keys and dimensions D / 16 (l % 16) ..,
 //     and widens each key's to fp16 under its scale, exactly: two keys' halves side by side are the operand, so
 //     V is turned inside a lane. Row i of O^T tile n is dimension (D / 16) i + n.
+// What it costs (2.4 GHz): an item's chain of waits (its request, page ids, K, the join) is 16,000 clocks, most of
+// them loads on loads and code that is fetched for the first time; a tile of 32 keys and 16 columns some 1,100 clocks
+// of a SIMD's issue, whatever the order: products and the VALU's work were measured to add up, also where two waves
+// share the SIMD. Long tails are bound by memory: 3 sequences of 120,000 tokens (8 kv heads x 128, fp16) 28 us, 4.7
+// TB/s; many columns by instructions: 624 over 24,000 tokens 50 us, 620 TFLOP/s. Tried and no faster: the workgroup's
+// waves on columns of their own around V widened once in LDS (64 us), K and V one more tile ahead (+2 us), 3 waves to
+// a SIMD of 16 columns (168 registers, +5 us), products and VALU interleaved by hand, wave priorities.
 //   A lane's 8 scores are of the keys 4 q .. 4 q + 3 of either 16, q = l / 16, and those are the keys of its part of
 //     the weights' operand; V's rows are read in that order.
 typedef int ka4_i8 __attribute__((ext_vector_type(8)));
@@ -629,7 +637,8 @@ __device__ __forceinline__ int ka4_scan(int x) {
 }
 
 // ka_runs for up to 64 N requests, by each wave on its own: no LDS and no barriers, and what is found is the same
-// for the wave's lanes as the compiler sees it, so that page ids are scalar loads.
+// for the wave's lanes as the compiler sees it. 1 sequence 8.9 us (by the workgroup 9.8), 40 behind a prompt 15.6
+// (17.0), 200 of up to 300 tokens 18.3 (17.8); more would cost registers.
 template <int N>
 __device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found, int cols) {
     const int lane = threadIdx.x & 63;
@@ -730,8 +739,8 @@ static int ka4_launch(const KaArgs& a, hipStream_t st) {
 }
 template <int D>
 static int ka4_route(const KaArgs& a, int nc, hipStream_t st) {
-    if (a.q16) return nc == 1 ? ka4_launch<D, true, 1>(a, st) : ka4_launch<D, true, 2>(a, st);
-    return nc == 1 ? ka4_launch<D, false, 1>(a, st) : ka4_launch<D, false, 2>(a, st);
+    if (!a.q16) return ka4_launch<D, false, 1>(a, st);
+    return nc == 1 ? ka4_launch<D, true, 1>(a, st) : ka4_launch<D, true, 2>(a, st);
 }
 template <int D>
 static int ka4_join(const KaArgs& a, hipStream_t st) {
@@ -743,11 +752,13 @@ static int ka4_join(const KaArgs& a, hipStream_t st) {
     return PIO_OK;
 }
 
-// An item costs its rounds of keys and this many more.
+// An item costs its rounds of keys and this many more (2 to 12 make no difference but where the device is not full:
+// 40 sequences behind a prompt 15.6 us, with 2 19.0, with 8 16.0).
 constexpr float KA4_FIXED = 4.f;
-// Rounds of a run, at least, where a table row has no more for the most runs: below, what a wave saves is
-// less than what the join costs.
+// Rounds of a run at least, as a table row's pages allow: below, what the waves save is less than what the join costs.
+// Rows of 512 keys or less need none: 1 sequence of 301 tokens 8.9 us, in runs of a round 10.1.
 constexpr int KA4_LEAST = 4;
+// Keys of a prefix's run at most (below).
 constexpr int KA4_RUN = 8192;
 
 // Items for the matrix core kernels.
@@ -755,11 +766,21 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
     const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
     a.fixed = KA4_FIXED;
-    const int nc = tail_cols > 16 ? 2 : 1, width = 16 * nc, held = 2;
+    a.slots = 2 * cus;                             // two workgroups to a CU
+    // Items of 32 columns widen V once for both their tiles, and halve what crosses from L2; items of 16 are twice as
+    // many. fp16 queries, 8 heads to each of 4 kv heads of 128: 40 windows of 3 behind 24,000 tokens 50 us (16 columns:
+    // 86), 24 behind 12,000 33 (36), behind 6,000 24.5 (24.7), behind 2,000 18.5 (14.7), over 3,000 own tokens 15.2
+    // (12.4); 4 windows of 100 over those 33 (29); two prompts of 509 over 4,090, 4 heads to each of 8, 54 (71). fp32
+    // queries, whose parts and weights need the registers, were 6 % faster at those prompts and slower at all others.
+    // Of 64 dimensions, 7 heads to each of 2 kv heads, 24 windows over up to 2,100 tokens: of 3 14.4 us (12.5), of 6
+    // 15.7 (17.3), of 12 17.5 (20.6), 8 of 40 23.0 (21.4).
+    const bool many = cols * Hk > 16 * a.slots || (double)cols * Hk * a.shared * a.c.head_dim >= 0x1p30;
+    const bool small = a.c.head_dim == 64 && tail_cols > 32 && tail_cols <= 128;
+    const int nc = a.q16 && tail_cols > 16 && (many || small) ? 2 : 1;
+    const int width = 16 * nc;
     a.tail_tiles = ceil_div(tail_cols, width);
     PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);
     const int64_t items = std::min((int64_t)a.n * a.tail_tiles, cols / width + a.n) * Hk;
-    a.slots = cus * held;
     const int64_t units = (int64_t)Hk * a.tail_tiles;
     a.tail_runs = (int)std::max<int64_t>(1, a.slots / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);

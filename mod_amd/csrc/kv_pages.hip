@@ -415,7 +415,8 @@ typedef uint32_t KvU4 __attribute__((ext_vector_type(4)));
 // then moves k and v in pieces of 8 elements. Bytes bound it: 336 rows of 28 layers,
 // fp32 to fp16, 32 us, 3.5 TB/s; few rows, the chain of loads that says where a row goes
 // and whether it may: 8 rows of one layer 4.3 us, 3.6 without its checks. In 4 bits the four
-// threads of a block of 32 values share its largest magnitude.
+// threads of a block of 32 values share its largest magnitude; 3,941 rows of 28 layers of 8 x 128, fp16, 113 us,
+// 5.1 TB/s (150 with loads through the caches).
 template <typename XT, typename KT>
 __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int layer, int layers,
                                                           const int32_t* __restrict__ seq,
@@ -531,7 +532,9 @@ __global__ __launch_bounds__(KV_COPY) void kv_write_kernel(pio_kv_cache c, int l
 }
 
 // ------------------------------------------------------------------ read ----
-// The way back: a workgroup takes one row through a few layers, in pieces of 8 elements.
+// The way back: a workgroup takes one row through a few layers, in pieces of 8 elements. Bytes bound it: 1,805 rows of
+// 28 layers of 8 x 128 out of 4 bits to fp16 40 us, 6.5 TB/s (67 with stores through the caches; some pages are in the
+// memory-side cache).
 template <typename KT, typename YT>
 __global__ __launch_bounds__(KV_COPY) void kv_read_kernel(pio_kv_cache c, int layer, int layers,
                                                          const int32_t* __restrict__ seq,
