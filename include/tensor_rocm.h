@@ -441,7 +441,7 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * parts of a row that are computed apart (runs of its own tokens, of the shared
  * ones) meet in a workspace, rows * n_heads * (head_dim + 2) * 4 bytes each: up to
  * 256 MB for its own tokens or one part, whichever is more, and the shared ones'
- * on top (one part where rows are many). */
+ * on top (one part where rows are many; over 4 bits, up to 256 MB). */
 int pio_kv_attention(const pio_kv_cache* cache, int layer, const int32_t* seq, const int32_t* row_start, int n,
                      int shared, const void* q, void* out, int dtype, int rows, int n_heads, int64_t q_stride,
                      int64_t out_stride, int max_rows, float scale, void* stream);
