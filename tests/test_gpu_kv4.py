@@ -342,6 +342,40 @@ def test_attention_masked_places(torch, ops, x, D):
     ops.kv_status(p.c)
 
 
+@pytest.mark.parametrize("D,H,rows,tokens", [(128, 32, 300, 300), (64, 32, 300, 333), (64, 14, 8, 100), (128, 32, 300, 290)])
+def test_attention_masked_columns(torch, ops, D, H, rows, tokens):
+    """Items of 32 columns: NaN blocks of values and keys, and what lies behind the end, reach the rows that see them alone;
+    more rows than tokens."""
+    _say(f"masked columns D{D} {rows} rows of {tokens}")
+    rng = np.random.default_rng(D + rows)
+    p = _held(torch, ops, rng, [tokens, 70], 2, D, 16)
+    codes, scales = p.ref.blocks()
+    scales = scales.copy()
+    for kind, pos, block in ((1, tokens - 5, 1), (0, tokens - 2, 0), (1, tokens - 1, 0)):
+        scales[0, kind, p.ref.table[0, pos // 16], :, block, pos % 16] = 255
+    end = p.ref.table[0, (tokens - 1) // 16]
+    if tokens % 16:
+        scales[0, :, end, :, :, tokens % 16:] = rng.choice([0, 200, 255], scales[0, :, end, :, :, tokens % 16:].shape)
+    p.ref.kv = np.concatenate([codes.reshape(*codes.shape[:4], -1), scales.reshape(*scales.shape[:4], -1)],
+                              4).reshape(p.ref.kv.shape)
+    p.upload()
+    q = rng.standard_normal((rows + 2, H, D)).astype(np.float16)
+    seq, start = [0, 1], [0, rows, rows + 2]
+    ref = p.ref.attention(0, seq, start, q, D ** -0.5, np.zeros(q.shape))
+    assert np.isnan(ref[rows - 1]).all() and np.isnan(ref[rows - 5, :, 32:64]).all() and np.isfinite(ref[rows - 5, :, :32]).all()
+    tol = _tolerance(p, 0, seq, start, q, D ** -0.5, True)
+    for shared in (0, 64):
+        if shared:
+            p.table[1] = p.table[0]                 # one prefix, and the tokens behind it
+            p.ref.table[1] = p.ref.table[0]
+            torch.cuda.synchronize()
+            ref = p.ref.attention(0, seq, start, q, D ** -0.5, np.zeros(q.shape))
+        got = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, rows).astype(np.float64)
+        fine = np.isfinite(ref)
+        assert np.array_equal(np.isfinite(got), fine) and np.abs(got[fine] - ref[fine]).max() <= tol
+    ops.kv_status(p.c)
+
+
 @pytest.mark.parametrize("x", ["float32", "float16"])
 @pytest.mark.parametrize("D", [64, 128, 32])
 def test_queries_of_any_size(torch, ops, x, D):
@@ -493,6 +527,10 @@ def test_attention_many_requests(torch, ops, n, x, D):
     (16, 2, 128, 32, "float16", 37, 3, 12320),      # a long prefix of many columns
     (16, 2, 64, 16, "float32", 700, 1, 17001),
     (24, 2, 128, 16, "float32", 3, 7, 2999),        # rows that stand inside the prefix
+    (32, 4, 128, 32, "float16", 37, 3, 12320),      # items of 32 columns, for a prefix and for a prompt
+    (32, 4, 128, 16, "float16", 2, 4, 17003),
+    (32, 2, 128, 16, "float16", 313, 300, 0),
+    (32, 2, 64, 64, "float16", 1313, 300, 0),
 ])
 def test_attention_long(torch, ops, H, Hk, D, page, x, tail, window, shared):
     """Many tiles of a wave, more than one load of page ids holds, and runs that are joined."""
@@ -558,6 +596,24 @@ def test_far_pages(torch, ops):
         assert np.array_equal(out.cpu().numpy(), want)
     ops.kv_status(c)
     c.close()
+
+
+def test_write_leaves_the_rest(torch, ops):
+    """Strided rows and layers, rows behind the last request, a layer in the middle."""
+    rng = np.random.default_rng(14)
+    p = Pair4(torch, ops, 3, 2, 32, 16, 12, 4, 3, fill=0)
+    p.reserve([3, 1], [21, 7])
+    start = [0, 19, 24]                             # the last 19 of 21, and 5 of 7
+    k, v = (rng.standard_normal((2, 27, 80)).astype(np.float32) for _ in range(2))
+    k[:, 24:], v[:, 24:] = np.nan, np.nan
+    for row_stride, layer_stride in ((80, 27 * 80), (160, 80)):
+        a, b = ((x if layer_stride > 80 else np.ascontiguousarray(x.transpose(1, 0, 2))) for x in (k, v))
+        ops.kv_write(p.c, 1, 2, p.ints([3, 1]), p.ints(start), 2, p.dev(a), p.dev(b), 27, row_stride=row_stride,
+                     layer_stride=layer_stride)
+        p.ref.write(1, [3, 1], start, *(x[:, :, :64].reshape(2, 27, 2, 32) for x in (k, v)))
+        p.same()
+        k, v = k * 3, v * 0.1
+    ops.kv_status(p.c)
 
 
 def test_refused_writes(torch, ops):
