@@ -752,9 +752,10 @@ static int ka4_join(const KaArgs& a, hipStream_t st) {
     return PIO_OK;
 }
 
-// An item costs its rounds of keys and this many more (2 to 12 make no difference but where the device is not full:
-// 40 sequences behind a prompt 15.6 us, with 2 19.0, with 8 16.0).
-constexpr float KA4_FIXED = 4.f;
+// An item costs its rounds of keys and this many more. A small figure cuts long rows into more runs than pay for their
+// join: 32 sequences of up to 16,000 tokens 19.9 us with 4, 17.0 with 6, 17.1 with 8, and 96 of them 43.0 us with any of
+// these; with 2, 40 sequences behind a prompt 19.0 us against 15.5.
+constexpr float KA4_FIXED = 6.f;
 // Rounds of a run at least, as a table row's pages allow: below, what the waves save is less than what the join costs.
 // Rows of 512 keys or less need none: 1 sequence of 301 tokens 8.9 us, in runs of a round 10.1.
 constexpr int KA4_LEAST = 4;
