@@ -726,7 +726,11 @@ __global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
         for (int i = tid; i < r.r1 - r.r0; i += 64 * KA4_WAVES) a.part_n[r.r0 + i] = it.direct ? 0 : r.runs;
     // columns beyond the tiles of the grid (a request of more rows than announced): more rounds
     for (int c0 = r.ct * COLS; c0 < it.ncols; c0 += r.tiles * COLS) {
-        ka4_item<D, X16, NC, NC == 1>(a, it, lds, ml, nullptr, c0, w, lane);
+        // (opaque: else the addresses that the lane alone decides are formed ahead of the loop, and 32 columns of 128
+        // have no registers for them: their reloads put the first loads in a row, two prompts 57 us, so 55)
+        int own = lane;
+        if constexpr (NC > 1) asm volatile("" : "+v"(own));
+        ka4_item<D, X16, NC, NC == 1>(a, it, lds, ml, nullptr, c0, w, own);
         __syncthreads();                                   // its output is out of LDS
     }
 }
