@@ -170,7 +170,10 @@ __device__ __forceinline__ ka4_v32 ka4_from6(const ka4_u6& c, float scale) {
 template <int D, bool X16>
 struct Ka4Q {
     ka4_u6 p[Ka4<D, X16>::QM];
-    int e[Ka4<D, X16>::QM];
+    uint32_t e[(Ka4<D, X16>::QM + 3) / 4];         // four scales to a word
+    __device__ __forceinline__ void scale(int m, int to) {
+        e[m / 4] = (e[m / 4] & ~(255u << 8 * (m & 3))) | (uint32_t)to << 8 * (m & 3);
+    }
 };
 // Its elements as they lie in memory, loaded ahead of the keys (waits for loads are in order).
 template <bool X16>
@@ -206,6 +209,8 @@ __device__ __forceinline__ void ka4_set_q(const KaArgs& a, const Ka4Raw<X16>& ra
 #pragma unroll
         for (int i = 0; i < 16; i++) xa[i] = xb[i] = 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < (T::QM + 3) / 4; i++) q.e[i] = 0;
     // the least power of two (a byte of exponent) that the largest is below 7.5 of, with what rounds up to 8; a
     // part's rest is at most a quarter of its step's unit, or an eighth from the second part on: 4 and 5 bits
     const int first = (int)((most + 0x100000u) >> 23) - 2;
@@ -217,14 +222,14 @@ __device__ __forceinline__ void ka4_set_q(const KaArgs& a, const Ka4Raw<X16>& ra
         if (live && odd) e = KV_MX4_NAN;
         if constexpr (D == 128) {
             q.p[p] = c;
-            q.e[p] = e;
+            q.scale(p, e);
         } else if (p % 2 == 0) {
             q.p[p / 2] = c;
-            q.e[p / 2] = e;
+            q.scale(p / 2, e);
             if (half && p == T::PARTS - 1) q.p[p / 2] = ka4_u6{0, 0, 0, 0, 0, 0};
         } else if (half) {
             q.p[p / 2] = c;
-            q.e[p / 2] = e;
+            q.scale(p / 2, e);
         }
         if (p + 1 < T::PARTS) {
             const ka4_v32 y = ka4_from6(c, unit);
@@ -242,10 +247,10 @@ __device__ __forceinline__ void ka4_set_q(const KaArgs& a, const Ka4Raw<X16>& ra
 // (of the rounded weights, as O^T is), in all elements.
 template <int D>
 struct Ka4Acc {
-    float m;                       // the reference; -FLT_MAX: saw no key
     ka_f4 ref, l, o[D / 16];
+    // The reference; -FLT_MAX: saw no key (the largest weight of a tile is never lost in l).
+    __device__ __forceinline__ float m() const { return l[0] == 0.f ? -FLT_MAX : -ref[0]; }
     __device__ void clear() {
-        m = -FLT_MAX;
         ref = l = ka_f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int n = 0; n < D / 16; n++) o[n] = ka_f4{0.f, 0.f, 0.f, 0.f};
@@ -260,6 +265,31 @@ struct Ka4K {
 struct Ka4V {
     uint32_t v[8], vs[2];
 };
+
+// Sums over the lanes up to each.
+__device__ __forceinline__ int ka4_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);      // row_bcast 15, into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);      // row_bcast 31, into rows 2 and 3
+    return x;
+}
+
+// The least of the wave's.
+__device__ __forceinline__ int ka4_least(int x) {
+    auto with = [&](auto ctrl, auto rows) {
+        x = min(x, __builtin_amdgcn_update_dpp(INT_MAX, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    with(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});      // as above
+    with(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    with(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    with(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    with(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});
+    with(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});
+    return __builtin_amdgcn_readlane(x, 63);
+}
 
 // A wave's tiles, every KA4_WAVES-th. The scores run one tile ahead of the softmax, in one piece of code without
 // branches: their products fill the matrix cores while the VALU forms the weights and widens the values. K is
@@ -296,7 +326,7 @@ struct Ka4Walk {
             const int t = half_of(i, lane);
             const bool ok = (unsigned)id < (unsigned)a.c.n_pages;
             if (__any(!ok))
-                bad_at = min(bad_at, ka_wave_min(ok ? INT_MAX : max(min(max(t, it.k0), it.k1 - 1) & -16, it.k0)));
+                bad_at = min(bad_at, ka4_least(ok ? INT_MAX : max(min(max(t, it.k0), it.k1 - 1) & -16, it.k0)));
             base = (uint64_t)(uintptr_t)kb + (uint64_t)(ok ? (uint32_t)id : 0u) * page_b + (t & mask) * T::RB;
             if (i + 32 < count) look_up(it, i + 32, lane);
         }
@@ -381,7 +411,11 @@ struct Ka4Walk {
                 for (int m = T::QM - 1; m >= 0; m--) {             // the small parts first
                     const ka4_u6& p = q[c].p[m];
                     const ka4_i8 qm = {(int)p[0], (int)p[1], (int)p[2], (int)p[3], (int)p[4], (int)p[5], 0, 0};
-                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 0, q[c].e[m]);
+                    const int at = (int)q[c].e[m / 4];             // (which byte of it is in the instruction)
+                    if ((m & 3) == 0) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 0, at);
+                    if ((m & 3) == 1) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 1, at);
+                    if ((m & 3) == 2) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 2, at);
+                    if ((m & 3) == 3) acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kt, qm, acc, 4, 2, 0, k.ks[t], 3, at);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; e++) s[c][4 * t + e] = acc[e];
@@ -423,7 +457,6 @@ struct Ka4Walk {
 #pragma unroll
                 for (int n = 0; n < T::NT; n++) x[c].o[n] *= corr;
             }
-            if (sees) x[c].m = -x[c].ref[0];
 #pragma unroll
             for (int i = 0; i < 8; i++) s[c][i] += by;
         }
@@ -490,7 +523,7 @@ struct Ka4Walk {
         int least = limit[0];
 #pragma unroll
         for (int c = 1; c < NC; c++) least = min(least, limit[c]);
-        least = __builtin_amdgcn_readfirstlane(ka_wave_min(least));
+        least = ka4_least(least);
         auto begins = [&](int i) { return first + i * (KA4_WAVES * KA4_TILE); };
         const int whole = least >= first ? (least - first) / (KA4_WAVES * KA4_TILE) + (((least - first) & (KA4_WAVES * KA4_TILE - 1)) >= KA4_TILE) : 0;
         const int low = first < it.k0 ? 0 : -1;
@@ -589,14 +622,14 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
         if (c) __syncthreads();                            // the last columns are out of LDS
         const int col = lane & 15, part = lane >> 4;
         if (part == 0) {
-            ml[w][col][0] = x[c].m;
+            ml[w][col][0] = x[c].m();
             ml[w][col][1] = x[c].l[0];
         }
         __syncthreads();
         float mx = ml[0][col][0];
 #pragma unroll
         for (int i = 1; i < KA4_WAVES; i++) mx = fmaxf(mx, ml[i][col][0]);
-        const float f = __builtin_amdgcn_exp2f(x[c].m - mx);
+        const float f = __builtin_amdgcn_exp2f(x[c].m() - mx);
         float* to = lds + (w * 16 + col) * T::OP;
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -623,17 +656,6 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
             ka_emit(a, D, it, at, d, v, m, l);
         }
     }
-}
-
-// Sums over the lanes up to each.
-__device__ __forceinline__ int ka4_scan(int x) {
-    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);      // row_shr 1, 2, 4, 8
-    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
-    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);      // row_bcast 15, into rows 1 and 3
-    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);      // row_bcast 31, into rows 2 and 3
-    return x;
 }
 
 // ka_runs for up to 64 N requests, by each wave on its own: no LDS and no barriers, and what is found is the same
