@@ -127,7 +127,7 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 // them loads on loads and code that is fetched for the first time; a tile of 32 keys and 16 columns some 1,100 clocks
 // of a SIMD's issue, whatever the order: products and the VALU's work were measured to add up, also where two waves
 // share the SIMD. Long tails are bound by memory: 3 sequences of 120,000 tokens (8 kv heads x 128, fp16) 28 us, 4.7
-// TB/s; many columns by instructions: 624 over 24,000 tokens 50 us, 620 TFLOP/s. Tried and no faster: the workgroup's
+// TB/s; many columns by instructions: 624 over 24,000 tokens 48 us, 646 TFLOP/s. Tried and no faster: the workgroup's
 // waves on columns of their own around V widened once in LDS (64 us), K and V one more tile ahead (+2 us), 3 waves to
 // a SIMD of 16 columns (168 registers, +5 us), products and VALU interleaved by hand, wave priorities.
 //   A lane's 8 scores are of the keys 4 q .. 4 q + 3 of either 16, q = l / 16, and those are the keys of its part of
@@ -765,7 +765,7 @@ static int ka4_launch(const KaArgs& a, hipStream_t st) {
 }
 template <int D>
 static int ka4_route(const KaArgs& a, int nc, hipStream_t st) {
-    if (!a.q16) return ka4_launch<D, false, 1>(a, st);
+    if (!a.q16) return nc == 1 ? ka4_launch<D, false, 1>(a, st) : ka4_launch<D, false, 2>(a, st);
     return nc == 1 ? ka4_launch<D, true, 1>(a, st) : ka4_launch<D, true, 2>(a, st);
 }
 template <int D>
@@ -795,15 +795,19 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     a.fixed = KA4_FIXED;
     a.slots = 2 * cus;                             // two workgroups to a CU
     // Items of 32 columns widen V once for both their tiles, and halve what crosses from L2; items of 16 are twice as
-    // many. fp16 queries, 8 heads to each of 4 kv heads of 128: 40 windows of 3 behind 24,000 tokens 50 us (16 columns:
+    // many. fp16 queries, 8 heads to each of 4 kv heads of 128: 40 windows of 3 behind 24,000 tokens 48 us (16 columns:
     // 86), 24 behind 12,000 33 (36), behind 6,000 24.5 (24.7), behind 2,000 18.5 (14.7), over 3,000 own tokens 15.2
-    // (12.4); 4 windows of 100 over those 33 (29); two prompts of 509 over 4,090, 4 heads to each of 8, 54 (71). fp32
-    // queries, whose parts and weights need the registers, were 6 % faster at those prompts and slower at all others.
-    // Of 64 dimensions, 7 heads to each of 2 kv heads, 24 windows over up to 2,100 tokens: of 3 14.4 us (12.5), of 6
-    // 15.7 (17.3), of 12 17.5 (20.6), 8 of 40 23.0 (21.4).
-    const bool many = cols * Hk > 16 * a.slots || (double)cols * Hk * a.shared * a.c.head_dim >= 0x1p30;
-    const bool small = a.c.head_dim == 64 && tail_cols > 32 && tail_cols <= 128;
-    const int nc = a.q16 && tail_cols > 16 && (many || small) ? 2 : 1;
+    // (12.4); 4 windows of 100 over those 33 (29); two prompts of 509 over 4,090, 4 heads to each of 8, 50 (71). Of 64
+    // dimensions, 7 heads to each of 2 kv heads, 24 windows over up to 2,100 tokens: of 3 14.4 us (12.5), of 6 15.7
+    // (17.3), of 12 17.5 (20.6), 8 of 40 23.0 (21.4).
+    // fp32 queries, whose parts and weights take the registers, need more: those prompts 75 (86), over 1,000 53 (61); 24
+    // windows of up to 40, 320 columns each, over 3,000 own tokens 47 (42); of 200, 1,400 columns of 64, 143 (178). 40 windows
+    // of up to 3 behind 48,000 124 (145), 24,000 76 (111), 12,000 65 (59), 6,000 42 (42), 2,000 26 (25); 80 behind 6,000 63
+    // (85), 12,000 97 (89); 20 behind 24,000 56 (70), 48,000 94 (79); of 64 dimensions, 40 behind 24,000 58 (89).
+    const double over = (double)cols * Hk * a.shared * a.c.head_dim;
+    const bool many = a.q16 ? cols * Hk > 16 * a.slots || over >= 0x1p30 : tail_cols > 1024 || over >= 0x1p31;
+    const bool small = a.q16 && a.c.head_dim == 64 && tail_cols > 32 && tail_cols <= 128;
+    const int nc = tail_cols > 16 && (many || small) ? 2 : 1;
     const int width = 16 * nc;
     a.tail_tiles = ceil_div(tail_cols, width);
     PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);

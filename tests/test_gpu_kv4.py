@@ -342,11 +342,10 @@ def test_attention_masked_places(torch, ops, x, D):
     ops.kv_status(p.c)
 
 
-@pytest.mark.parametrize("D,H,rows,tokens", [(128, 32, 300, 300), (64, 32, 300, 333), (64, 14, 8, 100), (128, 32, 300, 290)])
-def test_attention_masked_columns(torch, ops, D, H, rows, tokens):
+def _masked_columns(torch, ops, D, H, rows, tokens, x):
     """Items of 32 columns: NaN blocks of values and keys, and what lies behind the end, reach the rows that see them alone;
     more rows than tokens."""
-    _say(f"masked columns D{D} {rows} rows of {tokens}")
+    _say(f"masked columns D{D} {rows} rows of {tokens} {x}")
     rng = np.random.default_rng(D + rows)
     p = _held(torch, ops, rng, [tokens, 70], 2, D, 16)
     codes, scales = p.ref.blocks()
@@ -359,11 +358,11 @@ def test_attention_masked_columns(torch, ops, D, H, rows, tokens):
     p.ref.kv = np.concatenate([codes.reshape(*codes.shape[:4], -1), scales.reshape(*scales.shape[:4], -1)],
                               4).reshape(p.ref.kv.shape)
     p.upload()
-    q = rng.standard_normal((rows + 2, H, D)).astype(np.float16)
+    q = rng.standard_normal((rows + 2, H, D)).astype(x)
     seq, start = [0, 1], [0, rows, rows + 2]
     ref = p.ref.attention(0, seq, start, q, D ** -0.5, np.zeros(q.shape))
     assert np.isnan(ref[rows - 1]).all() and np.isnan(ref[rows - 5, :, 32:64]).all() and np.isfinite(ref[rows - 5, :, :32]).all()
-    tol = _tolerance(p, 0, seq, start, q, D ** -0.5, True)
+    tol = _tolerance(p, 0, seq, start, q, D ** -0.5, x == "float16")
     for shared in (0, 64):
         if shared:
             p.table[1] = p.table[0]                 # one prefix, and the tokens behind it
@@ -374,6 +373,16 @@ def test_attention_masked_columns(torch, ops, D, H, rows, tokens):
         fine = np.isfinite(ref)
         assert np.array_equal(np.isfinite(got), fine) and np.abs(got[fine] - ref[fine]).max() <= tol
     ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("D,H,rows,tokens", [(128, 32, 300, 300), (64, 32, 300, 333), (64, 14, 8, 100), (128, 32, 300, 290)])
+def test_attention_masked_columns(torch, ops, D, H, rows, tokens):
+    _masked_columns(torch, ops, D, H, rows, tokens, "float16")
+
+
+@pytest.mark.parametrize("D,H,rows,tokens", [(128, 32, 300, 300), (64, 14, 200, 213)])
+def test_attention_masked_columns_fp32(torch, ops, D, H, rows, tokens):
+    _masked_columns(torch, ops, D, H, rows, tokens, "float32")
 
 
 @pytest.mark.parametrize("x", ["float32", "float16"])
@@ -555,6 +564,17 @@ def test_attention_long(torch, ops, H, Hk, D, page, x, tail, window, shared):
     if shared:
         assert np.abs(_attend(p, torch, ops, 0, seq, np.concatenate([[0], np.cumsum(counts)]), q, D ** -0.5, 0, 1)
                       .astype(np.float64) - got).max() <= 2 * _tolerance(p, 0, seq[:1], [0, 1], q[:1], D ** -0.5, x == "float16")
+
+
+@pytest.mark.parametrize("H,Hk,D,page,tail,window,shared", [
+    (32, 2, 128, 16, 313, 300, 0),                  # prompts
+    (32, 2, 64, 64, 1313, 300, 0),
+    (32, 2, 128, 32, 90, 70, 6000),                 # windows behind a prefix
+    (14, 2, 64, 16, 190, 150, 2999),
+])
+def test_attention_long_fp32(torch, ops, H, Hk, D, page, tail, window, shared):
+    """Items of 32 columns of fp32 queries."""
+    test_attention_long(torch, ops, H, Hk, D, page, "float32", tail, window, shared)
 
 
 def test_far_pages(torch, ops):
