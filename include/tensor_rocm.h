@@ -378,8 +378,8 @@ int pio_kv_status(const pio_kv_cache* cache, void* stream);
  * rows in use, in every layer (two requests that share such a page each get
  * one). All or nothing: if any request is refused, or the free pages do not
  * suffice, no request is served. Behind a refused call its sequences are held up:
- * pio_kv_write and pio_kv_drop with counts leave them as they are, so that a step's
- * calls need not wait for its outcome (the attention and verification of such a
+ * pio_kv_write and pio_kv_drop with counts leave them as they are, and pio_kv_read of
+ * their last tokens gives NaN, so that a step's calls need not wait for its outcome (the attention and verification of such a
  * step mean nothing: ask pio_kv_status before their results are used). That ends
  * with pio_kv_status, with a pio_kv_reserve that serves the sequence, and with its
  * end (pio_kv_drop without counts, pio_kv_fork onto it). */
@@ -403,7 +403,9 @@ int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t
  * pio_kv_write's, and rows and layers may not overlap. fp32|fp16, rounded to
  * it from an fp32 cache. A row whose sequence, token or page is not there becomes NaN, and
  * pio_kv_status reports it; rows at and behind row_start[n] are left as they are. One
- * sequence may come often. */
+ * sequence may come often. Behind a refused pio_kv_reserve the rows of its sequences
+ * that are counted from the end, or lie behind it, become NaN: their tokens never came
+ * (which the reserve has reported). */
 int pio_kv_read(const pio_kv_cache* cache, int layer, int layers, const int32_t* seq, const int32_t* row_start,
                 const int32_t* first, int n, void* k, void* v, int dtype, int rows, int64_t row_stride,
                 int64_t layer_stride, void* stream);

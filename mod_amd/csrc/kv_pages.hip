@@ -551,11 +551,20 @@ __global__ __launch_bounds__(KV_COPY) void kv_read_kernel(pio_kv_cache c, int la
         if (row < r0 || row >= r1) continue;
         const int L = kv_seq_len(c, s);
         const int64_t pos = first ? f + ((int64_t)row - r0) : L - ((int64_t)r1 - row);
-        const int page = pos >= 0 && pos < L ? c.table[(int64_t)s * c.max_pages + (pos >> lg)] : -1;
+        bool has = pos >= 0 && pos < L;
+        int page = -1, held_up = 0;
+        if (L >= 0) {                      // (both loads at once)
+            held_up = kv_work(c).held_up[s];
+            page = c.table[(int64_t)s * c.max_pages + (has ? pos >> lg : 0)];
+        }
+        // Behind a refused reserve the last tokens are not those that the caller counts from, and what is not there the
+        // reserve has reported.
+        has = has && (first || !held_up);
+        if (!has) page = -1;
         if (page >= 0 && page < c.n_pages) {
             where[0] = page;
             where[1] = (int)(pos & (c.page_size - 1));
-        } else {
+        } else if (has || !held_up) {
             atomicOr(kv_work(c).status, KV_BAD);
         }
         where[2] = i;

@@ -433,7 +433,8 @@ def kv_write(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k,
 
 def kv_read(cache: KvCache, layer: int, layers: int, seq, row_start, n: int, k, v, rows: int, first=None,
             row_stride: int = 0, layer_stride: int = 0, stream=None) -> None:
-    """Each sequence's tokens from first[i] on (None: its last ones) into k and v, as kv_write takes them."""
+    """Each sequence's tokens from first[i] on (None: its last ones) into k and v, as kv_write takes them. Behind a
+    refused kv_reserve its sequences' last ones are NaN."""
     dt = _dt(k)
     if _dt(v) != dt:
         raise TypeError("kv_read: k and v differ in dtype")

@@ -1,0 +1,90 @@
+"""Tokens read out of a paged cache (mod_amd/csrc/kv_pages.hip, kv_read_kernel) against
+oracle/kv_ref.py: behind a refused reserve, and out of caches of every type, head
+dimension and page size. A value is a function of one stored value: held to equality."""
+import numpy as np
+import pytest
+
+from oracle import kv_ref
+from test_gpu_kv4 import Pair4
+from test_gpu_kv_cache import Pair, _say
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch(torch_dev):
+    import torch
+    return torch
+
+
+@pytest.fixture(scope="module")
+def ops(torch_dev):
+    from mod_amd import ops
+    return ops
+
+
+def _pair(torch, ops, kind, layers, heads, dim, page, pages, seqs, width):
+    if kind == "mx4":
+        return Pair4(torch, ops, layers, heads, dim, page, pages, seqs, width)
+    p = Pair(torch, ops, layers, heads, dim, page, pages, seqs, width, kind)
+    p.ref.D = dim
+    return p
+
+
+@pytest.mark.parametrize("kind", ["float32", "float16", "mx4"])
+def test_behind_a_refused_reserve(torch, ops, kind):
+    """Rows counted from the end of a sequence that is held up are NaN, and the status stays that of the reserve: until
+    the status is asked, a reserve serves the sequence, or it ends."""
+    _say(f"read behind a refused reserve {kind}")
+    rng = np.random.default_rng(21)
+    p = _pair(torch, ops, kind, 2, 2, 32, 16, 8, 5, 4)
+    p.add(rng, [0, 1, 2], [20, 17, 5])
+
+    def read(seq, start, first=None):
+        got = Pair4.read(p, 0, 2, seq, start, first, torch.float32)
+        return [x.reshape(2, start[-1], 64) for x in got]
+
+    def want(s, at):
+        return [[x[at].reshape(-1, 64) for x in p.ref.rows(layer, s, int(p.ref.lens[s]))] for layer in range(2)]
+
+    def same(got, rows, s, at):
+        return all(np.array_equal(got[kind][layer, rows], want(s, at)[layer][kind]) for kind in range(2) for layer in range(2))
+    same_seq = lambda got: same(got, slice(3, 5), 2, slice(3, 5))  # noqa: E731
+
+    def refuse(seq, count):
+        ops.kv_reserve(p.c, p.ints(seq), p.ints(count), len(seq))
+        with pytest.raises(kv_ref.Refused):
+            p.ref.reserve(seq, count)
+    refuse([0, 1], [3, 200])
+    got = read([0, 2, 1], [0, 3, 5, 6])
+    assert all(np.isnan(x[:, :3]).all() and np.isnan(x[:, 5]).all() for x in got) and same_seq(got)
+    # tokens named by their place are what they are; those that the reserve did not bring are not there
+    got = read([0, 1], [0, 4, 6], [18, 3])
+    assert all(np.isnan(x[:, 2:4]).all() for x in got)
+    assert same(got, slice(0, 2), 0, slice(18, 20)) and same(got, slice(4, 6), 1, slice(3, 5))
+    with pytest.raises(ops.RocmError, match="too few free pages"):
+        ops.kv_status(p.c)
+    got = read([0, 1], [0, 3, 4])
+    assert same(got, slice(0, 3), 0, slice(17, 20)) and same(got, slice(3, 4), 1, slice(16, 17))
+    ops.kv_status(p.c)
+    # a reserve that serves one of them
+    refuse([0, 1], [200, 1])
+    p.reserve([0], [2])
+    k, v = (rng.standard_normal((2, 2, 2, 32)).astype(np.float32) for _ in range(2))
+    p.write(0, [0], [0, 2], k, v)
+    got = read([0, 1], [0, 4, 5])
+    assert same(got, slice(0, 4), 0, slice(18, 22)) and all(np.isnan(x[:, 4]).all() for x in got)
+    # and the end of the other
+    p.drop([1])
+    p.fork([0], [1])
+    got = read([1], [0, 22])
+    assert same(got, slice(0, 22), 1, slice(0, 22))
+    with pytest.raises(ops.RocmError, match="too few free pages"):
+        ops.kv_status(p.c)
+    # a page outside the cache is still reported where its sequence is held up
+    refuse([0], [200])
+    p.table[0, 0] = -1
+    got = read([0], [0, 3], [14])
+    assert all(np.isnan(x[:, :2]).all() and not np.isnan(x[:, 2]).any() for x in got)
+    with pytest.raises(ops.RocmError, match="does not have"):
+        ops.kv_status(p.c)
