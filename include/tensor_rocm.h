@@ -437,8 +437,8 @@ int pio_kv_compact(const pio_kv_cache* cache, void* stream);
  * the fp16 matrix cores with the softmax's weights rounded to fp16; of fp32
  * queries over an fp16 cache with queries and weights as two fp16 parts each;
  * over an fp32 cache on the fp32 matrix cores. Over a cache of 4 bits the keys are
- * operands of the scaled matrix cores as they lie there and the queries the sum of 3 (fp16) or
- * 5 (fp32) parts of 6 bits, exact to 2^-13 (2^-23) of the largest of 32 dimensions; the values
+ * operands of the scaled matrix cores as they lie there and the queries the sum of 4 (fp16) or
+ * 5 (fp32) parts of 6 bits, exact to 2^-18 (2^-23) of the largest of 32 dimensions; the values
  * are exact in fp16, the weights as over an fp16 cache. Where head_dim is 64 or 128 the
  * parts of a row that are computed apart (runs of its own tokens, of the shared
  * ones) meet in a workspace, rows * n_heads * (head_dim + 2) * 4 bytes each: up to
