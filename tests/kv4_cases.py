@@ -98,3 +98,111 @@ PARTS_CASES = [
     (4, 2, 128, 3, "float16"), (4, 2, 64, 3, "float16"), (32, 1, 128, 300, "float16"), (16, 1, 64, 4, "float16"),
     (4, 2, 128, 3, "float32"), (4, 2, 64, 3, "float32"), (16, 1, 128, 70, "float32"), (16, 1, 64, 70, "float32"),
 ]
+
+
+# ------------------------------------------------------------------ every key counts
+def held(rng, lens, layers, Hk, D, page, common=0, spare=3):
+    """A cache with sequences of the given lengths, in pages in any order; the pages of the first `common` tokens that
+    these fill are the same."""
+    need = [-(-n // page) for n in lens]
+    same = common // page
+    pages = same + sum(max(n - same, 0) for n in need) + spare
+    c = kv_ref.Cache4(layers, Hk, D, page, pages, len(lens), max(need) + 1)
+    free = [int(i) for i in rng.permutation(pages)]
+    first = [free.pop() for _ in range(same)]
+    for s, (n, k) in enumerate(zip(lens, need)):
+        c.table[s, :k] = (first + [free.pop() for _ in range(max(k - same, 0))])[:k]
+        c.lens[s] = n
+    np.add.at(c.refs, c.table[c.table >= 0], 1)
+    return c
+
+
+def flat(rng, c, key=119):
+    """Keys so small (under scales of 2^-8) that all weights are nearly the same, and values of 1 with signs of their own
+    for every 16 rows of a page and each dimension: 32 keys that are left out, or taken twice, move some dimension of an
+    output by 32 of the keys that a query sees."""
+    codes, scales = c.blocks()
+    codes[:, 0] = rng.integers(0, 256, codes[:, 0].shape)
+    scales[:, 0], scales[:, 1] = key, 127
+    sign = np.repeat(rng.integers(0, 4, (*codes[:, 1].shape[:3], c.P // 16, c.D // 2)), 16, 3).astype(np.uint8)
+    codes[:, 1] = 0x22 | (sign & 1) << 3 | (sign & 2) << 6
+
+
+def share(c, common):
+    """The tokens of a prefix that lie in a page of each sequence's own are those of sequence 0."""
+    part, at = common % c.P, common // c.P
+    codes, scales = c.blocks()
+    for s in range(1, len(c.lens)):
+        n = min(part, int(c.lens[s]) - at * c.P)
+        if n > 0:
+            codes[:, :, c.table[s, at], :, :n] = codes[:, :, c.table[0, at], :, :n]
+            scales[:, :, c.table[s, at], :, :, :n] = scales[:, :, c.table[0, at], :, :, :n]
+
+
+def attend(c, layer, s, q, scale, times=None):
+    """Outputs of q [rows, H, D], the last tokens of sequence s; times: how often each key is taken."""
+    n, rows = int(c.lens[s]), len(q)
+    k, v = c.rows(layer, s, n)
+    times = np.ones(n) if times is None else times
+    G = q.shape[1] // k.shape[1]
+    out = np.zeros(q.shape)
+    hidden = np.arange(n) > np.arange(n - rows, n)[:, None]
+    for h in range(k.shape[1]):
+        sc = np.einsum("rgd,td->rgt", q[:, h * G:(h + 1) * G].astype(np.float64), k[:, h], optimize=True) * scale
+        sc[np.broadcast_to(hidden[:, None], sc.shape)] = -np.inf
+        top = sc.max(2, keepdims=True)
+        w = np.exp(sc - np.where(np.isfinite(top), top, 0)) * times
+        out[:, h * G:(h + 1) * G] = w @ v[:, h] / np.maximum(w.sum(2, keepdims=True), 1e-300)
+    return out
+
+
+def flat_tolerance(x, out, largest):
+    """Of outputs of values of 1 where scores are no larger than `largest`. fp16: each weight is off by up to 2^-11 of it,
+    which moves an output by that much of the weight times |v - out|; then the output is rounded. fp32: two parts of a
+    weight, 2^-22. Scores, of a running sum of exponents up to 16: PARTS + 4 roundings, and what the parts drop."""
+    off = (PARTS[x] + 4) * 2.0 ** -24 * 16 / LOG2E + OFF[x] * largest
+    each = 2.0 ** -11 if x == "float16" else 2.0 ** -22
+    return (each + 2 * off) * (1 + np.abs(out)) + each * np.abs(out)
+
+
+FLAT_CASES = [
+    # heads, kv heads, dim, page, queries; shared, the longest tail, how many; queries of each
+    (8, 1, 128, 16, "float16", 0, 20011, 1, 1),          # runs of one sequence, over one kv head
+    (8, 1, 128, 128, "float32", 0, 20011, 1, 2),
+    (8, 4, 64, 64, "float16", 0, 9973, 1, 5),
+    (8, 2, 64, 16, "float32", 0, 33001, 2, 1),
+    (16, 2, 128, 32, "float16", 12320, 37, 12, 3),       # a long prefix
+    (16, 2, 64, 16, "float32", 17001, 700, 12, 1),
+    (24, 2, 128, 16, "float32", 2999, 3, 12, 7),         # rows that stand inside it
+    (32, 4, 128, 32, "float16", 12320, 400, 12, 3),      # items of 32 columns
+    (32, 4, 128, 16, "float16", 17003, 2, 12, 4),
+    (32, 2, 128, 16, "float16", 0, 313, 1, 300),
+    (32, 2, 64, 64, "float16", 0, 1313, 1, 300),
+    (14, 2, 64, 16, "float16", 250, 2100, 24, 6),
+    (32, 2, 128, 16, "float32", 0, 313, 1, 300),
+    (32, 2, 64, 64, "float32", 0, 1313, 1, 300),
+    (32, 2, 128, 32, "float32", 6000, 90, 12, 70),
+    (8, 2, 128, 16, "float16", 0, 3000, 60, 1),          # ragged ones, cut into runs
+    (8, 2, 128, 16, "float32", 0, 600, 300, 2),          # more than the waves find on their own
+]
+
+
+class Flat:
+    def __init__(self, H, Hk, D, page, x, shared, tail, n, window):
+        rng = np.random.default_rng(shared + tail)
+        tails = [tail] + [max(1, int(t)) for t in np.exp(rng.uniform(np.log(max(1, tail / 40)), np.log(tail), n - 1))]
+        self.c = held(rng, [shared + t for t in tails], 1, Hk, D, page, shared)
+        flat(rng, self.c)
+        share(self.c, shared)
+        self.seq = [int(s) for s in rng.permutation(n)]
+        self.counts = [min(window, int(self.c.lens[s])) if s == 0 else int(rng.integers(1, min(window, self.c.lens[s]) + 1))
+                       for s in self.seq]
+        self.start = np.concatenate([[0], np.cumsum(self.counts)]).astype(int)
+        self.q = rng.standard_normal((int(self.start[-1]), H, D)).astype(x)
+        self.scale, self.shared, self.window, self.x = D ** -0.5, shared, window, x
+        # a score's most: queries times keys of up to 6 * 2^-8 in every dimension
+        self.largest = float(np.abs(self.q).max()) * 6 * 2.0 ** -8 * D * self.scale
+
+    def of(self, s):
+        i = self.seq.index(s)
+        return slice(self.start[i], self.start[i + 1])

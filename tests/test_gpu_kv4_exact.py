@@ -23,30 +23,24 @@ def ops(torch_dev):
     return ops
 
 
-def _fill(p, layer, s, k, v):
+def _fill(c, layer, s, k, v):
     """The first tokens of sequence s, k and v [tokens, heads, D], by the oracle."""
     t = np.arange(len(k))
-    page, at = p.ref.table[s, t // p.ref.P], t % p.ref.P
-    codes, scales = p.ref.blocks()
+    page, at = c.table[s, t // c.P], t % c.P
+    codes, scales = c.blocks()
     for kind, x in enumerate((k, v)):
         code, scale = kv_ref.mx4_encode(x)
         codes[layer, kind, page, :, at] = code[..., 0::2] | code[..., 1::2] << 4
         scales[layer, kind, page, :, :, at] = scale
 
 
-def _sequences(torch, ops, rng, lens, layers, Hk, D, page, common=0):
-    """Sequences of the given lengths, in pages in any order; the first `common` tokens' pages are the same."""
-    need = [-(-n // page) for n in lens]
-    same = common // page
-    pages = same + sum(n - same for n in need) + 3
-    p = Pair4(torch, ops, layers, Hk, D, page, pages, len(lens), max(need) + 1)
-    free = [int(i) for i in rng.permutation(pages)]
-    first = [free.pop() for _ in range(same)]
-    for s, (n, k) in enumerate(zip(lens, need)):
-        p.ref.table[s, :k] = first + [free.pop() for _ in range(k - same)]
-        p.ref.lens[s] = n
-    np.add.at(p.ref.refs, p.ref.table[p.ref.table >= 0], 1)
-    for dev, ref in ((p.table, p.ref.table), (p.lens, p.ref.lens), (p.refs, p.ref.refs)):
+def _upload(torch, ops, c):
+    """The oracle's cache on the GPU."""
+    layers, _, pages, Hk, P, _ = c.kv.shape
+    p = Pair4(torch, ops, layers, Hk, c.D, P, pages, *c.table.shape)
+    p.ref = c
+    p.upload()
+    for dev, ref in ((p.table, c.table), (p.lens, c.lens), (p.refs, c.refs)):
         dev.copy_(torch.from_numpy(ref))
     torch.cuda.synchronize()
     return p
@@ -59,9 +53,9 @@ def test_query_parts(torch, ops, H, Hk, D, rows, x, own):
     _say(f"parts H{H}/{Hk} D{D} {rows} rows {x} own {own}")
     rng = np.random.default_rng(D + rows)
     c = kv4_cases.Parts(rng, D, H, Hk, rows, x, own)
-    p = _sequences(torch, ops, rng, [D + rows], 1, Hk, D, 16)
-    _fill(p, 0, 0, c.k, c.v)
-    p.upload()
+    ref = kv4_cases.held(rng, [D + rows], 1, Hk, D, 16)
+    _fill(ref, 0, 0, c.k, c.v)
+    p = _upload(torch, ops, ref)
     for shared in (0, D, D // 2 + 5):
         got = _attend(p, torch, ops, 0, [0], [0, rows], c.q, c.scale, shared, rows).astype(np.float64)
         wrong = c.wrong(got)
@@ -72,7 +66,7 @@ def test_query_parts(torch, ops, H, Hk, D, rows, x, own):
 
 def _off(p, layer, s, rows, q, got, scale):
     """Relative error of the rows of sequence s, its last, in the 2-norm."""
-    want = p.ref.attention(layer, [s], [0, rows], q, scale, np.zeros(q.shape))
+    want = kv4_cases.attend(p.ref, layer, s, q, scale)
     return np.linalg.norm(got.astype(np.float64) - want) / np.linalg.norm(want)
 
 
@@ -86,9 +80,9 @@ def test_error_of_normal_inputs(torch, ops, H, Hk, D, n, rows, x):
     parts of a weight, 2^-22. Both: a query's parts, uniform within their bound over D dimensions of keys of 1."""
     _say(f"normal H{H}/{Hk} D{D} {n} keys {x}")
     rng = np.random.default_rng(n)
-    p = _sequences(torch, ops, rng, [n], 1, Hk, D, 16)
-    _fill(p, 0, 0, *(rng.standard_normal((n, Hk, D)) for _ in range(2)))
-    p.upload()
+    ref = kv4_cases.held(rng, [n], 1, Hk, D, 16)
+    _fill(ref, 0, 0, *(rng.standard_normal((n, Hk, D)) for _ in range(2)))
+    p = _upload(torch, ops, ref)
     q = rng.standard_normal((rows, H, D)).astype(x)
     scale = D ** -0.5
     most = np.abs(q.astype(np.float64)).reshape(-1, 32).max(1).max()
@@ -111,9 +105,9 @@ def test_one_large_dimension(torch, ops, D, ratio):
     _say(f"one large dimension D{D} {ratio}")
     rng = np.random.default_rng(ratio)
     n, H, scale = 4096, 16, D ** -0.5
-    p = _sequences(torch, ops, rng, [n], 1, 1, D, 16)
-    _fill(p, 0, 0, *(rng.standard_normal((n, 1, D)) for _ in range(2)))
-    p.upload()
+    ref = kv4_cases.held(rng, [n], 1, 1, D, 16)
+    _fill(ref, 0, 0, *(rng.standard_normal((n, 1, D)) for _ in range(2)))
+    p = _upload(torch, ops, ref)
     q = rng.standard_normal((4, H, D))
     q[:, :, 17] = ratio
     q = q.astype("float16")
@@ -123,3 +117,135 @@ def test_one_large_dimension(torch, ops, D, ratio):
     off = _off(p, 0, 0, 4, q, _attend(p, torch, ops, 0, [0], [0, 4], q, scale, 0, 4), scale)
     _say(f"  {off:.2e} of {tol:.2e}")
     assert off <= tol
+
+
+@pytest.mark.parametrize("H,Hk,D,page,x,shared,tail,n,window", kv4_cases.FLAT_CASES)
+def test_every_key_counts(torch, ops, H, Hk, D, page, x, shared, tail, n, window):
+    """Weights that are nearly the same: a tile of keys left out of any sequence, or taken twice, would show."""
+    _say(f"every key H{H}/{Hk} D{D} page {page} {x} {n} x {shared} + {tail}")
+    f = kv4_cases.Flat(H, Hk, D, page, x, shared, tail, n, window)
+    p = _upload(torch, ops, f.c)
+    want = np.zeros(f.q.shape)
+    for s in f.seq:
+        want[f.of(s)] = kv4_cases.attend(f.c, 0, s, f.q[f.of(s)], f.scale)
+    tol = kv4_cases.flat_tolerance(x, want, f.largest)
+    # (the prefix read for all of them, for none, and in part; windows longer than announced)
+    for same, hint in ((shared, window), (0, window), (shared // 2, window), (shared, 1)):
+        got = _attend(p, torch, ops, 0, f.seq, f.start, f.q, f.scale, same, hint).astype(np.float64)
+        wrong = (np.abs(got - want) / tol).max()
+        _say(f"  shared {same}, {hint} rows: {wrong:.2f} of the bound")
+        assert wrong <= 1
+    ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("x", ["float32", "float16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("way", ["up", "down", "both"])
+def test_references_follow(torch, ops, D, x, way):
+    """Scores that climb by more than the references stay behind, fall, or do both, over runs and a prefix: values of 1
+    with the signs of kv4_cases.flat, keys 0 to 6 in one dimension, 4 (fp16) or 12 (fp32) a step."""
+    _say(f"references D{D} {x} {way}")
+    rng = np.random.default_rng(D)
+    n, H, step = 4000, 8, 4.0 if x == "float16" else 12.0
+    c = kv4_cases.held(rng, [n, n], 1, 2, D, 16, 2000)
+    kv4_cases.flat(rng, c)
+    level = np.arange(n) * 8 // n
+    level = {"up": level, "down": 7 - level, "both": np.where(level < 4, 2 * level, 15 - 2 * level)}[way]
+    for s in range(2):
+        k = np.zeros((n, 2, D))
+        k[:, :, 9] = kv_ref.MX4_VALUES[level][:, None]
+        v = c.rows(0, s, n)[1]
+        _fill(c, 0, s, k, v)
+    p = _upload(torch, ops, c)
+    q = np.zeros((6, H, D))
+    q[:, :, 9] = np.array([1.0, -1.0, 0.5, 2.0])[np.arange(H) % 4]
+    q = q.astype(x)
+    want = np.concatenate([kv4_cases.attend(c, 0, s, q[3 * s:3 * s + 3], step) for s in range(2)])
+    # scores of up to 12 steps: their sums' roundings are of exponents up to that, and 16
+    largest = 12 * step
+    tol = kv4_cases.flat_tolerance(x, want, largest) + 2 * 9 * 2.0 ** -24 * largest * 2
+    for shared in (0, 2000, 1001):
+        got = _attend(p, torch, ops, 0, [0, 1], [0, 3, 6], q, step, shared, 3).astype(np.float64)
+        wrong = (np.abs(got - want) / tol).max()
+        _say(f"  shared {shared}: {wrong:.2f} of the bound")
+        assert wrong <= 1
+    ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("big", [False, True])
+@pytest.mark.parametrize("x", ["float32", "float16"])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (4, 2, 128), (16, 1, 64), (64, 1, 128), (2, 2, 96)])
+def test_one_token_picked(torch, ops, H, Hk, D, x, big):
+    """Each query picks one token, whose weight is 1 and the others' 0: outputs are that token's values, of every scale
+    that the cache has and every code, side by side. big: queries as large as their type holds."""
+    _say(f"picked H{H}/{Hk} D{D} {x} big {big}")
+    rng = np.random.default_rng(D)
+    rows = 2 * D
+    c = kv4_cases.held(rng, [2 * D + rows], 1, Hk, D, 16)
+    codes, scales = c.blocks()
+    codes[:] = rng.integers(0, 256, codes.shape)
+    scales[:] = 104 + rng.permutation(scales.size).reshape(scales.shape) % 37
+    v = c.rows(0, 0, 2 * D + rows)[1]
+    k = np.zeros((2 * D + rows, Hk, D))
+    k[np.arange(D), :, np.arange(D)] = 4.0         # 4 or -4 in a dimension of its own; the last tokens: none
+    k[D + np.arange(D), :, np.arange(D)] = -4.0
+    # (its keys alone: the values' scales are not what an encoder would choose)
+    kept = c.kv[:, 1].copy()
+    _fill(c, 0, 0, k, v)
+    c.kv[:, 1] = kept
+    v = c.rows(0, 0, 2 * D + rows)[1]
+    p = _upload(torch, ops, c)
+    which = np.stack([rng.permutation(2 * D) for _ in range(H)], 1)                  # [rows, H]
+    q = np.zeros((rows, H, D))
+    size = 64.0 if not big else 6e4 if x == "float16" else 1e30
+    np.put_along_axis(q, (which % D)[..., None], np.where(which < D, size, -size)[..., None], 2)
+    got = _attend(p, torch, ops, 0, [0], [0, rows], q.astype(x), 2.0, 0, rows).astype(np.float64)
+    want = np.stack([v[which[:, h], h // (H // Hk)] for h in range(H)], 1)
+    # a weight and the sum are the same number but for 2^-21; fp16: the values are its numbers
+    tol = 2.0 ** -20 * np.abs(want) + (2.0 ** -11 * np.abs(want) if x == "float16" else 0)
+    assert (np.abs(got - want) <= tol).all()
+    ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("x", ["float32", "float16"])
+@pytest.mark.parametrize("H,Hk,D,rows", [(4, 2, 64, 2), (4, 2, 128, 2), (16, 1, 64, 4), (64, 1, 128, 140)])
+def test_every_scale(torch, ops, H, Hk, D, rows, x):
+    """Values of a whole sequence under one scale, the least to the largest that the cache has, and keys likewise, with
+    queries and a factor that make ordinary scores of them: relative to that sequence's values. (fp16: an output below
+    2^-14 is rounded by up to 2^-25.)"""
+    _say(f"scales H{H}/{Hk} D{D} {rows} rows {x}")
+    rng = np.random.default_rng(D)
+    lens = [rows + 30 + int(i) for i in rng.integers(0, 40, 37)]
+    c = kv4_cases.held(rng, lens, 1, Hk, D, 16)
+    kv4_cases.flat(rng, c, 126)
+    codes, scales = c.blocks()
+    for i, n in enumerate(lens):
+        pages = c.table[i, :-(-n // 16)]
+        scales[0, 1, pages] = 104 + i
+    p = _upload(torch, ops, c)
+    seq, counts = list(range(37)), [rows] + [1 + i % 3 for i in range(36)]
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+    q = rng.standard_normal((int(start[-1]), H, D)).astype(x)
+    scale = D ** -0.5
+    most = np.abs(q).max() * 6 * 0.5 * D * scale   # a score's most
+    off = kv4_cases.OFF[x] * most + (kv4_cases.PARTS[x] + 4) * 2.0 ** -24 * (most + 16 / kv4_cases.LOG2E)
+
+    def check(got, i, want, unit):
+        each = 2.0 ** -11 if x == "float16" else 2.0 ** -22
+        tol = (2 * each + 4 * off) * unit + (2.0 ** -25 if x == "float16" else 0)
+        assert np.isfinite(got).all() and np.abs(got - want).max() <= tol, (i, np.abs(got - want).max(), tol)
+    got = _attend(p, torch, ops, 0, seq, start, q, scale, 0, rows).astype(np.float64)
+    for i in seq:
+        rows_ = slice(start[i], start[i + 1])
+        check(got[rows_], i, kv4_cases.attend(c, 0, i, q[rows_], scale), 2.0 ** (i - 23))
+    # keys: the same codes under another scale, and a factor against it
+    for i in seq:
+        scales[0, 0, c.table[i, :-(-lens[i] // 16)]] = 104 + i
+    scales[:, 1] = 127
+    p.upload()
+    for i in seq:
+        rows_ = slice(start[i], start[i + 1])
+        factor = scale * 2.0 ** (22 - i)
+        got = _attend(p, torch, ops, 0, [i], [0, counts[i]], q[rows_], factor, 0, rows).astype(np.float64)
+        check(got, i, kv4_cases.attend(c, 0, i, q[rows_], factor), 1.0)
+    ops.kv_status(p.c)
