@@ -88,3 +88,51 @@ def test_behind_a_refused_reserve(torch, ops, kind):
     assert all(np.isnan(x[:, :2]).all() and not np.isnan(x[:, 2]).any() for x in got)
     with pytest.raises(ops.RocmError, match="does not have"):
         ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("x", ["float32", "float16"])
+@pytest.mark.parametrize("kind,heads,dim,page,layers", [
+    ("float32", 1, 8, 1, 1), ("float32", 3, 40, 2, 3), ("float32", 8, 128, 16, 2), ("float32", 2, 256, 1024, 2),
+    ("float16", 1, 8, 1, 2), ("float16", 5, 72, 4, 1), ("float16", 8, 128, 16, 3), ("float16", 2, 64, 32, 2),
+    ("float16", 1, 256, 1024, 2), ("float32", 33, 64, 8, 2), ("mx4", 1, 32, 16, 1), ("mx4", 3, 96, 32, 3),
+    ("mx4", 8, 128, 1024, 2), ("mx4", 5, 256, 16, 2), ("mx4", 33, 64, 64, 2)])
+def test_every_geometry(torch, ops, kind, heads, dim, page, layers, x):
+    """Head dimensions, heads and page sizes up to their limits: pieces of sequences, some twice, rows at the ends of
+    pages, one layer and all of them."""
+    _say(f"read {kind} {heads} x {dim} page {page} {layers} layers {x}")
+    rng = np.random.default_rng(heads + dim)
+    lens = [page + 3, 2 * page, 1, page]
+    need = [-(-n // page) for n in lens]
+    p = _pair(torch, ops, kind, layers, heads, dim, page, sum(need) + 2, 5, max(need) + 1)
+    order = [3, 0, 4, 2]
+    p.reserve(order, lens)
+    n = sum(lens)
+    k, v = ((rng.standard_normal((layers, n, heads, dim)) * 3).astype(np.float32) for _ in range(2))
+    p.write(0, order, np.concatenate([[0], np.cumsum(lens)]).astype(int), k, v)
+    seq, first, count = [], [], []
+    for s, m in zip(order, lens):
+        for a, b in ((0, m), (max(0, page - 2), m), (m - 1, m), (0, min(m, page))):
+            seq.append(s)
+            first.append(a if a < m else 0)
+            count.append(max(0, b - first[-1]))
+    pick = rng.permutation(len(seq))
+    seq, first, count = ([int(a[i]) for i in pick] for a in (seq, first, count))
+    start = np.concatenate([[0], np.cumsum(count)]).astype(int)
+    for layer, m in ((0, layers), (layers - 1, 1)):
+        got = Pair4.read(p, layer, m, seq, start, first, getattr(torch, x))
+        for kind_ in range(2):
+            rows = got[kind_].reshape(m, start[-1], heads, dim)
+            for i, s in enumerate(seq):
+                for l in range(m):
+                    want = p.ref.rows(layer + l, s, first[i] + count[i])[kind_][first[i]:].astype(x)
+                    assert np.array_equal(rows[l, start[i]:start[i + 1]], want)
+    # the last ones
+    last = [min(2, m) for m in lens]
+    start = np.concatenate([[0], np.cumsum(last)]).astype(int)
+    got = Pair4.read(p, 0, layers, order, start, None, getattr(torch, x))
+    for kind_ in range(2):
+        rows = got[kind_].reshape(layers, start[-1], heads, dim)
+        for i, s in enumerate(order):
+            want = p.ref.rows(0, s, lens[i])[kind_][-last[i]:].astype(x)
+            assert np.array_equal(rows[0, start[i]:start[i + 1]], want)
+    ops.kv_status(p.c)
