@@ -302,7 +302,7 @@ __device__ __forceinline__ int ka4_least(int x) {
 // A wave's tiles, every KA4_WAVES-th. The scores run one tile ahead of the softmax, in one piece of code without
 // branches: their products fill the matrix cores while the VALU forms the weights and widens the values. K is
 // loaded two tiles ahead, V one, by turns into two sets of registers.
-// ONCE: nothing else reads these keys.
+// ONCE: no other column tile reads these keys (a request of more rows than announced does so itself).
 template <int D, bool X16, int NC, bool ONCE>
 struct Ka4Walk {
     using T = Ka4<D, X16>;
@@ -357,8 +357,9 @@ struct Ka4Walk {
         const uint32_t o = here(ko);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            // (past the caches where the keys are read once: 3 sequences of 120,000 36.4 us, so 32.9. V's rows, whose lines
-            // two loads share, are not: 35.1)
+            // (past the caches where the keys are read once: sequences of 120,011, 3,323 and 2,565 tokens 36.4 us, so 32.9. V's
+            // rows, whose lines two loads share, are not: 35.1. Where several tiles read them: 24 windows of up to 6 over
+            // 16,000 tokens, 3 tiles each, 26.6 past the caches, 25.2 through them)
             if constexpr (ONCE)
                 to.k[h] = __builtin_nontemporal_load((const __attribute__((address_space(1))) ka4_u4*)(kc[h] + o));
             else
@@ -724,7 +725,7 @@ __device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found
 }
 
 // The prefix's items, then the tails'.
-template <int D, bool X16, int NC>
+template <int D, bool X16, int NC, bool ONCE>
 __global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[KA4_WAVES * 16 * Ka4<D, X16>::OP];
     __shared__ float ml[KA4_WAVES][16][2];
@@ -760,21 +761,25 @@ __global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
         // have no registers for them: their reloads put the first loads in a row, two prompts 57 us, so 55)
         int own = lane;
         if constexpr (NC > 1) asm volatile("" : "+v"(own));
-        ka4_item<D, X16, NC, NC == 1>(a, it, lds, ml, nullptr, c0, w, own);
+        ka4_item<D, X16, NC, ONCE>(a, it, lds, ml, nullptr, c0, w, own);
         __syncthreads();                                   // its output is out of LDS
     }
 }
 
-template <int D, bool X16, int NC>
+template <int D, bool X16, int NC, bool ONCE>
 static int ka4_launch(const KaArgs& a, hipStream_t st) {
-    ka4_kernel<D, X16, NC><<<a.pre_items + a.tail_items, 256, 0, st>>>(a);
+    ka4_kernel<D, X16, NC, ONCE><<<a.pre_items + a.tail_items, 256, 0, st>>>(a);
     PIO_LAUNCHED();
     return PIO_OK;
 }
+template <int D, bool X16>
+static int ka4_width(const KaArgs& a, int nc, hipStream_t st) {
+    if (nc > 1) return ka4_launch<D, X16, 2, false>(a, st);
+    return a.tail_tiles == 1 ? ka4_launch<D, X16, 1, true>(a, st) : ka4_launch<D, X16, 1, false>(a, st);
+}
 template <int D>
 static int ka4_route(const KaArgs& a, int nc, hipStream_t st) {
-    if (!a.q16) return nc == 1 ? ka4_launch<D, false, 1>(a, st) : ka4_launch<D, false, 2>(a, st);
-    return nc == 1 ? ka4_launch<D, true, 1>(a, st) : ka4_launch<D, true, 2>(a, st);
+    return a.q16 ? ka4_width<D, true>(a, nc, st) : ka4_width<D, false>(a, nc, st);
 }
 template <int D>
 static int ka4_join(const KaArgs& a, hipStream_t st) {
