@@ -724,9 +724,13 @@ __device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found
     }
 }
 
+// Workgroups to a CU, by registers: 168 hold 16 columns of fp16 queries of 64 dimensions (60 sequences of up to 492 tokens,
+// 16 heads of their own, 15.0 us, two to a CU 17.2), the others take 187 to 256.
+__host__ __device__ constexpr int ka4_held(int D, bool x16, int nc) { return D == 64 && x16 && nc == 1 ? 3 : 2; }
+
 // The prefix's items, then the tails'.
 template <int D, bool X16, int NC, bool ONCE>
-__global__ __launch_bounds__(256, 2) void ka4_kernel(KaArgs a) {
+__global__ __launch_bounds__(256, ka4_held(D, X16, NC)) void ka4_kernel(KaArgs a) {
     __shared__ __attribute__((aligned(16))) float lds[KA4_WAVES * 16 * Ka4<D, X16>::OP];
     __shared__ float ml[KA4_WAVES][16][2];
     __shared__ int limits[16 * NC];
