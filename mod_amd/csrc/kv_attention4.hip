@@ -805,50 +805,82 @@ constexpr int KA4_LEAST = 4;
 // Keys of a prefix's run at most (below).
 constexpr int KA4_RUN = 8192;
 
+// Rounds of a request's own tokens, which the host does not know: taken for all where the width of the items is chosen.
+constexpr int KA4_TAIL = 8;
+
+// How the columns are cut into items of `width`, and the rounds of 16 columns that the device takes for them: as long as an
+// item, and as all of them over its `places`. A round of 32 columns is `round` of 16.
+struct Ka4Cut {
+    int64_t tail_tiles, items;                     // column tiles of a request at most; items of one run to a request
+    int64_t pre_tiles, pre_splits, pre_keys;
+    float cost;
+};
+static Ka4Cut ka4_cut(const KaArgs& a, int64_t tail_cols, int64_t part, int width, float round, int places) {
+    Ka4Cut k{};
+    const int64_t Hk = a.c.n_kv_heads, cols = (int64_t)a.rows * a.G;
+    const float tail = a.fixed + round * KA4_TAIL;
+    k.tail_tiles = (tail_cols + width - 1) / width;
+    k.items = std::min(a.n * k.tail_tiles, cols / width + a.n) * Hk;
+    k.cost = std::max(tail, k.items * tail / places);
+    if (a.shared == 0) return k;
+    k.pre_tiles = (cols + width - 1) / width;
+    const int64_t units = Hk * k.pre_tiles, rounds = (a.shared + KA_ROUND - 1) / KA_ROUND, most = a.slots / units;
+    // As many runs as fill the device, a quarter of that where the prefix is short (the tails need some of it), and
+    // none longer than KA4_RUN keys where several column tiles read them: an XCD's workgroups then stay within what
+    // its L2 holds (and no more of these than 256 MB of partial results hold). 624 columns x 4 kv heads over 96,000
+    // tokens 185 us, 240 in longer runs; over 48,000 the same, in runs of 6,144 83 -> 93.
+    const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most),
+                                              k.pre_tiles > 1 ? std::min<int64_t>((a.shared + KA4_RUN - 1) / KA4_RUN, (256 << 20) / part) : 1});
+    const int64_t each = std::min(splits, rounds), run = (rounds + each - 1) / each;
+    k.pre_keys = run * KA_ROUND;
+    k.pre_splits = (a.shared + k.pre_keys - 1) / k.pre_keys;
+    const float pre = a.fixed + round * run;
+    k.cost = std::max({pre, tail, (units * k.pre_splits * pre + k.items * tail) / places});
+    return k;
+}
+
 // Items for the matrix core kernels.
 static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     const int Hk = a.c.n_kv_heads, cus = 256;
-    const int64_t cols = (int64_t)a.rows * a.G, tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
+    const int64_t tail_cols = (int64_t)std::min(max_rows, a.rows) * a.G;
+    const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
     a.fixed = KA4_FIXED;
     a.slots = 2 * cus;                             // two workgroups to a CU
-    // Items of 32 columns widen V once for both their tiles, and halve what crosses from L2; items of 16 are twice as
-    // many. fp16 queries, 8 heads to each of 4 kv heads of 128: 40 windows of 3 behind 24,000 tokens 48 us (16 columns:
-    // 86), 24 behind 12,000 33 (36), behind 6,000 24.5 (24.7), behind 2,000 18.5 (14.7), over 3,000 own tokens 15.2
-    // (12.4); 4 windows of 100 over those 33 (29); two prompts of 509 over 4,090, 4 heads to each of 8, 50 (71). Of 64
-    // dimensions, 7 heads to each of 2 kv heads, 24 windows over up to 2,100 tokens: of 3 14.4 us (12.5), of 6 15.7
-    // (17.3), of 12 17.5 (20.6), 8 of 40 23.0 (21.4).
-    // fp32 queries, whose parts and weights take the registers, need more: those prompts 75 (86), over 1,000 53 (61); 24
-    // windows of up to 40, 320 columns each, over 3,000 own tokens 47 (42); of 200, 1,400 columns of 64, 143 (178). 40 windows
-    // of up to 3 behind 48,000 124 (145), 24,000 76 (111), 12,000 65 (59), 6,000 42 (42), 2,000 26 (25); 80 behind 6,000 63
-    // (85), 12,000 97 (89); 20 behind 24,000 56 (70), 48,000 94 (79); of 64 dimensions, 40 behind 24,000 58 (89).
-    const double over = (double)cols * Hk * a.shared * a.c.head_dim;
-    const bool many = a.q16 ? cols * Hk > 16 * a.slots || over >= 0x1p30 : tail_cols > 1024 || over >= 0x1p31;
-    const bool small = a.q16 && a.c.head_dim == 64 && tail_cols > 32 && tail_cols <= 128;
-    const int nc = tail_cols > 16 && (many || small) ? 2 : 1;
-    const int width = 16 * nc;
-    a.tail_tiles = ceil_div(tail_cols, width);
     PIO_REQUIRE((int64_t)a.n * Hk <= 1 << 22, "pio_kv_attention: %d requests are too many", a.n);
-    const int64_t items = std::min((int64_t)a.n * a.tail_tiles, cols / width + a.n) * Hk;
+    // Items of 32 columns widen V once for both their tiles and halve what crosses from L2, items of 16 are twice as
+    // many: 32 where their cost is the lower (where a request has 16 columns at most, half of them would be empty). Over
+    // 4,000 random shapes of 17 columns a request and more, up to 60,000 shared tokens and tails of 20,000, which were not
+    // used to choose this, what is taken costs 1.1 % more than the better of both (fp16 of 64 dimensions 2.1 %; one in 20
+    // costs 9 to 17 %), always 16 columns 5 to 10 %, always 32 12 to 14 %. fp16 queries, 8 heads to each of 4 kv heads of
+    // 128, 40 windows of up to 3 (78 rows): behind 24,000 tokens 50.0 us (16 columns: 84.2), 12,000 47.8 (46.0), 6,000 34.5
+    // (29.3), 2,000 20.2 (18.1); prompts of 509 and 111 rows over 4,090 and 1,065 tokens, 4 heads to each of 8, 53.2 (63.3).
+    // Of 64 dimensions, 7 heads to each of 2, 24 windows of up to 3 12.5 (32 columns: 15.0), 6 14.9 (16.3), 12 19.8 (17.9).
+    // fp32, those windows of 3 behind 48,000 112.6 (16 columns: 132.7), 24,000 68.5 (100.0), 12,000 61.3 (55.2), the prompts
+    // 66.3 (76.2).
+    // What the cost does not see is how the tails fit beside the prefix's items.
+    Ka4Cut cut = ka4_cut(a, tail_cols, part, 16, 1.f, cus * ka4_held(a.c.head_dim, a.q16, 1));
+    int nc = 1;
+    if (tail_cols > 16) {
+        const Ka4Cut wide = ka4_cut(a, tail_cols, part, 32, a.q16 ? 1.3f : 1.45f,
+                                    cus * ka4_held(a.c.head_dim, a.q16, 2));
+        if (wide.cost < cut.cost) {
+            cut = wide;
+            nc = 2;
+        }
+    }
+    a.tail_tiles = (int)cut.tail_tiles;
     const int64_t units = (int64_t)Hk * a.tail_tiles;
     a.tail_runs = (int)std::max<int64_t>(1, a.slots / units);
     const int64_t longest = std::max<int64_t>((int64_t)a.c.max_pages * a.c.page_size - a.shared, 1);
-    const int64_t part = (int64_t)a.rows * a.H * (a.c.head_dim + 2) * 4;
     a.max_runs = (int)std::min<int64_t>({a.tail_runs, 64, ceil_div(longest, KA4_LEAST * KA_ROUND), std::max<int64_t>(1, (256 << 20) / part)});
     a.direct = a.shared == 0 && a.max_runs == 1;
-    a.tail_items = (int)(items + (a.max_runs == 1 ? 0 : (int64_t)a.tail_runs * units));
+    a.tail_items = (int)(cut.items + (a.max_runs == 1 ? 0 : (int64_t)a.tail_runs * units));
     if (a.shared > 0) {
-        a.pre_tiles = ceil_div(cols, width);
-        const int64_t pre_units = (int64_t)Hk * a.pre_tiles, rounds = ceil_div(a.shared, KA_ROUND);
-        const int64_t most = a.slots / pre_units;
-        // As many runs as fill the device, a quarter of that where the prefix is short (the tails need some of it), and
-        // none longer than KA4_RUN keys where several column tiles read them: an XCD's workgroups then stay within what
-        // its L2 holds (and no more of these than 256 MB of partial results hold). 624 columns x 4 kv heads over 96,000
-        // tokens 185 us, 240 in longer runs; over 48,000 the same, in runs of 6,144 83 -> 93.
-        const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most),
-                                                  a.pre_tiles > 1 ? std::min<int64_t>(ceil_div(a.shared, KA4_RUN), (256 << 20) / part) : 1});
-        a.pre_keys = (int)ceil_div(rounds, std::min(splits, rounds)) * KA_ROUND;
-        a.pre_splits = ceil_div(a.shared, a.pre_keys);
-        a.pre_work = (float)pre_units * (a.pre_splits * a.fixed + rounds);
+        const int64_t pre_units = Hk * cut.pre_tiles;
+        a.pre_tiles = (int)cut.pre_tiles;
+        a.pre_keys = (int)cut.pre_keys;
+        a.pre_splits = (int)cut.pre_splits;
+        a.pre_work = (float)pre_units * (a.pre_splits * a.fixed + ceil_div(a.shared, KA_ROUND));
         const int64_t pre = (int64_t)ceil_div((int64_t)Hk * a.pre_splits, 8) * 8 * a.pre_tiles;
         PIO_REQUIRE(pre <= 1 << 22, "pio_kv_attention: too many rows over %d shared tokens", a.shared);
         a.pre_items = (int)pre;

@@ -95,8 +95,10 @@ class Parts:
 
 PARTS_CASES = [
     # heads, kv heads, dim, rows; the last of each type run in items of 32 columns
-    (4, 2, 128, 3, "float16"), (4, 2, 64, 3, "float16"), (32, 1, 128, 300, "float16"), (16, 1, 64, 4, "float16"),
+    (4, 2, 128, 3, "float16"), (4, 2, 64, 3, "float16"), (16, 1, 64, 4, "float16"), (32, 1, 128, 300, "float16"),
+    (32, 1, 128, 400, "float16"), (32, 1, 64, 400, "float16"),
     (4, 2, 128, 3, "float32"), (4, 2, 64, 3, "float32"), (16, 1, 128, 70, "float32"), (16, 1, 64, 70, "float32"),
+    (32, 1, 128, 400, "float32"), (32, 1, 64, 400, "float32"),
 ]
 
 
@@ -182,6 +184,12 @@ FLAT_CASES = [
     (32, 2, 128, 16, "float32", 0, 313, 1, 300),
     (32, 2, 64, 64, "float32", 0, 1313, 1, 300),
     (32, 2, 128, 32, "float32", 6000, 90, 12, 70),
+    (32, 2, 64, 32, "float32", 6000, 90, 12, 70),
+    (14, 2, 64, 32, "float16", 6000, 90, 40, 20),
+    (32, 2, 128, 16, "float16", 0, 513, 1, 500),
+    (32, 2, 64, 16, "float16", 0, 513, 1, 500),
+    (32, 2, 128, 16, "float32", 0, 513, 1, 500),
+    (32, 2, 64, 16, "float32", 0, 513, 1, 500),
     (8, 2, 128, 16, "float16", 0, 3000, 60, 1),          # ragged ones, cut into runs
     (8, 2, 128, 16, "float32", 0, 600, 300, 2),          # more than the waves find on their own
 ]

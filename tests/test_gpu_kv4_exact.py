@@ -5,7 +5,7 @@ import pytest
 
 import kv4_cases
 from oracle import kv_ref
-from test_gpu_kv4 import Pair4
+from test_gpu_kv4 import Pair4, _masked_columns
 from test_gpu_kv_cache import _attend, _say
 
 pytestmark = pytest.mark.gpu
@@ -141,12 +141,13 @@ def test_every_key_counts(torch, ops, H, Hk, D, page, x, shared, tail, n, window
 @pytest.mark.parametrize("x", ["float32", "float16"])
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("way", ["up", "down", "both"])
-def test_references_follow(torch, ops, D, x, way):
+@pytest.mark.parametrize("H,rows", [(8, 3), (64, 150)])
+def test_references_follow(torch, ops, H, rows, D, x, way):
     """Scores that climb by more than the references stay behind, fall, or do both, over runs and a prefix: values of 1
     with the signs of kv4_cases.flat, keys 0 to 6 in one dimension, 4 (fp16) or 12 (fp32) a step."""
-    _say(f"references D{D} {x} {way}")
+    _say(f"references H{H} D{D} {rows} rows {x} {way}")
     rng = np.random.default_rng(D)
-    n, H, step = 4000, 8, 4.0 if x == "float16" else 12.0
+    n, step = 4000, 4.0 if x == "float16" else 12.0
     c = kv4_cases.held(rng, [n, n], 1, 2, D, 16, 2000)
     kv4_cases.flat(rng, c)
     level = np.arange(n) * 8 // n
@@ -157,15 +158,15 @@ def test_references_follow(torch, ops, D, x, way):
         v = c.rows(0, s, n)[1]
         _fill(c, 0, s, k, v)
     p = _upload(torch, ops, c)
-    q = np.zeros((6, H, D))
+    q = np.zeros((2 * rows, H, D))
     q[:, :, 9] = np.array([1.0, -1.0, 0.5, 2.0])[np.arange(H) % 4]
     q = q.astype(x)
-    want = np.concatenate([kv4_cases.attend(c, 0, s, q[3 * s:3 * s + 3], step) for s in range(2)])
+    want = np.concatenate([kv4_cases.attend(c, 0, s, q[rows * s:rows * (s + 1)], step) for s in range(2)])
     # scores of up to 12 steps: their sums' roundings are of exponents up to that, and 16
     largest = 12 * step
     tol = kv4_cases.flat_tolerance(x, want, largest) + 2 * 9 * 2.0 ** -24 * largest * 2
     for shared in (0, 2000, 1001):
-        got = _attend(p, torch, ops, 0, [0, 1], [0, 3, 6], q, step, shared, 3).astype(np.float64)
+        got = _attend(p, torch, ops, 0, [0, 1], [0, rows, 2 * rows], q, step, shared, rows).astype(np.float64)
         wrong = (np.abs(got - want) / tol).max()
         _say(f"  shared {shared}: {wrong:.2f} of the bound")
         assert wrong <= 1
@@ -174,7 +175,7 @@ def test_references_follow(torch, ops, D, x, way):
 
 @pytest.mark.parametrize("big", [False, True])
 @pytest.mark.parametrize("x", ["float32", "float16"])
-@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (4, 2, 128), (16, 1, 64), (64, 1, 128), (2, 2, 96)])
+@pytest.mark.parametrize("H,Hk,D", [(4, 2, 64), (4, 2, 128), (16, 1, 64), (64, 1, 128), (128, 1, 64), (2, 2, 96)])
 def test_one_token_picked(torch, ops, H, Hk, D, x, big):
     """Each query picks one token, whose weight is 1 and the others' 0: outputs are that token's values, of every scale
     that the cache has and every code, side by side. big: queries as large as their type holds."""
@@ -208,7 +209,8 @@ def test_one_token_picked(torch, ops, H, Hk, D, x, big):
 
 
 @pytest.mark.parametrize("x", ["float32", "float16"])
-@pytest.mark.parametrize("H,Hk,D,rows", [(4, 2, 64, 2), (4, 2, 128, 2), (16, 1, 64, 4), (64, 1, 128, 140)])
+@pytest.mark.parametrize("H,Hk,D,rows", [(4, 2, 64, 2), (4, 2, 128, 2), (16, 1, 64, 4), (64, 1, 128, 140),
+                                         (64, 1, 64, 140)])
 def test_every_scale(torch, ops, H, Hk, D, rows, x):
     """Values of a whole sequence under one scale, the least to the largest that the cache has, and keys likewise, with
     queries and a factor that make ordinary scores of them: relative to that sequence's values. (fp16: an output below
@@ -249,3 +251,11 @@ def test_every_scale(torch, ops, H, Hk, D, rows, x):
         got = _attend(p, torch, ops, 0, [i], [0, counts[i]], q[rows_], factor, 0, rows).astype(np.float64)
         check(got, i, kv4_cases.attend(c, 0, i, q[rows_], factor), 1.0)
     ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("D,H,rows,tokens,x", [
+    (128, 32, 500, 520, "float16"), (64, 32, 500, 533, "float16"), (128, 32, 500, 490, "float32"),
+    (64, 32, 500, 533, "float32"), (64, 14, 30, 100, "float32")])
+def test_masked_columns(torch, ops, D, H, rows, tokens, x):
+    """Enough columns for items of 32 of each type and dimension, whatever the work: NaN blocks in them and behind the end."""
+    _masked_columns(torch, ops, D, H, rows, tokens, x)
