@@ -259,3 +259,38 @@ def test_every_scale(torch, ops, H, Hk, D, rows, x):
 def test_masked_columns(torch, ops, D, H, rows, tokens, x):
     """Enough columns for items of 32 of each type and dimension, whatever the work: NaN blocks in them and behind the end."""
     _masked_columns(torch, ops, D, H, rows, tokens, x)
+
+
+@pytest.mark.parametrize("x", ["float32", "float16"])
+@pytest.mark.parametrize("D,H,window", [(64, 4, 7), (128, 8, 40), (128, 64, 40), (64, 64, 40)])
+def test_a_nan_anywhere(torch, ops, D, H, window, x):
+    """One block of values that is NaN, in each sequence at another place: the rows that see it are NaN in its dimensions,
+    and no others, whichever tile, run or prefix it lies in."""
+    _say(f"NaN anywhere D{D} H{H} {window} rows {x}")
+    rng = np.random.default_rng(D + H)
+    n, common = 40, 90
+    lens = [common + window + int(k) for k in rng.integers(0, 900, n)]
+    c = kv4_cases.held(rng, lens, 1, 2, D, 16, common)
+    kv4_cases.flat(rng, c)
+    kv4_cases.share(c, common)
+    scales = c.blocks()[1]
+    # at the borders of tiles, the ends, and just before and behind what the first row sees; some in the prefix's last page
+    for s, L in enumerate(lens):
+        places = [L - 1, L - window, L - window + 1, L - window - 1, common, common + 5, (L - window) & -32, L & -32, L - 33,
+                  common + (L - common) // 2]
+        pos = max(common, min(L - 1, places[s % len(places)]))
+        scales[0, 1, c.table[s, pos // 16], :, int(rng.integers(0, D // 32)), pos % 16] = 255
+    p = _upload(torch, ops, c)
+    seq = [int(s) for s in rng.permutation(n)]
+    counts = [int(k) for k in rng.integers(1, window + 1, n)]
+    start = np.concatenate([[0], np.cumsum(counts)]).astype(int)
+    q = rng.standard_normal((int(start[-1]), H, D)).astype(x)
+    want = c.attention(0, seq, start, q, D ** -0.5, np.zeros(q.shape))
+    fine = np.isfinite(want)
+    assert 0.01 < (~fine).mean() < 0.9
+    tol = kv4_cases.flat_tolerance(x, np.where(fine, want, 0), float(np.abs(q).max()) * 6 * 2.0 ** -8 * D ** 0.5)
+    for shared in (0, common, 37):
+        got = _attend(p, torch, ops, 0, seq, start, q, D ** -0.5, shared, window).astype(np.float64)
+        assert np.array_equal(np.isfinite(got), fine)
+        assert (np.abs(got - want)[fine] <= tol[fine]).all()
+    ops.kv_status(p.c)
