@@ -400,7 +400,7 @@ int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t
 /* Tokens out of the cache: rows row_start[i] .. row_start[i + 1] - 1 of k and v
  * become the keys and values of seq[i]'s tokens from first[i] on (its last ones,
  * where first is null), in `layers` layers from `layer`; the layouts and limits are
- * pio_kv_write's, and rows and layers may not overlap. fp32|fp16, rounded to
+ * pio_kv_write's, and neither rows nor layers nor k and v may overlap (k and v may take turns). fp32|fp16, rounded to
  * it from an fp32 cache. A row whose sequence, token or page is not there becomes NaN, and
  * pio_kv_status reports it; rows at and behind row_start[n] are left as they are. One
  * sequence may come often. Behind a refused pio_kv_reserve the rows of its sequences

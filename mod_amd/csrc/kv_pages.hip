@@ -12,6 +12,7 @@
 #include <algorithm>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 #include <type_traits>
 
 namespace pio {
@@ -777,6 +778,22 @@ PIO_EXPORT int pio_kv_write(const pio_kv_cache* c, int layer, int layers, const 
     return PIO_OK;
 }
 
+// Whether a row of k shares elements with one of v, `bytes` behind k: rows and layers of `width` elements that do not overlap
+// among themselves. The greater of the strides is at least as long as all that the smaller one spans.
+static bool kv_rows_meet(int64_t bytes, int size, int64_t width, int rows, int64_t row_stride, int layers, int64_t layer_stride) {
+    if (layers == 1) layer_stride = INT64_MAX / 4;
+    const bool rows_within = row_stride <= layer_stride;
+    const int64_t s2 = rows_within ? layer_stride : row_stride, s1 = rows_within ? row_stride : layer_stride;
+    const int64_t n2 = rows_within ? layers : rows, n1 = rows_within ? rows : layers;
+    const int64_t d = (bytes < 0 ? -bytes : bytes) / size;                 // (both are 16-byte aligned)
+    for (int k2 = 0; k2 < 2; k2++) {
+        const int64_t off = std::abs(d - std::min(d / s2 + k2, n2 - 1) * s2);
+        for (int k1 = 0; k1 < 2; k1++)
+            if (std::abs(off - std::min(off / s1 + k1, n1 - 1) * s1) < width) return true;
+    }
+    return false;
+}
+
 PIO_EXPORT int pio_kv_read(const pio_kv_cache* c, int layer, int layers, const int32_t* seq, const int32_t* row_start,
                            const int32_t* first, int n, void* k, void* v, int dtype, int rows, int64_t row_stride,
                            int64_t layer_stride, void* stream) {
@@ -803,6 +820,9 @@ PIO_EXPORT int pio_kv_read(const pio_kv_cache* c, int layer, int layers, const i
     PIO_REQUIRE(layers == 1 || (layer_stride >= width && ((layer_stride - width) / row_stride >= rows - 1 ||
                                                           (row_stride - width) / layer_stride >= layers - 1)),
                 "%s: strides %lld, %lld: rows or layers overlap", nm, (long long)row_stride, (long long)layer_stride);
+    PIO_REQUIRE(!kv_rows_meet((const char*)v - (const char*)k, dtype == PIO_F32 ? 4 : 2, width, rows, row_stride, layers,
+                              layer_stride),
+                "%s: k and v overlap", nm);
     const int per_block = (int)std::max<int64_t>(1, std::min<int64_t>({layers, (int64_t)rows * layers / 4096, (1 << 28) / width}));
     const dim3 grid(rows, ceil_div(layers, per_block));
     PIO_REQUIRE(grid.y <= 65535, "%s: too many layers", nm);

@@ -136,3 +136,27 @@ def test_every_geometry(torch, ops, kind, heads, dim, page, layers, x):
             want = p.ref.rows(0, s, lens[i])[kind_][-last[i]:].astype(x)
             assert np.array_equal(rows[0, start[i]:start[i + 1]], want)
     ops.kv_status(p.c)
+
+
+@pytest.mark.parametrize("x", ["float32", "float16"])
+def test_k_and_v_in_turns(torch, ops, x):
+    """k and v of a row side by side, and of a layer: taken, as they share no element; half a row apart: refused."""
+    rng = np.random.default_rng(9)
+    p = _pair(torch, ops, "mx4", 3, 2, 32, 16, 4, 2, 2)
+    p.add(rng, [1], [21])
+    dtype = getattr(torch, x)
+    for row_stride, layer_stride, apart in ((128, 21 * 128, 64), (64, 2 * 21 * 64, 21 * 64), (6 * 64, 128, 64)):
+        both = torch.full((3 * 21 * 128,), 7.0, dtype=dtype, device="cuda")
+        torch.cuda.synchronize()
+        args = (p.c, 0, 3, p.ints([1]), p.ints([0, 21]), 1)
+        ops.kv_read(*args, both, both[apart:], 21, row_stride=row_stride, layer_stride=layer_stride)
+        torch.cuda.synchronize()
+        got = both.cpu().numpy()
+        for layer in range(3):
+            for kind, rows in enumerate(p.ref.rows(layer, 1, 21)):
+                for r in range(21):
+                    at = layer * layer_stride + r * row_stride + kind * apart
+                    assert np.array_equal(got[at:at + 64], rows[r].reshape(-1).astype(x))
+        with pytest.raises(ops.RocmError, match="k and v overlap"):
+            ops.kv_read(*args, both, both[apart - 32:], 21, row_stride=row_stride, layer_stride=layer_stride)
+    ops.kv_status(p.c)
