@@ -124,12 +124,13 @@ __global__ __launch_bounds__(KA_THREADS) void ka4_simple_kernel(KaArgs a) {
 //     and widens each key's to fp16 under its scale, exactly: two keys' halves side by side are the operand, so
 //     V is turned inside a lane. Row i of O^T tile n is dimension (D / 16) i + n.
 // What it costs (2.4 GHz): an item's chain of waits (its request, page ids, K, the join) is 16,000 clocks, most of
-// them loads on loads and code that is fetched for the first time; a tile of 32 keys and 16 columns some 1,100 clocks
-// of a SIMD's issue, whatever the order: products and the VALU's work were measured to add up, also where two waves
-// share the SIMD. Long tails are bound by memory: 3 sequences of 120,000 tokens (8 kv heads x 128, fp16) 28 us, 4.7
-// TB/s; many columns by instructions: 624 over 24,000 tokens 48 us, 646 TFLOP/s. Tried and no faster: the workgroup's
-// waves on columns of their own around V widened once in LDS (64 us), K and V one more tile ahead (+2 us), 3 waves to
-// a SIMD of 16 columns (168 registers, +5 us), products and VALU interleaved by hand, wave priorities.
+// them loads on loads and code that is fetched for the first time; a tile of 32 keys and 32 columns of 128 dimensions, 34
+// products (544 clocks) and 130 VALU instructions with fp16 queries, 1,100 clocks of a SIMD's issue, whatever the order:
+// products and the VALU's work were measured to add up, also where two waves share the SIMD. Long tails are bound by
+// memory: 3 sequences of 120,000 tokens (8 kv heads x 128, fp16) 70 us with their join, 5.6 TB/s; many columns by
+// instructions: 78 rows of 32 heads over 24,000 tokens 49 us, 620 TFLOP/s. Tried and no faster (of 128 dimensions): the
+// workgroup's waves on columns of their own around V widened once in LDS, K and V one more tile ahead, 3 waves to a SIMD
+// of 16 columns, products and VALU interleaved by hand, wave priorities.
 //   A lane's 8 scores are of the keys 4 q .. 4 q + 3 of either 16, q = l / 16, and those are the keys of its part of
 //     the weights' operand; V's rows are read in that order.
 typedef int ka4_i8 __attribute__((ext_vector_type(8)));
@@ -148,8 +149,8 @@ constexpr int KA4_TILE = 32, KA4_WAVES = 4;
 // for what is smaller the loss of a block is a 20th of what rounding its largest to fp16 was. One dimension 30, 300,
 // 3,000 times the others, 4,096 normal keys: 5e-6, 3e-5 and 2e-4 to 1e-3 of the output in the 2-norm, whose rounding is
 // 2e-4 (3 parts: 2e-4, 5e-4 to 3e-3, 7e-3 to 3e-2; 5, as fp32 queries have: 2e-7, 7e-7, 4e-6, as fp32 products). 78 rows behind 24,000
-// tokens 49.8 us (3 parts 47.6, 5 52.4), prompts of 509 and 111 rows 53.1 (50.6, 56.2), 24 windows of up to 6 of 64
-// dimensions, where an operand holds two parts, 16.0 (15.8, 16.9).
+// tokens 49.8 us (3 parts 47.6, 5 52.4), prompts of 509 and 111 rows 53.1 (50.6, 56.2); of 64 dimensions, where an operand
+// holds two parts, 24 windows of up to 6 in 32 columns 16.0 (15.8, 16.9).
 //   Weights: rounding them costs normal inputs as much as rounding the output, 2.0e-4 each; a second part is a third of
 // the products.
 template <int D, bool X16>
@@ -357,9 +358,10 @@ struct Ka4Walk {
         const uint32_t o = here(ko);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            // (past the caches where the keys are read once: sequences of 120,011, 3,323 and 2,565 tokens 36.4 us, so 32.9. V's
-            // rows, whose lines two loads share, are not: 35.1. Where several tiles read them: 24 windows of up to 6 over
-            // 16,000 tokens, 3 tiles each, 26.6 past the caches, 25.2 through them)
+            // (past the caches where the keys are read once: 3 sequences of 120,000 tokens 70.3 us, through them 76.8, 32 of
+            // 16,000 54.7 and 58.8, where no cache holds them before the call; where the memory-side cache does, the same 137
+            // MB again and again, 43.6 and 41.2. V's rows, whose lines two loads share, are not. Where several tiles read the
+            // keys: 24 windows of up to 6 over 16,000 tokens, 3 tiles each, 26.6 past the caches, 25.2 through them)
             if constexpr (ONCE)
                 to.k[h] = __builtin_nontemporal_load((const __attribute__((address_space(1))) ka4_u4*)(kc[h] + o));
             else
@@ -682,8 +684,8 @@ __device__ __forceinline__ void ka4_item(const KaArgs& a, const KaItem& it, floa
 }
 
 // ka_runs for up to 64 N requests, by each wave on its own: no LDS and no barriers, and what is found is the same
-// for the wave's lanes as the compiler sees it. 1 sequence 8.9 us (by the workgroup 9.8), 40 behind a prompt 15.6
-// (17.0), 200 of up to 300 tokens 18.3 (17.8); more would cost registers.
+// for the wave's lanes as the compiler sees it. 1 sequence 8.9 us (by the workgroup 9.6), 40 behind a prompt 15.7
+// (16.8), 200 of up to 300 tokens 31.8 (32.2); more would cost registers.
 template <int N>
 __device__ __forceinline__ void ka4_runs(const KaArgs& a, int unit, KaRun& found, int cols) {
     const int lane = threadIdx.x & 63;
@@ -810,11 +812,11 @@ static int ka4_join(const KaArgs& a, hipStream_t st) {
 }
 
 // An item costs its rounds of keys and this many more. A small figure cuts long rows into more runs than pay for their
-// join: 32 sequences of up to 16,000 tokens 19.9 us with 4, 17.0 with 6, 17.1 with 8, and 96 of them 43.0 us with any of
-// these; with 2, 40 sequences behind a prompt 19.0 us against 15.5.
+// join: 32 sequences of up to 16,000 tokens 19.8 us with 4, 17.2 with 6, 17.0 with 8, and 96 of them 43.5 us with any of
+// these; with 2, 40 sequences behind a prompt 16.3 us against 15.6.
 constexpr float KA4_FIXED = 6.f;
 // Rounds of a run at least, as a table row's pages allow: below, what the waves save is less than what the join costs.
-// Rows of 512 keys or less need none: 1 sequence of 301 tokens 8.9 us, in runs of a round 10.1.
+// 1 sequence of 301 tokens 8.9 us, in runs of a round 10.1; of 200 8.2 and 10.0, of 500 10.7 and 10.2.
 constexpr int KA4_LEAST = 4;
 // Keys of a prefix's run at most (below).
 constexpr int KA4_RUN = 8192;
@@ -841,8 +843,8 @@ static Ka4Cut ka4_cut(const KaArgs& a, int64_t tail_cols, int64_t part, int widt
     const int64_t units = Hk * k.pre_tiles, rounds = (a.shared + KA_ROUND - 1) / KA_ROUND, most = a.slots / units;
     // As many runs as fill the device, a quarter of that where the prefix is short (the tails need some of it), and
     // none longer than KA4_RUN keys where several column tiles read them: an XCD's workgroups then stay within what
-    // its L2 holds (and no more of these than 256 MB of partial results hold). 624 columns x 4 kv heads over 96,000
-    // tokens 185 us, 240 in longer runs; over 48,000 the same, in runs of 6,144 83 -> 93.
+    // its L2 holds (and no more of these than 256 MB of partial results hold). 78 rows of 32 heads on 4 over 96,000 tokens
+    // 178 us, 240 in longer runs, 171 in runs of 6,144; over 48,000 78, 78 and 90.
     const int64_t splits = std::max<int64_t>({1, most / 4, std::min(rounds / 8, most),
                                               k.pre_tiles > 1 ? std::min<int64_t>((a.shared + KA4_RUN - 1) / KA4_RUN, (256 << 20) / part) : 1});
     const int64_t each = std::min(splits, rounds), run = (rounds + each - 1) / each;
@@ -866,11 +868,11 @@ static int ka4_matrix(KaArgs& a, int max_rows, hipStream_t st) {
     // 4,000 random shapes of 17 columns a request and more, up to 60,000 shared tokens and tails of 20,000, which were not
     // used to choose this, what is taken costs 1.1 % more than the better of both (fp16 of 64 dimensions 2.1 %; one in 20
     // costs 9 to 17 %), always 16 columns 5 to 10 %, always 32 12 to 14 %. fp16 queries, 8 heads to each of 4 kv heads of
-    // 128, 40 windows of up to 3 (78 rows): behind 24,000 tokens 50.0 us (16 columns: 84.2), 12,000 47.8 (46.0), 6,000 34.5
-    // (29.3), 2,000 20.2 (18.1); prompts of 509 and 111 rows over 4,090 and 1,065 tokens, 4 heads to each of 8, 53.2 (63.3).
-    // Of 64 dimensions, 7 heads to each of 2, 24 windows of up to 3 12.5 (32 columns: 15.0), 6 14.9 (16.3), 12 19.8 (17.9).
-    // fp32, those windows of 3 behind 48,000 112.6 (16 columns: 132.7), 24,000 68.5 (100.0), 12,000 61.3 (55.2), the prompts
-    // 66.3 (76.2).
+    // 128, 40 windows of up to 3 (78 rows): behind 48,000 tokens 78.6 us (16 columns: 105.0), 24,000 49.7 (84.4), 12,000
+    // 47.9 (46.0), 6,000 34.8 (29.2), 2,000 19.9 (17.7); prompts of 509 and 111 rows over 4,090 and 1,065 tokens, 4 heads to
+    // each of 8, 53.3 (64.5), of 2,000 tokens 113 (158). Of 64 dimensions, 7 heads to each of 2, 24 windows of up to 3 12.6
+    // (32 columns: 14.9), 6 14.9 (16.3), 12 19.9 (17.9). fp32, those 40 windows behind 48,000 109 (16 columns: 130), 24,000
+    // 68.2 (99.8), 12,000 60.8 (55.1), 2,000 25.2 (23.9), those prompts 66.4 (75.2).
     // What the cost does not see is how the tails fit beside the prefix's items.
     Ka4Cut cut = ka4_cut(a, tail_cols, part, 16, 1.f, cus * ka4_held(a.c.head_dim, a.q16, 1));
     int nc = 1;
