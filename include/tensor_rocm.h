@@ -379,8 +379,8 @@ int pio_kv_status(const pio_kv_cache* cache, void* stream);
  * one). All or nothing: if any request is refused, or the free pages do not
  * suffice, no request is served. Behind a refused call its sequences are held up:
  * pio_kv_write and pio_kv_drop with counts leave them as they are, and pio_kv_read of
- * their last tokens gives NaN, so that a step's calls need not wait for its outcome (the attention and verification of such a
- * step mean nothing: ask pio_kv_status before their results are used). That ends
+ * their last tokens gives NaN, so that a step's calls need not wait for its outcome
+ * (the attention and verification of such a step mean nothing: ask pio_kv_status before their results are used). That ends
  * with pio_kv_status, with a pio_kv_reserve that serves the sequence, and with its
  * end (pio_kv_drop without counts, pio_kv_fork onto it). */
 int pio_kv_reserve(const pio_kv_cache* cache, const int32_t* seq, const int32_t* count, int n, void* stream);
@@ -400,8 +400,8 @@ int pio_kv_write(const pio_kv_cache* cache, int layer, int layers, const int32_t
 /* Tokens out of the cache: rows row_start[i] .. row_start[i + 1] - 1 of k and v
  * become the keys and values of seq[i]'s tokens from first[i] on (its last ones,
  * where first is null), in `layers` layers from `layer`; the layouts and limits are
- * pio_kv_write's, and neither rows nor layers nor k and v may overlap (k and v may take turns). fp32|fp16, rounded to
- * it from an fp32 cache. A row whose sequence, token or page is not there becomes NaN, and
+ * pio_kv_write's, and neither rows nor layers nor k and v may overlap (k and v may
+ * take turns). fp32|fp16, rounded to it from an fp32 cache. A row whose sequence, token or page is not there becomes NaN, and
  * pio_kv_status reports it; rows at and behind row_start[n] are left as they are. One
  * sequence may come often. Behind a refused pio_kv_reserve the rows of its sequences
  * that are counted from the end, or lie behind it, become NaN: their tokens never came

@@ -148,9 +148,9 @@ constexpr int KA4_TILE = 32, KA4_WAVES = 4;
 //   4 parts are within 2^-18 of the largest of 32 dimensions: what is a 128th of that or more keeps all 11 bits, and
 // for what is smaller the loss of a block is a 20th of what rounding its largest to fp16 was. One dimension 30, 300,
 // 3,000 times the others, 4,096 normal keys: 5e-6, 3e-5 and 2e-4 to 1e-3 of the output in the 2-norm, whose rounding is
-// 2e-4 (3 parts: 2e-4, 5e-4 to 3e-3, 7e-3 to 3e-2; 5, as fp32 queries have: 2e-7, 7e-7, 4e-6, as fp32 products). 78 rows behind 24,000
-// tokens 49.8 us (3 parts 47.6, 5 52.4), prompts of 509 and 111 rows 53.1 (50.6, 56.2); of 64 dimensions, where an operand
-// holds two parts, 24 windows of up to 6 in 32 columns 16.0 (15.8, 16.9).
+// 2e-4 (3 parts: 2e-4, 5e-4 to 3e-3, 7e-3 to 3e-2; 5, as fp32 queries have: 2e-7, 7e-7, 4e-6, as fp32 products). 78
+// rows behind 24,000 tokens 49.8 us (3 parts 47.6, 5 52.4), prompts of 509 and 111 rows 53.1 (50.6, 56.2); of 64
+// dimensions, where an operand holds two parts, 24 windows of up to 6 in 32 columns 16.0 (15.8, 16.9).
 //   Weights: rounding them costs normal inputs as much as rounding the output, 2.0e-4 each; a second part is a third of
 // the products.
 template <int D, bool X16>
